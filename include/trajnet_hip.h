@@ -659,6 +659,49 @@ TNP_API int64_t tnp_format_predictions(const double *pred, int n_modes, int pred
                                        const int64_t *scene_end, char *out, size_t cap);
 TNP_API size_t tnp_format_predictions_bound(int n_modes, int pred_length, int64_t M, int64_t n_scenes);
 
+/* ---- motions as tokens: embedding table and cross entropy over a vocabulary --------------------------------------------------
+ * No counterpart in the reference (its input and output are continuous positions); they stand beside InputEmbedding
+ * (lstm/modules.py:4-48) and PredictionLoss (lstm/loss.py:6-91) for models whose motions are entries of a vocabulary.
+ * A negative token or target marks an absent track everywhere. */
+#define TNP_F32  0
+#define TNP_BF16 1
+#define TNP_F16  2
+
+/* out[i, :] = scale * weight[tokens[i], :];  tokens int32 / int64 (token_bytes 4 / 8), tokens[i] < 0: a zero row,
+ * tokens[i] >= V: a NaN row.  ldw / ldo: elements per row. */
+TNP_API int tnp_token_embedding_forward(const void *tokens, int token_bytes, int64_t N, const void *weight, int64_t ldw,
+                                        int64_t V, int D, int dtype, float scale, void *out, int64_t ldo, void *stream);
+/* dweight[v, :] = scale * sum of grad[i, :] over tokens[i] == v, every row of dweight written (zero where no token names it);
+ * fp32 sums in a fixed order.  Tokens outside [0, V) contribute nothing. */
+TNP_API size_t tnp_token_embedding_backward_workspace_bytes(int64_t N, int64_t V, int D);
+TNP_API int tnp_token_embedding_backward(const void *tokens, int token_bytes, int64_t N, const void *grad, int64_t ldg,
+                                         int64_t V, int D, int dtype, float scale, void *dweight, int64_t ldd, void *workspace,
+                                         size_t workspace_bytes, void *stream);
+
+/* loss_i = log sum_v exp(hidden_i . weight_v + bias_v) - (hidden_i . weight_t + bias_t), t = target[i], without keeping the
+ * logits.  target[i] < 0: loss and gradients 0, hidden_i is not read; target[i] >= V: NaN.  bias may hold -inf (masked entries). */
+typedef struct tnp_vocab_ce {
+    int32_t dtype;              /* TNP_F32 / TNP_BF16 / TNP_F16: hidden, weight, bias and their gradients */
+    int32_t reduction;          /* 0 none, 1 mean over the rows that are there (0 if there are none), 2 sum */
+    int64_t M;                  /* rows */
+    int32_t V, D;
+    const void *hidden;         /* [M, D], ld_hidden elements per row */
+    int64_t ld_hidden;
+    const void *weight;         /* [V, D], ld_weight elements per row */
+    int64_t ld_weight;
+    const void *bias;           /* [V] or NULL */
+    const int64_t *target;      /* [M] */
+    void *saved;                /* tnp_vocab_ce_saved_bytes() bytes that the forward pass fills for the backward pass (which
+                                   reads them, weight, bias and target); NULL: no backward pass will follow */
+} tnp_vocab_ce;
+TNP_API size_t tnp_vocab_ce_saved_bytes(const tnp_vocab_ce *args);
+TNP_API size_t tnp_vocab_ce_workspace_bytes(const tnp_vocab_ce *args, int backward);
+/* loss: fp32, [M] (none) or [1] */
+TNP_API int tnp_vocab_ce_forward(const tnp_vocab_ce *args, float *loss, void *workspace, size_t workspace_bytes, void *stream);
+/* grad: fp32, [M] (none) or [1]; dhidden [M, D], dweight [V, D], dbias [V] contiguous, each may be NULL */
+TNP_API int tnp_vocab_ce_backward(const tnp_vocab_ce *args, const float *grad, void *dhidden, void *dweight, void *dbias,
+                                  void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

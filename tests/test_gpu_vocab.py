@@ -1,0 +1,452 @@
+"""Token embedding and vocabulary cross entropy on the GPU against their formulas in 64 bits.
+
+Tolerances come from the arithmetic, not from runs.  u(t) = finfo(t).eps / 2 is the unit round-off of a type.
+ * A sum of n fp32 terms in any order is off by at most n 2^-24 times the sum of their magnitudes; the matrix instructions' own
+   accumulation is counted as 2^-23 per term.
+ * fp32 operands of the cross entropy are two fp16 numbers: |x - hi - lo| <= 2^-22 |x| + 2^-39 max|x|; the product lo * lo is left
+   out (2^-22): a product is off by at most 3 * 2^-22 |x w| (+ the 2^-38 term).  bf16 / fp16 operands are exact down to 2^-39 max|x|.
+ * G = g (p - y) is rounded to fp16 (2^-11) or two fp16 numbers (2^-22), with 2^-40 max|g| of absolute error.
+"""
+import math
+
+import pytest
+import torch
+
+from trajnetplusplusbaselines_amd import vocab
+from trajnetplusplusbaselines_amd.lstm import TokenEmbedding, VocabularyLoss
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def _u(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _gen(seed):
+    return torch.Generator(device='cuda').manual_seed(seed)
+
+
+def _within(got, want, bound):
+    got, want = got.double(), want.double()
+    assert got.shape == want.shape
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    ok = torch.isfinite(want)
+    assert torch.equal(got[~ok & ~torch.isnan(want)], want[~ok & ~torch.isnan(want)])
+    worst = ((got - want).abs() / bound.clamp(min=1e-300))[ok]
+    assert worst.numel() == 0 or worst.max() <= 1.0, 'off by %.3g of the bound' % float(worst.max())
+
+
+# ---- token embedding --------------------------------------------------------------------------------------------------------
+def _round_bound(v, dtype):
+    # one rounding to fp32 of the product, one to the type; half a step of the smallest numbers
+    return v.abs() * (_u(dtype) + 2.0 ** -24) * 1.0001 + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+
+
+def _tokens(n, vocab_size, kind, g):
+    if kind == 'one':                                   # every track the same token
+        return torch.full((n,), vocab_size // 2, device='cuda')
+    t = torch.rand(n, device='cuda', generator=g, dtype=torch.float64)
+    t = (t ** (4 if kind == 'skew' else 1) * vocab_size).long().clamp(max=vocab_size - 1)
+    if kind == 'absent':
+        t[torch.rand(n, device='cuda', generator=g) < 0.5] = -1
+    if kind == 'none':
+        t[:] = -1
+    return t
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('n,v,d,kind', [
+    (1, 1, 1, 'one'), (1, 7, 64, 'even'), (36, 256, 64, 'skew'), (31, 5, 3, 'one'), (33, 5, 8, 'one'), (65, 3, 17, 'absent'),
+    (1000, 1023, 33, 'even'), (1000, 1024, 128, 'skew'), (5000, 2, 100, 'skew'), (8192, 300, 16, 'one'), (8193, 300, 16, 'one'),
+    (20011, 70001, 12, 'even'), (40000, 257, 64, 'absent'), (100, 1300000, 4, 'even'), (777, 50, 1030, 'skew'), (50, 9, 24, 'none')])
+def test_embedding_lookup_and_gradient(dtype, n, v, d, kind):
+    g = _gen(n + v + d)
+    tok = _tokens(n, v, kind, g)
+    w = torch.randn(v, d, device='cuda', generator=g).to(dtype).requires_grad_()
+    scale = 3.7
+    s32 = torch.tensor(scale, dtype=torch.float32).double().item()      # the C entry takes a float
+    out = vocab.token_embedding(tok, w, scale)
+    there = (tok >= 0)[:, None]
+    want = torch.where(there, w.detach().double()[tok.clamp(min=0)] * s32, 0.0)
+    assert out.dtype == dtype
+    _within(out, want, _round_bound(want, dtype))
+    grad = torch.randn(n, d, device='cuda', generator=g).to(dtype)
+    dw, = torch.autograd.grad(out, w, grad)
+    contrib = torch.where(there, grad.double() * s32, 0.0)
+    zero = torch.zeros(v, d, dtype=torch.float64, device='cuda')
+    want_dw = zero.index_add(0, tok.clamp(min=0), contrib)
+    mag = zero.index_add(0, tok.clamp(min=0), contrib.abs())
+    count = zero[:, :1].index_add(0, tok.clamp(min=0), there.double())
+    _within(dw, want_dw, mag * count * 2.0 ** -24 + _round_bound(want_dw, dtype))
+    assert bool((dw[count[:, 0] == 0] == 0).all())
+    again, = torch.autograd.grad(vocab.token_embedding(tok, w, scale), w, grad)
+    assert torch.equal(dw, again)                                       # fixed order: the same bits
+
+
+def test_embedding_layouts():
+    g = _gen(1)
+    big = torch.randn(50, 40, device='cuda', generator=g)
+    tok = torch.randint(50, (6, 14), device='cuda', generator=g)
+    want = big[:, 3:27].double()[tok] * 0.5
+    for w, t in ((big[:, 3:27], tok), (big.t().contiguous().t()[:, 3:27], tok), (big[:, 3:27].contiguous(), tok.int()),
+                 (big[:, 3:27], tok.t().contiguous().t())):
+        out = vocab.token_embedding(t, w, 0.5)
+        assert out.shape == (6, 14, 24) and out.is_contiguous()
+        _within(out, want, _round_bound(want, torch.float32))
+    w = big.clone().requires_grad_()
+    out = vocab.token_embedding(tok, w)
+    up = torch.randn(14, 6, 40, device='cuda', generator=g).transpose(0, 1)             # gradient in another order
+    dw, = torch.autograd.grad(out, w, up)
+    want = torch.zeros(50, 40, dtype=torch.float64, device='cuda').index_add(0, tok.reshape(-1), up.double().reshape(-1, 40))
+    _within(dw, want, 84 * 2.0 ** -23 * torch.full_like(want, 10.0))
+    up1 = torch.ones((), device='cuda').expand(6, 14, 40)                                # a broadcast gradient
+    dw, = torch.autograd.grad(vocab.token_embedding(tok, w), w, up1)
+    assert torch.equal(dw, torch.bincount(tok.reshape(-1), minlength=50)[:, None].float().expand(50, 40))
+
+
+def test_embedding_tokens_outside_the_table():
+    w = torch.ones(4, 8, device='cuda', requires_grad=True)
+    tok = torch.tensor([-5, 0, 4, 3, 2 ** 40, -2 ** 40, 3], device='cuda')
+    out = vocab.token_embedding(tok, w, 2.0)
+    assert torch.isnan(out[[2, 4]]).all() and (out[[0, 5]] == 0).all() and (out[[1, 3, 6]] == 2.0).all()
+    dw, = torch.autograd.grad(out, w, torch.ones_like(out))
+    assert dw[:, 0].tolist() == [2.0, 0.0, 0.0, 4.0]
+    empty = vocab.token_embedding(tok[:0], w)
+    assert empty.shape == (0, 8)
+    dw, = torch.autograd.grad(empty, w, torch.ones_like(empty))
+    assert bool((dw == 0).all())
+    nan = torch.full((4, 8), float('nan'), device='cuda')
+    assert bool((vocab.token_embedding(torch.tensor([-1], device='cuda'), nan) == 0).all())
+
+
+def test_embedding_half_rows_that_are_not_sixteen_bytes():
+    """every width of access: row lengths and base addresses of 2, 4 and 16 bytes"""
+    g = _gen(3)
+    for d, off in ((7, 0), (6, 1), (6, 2), (8, 4), (8, 8), (24, 1)):
+        base = torch.randn(40 * 32 + 16, device='cuda', generator=g).half()
+        w = base[off:off + 40 * 32].view(40, 32)[:, :d]
+        tok = torch.randint(40, (100,), device='cuda', generator=g)
+        want = w.double()[tok] * 1.5
+        _within(vocab.token_embedding(tok, w, 1.5), want, _round_bound(want, torch.float16))
+
+
+# ---- cross entropy ----------------------------------------------------------------------------------------------------------
+def _case(m, v, d, dtype, seed, bias=True, absent=0.0, masked=0.0):
+    g = _gen(seed)
+    t = torch.randint(v, (m,), device='cuda', generator=g)
+    w = torch.randn(v, d, device='cuda', generator=g) * (2.0 / math.sqrt(d))
+    x = torch.tanh(2.0 * torch.rand(m, 1, device='cuda', generator=g) * w[t] + 0.7 * torch.randn(m, d, device='cuda', generator=g))
+    b = torch.randn(v, device='cuda', generator=g) if bias else None
+    if masked:
+        b[torch.rand(v, device='cuda', generator=g) < masked] = float('-inf')
+        b[0] = 0.0
+        t[b[t] == float('-inf')] = 0
+    if absent:
+        gone = torch.rand(m, device='cuda', generator=g) < absent
+        t[gone] = -1 - torch.randint(200, (int(gone.sum()),), device='cuda', generator=g)
+        x[gone] = float('nan')
+    leaf = lambda z: None if z is None else z.to(dtype).requires_grad_()
+    return leaf(x), leaf(w), leaf(b), t
+
+
+def _formula(x, w, b, t, grad_rows):
+    """loss per row, gradients and their bounds, everything in 64 bits"""
+    dtype = x.dtype
+    split = dtype == torch.float32
+    there = t >= 0
+    xd = torch.where(there[:, None], x.detach().double(), 0.0)
+    wd = w.detach().double()
+    k, v = xd.shape[1], wd.shape[0]
+    l = xd @ wd.t() + (b.detach().double() if b is not None else 0.0)
+    at = t.clamp(min=0)[:, None]
+    lse = torch.logsumexp(l, 1)
+    loss = torch.where(there, lse - l.gather(1, at)[:, 0], 0.0)
+    p = torch.exp(l - lse[:, None])
+    # logits: products, their sum, scale and bias
+    per = (3 * 2.0 ** -22 if split else 0.0) + (3 if split else 1) * k * 2.0 ** -23
+    delta = per * (xd.abs() @ wd.abs().t()) + k * 2.0 ** -38 * xd.abs().max() * wd.abs().max()
+    delta += 4 * 2.0 ** -24 * torch.nan_to_num(l.abs(), posinf=0.0)
+    worst = delta.max(1).values
+    # exponentials (2^-22, and the rounding of their argument) and their sum (lane sums of up to 64 terms, wave tiles, joins)
+    sums = 2.0 ** -22 + 2 * 2.0 ** -24 * torch.nan_to_num(l.abs(), posinf=0.0).max(1).values + (64 + v / 16 + 32) * 2.0 ** -24
+    loss_bound = torch.where(there, 2 * worst + sums + 4 * 2.0 ** -24 * (loss.abs() + lse.abs()), 0.0) + 1e-30
+    g = torch.where(there, grad_rows.double(), 0.0)[:, None]
+    gp = p * g
+    G = gp.scatter_add(1, at, -g)
+    dp = p * g.abs() * (2 * worst + 2 * sums)[:, None] * 1.01
+    dG = dp + G.abs() * (2.0 ** -22 if split else 2.0 ** -11) + 4 * 2.0 ** -24 * G.abs() + 2.0 ** -39 * g.abs().max()
+    dG = torch.where(there[:, None], dG, 0.0)
+    m = xd.shape[0]
+    both = 3 * 2.0 ** -22 if split else 0.0
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    dx, dw, db = G @ wd, G.t() @ xd, G.sum(0)
+    near = lambda val, a, c, n: a + c * (both + (3 if split else 1) * n * 2.0 ** -23) + val.abs() * (_u(dtype) + 3 * 2.0 ** -24) + tiny + 1e-30
+    bx = near(dx, dG @ wd.abs(), G.abs() @ wd.abs(), v) + v * 2.0 ** -38 * wd.abs().max() * G.abs().max()
+    bw = near(dw, dG.t() @ xd.abs(), G.t().abs() @ xd.abs(), m) + m * 2.0 ** -38 * xd.abs().max() * G.abs().max()
+    bb = near(db, dG.sum(0), G.abs().sum(0), m)
+    return loss, loss_bound, (dx, dw, db), (bx, bw, bb)
+
+
+SHAPES = [(1, 1, 1), (1, 300, 64), (2, 17, 3), (16, 255, 8), (17, 257, 33), (64, 1000, 128), (65, 1000, 128), (100, 31, 200), (257, 513, 65),
+          (300, 700, 96), (1000, 130, 256), (511, 4099, 40)]
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('m,v,d', SHAPES)
+def test_scoring_without_gradient(dtype, m, v, d):
+    x, w, b, t = _case(m, v, d, dtype, 1000 * m + v, absent=0.3 if m > 4 else 0.0)
+    loss, bound, _, _ = _formula(x, w, b, t, torch.ones(m, device='cuda'))
+    with torch.no_grad():
+        _within(vocab.vocab_cross_entropy(x, w, t, bias=b, reduction='none'), loss, bound)
+        n = max(1, int((t >= 0).sum()))
+        mean = vocab.vocab_cross_entropy(x, w, t, bias=b)
+        _within(mean, loss.sum() / n, bound.sum() / n + 2.0 ** -23 * loss.sum() / n)
+        _within(vocab.vocab_cross_entropy(x, w, t, bias=b, reduction='sum'), loss.sum(), bound.sum() + 2.0 ** -23 * loss.sum())
+        no_bias, nb, _, _ = _formula(x, w, None, t, torch.ones(m, device='cuda'))
+        _within(vocab.vocab_cross_entropy(x, w, t, reduction='none'), no_bias, nb)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('reduction', ['mean', 'none', 'sum'])
+@pytest.mark.parametrize('m,v,d', SHAPES)
+def test_gradients(dtype, reduction, m, v, d):
+    x, w, b, t = _case(m, v, d, dtype, 7 * m + v + d, bias=reduction != 'sum', absent=0.25 if m > 4 else 0.0)
+    n = max(1, int((t >= 0).sum()))
+    up = torch.randn(m, device='cuda', generator=_gen(5)) if reduction == 'none' else torch.tensor(0.7, device='cuda')
+    rows = up if reduction == 'none' else (up.double() / (n if reduction == 'mean' else 1)).expand(m)
+    loss, bound, want, bounds = _formula(x, w, b, t, rows)
+    out = vocab.vocab_cross_entropy(x, w, t, bias=b, reduction=reduction)
+    if reduction == 'none':
+        _within(out.detach(), loss, bound)
+    else:
+        k = n if reduction == 'mean' else 1
+        _within(out.detach(), loss.sum() / k, (bound.sum() + 2.0 ** -23 * loss.sum()) / k)
+    leaves = (x, w) if b is None else (x, w, b)
+    got = torch.autograd.grad(out, leaves, up)
+    for a, e, lim in zip(got, want, bounds):
+        assert a.dtype == dtype
+        _within(a, e, lim)
+    assert bool((got[0][t < 0] == 0).all())
+    again = torch.autograd.grad(vocab.vocab_cross_entropy(x, w, t, bias=b, reduction=reduction), leaves, up)
+    assert all(torch.equal(p, q) for p, q in zip(got, again))
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_large_tiles(dtype):
+    x, w, b, t = _case(4000, 8200, 72, dtype, 11, absent=0.2)
+    n = int((t >= 0).sum())
+    loss, bound, want, bounds = _formula(x, w, b, t, torch.full((4000,), 1.0 / n, device='cuda', dtype=torch.float64))
+    out = vocab.vocab_cross_entropy(x, w, t, bias=b)
+    _within(out.detach(), loss.sum() / n, (bound.sum() + 2.0 ** -23 * loss.sum()) / n)
+    for a, e, lim in zip(torch.autograd.grad(out, (x, w, b)), want, bounds):
+        _within(a, e, lim)
+
+
+def test_several_pieces_of_the_vocabulary():
+    """more than 512 MB of G: the hidden states' gradient is summed over pieces"""
+    x, w, b, t = _case(20000, 17000, 40, torch.bfloat16, 12, absent=0.1)
+    out = vocab.vocab_cross_entropy(x, w, t, bias=b, reduction='sum')
+    got = torch.autograd.grad(out, (x, w, b))
+    keep = torch.cat([torch.arange(0, 20000, 997, device='cuda'), torch.tensor([19999], device='cuda')])
+    loss, bound, want, bounds = _formula(x[keep], w, b, t[keep], torch.ones(keep.numel(), device='cuda'))
+    _within(got[0][keep], want[0], bounds[0])
+    # dbias and dweight in pieces of rows, in 64 bits
+    db = torch.zeros(17000, dtype=torch.float64, device='cuda')
+    dw = torch.zeros(17000, 40, dtype=torch.float64, device='cuda')
+    lb, lw = torch.zeros_like(db), torch.zeros_like(dw)
+    for rows in torch.arange(20000, device='cuda').split(2500):
+        _, _, part, lim = _formula(x[rows], w, b, t[rows], torch.ones(rows.numel(), device='cuda'))
+        db += part[2]; dw += part[1]; lb += lim[2]; lw += lim[1]
+    _within(got[2], db, lb * 8)          # the bound's n 2^-23 term grows with the rows: 8 pieces
+    _within(got[1], dw, lw * 8)
+
+
+@pytest.mark.parametrize('m', [5, 200])
+def test_masked_entries_and_rows(m):
+    x, w, b, t = _case(m, 600, 48, torch.float32, 21, masked=0.4, absent=0.2)
+    loss, bound, want, bounds = _formula(x, w, b, t, torch.ones(m, device='cuda'))
+    with torch.no_grad():
+        _within(vocab.vocab_cross_entropy(x, w, t, bias=b, reduction='none'), loss, bound)
+    out = vocab.vocab_cross_entropy(x, w, t, bias=b, reduction='sum')
+    for a, e, lim in zip(torch.autograd.grad(out, (x, w, b)), want, bounds):
+        _within(a, e, lim)
+    # a whole tile and more of masked entries; the lowest finite value masks as well
+    for low in (float('-inf'), torch.finfo(torch.float32).min):
+        b2 = b.detach().clone()
+        b2[100:600] = low
+        t2 = torch.where(t >= 100, 0, t)
+        b2[0] = 0.0
+        loss, bound, want, bounds = _formula(x, w, b2, t2, torch.ones(m, device='cuda'))
+        bound = bound if math.isinf(low) else _formula(x, w, torch.where(b2 == low, float('-inf'), b2), t2, torch.ones(m, device='cuda'))[1]
+        with torch.no_grad():
+            _within(vocab.vocab_cross_entropy(x, w, t2, bias=b2, reduction='none'), loss, bound)
+    # a masked target: infinite loss; every entry masked: NaN; others keep their values
+    with torch.no_grad():
+        b3 = b.detach().clone()
+        hit = int(t[t >= 0][0])
+        b3[hit] = float('-inf')
+        got = vocab.vocab_cross_entropy(x, w, t, bias=b3, reduction='none')
+        assert torch.equal(torch.isinf(got), t == hit)
+        none = vocab.vocab_cross_entropy(x, w, t, bias=torch.full_like(b3, float('-inf')), reduction='none')
+        assert torch.equal(torch.isnan(none), t >= 0) and bool((none[t < 0] == 0).all())
+
+
+@pytest.mark.parametrize('m', [8, 300])
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_no_row_is_there(m, dtype):
+    x, w, b, t = _case(m, 100, 32, dtype, 31)
+    x = torch.full_like(x, float('nan')).requires_grad_()
+    gone = torch.full_like(t, -1)
+    for red in ('mean', 'sum', 'none'):
+        out = vocab.vocab_cross_entropy(x, w, gone, bias=b, reduction=red)
+        assert bool((out == 0).all())
+        for g in torch.autograd.grad(out, (x, w, b), torch.ones_like(out)):
+            assert bool((g == 0).all())
+    out = vocab.vocab_cross_entropy(x[:0], w, gone[:0], bias=b)
+    assert float(out) == 0.0
+    assert all(bool((g == 0).all()) for g in torch.autograd.grad(out, (w, b)))
+    assert vocab.vocab_cross_entropy(x[:0], w, gone[:0], reduction='none').shape == (0,)
+
+
+@pytest.mark.parametrize('m', [9, 150])
+def test_targets_past_the_vocabulary_show(m):
+    x, w, b, t = _case(m, 90, 16, torch.float32, 41)
+    t[3] = 90
+    t[5] = 2 ** 40
+    with torch.no_grad():
+        got = vocab.vocab_cross_entropy(x, w, t, bias=b, reduction='none')
+    bad = torch.zeros_like(t, dtype=torch.bool)
+    bad[3] = bad[5] = True
+    assert torch.equal(torch.isnan(got), bad)
+    out = vocab.vocab_cross_entropy(x, w, t, bias=b, reduction='none')
+    assert torch.equal(torch.isnan(out), bad)
+    dx, dw = torch.autograd.grad(out, (x, w), torch.ones_like(out))
+    assert torch.equal(torch.isnan(dx).all(1), bad) and bool(torch.isnan(dw).all())
+    assert torch.isnan(vocab.vocab_cross_entropy(x, w, t, bias=b))
+
+
+def test_cross_entropy_layouts_and_single_gradients():
+    x, w, b, t = _case(6 * 35, 333, 56, torch.float32, 51, absent=0.1)
+    ones = torch.full((210,), 1.0, device='cuda')
+    loss, bound, want, bounds = _formula(x, w, b, t, ones)
+    xs = torch.zeros(210, 80, device='cuda')
+    xs[:, 9:65] = x.detach()
+    ws = torch.zeros(56, 333, device='cuda')
+    ws.copy_(w.detach().t())
+    views = [(x.detach().reshape(6, 35, 56), w.detach(), t.reshape(6, 35)), (xs[:, 9:65], ws.t(), t.int()),
+             (x.detach().reshape(35, 6, 56).transpose(0, 1), w.detach(), t.reshape(35, 6).t())]
+    for xv, wv, tv in views:
+        with torch.no_grad():
+            got = vocab.vocab_cross_entropy(xv, wv, tv, bias=b, reduction='none')
+        assert got.shape == tv.shape
+        back = got if got.dim() == 1 else got.reshape(-1) if tv.is_contiguous() else got.t().reshape(-1)
+        _within(back, loss, bound)
+    for i in range(3):
+        leaves = [z.detach().requires_grad_(j == i) for j, z in enumerate((x, w, b))]
+        out = vocab.vocab_cross_entropy(leaves[0], leaves[1], t, bias=leaves[2], reduction='sum')
+        _within(torch.autograd.grad(out, leaves[i])[0], want[i], bounds[i])
+
+
+def test_gradient_against_differences():
+    x, w, b, t = _case(70, 40, 12, torch.float32, 61, absent=0.1)
+    t_bad = t < 0
+    out = vocab.vocab_cross_entropy(x, w, t, bias=b)
+    got = torch.autograd.grad(out, (x, w, b))
+
+    def f(xd, wd, bd):
+        l = torch.where(t_bad[:, None], 0.0, xd) @ wd.t() + bd
+        nll = torch.logsumexp(l, 1) - l.gather(1, t.clamp(min=0)[:, None])[:, 0]
+        return torch.where(t_bad, 0.0, nll).sum() / (~t_bad).sum()
+
+    base = [z.detach().double() for z in (x, w, b)]
+    g = _gen(9)
+    for i in range(3):
+        d = torch.randn(base[i].shape, device='cuda', generator=g, dtype=torch.float64)
+        if i == 0:
+            d[t_bad] = 0.0
+        h = 1e-5
+        up, dn = list(base), list(base)
+        up[i], dn[i] = torch.nan_to_num(base[i]) + h * d, torch.nan_to_num(base[i]) - h * d
+        want = float((f(*up) - f(*dn)) / (2 * h))
+        have = float((got[i].double() * d).sum())
+        # the quotient's own error: h^2 times a third derivative of order |d|^3; the gradient's: fp32 bounds of test_gradients
+        assert abs(want - have) < 1e-5 * float(d.abs().sum()) / 10
+
+
+def test_other_stream_and_two_calls_at_once():
+    x, w, b, t = _case(500, 700, 64, torch.bfloat16, 71, absent=0.1)
+    x2, w2, b2, t2 = _case(500, 700, 64, torch.bfloat16, 72, absent=0.1)
+    step = lambda *a: torch.autograd.grad(vocab.vocab_cross_entropy(a[0], a[1], a[3], bias=a[2]), a[:3])
+    want, want2 = step(x, w, b, t), step(x2, w2, b2, t2)
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(3):
+        with torch.cuda.stream(s1):
+            got = step(x, w, b, t)
+        with torch.cuda.stream(s2):
+            got2 = step(x2, w2, b2, t2)
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, want)) and all(torch.equal(p, q) for p, q in zip(got2, want2))
+
+
+@pytest.mark.parametrize('m', [20, 400])
+def test_captured_and_replayed(m):
+    """a step captured once and replayed on new inputs gives the eager step's bits, with eager work in between"""
+    cases = [_case(m, 500, 48, torch.float32, 80 + k, absent=0.2) for k in range(4)]
+    emb = [torch.randint(-1, 500, (m,), device='cuda', generator=_gen(90 + k)) for k in range(4)]
+
+    def step(x, w, b, t, tok):
+        out = vocab.token_embedding(tok, w, 2.0)
+        loss = vocab.vocab_cross_entropy(x, w, t, bias=b)
+        return [out, loss] + list(torch.autograd.grad(loss + out.sum(), (x, w, b)))
+
+    bufs = [z.detach().clone().requires_grad_(i < 3) for i, z in enumerate(cases[0])]
+    tok = emb[0].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*bufs, tok)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(*bufs, tok)
+    for k in (1, 2, 3, 1):
+        with torch.no_grad():
+            for buf, src in zip(bufs, cases[k]):
+                buf.copy_(src)
+            tok.copy_(emb[k])
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [h.detach().clone() for h in held]
+        want = step(*[z.detach().clone().requires_grad_(i < 3) for i, z in enumerate(cases[k])], emb[k])
+        assert all(torch.equal(p, q.detach()) for p, q in zip(got, want))
+
+
+def test_token_model_trains_a_run_of_the_operators():
+    """embedding -> recurrent cell -> vocabulary loss with a tied table, as a token model uses them: gradients against the same run
+    from torch's own operators in 64 bits"""
+    torch.manual_seed(0)
+    emb = TokenEmbedding(290, 64, scale=8.0).cuda()
+    cell = torch.nn.Linear(64, 64).cuda()
+    crit = VocabularyLoss(64, 290).cuda()
+    crit.linear.weight = emb.weight
+    tok = torch.randint(290, (5, 77), device='cuda', generator=_gen(100))
+    tok[torch.rand(5, 77, device='cuda', generator=_gen(101)) < 0.2] = -1
+    hidden = torch.tanh(cell(emb(tok[:-1])))
+    loss = crit(hidden, tok[1:])
+    got = torch.autograd.grad(loss, (emb.weight, cell.weight, crit.linear.bias))
+    w, cw, cb, b = (p.detach().double().requires_grad_() for p in (emb.weight, cell.weight, cell.bias, crit.linear.bias))
+    e = torch.where((tok[:-1] >= 0)[..., None], w[tok[:-1].clamp(min=0)] * 8.0, 0.0)
+    l = torch.tanh(e @ cw.t() + cb) @ w.t() + b
+    nll = torch.logsumexp(l, -1) - l.gather(-1, tok[1:].clamp(min=0)[..., None])[..., 0]
+    there = tok[1:] >= 0
+    ref = torch.where(there, nll, 0.0).sum() / there.sum()
+    want = torch.autograd.grad(ref, (w, cw, b))
+    # sums of a few hundred fp32 terms through three layers: (77 * 4 + 3 * 290) 2^-23 of the magnitudes, which stay below 0.1
+    lim = (77 * 4 + 3 * 290) * 2.0 ** -23
+    assert abs(float(loss) - float(ref)) < lim * float(ref)
+    for a, c in zip(got, want):
+        assert float((a.double() - c).abs().max()) < lim * max(0.1, float(c.abs().max()))

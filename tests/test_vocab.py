@@ -1,0 +1,81 @@
+"""Refusals and host-side checks of the vocabulary operators (no GPU): every call that the documentation does not allow raises before
+anything is launched."""
+import ctypes
+
+import pytest
+import torch
+
+from trajnetplusplusbaselines_amd import _lib, vocab
+from trajnetplusplusbaselines_amd.lstm import TokenEmbedding, VocabularyLoss
+
+
+def test_host_tensors_are_refused():
+    with pytest.raises(RuntimeError, match='no CPU fallback'):
+        vocab.token_embedding(torch.zeros(3, dtype=torch.int64), torch.zeros(4, 8))
+    with pytest.raises(RuntimeError, match='no CPU fallback'):
+        vocab.vocab_cross_entropy(torch.zeros(3, 8), torch.zeros(4, 8), torch.zeros(3, dtype=torch.int64))
+    with pytest.raises(RuntimeError, match='no CPU fallback'):
+        TokenEmbedding(4, 8)(torch.zeros(3, dtype=torch.int64))
+    with pytest.raises(RuntimeError, match='no CPU fallback'):
+        VocabularyLoss(8, 4)(torch.zeros(3, 8), torch.zeros(3, dtype=torch.int64))
+
+
+@pytest.mark.parametrize('tokens,weight,error', [
+    (torch.zeros(3), torch.zeros(4, 8), TypeError), (torch.zeros(3, dtype=torch.int16), torch.zeros(4, 8), TypeError),
+    ([0, 1], torch.zeros(4, 8), TypeError), (torch.zeros(3, dtype=torch.int64), torch.zeros(4, 8, dtype=torch.float64), TypeError),
+    (torch.zeros(3, dtype=torch.int64), torch.zeros(4), ValueError), (torch.zeros(3, dtype=torch.int64), torch.zeros(0, 8), ValueError)])
+def test_embedding_arguments(tokens, weight, error):
+    with pytest.raises(error):
+        vocab.token_embedding(tokens, weight)
+
+
+def _ce(**kw):
+    a = dict(hidden=torch.zeros(3, 8), weight=torch.zeros(4, 8), target=torch.zeros(3, dtype=torch.int64), bias=torch.zeros(4))
+    a.update(kw)
+    return vocab.vocab_cross_entropy(**a)
+
+
+@pytest.mark.parametrize('kw,error', [
+    (dict(reduction='max'), ValueError), (dict(hidden=torch.zeros(3, 7)), ValueError), (dict(hidden=torch.zeros(2, 8)), ValueError),
+    (dict(target=torch.zeros(3)), TypeError), (dict(bias=torch.zeros(5)), ValueError), (dict(bias=torch.zeros(4).half()), TypeError),
+    (dict(hidden=torch.zeros(3, 8).half()), TypeError), (dict(weight=torch.zeros(4, 8).double()), TypeError),
+    (dict(weight=torch.zeros(0, 8)), ValueError), (dict(target=[0, 1, 2]), TypeError), (dict(target=torch.zeros(3, 1, dtype=torch.int64)), ValueError)])
+def test_cross_entropy_arguments(kw, error):
+    with pytest.raises(error):
+        _ce(**kw)
+
+
+def test_c_entries_refuse_on_the_host():
+    L = _lib.lib()
+    p = ctypes.c_void_p(1 << 20)        # never followed: every call below is refused first
+    fwd = lambda **k: L.tnp_token_embedding_forward(*[k.get(n, d) for n, d in (
+        ('tokens', p), ('token_bytes', 8), ('N', 4), ('weight', p), ('ldw', 8), ('V', 4), ('D', 8), ('dtype', 0), ('scale', 1.0), ('out', p),
+        ('ldo', 8), ('stream', None))])
+    for bad in (dict(token_bytes=2), dict(N=-1), dict(N=1 << 40), dict(V=0), dict(D=0), dict(dtype=7), dict(ldw=7), dict(ldo=1), dict(tokens=None)):
+        assert fwd(**bad) == -1
+        assert b'tnp_token_embedding_forward' in L.tnp_last_error()
+    assert fwd(N=0, tokens=None) == 0
+    need = L.tnp_token_embedding_backward_workspace_bytes(100, 50, 8)
+    assert need > 0
+    args = [p, 8, 100, p, 8, 50, 8, 0, 1.0, p, 8, p, need - 1, None]
+    assert L.tnp_token_embedding_backward(*args) == -1 and b'workspace' in L.tnp_last_error()
+    a = vocab.VocabCe(dtype=0, reduction=1, M=10, V=20, D=8, hidden=1 << 20, ld_hidden=8, weight=1 << 20, ld_weight=8, target=1 << 20)
+    ref = ctypes.byref(a)
+    assert L.tnp_vocab_ce_saved_bytes(ref) > 0
+    need = L.tnp_vocab_ce_workspace_bytes(ref, 0)
+    assert L.tnp_vocab_ce_forward(ref, p, p, need - 1, None) == -1 and b'workspace' in L.tnp_last_error()
+    assert L.tnp_vocab_ce_backward(ref, p, p, p, None, p, 1 << 40, None) == -1          # nothing saved
+    a.saved = 1 << 20
+    assert L.tnp_vocab_ce_backward(ref, p, p, p, p, p, 1 << 40, None) == -1 and b'bias' in L.tnp_last_error()
+    for field, value in (('dtype', 3), ('reduction', 3), ('V', 0), ('D', 0), ('D', 20000), ('M', -1), ('ld_hidden', 7), ('ld_weight', 7)):
+        b = vocab.VocabCe.from_buffer_copy(a)
+        setattr(b, field, value)
+        assert L.tnp_vocab_ce_saved_bytes(ctypes.byref(b)) == 0
+        assert L.tnp_vocab_ce_workspace_bytes(ctypes.byref(b), 1) == 0
+        assert L.tnp_vocab_ce_forward(ctypes.byref(b), p, p, 1 << 40, None) == -1
+    a.M = 0
+    assert L.tnp_vocab_ce_forward(ref, p, p, 1 << 40, None) == -1
+
+
+def test_struct_mirror():
+    assert _lib.lib().tnp_abi_sizeof(8) == ctypes.sizeof(vocab.VocabCe)

@@ -19,6 +19,7 @@ HEADER_PATH = os.path.join(os.path.dirname(_HERE), 'include', 'trajnet_hip.h')
 POOL_NONE, POOL_OCCUPANCY, POOL_DIRECTIONAL, POOL_SOCIAL = -1, 0, 1, 2
 POOL_NN, POOL_HIDDENMLP, POOL_ATTNMLP, POOL_NNLSTM, POOL_TRAJ = 4, 5, 6, 7, 8
 ABI_VERSION = 7   # TNP_ABI_VERSION of include/trajnet_hip.h this binding was written against
+F32, BF16, F16 = 0, 1, 2   # TNP_F32 / TNP_BF16 / TNP_F16
 POOL_TYPES = {None: POOL_NONE, 'occupancy': POOL_OCCUPANCY, 'directional': POOL_DIRECTIONAL, 'social': POOL_SOCIAL}
 
 _fp = ctypes.c_void_p
@@ -196,6 +197,18 @@ def lib():
                                       ctypes.c_float, ctypes.c_float, _fp, _fp]
     L.tnp_pool_pair_cells_autograd.argtypes = [_fp, _fp, _fp, _fp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                                ctypes.c_float, ctypes.c_float, ctypes.c_float, ctypes.c_float, _fp, _fp, _fp, _fp]
+    L.tnp_token_embedding_forward.argtypes = [_fp, ctypes.c_int, ctypes.c_int64, _fp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int,
+                                              ctypes.c_int, ctypes.c_float, _fp, ctypes.c_int64, _fp]
+    L.tnp_token_embedding_backward_workspace_bytes.restype = ctypes.c_size_t
+    L.tnp_token_embedding_backward_workspace_bytes.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.c_int]
+    L.tnp_token_embedding_backward.argtypes = [_fp, ctypes.c_int, ctypes.c_int64, _fp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int,
+                                               ctypes.c_int, ctypes.c_float, _fp, ctypes.c_int64, _fp, ctypes.c_size_t, _fp]
+    L.tnp_vocab_ce_saved_bytes.restype = ctypes.c_size_t
+    L.tnp_vocab_ce_saved_bytes.argtypes = [_fp]
+    L.tnp_vocab_ce_workspace_bytes.restype = ctypes.c_size_t
+    L.tnp_vocab_ce_workspace_bytes.argtypes = [_fp, ctypes.c_int]
+    L.tnp_vocab_ce_forward.argtypes = [_fp, _fp, _fp, ctypes.c_size_t, _fp]
+    L.tnp_vocab_ce_backward.argtypes = [_fp, _fp, _fp, _fp, _fp, _fp, ctypes.c_size_t, _fp]
     if L.tnp_abi_version() != ABI_VERSION:
         raise RuntimeError('libtrajnet_hip.so ABI version mismatch')
     _LIB = L

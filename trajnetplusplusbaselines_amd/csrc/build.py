@@ -9,9 +9,11 @@ PKG = os.path.dirname(HERE)
 OUT_DIR = os.path.join(PKG, 'lib')
 OUT = os.path.join(OUT_DIR, 'libtrajnet_hip.so')
 SOURCES = ['gemm_f32_mfma.hip', 'gemm_skinny.hip', 'gemm_wgrad.hip', 'pool_grid.hip', 'pool_embed_sparse.hip', 'pool_nongrid.hip', 'lstm_seq.hip', 'lstm_bwd.hip', 'loss.hip',
-           'optim.hip', 'classical.hip', 'ndjson_io.cpp']
+           'optim.hip', 'classical.hip', 'token_embed.hip', 'vocab_ce.hip', 'ndjson_io.cpp']
 EXACT = ('classical.hip', 'pool_grid.hip', 'optim.hip')
-HEADERS = ['tnp_internal.h', 'lstm_cell.h', 'classical_core.h', 'grid_build_body.h', os.path.join('..', '..', 'include', 'trajnet_hip.h'),
+# units compiled without v_pk_{add,mul,fma}_f32
+NO_PACKED_FP32 = ('token_embed.hip', 'vocab_ce.hip')
+HEADERS = ['tnp_internal.h', 'vocab_types.h', 'vocab_gemm.h', 'lstm_cell.h', 'classical_core.h', 'grid_build_body.h', os.path.join('..', '..', 'include', 'trajnet_hip.h'),
            os.path.join('..', '..', 'include', 'trajnet_hip_profile.h')]
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-fno-fast-math', '-fvisibility=hidden',
          '-Wall', '-Wno-unused-function']
@@ -44,6 +46,8 @@ def build(force=False, verbose=False):
         obj = os.path.join(OUT_DIR, os.path.splitext(src)[0] + '.o')
         # exact-arithmetic units (cell indexing, float64 / float32 simulators): no fma contraction
         extra = ['-ffp-contract=off'] if src in EXACT else []
+        if src in NO_PACKED_FP32:
+            extra = extra + ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
         cmd = [hipcc()] + FLAGS + extra + os.environ.get('TNP_HIPCC_EXTRA', '').split() + ['-c', path, '-o', obj]
         if verbose:
             print(' '.join(cmd))

@@ -1605,6 +1605,7 @@ extern "C" TNP_API size_t tnp_abi_sizeof(int which) {
         case 5: return sizeof(tnp_wgrad_problem);
         case 6: return sizeof(tnp_adam_tensor);
         case 7: return sizeof(tnp_transpose_problem);
+        case 8: return sizeof(tnp_vocab_ce);
         default: return 0;
     }
 }

@@ -1,0 +1,489 @@
+// Token embedding (gfx950): out[i] = scale * weight[token[i]], and the gradient of the table,
+//     dweight[v] = scale * sum over { i : token[i] == v } of grad[i]
+// summed in ascending i within fixed chunks, so that two calls on the same inputs give the same bits.  A negative token is an
+// absent track: a zero row forward, nothing backward.  A token >= V has no row: NaN forward (an error that shows and cannot
+// fault), nothing backward.
+//
+// Forward: one pass, bound by memory.  Backward: the tokens are sorted (a stable radix sort of (token, i) pairs, digits of up to
+// 10 bits), so that all rows of one token are neighbours; chunks of 32 sorted positions are summed by one group of lanes each,
+// whatever the distribution of the tokens -- a table row that owns half of the batch is split over thousands of chunks and joined.
+// Every gradient row is read once and every table row written once; table rows without a token are zeroed by their own workgroups,
+// which find them by binary search in the sorted tokens.
+#include "vocab_types.h"
+
+namespace tnp {
+
+static constexpr int EMB_CHUNK = 32;          // sorted positions per group of lanes
+static constexpr int EMB_ROWS = 16;           // rows of 64 pairs per wave of the sort
+static constexpr int EMB_SORT_THREADS = 512;  // eight waves: 8192 pairs per workgroup
+static constexpr int EMB_SORT_ITEMS = EMB_SORT_THREADS / 64 * EMB_ROWS * 64;
+static constexpr int EMB_MAX_BITS = 10;      // eight waves' counters of 2^10 digits: 32 KB of LDS
+static constexpr int64_t EMB_MAX_TOKENS = 1 << 28;
+
+// ---- forward ----------------------------------------------------------------------------------------------------------------
+// 2^lsh lanes per row; U rows per lane whose loads are in flight together.
+template <typename T, int VE, typename I, int U>
+__global__ void __launch_bounds__(256) embed_forward_kernel(const I *tokens, int64_t N, const T *weight, int64_t ldw, int64_t V,
+                                                            int D, int lsh, float scale, T *out, int64_t ldo) {
+    const int lanes = 1 << lsh, rows = 256 >> lsh;
+    const int64_t i0 = (int64_t)blockIdx.x * rows * U + (threadIdx.x >> lsh);
+    int64_t tok[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) tok[u] = i0 + u * rows < N ? (int64_t)tokens[i0 + u * rows] : -1;
+    for (int c = (threadIdx.x & (lanes - 1)) * VE; c < D; c += lanes * VE) {
+        Pack<T, VE> w[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (tok[u] >= 0 && tok[u] < V) {
+                w[u] = *(const Pack<T, VE> *)(weight + tok[u] * ldw + c);
+            } else {
+                const T fill = from_f32<T>(tok[u] < 0 ? 0.0f : __builtin_nanf(""));
+#pragma unroll
+                for (int e = 0; e < VE; ++e) w[u].v[e] = fill;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (i0 + u * rows >= N) continue;
+#pragma unroll
+            for (int e = 0; e < VE; ++e) w[u].v[e] = tok[u] < 0 ? from_f32<T>(0.0f) : from_f32<T>(to_f32(w[u].v[e]) * scale);
+            *(Pack<T, VE> *)(out + (i0 + u * rows) * ldo + c) = w[u];
+        }
+    }
+}
+
+// ---- stable radix sort of (token, i) ----------------------------------------------------------------------------------------
+// Keys: the token, or V for a token outside the table (sorted behind everything, skipped by the sums).
+template <typename I>
+__device__ __forceinline__ uint32_t embed_key(const I *tokens, const uint32_t *keys, int64_t i, uint32_t V) {
+    if (keys) return keys[i];
+    const int64_t t = (int64_t)tokens[i];
+    return t < 0 || t >= (int64_t)V ? V : (uint32_t)t;
+}
+
+// lanes of the wave that hold the same digit, among the lanes with `live`
+__device__ __forceinline__ uint64_t same_digit(uint32_t d, int bits, bool live) {
+    uint64_t m = __ballot(live);
+    for (int b = 0; b < bits; ++b) {
+        const bool one = (d >> b) & 1;
+        const uint64_t v = __ballot(one);
+        m &= one ? v : ~v;
+    }
+    return m;
+}
+
+// Ranks of a wave's pairs within (wave, digit), in ascending position, counts left in cnt[] (this wave's counters, zeroed by the
+// caller).  Only the first lane of a digit's group touches the counter, and LDS operations of a wave execute in order.
+template <typename I, bool RANK>
+__device__ __forceinline__ void embed_count(const I *tokens, const uint32_t *keys, int64_t base, int64_t N, uint32_t V, int shift,
+                                            int bits, uint32_t *cnt, uint32_t *key, uint32_t *rank) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int r = 0; r < EMB_ROWS; ++r) {
+        const int64_t i = base + r * 64 + lane;
+        key[r] = i < N ? embed_key(tokens, keys, i, V) : 0;
+    }
+#pragma unroll
+    for (int r = 0; r < EMB_ROWS; ++r) {
+        const bool live = base + r * 64 + lane < N;
+        const uint32_t d = (key[r] >> shift) & ((1u << bits) - 1);
+        const uint64_t m = same_digit(d, bits, live);
+        const int first = __ffsll((unsigned long long)m) - 1;
+        uint32_t before = 0;
+        if (live && lane == first) before = atomicAdd(&cnt[d], (uint32_t)__popcll(m));
+        if (RANK) rank[r] = __shfl(before, first & 63) + (uint32_t)__popcll(m & ((1ull << lane) - 1));
+    }
+}
+
+template <typename I>
+__global__ void __launch_bounds__(EMB_SORT_THREADS) embed_hist_kernel(const I *tokens, const uint32_t *keys, int64_t N, uint32_t V,
+                                                                      int shift, int bits, uint32_t *hist) {
+    extern __shared__ uint32_t cnt[];
+    const int nb = 1 << bits;
+    for (int b = threadIdx.x; b < nb; b += EMB_SORT_THREADS) cnt[b] = 0;
+    __syncthreads();
+    uint32_t key[EMB_ROWS];
+    const int64_t base = (int64_t)blockIdx.x * EMB_SORT_ITEMS + (threadIdx.x >> 6) * (EMB_ROWS * 64);
+    embed_count<I, false>(tokens, keys, base, N, V, shift, bits, cnt, key, nullptr);
+    __syncthreads();
+    for (int b = threadIdx.x; b < nb; b += EMB_SORT_THREADS) hist[(size_t)blockIdx.x * nb + b] = cnt[b];
+}
+
+// Every workgroup forms its own offsets from the histograms of all of them (nblk * 2^bits counters, L2-resident): one launch less
+// per pass than a scan kernel in between.  nblk == 1 needs no histogram at all.
+template <typename I>
+__global__ void __launch_bounds__(EMB_SORT_THREADS) embed_scatter_kernel(const I *tokens, const uint32_t *keys, const uint32_t *idx,
+                                                                         int64_t N, uint32_t V, int shift, int bits,
+                                                                         const uint32_t *hist, int nblk, uint32_t *keys_out,
+                                                                         uint32_t *idx_out) {
+    extern __shared__ uint32_t lds[];
+    const int nb = 1 << bits, nw = EMB_SORT_THREADS / 64;
+    uint32_t *cnt = lds;                // [waves][nb]: counts, then the first position of (wave, digit)
+    uint32_t *part = lds + nw * nb;     // [EMB_SORT_THREADS] partial sums of the scan over digits
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    for (int b = tid; b < nw * nb; b += EMB_SORT_THREADS) cnt[b] = 0;
+    __syncthreads();
+    uint32_t key[EMB_ROWS], rank[EMB_ROWS];
+    const int64_t base = (int64_t)blockIdx.x * EMB_SORT_ITEMS + wave * (EMB_ROWS * 64);
+    embed_count<I, true>(tokens, keys, base, N, V, shift, bits, cnt + wave * nb, key, rank);
+    __syncthreads();
+    const int per = (nb + EMB_SORT_THREADS - 1) / EMB_SORT_THREADS;       // digits per thread: 1 or 2
+    uint32_t total[2] = {0, 0}, before[2] = {0, 0}, sum = 0;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int b = tid * per + j;
+        if (j >= per || b >= nb) continue;
+        if (nblk == 1) {
+            for (int w = 0; w < nw; ++w) total[j] += cnt[w * nb + b];
+        } else {
+            for (int k = 0; k < nblk; ++k) {
+                const uint32_t h = hist[(size_t)k * nb + b];
+                if (k < (int)blockIdx.x) before[j] += h;
+                total[j] += h;
+            }
+        }
+        sum += total[j];
+    }
+    part[tid] = sum;
+    __syncthreads();
+    for (int off = 1; off < EMB_SORT_THREADS; off <<= 1) {
+        const uint32_t v = tid >= off ? part[tid - off] : 0;
+        __syncthreads();
+        part[tid] += v;
+        __syncthreads();
+    }
+    uint32_t start = part[tid] - sum;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int b = tid * per + j;
+        if (j >= per || b >= nb) continue;
+        uint32_t at = start + before[j];
+        for (int w = 0; w < nw; ++w) {
+            const uint32_t c = cnt[w * nb + b];
+            cnt[w * nb + b] = at;
+            at += c;
+        }
+        start += total[j];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < EMB_ROWS; ++r) {
+        const int64_t i = base + r * 64 + lane;
+        if (i >= N) continue;
+        const uint32_t d = (key[r] >> shift) & (nb - 1);
+        const uint32_t at = cnt[wave * nb + d] + rank[r];
+        keys_out[at] = key[r];
+        idx_out[at] = idx ? idx[i] : (uint32_t)i;
+    }
+}
+
+// ---- sums over the sorted pairs ---------------------------------------------------------------------------------------------
+// first position whose key is > k
+__device__ __forceinline__ uint32_t embed_upper(const uint32_t *keys, uint32_t lo, uint32_t hi, uint32_t k) {
+    while (lo < hi) {
+        const uint32_t mid = lo + ((hi - lo) >> 1);
+        if (keys[mid] > k) hi = mid; else lo = mid + 1;
+    }
+    return lo;
+}
+
+// Chunk c = sorted positions [32 c, 32 c + 32), 2^lsh lanes, fp32 sums.  A run (one token) inside the chunk is finished here; the
+// part of a run that came in from the chunk before goes to head[c], the first part of a run that goes on into the next to tail[c]
+// (embed_join_kernel adds those).  Workgroups from `sum_blocks` on zero the table rows that no token names.
+template <typename T, int VE>
+__global__ void __launch_bounds__(256) embed_reduce_kernel(const uint32_t *keys, const uint32_t *idx, uint32_t N, uint32_t V,
+                                                           const T *grad, int64_t ldg, int D, int lsh, float scale, T *dw,
+                                                           int64_t ldd, float *head, float *tail, uint32_t sum_blocks) {
+    const int lanes = 1 << lsh;
+    if (blockIdx.x >= sum_blocks) {                    // 64 table rows per wave
+        const uint32_t v0 = ((blockIdx.x - sum_blocks) * 4 + (threadIdx.x >> 6)) * 64, v = v0 + (threadIdx.x & 63);
+        bool none = v < V;
+        if (none && N > 0) {
+            const uint32_t at = v == 0 ? 0 : embed_upper(keys, 0, N, v - 1);
+            none = at >= N || keys[at] != v;
+        }
+        uint64_t m = __ballot(none);
+        const int c0 = blockIdx.y * lanes * VE;
+        const int rows = 64 >> lsh;                    // rows per trip (lsh <= 6)
+        const int sub = (threadIdx.x & 63) >> lsh;
+        const int c = c0 + (threadIdx.x & (lanes - 1)) * VE;
+        while (m) {
+            int mine = -1;
+            for (int r = 0; r < rows; ++r) {
+                const int b = m ? __ffsll((unsigned long long)m) - 1 : -1;
+                if (r == sub) mine = b;
+                if (m) m &= m - 1;
+            }
+            if (mine >= 0 && c < D) {
+                Pack<T, VE> z;
+#pragma unroll
+                for (int e = 0; e < VE; ++e) z.v[e] = from_f32<T>(0.0f);
+                *(Pack<T, VE> *)(dw + (int64_t)(v0 + mine) * ldd + c) = z;
+            }
+        }
+        return;
+    }
+    const uint32_t chunk = blockIdx.x * (256u >> lsh) + (threadIdx.x >> lsh);
+    const uint64_t a64 = (uint64_t)chunk * EMB_CHUNK;
+    if (a64 >= N) return;
+    const uint32_t a = (uint32_t)a64, b = min(a + EMB_CHUNK, N);
+    const int c = (blockIdx.y * lanes + (threadIdx.x & (lanes - 1))) * VE;
+    if (c >= D) return;
+    uint32_t cur = keys[a];
+    bool incoming = a > 0 && keys[a - 1] == cur;
+    float acc[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) acc[e] = 0.0f;
+    auto part = [&](float *where) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) where[(size_t)chunk * D + c + e] = acc[e];
+    };
+    auto finish = [&]() {
+        Pack<T, VE> o;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) o.v[e] = from_f32<T>(acc[e] * scale);
+        *(Pack<T, VE> *)(dw + (int64_t)cur * ldd + c) = o;
+    };
+    constexpr int U = 8;                               // rows in flight
+    for (uint32_t p = a; p < b; p += U) {
+        uint32_t k[U];
+        Pack<T, VE> g[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) k[u] = p + u < b ? keys[p + u] : V;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (k[u] < V) g[u] = *(const Pack<T, VE> *)(grad + (int64_t)idx[p + u] * ldg + c);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (p + u >= b) break;
+            if (k[u] != cur) {
+                if (incoming) part(head); else finish();
+                incoming = false;
+                cur = k[u];
+#pragma unroll
+                for (int e = 0; e < VE; ++e) acc[e] = 0.0f;
+            }
+            if (cur >= V) return;                      // only tokens outside the table are left
+#pragma unroll
+            for (int e = 0; e < VE; ++e) acc[e] += to_f32(g[u].v[e]);
+        }
+    }
+    if (cur >= V) return;
+    const bool goes_on = b < N && keys[b] == cur;
+    if (incoming) part(head);
+    else if (goes_on) part(tail);
+    else finish();
+}
+
+// One workgroup per chunk in which a run starts that goes on: tail[c] + head[c + 1] + ... of that run.  Groups of lanes stride over
+// the parts and meet in LDS in a fixed order.
+template <typename T, int VE>
+__global__ void __launch_bounds__(256) embed_join_kernel(const uint32_t *keys, uint32_t N, uint32_t V, int D, int lsh, float scale,
+                                                         T *dw, int64_t ldd, const float *head, const float *tail) {
+    extern __shared__ float sums[];                    // [256][VE]
+    const uint32_t chunk = blockIdx.x, a = chunk * EMB_CHUNK, b = a + EMB_CHUNK;
+    if (b >= N) return;
+    const uint32_t k = keys[b - 1];
+    if (k >= V || keys[b] != k || (a > 0 && keys[a - 1] == k)) return;      // uniform: no run starts here and goes on
+    const uint32_t last = (embed_upper(keys, b, N, k) - 1) / EMB_CHUNK;
+    const int lanes = 1 << lsh, groups = 256 >> lsh, grp = threadIdx.x >> lsh;
+    const int c = (blockIdx.y * lanes + (threadIdx.x & (lanes - 1))) * VE;
+    float acc[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) acc[e] = grp == 0 && c < D ? tail[(size_t)chunk * D + c + e] : 0.0f;
+    if (c < D) {
+        constexpr int U = 4;
+        for (uint32_t j = chunk + 1 + grp; j <= last; j += groups * U) {
+            float h[U][VE];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < VE; ++e) h[u][e] = j + u * groups <= last ? head[(size_t)(j + u * groups) * D + c + e] : 0.0f;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < VE; ++e) acc[e] += h[u][e];
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < VE; ++e) sums[threadIdx.x * VE + e] = acc[e];
+    __syncthreads();
+    if (grp != 0 || c >= D) return;
+    for (int g = 1; g < groups; ++g)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) acc[e] += sums[(g * lanes + threadIdx.x) * VE + e];
+    Pack<T, VE> o;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) o.v[e] = from_f32<T>(acc[e] * scale);
+    *(Pack<T, VE> *)(dw + (int64_t)k * ldd + c) = o;
+}
+
+// ---- host -------------------------------------------------------------------------------------------------------------------
+// elements per lane: 16 bytes where rows and pointers allow it, else 4, else one element
+static int embed_width(int dtype, int D, std::initializer_list<int64_t> lds, std::initializer_list<const void *> ptrs) {
+    const int sz = (int)dtype_bytes(dtype);
+    for (int bytes : {16, 4}) {
+        const int ve = bytes / sz;
+        bool ok = D % ve == 0;
+        for (int64_t ld : lds) ok = ok && ld % ve == 0;
+        for (const void *p : ptrs) ok = ok && (uintptr_t)p % bytes == 0;
+        if (ok) return ve;
+    }
+    return 1;
+}
+
+static int lane_shift(int D, int ve, int most) {
+    int s = 0;
+    while (s < most && ((int64_t)ve << s) < D) ++s;
+    return s;
+}
+
+struct EmbedSort { int bits, passes, nblk; };
+static EmbedSort embed_sort_plan(int64_t N, int64_t V) {
+    EmbedSort p;
+    int need = 1;
+    while (((int64_t)1 << need) <= V) ++need;          // keys 0 .. V
+    p.passes = (need + EMB_MAX_BITS - 1) / EMB_MAX_BITS;
+    p.bits = (need + p.passes - 1) / p.passes;
+    p.nblk = (int)((N + EMB_SORT_ITEMS - 1) / EMB_SORT_ITEMS);
+    return p;
+}
+
+static inline size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+template <typename T, int VE, typename I>
+static int embed_forward_run(const I *tokens, int64_t N, const T *w, int64_t ldw, int64_t V, int D, float scale, T *out, int64_t ldo,
+                             hipStream_t s) {
+    const int lsh = lane_shift(D, VE, 8);
+    const int64_t rows = 256 >> lsh;
+    // four rows per lane once one row per lane would be several rounds of workgroups
+    const bool four = N / rows >= 4096;
+    const int64_t most = rows << 22;                   // rows per launch: a grid holds fewer than 2^32 threads
+    for (int64_t i = 0; i < N; i += most) {
+        const int64_t n = N - i < most ? N - i : most, per = four ? rows * 4 : rows;
+        const dim3 grid((unsigned)((n + per - 1) / per));
+        if (four)
+            hipLaunchKernelGGL((embed_forward_kernel<T, VE, I, 4>), grid, dim3(256), 0, s, tokens + i, n, w, ldw, V, D, lsh, scale,
+                               out + i * ldo, ldo);
+        else
+            hipLaunchKernelGGL((embed_forward_kernel<T, VE, I, 1>), grid, dim3(256), 0, s, tokens + i, n, w, ldw, V, D, lsh, scale,
+                               out + i * ldo, ldo);
+        TNP_HIP(hipGetLastError());
+    }
+    return 0;
+}
+
+template <typename T, int VE>
+static int embed_forward_typed(const void *tokens, int tb, int64_t N, const void *w, int64_t ldw, int64_t V, int D, float scale, void *out,
+                               int64_t ldo, hipStream_t s) {
+    if (tb == 8) return embed_forward_run<T, VE, int64_t>((const int64_t *)tokens, N, (const T *)w, ldw, V, D, scale, (T *)out, ldo, s);
+    return embed_forward_run<T, VE, int32_t>((const int32_t *)tokens, N, (const T *)w, ldw, V, D, scale, (T *)out, ldo, s);
+}
+
+template <typename I>
+static int embed_sort(const I *tokens, int64_t N, uint32_t V, const EmbedSort &p, uint32_t *keys[2], uint32_t *idx[2], uint32_t *hist,
+                      hipStream_t s) {
+    for (int pass = 0; pass < p.passes; ++pass) {
+        const uint32_t *kin = pass ? keys[(pass + 1) & 1] : nullptr, *iin = pass ? idx[(pass + 1) & 1] : nullptr;
+        const size_t nb = (size_t)1 << p.bits;
+        if (p.nblk > 1) {
+            hipLaunchKernelGGL((embed_hist_kernel<I>), dim3(p.nblk), dim3(EMB_SORT_THREADS), nb * 4, s, tokens, kin, N, V, pass * p.bits, p.bits,
+                               hist);
+            TNP_HIP(hipGetLastError());
+        }
+        const size_t smem = (EMB_SORT_THREADS / 64 * nb + EMB_SORT_THREADS) * 4;
+        hipLaunchKernelGGL((embed_scatter_kernel<I>), dim3(p.nblk), dim3(EMB_SORT_THREADS), smem, s, tokens, kin, iin, N, V, pass * p.bits,
+                           p.bits, hist, p.nblk, keys[pass & 1], idx[pass & 1]);
+        TNP_HIP(hipGetLastError());
+    }
+    return 0;
+}
+
+template <typename T, int VE>
+static int embed_sums(const uint32_t *keys, const uint32_t *idx, uint32_t N, uint32_t V, const T *grad, int64_t ldg, int D, float scale, T *dw,
+                      int64_t ldd, float *head, float *tail, hipStream_t s) {
+    const int lsh = lane_shift(D, VE, 6);
+    const unsigned cols = (unsigned)((D + (VE << lsh) - 1) / (VE << lsh));
+    const unsigned chunks = (unsigned)(((uint64_t)N + EMB_CHUNK - 1) / EMB_CHUNK);
+    const unsigned sum_blocks = (unsigned)(((uint64_t)chunks + (256u >> lsh) - 1) / (256u >> lsh));
+    const unsigned zero_blocks = (unsigned)(((uint64_t)V + 255) / 256);
+    hipLaunchKernelGGL((embed_reduce_kernel<T, VE>), dim3(sum_blocks + zero_blocks, cols), dim3(256), 0, s, keys, idx, N, V, grad, ldg, D, lsh,
+                       scale, dw, ldd, head, tail, sum_blocks);
+    TNP_HIP(hipGetLastError());
+    if (chunks > 1) {
+        hipLaunchKernelGGL((embed_join_kernel<T, VE>), dim3(chunks - 1, cols), dim3(256), 256 * VE * 4, s, keys, N, V, D, lsh, scale, dw, ldd,
+                           head, tail);
+        TNP_HIP(hipGetLastError());
+    }
+    return 0;
+}
+
+}  // namespace tnp
+
+using namespace tnp;
+
+static int embed_check(const char *who, int token_bytes, int64_t N, int64_t V, int D, int dtype, int64_t ld1, int64_t ld2) {
+    if (token_bytes != 4 && token_bytes != 8) TNP_FAIL(-1, "%s: tokens are int32 or int64 (got %d bytes)", who, token_bytes);
+    if (!dtype_known(dtype)) TNP_FAIL(-1, "%s: unknown dtype %d", who, dtype);
+    if (N < 0 || N > EMB_MAX_TOKENS) TNP_FAIL(-1, "%s: %lld tokens (0 .. 2^28)", who, (long long)N);
+    if (V < 1 || V > (1 << 30) || D < 1 || D > (1 << 20)) TNP_FAIL(-1, "%s: table of %lld x %d", who, (long long)V, D);
+    if (ld1 < D || ld2 < D) TNP_FAIL(-1, "%s: a row stride is smaller than the %d columns", who, D);
+    return 0;
+}
+
+#define TNP_BY_WIDTH(FN, ve, dtype, ...)                                                                                   \
+    ((dtype) == TNP_F32 ? ((ve) == 4 ? FN<float, 4>(__VA_ARGS__) : FN<float, 1>(__VA_ARGS__))                               \
+     : (dtype) == TNP_BF16 ? ((ve) == 8 ? FN<bf16_t, 8>(__VA_ARGS__) : (ve) == 2 ? FN<bf16_t, 2>(__VA_ARGS__) : FN<bf16_t, 1>(__VA_ARGS__)) \
+                           : ((ve) == 8 ? FN<half_t, 8>(__VA_ARGS__) : (ve) == 2 ? FN<half_t, 2>(__VA_ARGS__) : FN<half_t, 1>(__VA_ARGS__)))
+
+extern "C" TNP_API int tnp_token_embedding_forward(const void *tokens, int token_bytes, int64_t N, const void *weight, int64_t ldw, int64_t V,
+                                                   int D, int dtype, float scale, void *out, int64_t ldo, void *stream) {
+    if (int rc = embed_check("tnp_token_embedding_forward", token_bytes, N, V, D, dtype, ldw, ldo)) return rc;
+    if (N == 0) return 0;
+    if (!tokens || !weight || !out) TNP_FAIL(-1, "tnp_token_embedding_forward: NULL pointer");
+    const int ve = embed_width(dtype, D, {ldw, ldo}, {weight, out});
+    return TNP_BY_WIDTH(embed_forward_typed, ve, dtype, tokens, token_bytes, N, weight, ldw, V, D, scale, out, ldo, (hipStream_t)stream);
+}
+
+extern "C" TNP_API size_t tnp_token_embedding_backward_workspace_bytes(int64_t N, int64_t V, int D) {
+    if (N <= 0 || V < 1 || D < 1) return 0;
+    const EmbedSort p = embed_sort_plan(N, V);
+    const size_t chunks = (size_t)((N + EMB_CHUNK - 1) / EMB_CHUNK);
+    return 4 * up256((size_t)N * 4) + up256((size_t)p.nblk * 4 << p.bits) + 2 * up256(chunks * (size_t)D * 4);
+}
+
+namespace tnp {
+template <typename T, int VE>
+static int embed_backward_typed(const uint32_t *keys, const uint32_t *idx, int64_t N, int64_t V, const void *grad, int64_t ldg, int D, float scale,
+                                void *dw, int64_t ldd, float *head, float *tail, hipStream_t s) {
+    return embed_sums<T, VE>(keys, idx, (uint32_t)N, (uint32_t)V, (const T *)grad, ldg, D, scale, (T *)dw, ldd, head, tail, s);
+}
+}  // namespace tnp
+
+extern "C" TNP_API int tnp_token_embedding_backward(const void *tokens, int token_bytes, int64_t N, const void *grad, int64_t ldg, int64_t V,
+                                                    int D, int dtype, float scale, void *dweight, int64_t ldd, void *workspace,
+                                                    size_t workspace_bytes, void *stream) {
+    if (int rc = embed_check("tnp_token_embedding_backward", token_bytes, N, V, D, dtype, ldg, ldd)) return rc;
+    if (!dweight || (N > 0 && (!tokens || !grad || !workspace))) TNP_FAIL(-1, "tnp_token_embedding_backward: NULL pointer");
+    const size_t need = tnp_token_embedding_backward_workspace_bytes(N, V, D);
+    if (workspace_bytes < need) TNP_FAIL(-1, "tnp_token_embedding_backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    hipStream_t s = (hipStream_t)stream;
+    uint32_t *keys[2] = {nullptr, nullptr}, *idx[2] = {nullptr, nullptr};
+    float *head = nullptr, *tail = nullptr;
+    int at = 0;
+    if (N > 0) {
+        const EmbedSort p = embed_sort_plan(N, V);
+        char *w = (char *)workspace;
+        for (int k = 0; k < 2; ++k) { keys[k] = (uint32_t *)w; w += up256((size_t)N * 4); idx[k] = (uint32_t *)w; w += up256((size_t)N * 4); }
+        uint32_t *hist = (uint32_t *)w;
+        w += up256((size_t)p.nblk * 4 << p.bits);
+        head = (float *)w;
+        tail = (float *)(w + up256((size_t)((N + EMB_CHUNK - 1) / EMB_CHUNK) * D * 4));
+        const int rc = token_bytes == 8 ? embed_sort((const int64_t *)tokens, N, (uint32_t)V, p, keys, idx, hist, s)
+                                        : embed_sort((const int32_t *)tokens, N, (uint32_t)V, p, keys, idx, hist, s);
+        if (rc) return rc;
+        at = (p.passes - 1) & 1;
+    }
+    const int ve = embed_width(dtype, D, {ldg, ldd}, {grad, dweight});
+    return TNP_BY_WIDTH(embed_backward_typed, ve, dtype, keys[at], idx[at], N, V, grad, ldg, D, scale, dweight, ldd, head, tail, s);
+}

@@ -1,0 +1,918 @@
+// Cross entropy over a vocabulary (gfx950): the output layer and its softmax loss as one operator,
+//     l_iv = hidden_i . weight_v + bias_v,   lse_i = log sum_v exp(l_iv),   loss_i = lse_i - l_i,target(i)
+//     G_iv = g_i (exp(l_iv - lse_i) - [v == target(i)]),   dhidden = G weight,   dweight = G^T hidden,   dbias_v = sum_i G_iv
+// The logits are never kept: the forward pass leaves per row the running maximum and sum of every vocabulary tile, the backward
+// pass forms the logits again, piece by piece of the vocabulary, as G in fp16 (twice fp16 for fp32 inputs), which both gradient
+// products read.  Forming them again costs 2 M D V operations; writing, reading and correcting the fp32 logits would cost 12 bytes
+// each, more than that for every D below about 2000.
+//
+// Numbers.  Inputs are packed once per call as fp16 times one power of two per tensor, so that its largest element lies in
+// [2^14, 2^15): bf16 and fp16 values are exact down to 2^-29 of the largest, fp32 values become two fp16 numbers (vocab_gemm.h) with an error
+// of 2^-23 of the value or 2^-40 of the largest.  G = 2^15 (g_i / max g) (p - y) is rounded to fp16 (11 bits, finer than bf16
+// by 8) or to two fp16 numbers.  All sums, maxima and statistics are fp32; the sum of the losses is fp64.
+//
+// A negative target marks an absent row: its hidden state is not read (it may be NaN), its loss and gradients are zero.  A target
+// >= V is an error that shows: NaN loss, NaN gradients.
+#include "vocab_gemm.h"
+
+#include <math.h>
+
+namespace tnp {
+
+static constexpr float CE_LOG2E = 1.4426950408889634f;
+static constexpr double CE_LN2 = 0.6931471805599453;
+static constexpr float CE_NEG_INF = -__builtin_inff();
+static constexpr int CE_AMAX_BLOCKS = 256;            // per tensor
+static constexpr int CE_ROW_PAD = 256, CE_COL_PAD = 256;
+static constexpr int CE_SCORE_ROWS = 64;              // rows up to which scoring reads the inputs in place
+
+struct CeScalars {            // head of the saved area
+    int ex, ew;               // packed = value * 2^-e
+    uint32_t ticket;          // last-workgroup counter of the loss sum
+    int pad;
+    float count;              // rows that are there
+    float gmax;               // largest |grad| (reduction none), else 1
+};
+
+struct CeShape {
+    int64_t M, Mp;            // rows, padded to 256
+    int V, Vp, D;             // vocabulary, padded to 256
+    int split;                // fp32: two planes
+    int64_t ld;               // stored elements per packed row
+    int steps;                // k steps of the logits
+};
+
+// ---- scales and packing -----------------------------------------------------------------------------------------------------
+template <typename T, int VE>
+__device__ __forceinline__ float ce_row_amax(const T *row, int D, int lane) {
+    float a = 0.0f;
+    for (int c = lane * VE; c < D; c += 64 * VE) {
+        const Pack<T, VE> p = *(const Pack<T, VE> *)(row + c);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+            const float v = fabsf(to_f32(p.v[e]));
+            if (v < __builtin_inff()) a = fmaxf(a, v);           // infinities and NaN do not set the scale
+        }
+    }
+    return a;
+}
+
+template <typename T, int VX, int VW>
+__global__ void __launch_bounds__(256) ce_amax_kernel(const T *x, int64_t ldx, int64_t M, const int64_t *target, const T *w, int64_t ldw, int V,
+                                                      int D, float *part, CeScalars *sc) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const bool is_w = blockIdx.x >= CE_AMAX_BLOCKS;
+    const int bid = is_w ? blockIdx.x - CE_AMAX_BLOCKS : blockIdx.x;
+    float a = 0.0f;
+    if (is_w) {
+        for (int64_t r = bid * 4 + wave; r < V; r += CE_AMAX_BLOCKS * 4) a = fmaxf(a, ce_row_amax<T, VW>(w + r * ldw, D, lane));
+    } else {
+        for (int64_t r = bid * 4 + wave; r < M; r += CE_AMAX_BLOCKS * 4)
+            if (target[r] >= 0) a = fmaxf(a, ce_row_amax<T, VX>(x + r * ldx, D, lane));
+    }
+    __shared__ float sh[4];
+    for (int o = 32; o; o >>= 1) a = fmaxf(a, __shfl_xor(a, o));
+    if (lane == 0) sh[wave] = a;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        part[blockIdx.x] = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
+        if (blockIdx.x == 0) sc->ticket = 0;
+    }
+}
+
+// exponent e with max |x| * 2^-e in [2^14, 2^15); 0 for an all-zero tensor
+__device__ __forceinline__ int ce_exponent(float a) {
+    if (a == 0.0f) return 0;
+    int e;
+    frexpf(a, &e);
+    return e - 15;
+}
+
+template <typename T, int VE, bool SPLIT>
+__device__ __forceinline__ void ce_pack_row(const T *src, bool live, int D, int e, half_t *dst, int64_t ld, int lane) {
+    // eight values per lane and trip; split rows hold 32 hi | 32 lo per block
+    const int per = SPLIT ? (int)ld / 2 : (int)ld;
+    for (int c = lane * 8; c < per; c += 512) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k += VE < 8 ? VE : 8) {
+            if (live && c + k < D) {
+                const Pack<T, (VE < 8 ? VE : 8)> p = *(const Pack<T, (VE < 8 ? VE : 8)> *)(src + c + k);
+#pragma unroll
+                for (int q = 0; q < (VE < 8 ? VE : 8); ++q) v[k + q] = ldexpf(to_f32(p.v[q]), -e);
+            } else {
+#pragma unroll
+                for (int q = 0; q < (VE < 8 ? VE : 8); ++q) v[k + q] = 0.0f;
+            }
+        }
+        half8 hi, lo;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            hi[k] = (half_t)v[k];
+            lo[k] = fabsf(v[k]) < 65504.0f ? (half_t)(v[k] - (float)hi[k]) : (half_t)0.0f;
+        }
+        if (SPLIT) {
+            half_t *o = dst + (c >> 5) * 64 + (c & 31);
+            *(half8 *)o = hi;
+            *(half8 *)(o + 32) = lo;
+        } else {
+            *(half8 *)(dst + c) = hi;
+        }
+    }
+}
+
+template <typename T, int VX, int VW, bool SPLIT>
+__global__ void __launch_bounds__(256) ce_pack_kernel(const T *x, int64_t ldx, const int64_t *target, const T *w, int64_t ldw, CeShape sh,
+                                                      const float *part, CeScalars *sc, half_t *xp, half_t *wp, int x_blocks) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const bool is_w = (int)blockIdx.x >= x_blocks;
+    __shared__ float red[4];
+    float a = part[(is_w ? CE_AMAX_BLOCKS : 0) + threadIdx.x];
+    for (int o = 32; o; o >>= 1) a = fmaxf(a, __shfl_xor(a, o));
+    if (lane == 0) red[wave] = a;
+    __syncthreads();
+    int e = ce_exponent(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+    if (threadIdx.x == 0 && (blockIdx.x == 0 || (int)blockIdx.x == x_blocks)) (is_w ? sc->ew : sc->ex) = e;
+    if (is_w) {
+        const int blocks = gridDim.x - x_blocks;
+        for (int64_t r = ((int)blockIdx.x - x_blocks) * 4 + wave; r < sh.Vp; r += blocks * 4)
+            ce_pack_row<T, VW, SPLIT>(w + r * ldw, r < sh.V, sh.D, e, wp + r * sh.ld, sh.ld, lane);
+    } else {
+        for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < sh.Mp; r += x_blocks * 4)
+            ce_pack_row<T, VX, SPLIT>(x + r * ldx, r < sh.M && target[r] >= 0, sh.D, e, xp + r * sh.ld, sh.ld, lane);
+    }
+}
+
+// ---- logits: statistics forward, G backward ---------------------------------------------------------------------------------
+// The vocabulary runs over the rows of the matrix instruction, so a lane holds 16 logits of ONE hidden row per 32 x 32 block and
+// maxima, sums and exponentials stay inside the lane; the two halves of a wave meet once per wave tile.
+struct CeLogits {
+    GemmOperand w, x;
+    const CeScalars *sc;
+    const int64_t *target;
+    int64_t M, Mp;
+    int V, v0, tiles_v, tiles_i, steps;
+    // forward
+    float2 *part;             // [wave tile along V][Mp]: (max, sum of 2^(l - max)), base 2
+    float *tlogit;            // [Mp] target's logit, base 2
+    // backward
+    const float *lse;         // [Mp] base 2; +inf: absent, NaN: no such target
+    const float *grad;        // reduction none: [M]
+    half_t *g;                // [Mp][ldg], column 0 = vocabulary entry v0
+    int64_t ldg;
+};
+
+template <typename T> __device__ __forceinline__ float ce_bias(const T *bias, int v) { return bias ? to_f32(bias[v]) * CE_LOG2E : 0.0f; }
+
+template <typename T, bool SPLIT, bool BACK, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(WM *WN * 64, 2) ce_logits_kernel(CeLogits a, const T *bias) {
+    constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    __shared__ __attribute__((aligned(16))) float sb[BM];
+    int tv, ti;
+    if (!gemm_tile_of(blockIdx.x, a.tiles_v, a.tiles_i, tv, ti)) return;
+    const int64_t vbase = a.v0 + (int64_t)tv * BM, ibase = (int64_t)ti * BN;
+    for (int j = threadIdx.x; j < BM; j += WM * WN * 64) sb[j] = vbase + j < a.V ? ce_bias(bias, (int)vbase + j) : CE_NEG_INF;
+    f32x16 acc[TM][TN];
+    gemm_tile<SPLIT, false, false, BM, BN, WM, WN>(a.w, a.x, vbase, 0, ibase, 0, 0, a.steps, lds, acc);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+    const int wm = wave / WN, wn = wave % WN;
+    const float scale = ldexpf(CE_LOG2E, a.sc->ex + a.sc->ew);
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const float4 b = *(const float4 *)(sb + wm * TM * 32 + i * 32 + 8 * q + 4 * h);
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                acc[i][j][4 * q + 0] = fmaf(acc[i][j][4 * q + 0], scale, b.x);
+                acc[i][j][4 * q + 1] = fmaf(acc[i][j][4 * q + 1], scale, b.y);
+                acc[i][j][4 * q + 2] = fmaf(acc[i][j][4 * q + 2], scale, b.z);
+                acc[i][j][4 * q + 3] = fmaf(acc[i][j][4 * q + 3], scale, b.w);
+            }
+        }
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+        const int64_t row = ibase + wn * TN * 32 + j * 32 + (lane & 31);
+        // the target's place in this lane's part of the wave tile: local - 4 h = 32 i + 8 q + e
+        const int64_t t = row < a.M ? a.target[row] : -1, off = t - vbase - wm * TM * 32 - 4 * h;
+        const bool mine = t >= 0 && off >= 0 && off < TM * 32 && (off & 4) == 0;
+        if (!BACK) {
+            float m = CE_NEG_INF;
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) m = fmaxf(m, acc[i][j][e]);
+            m = fmaxf(m, __shfl_xor(m, 32));
+            const float mm = m == CE_NEG_INF ? 0.0f : m;         // nothing but masked entries: a sum of zeros, not of NaN
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s += __builtin_amdgcn_exp2f(acc[i][j][e] - mm);
+            s += __shfl_xor(s, 32);
+            if (h == 0) a.part[(int64_t)(tv * WM + wm) * a.Mp + row] = make_float2(m, s);
+            if (__any(mine)) {
+                float l = 0.0f;
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (off == 32 * i + 8 * (e >> 2) + (e & 3)) l = acc[i][j][e];
+                if (mine) a.tlogit[row] = l;
+            }
+        } else {
+            const float lse = a.lse[row];
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_amdgcn_exp2f(acc[i][j][e] - lse);
+            if (__any(mine)) {
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (mine && off == 32 * i + 8 * (e >> 2) + (e & 3)) acc[i][j][e] -= 1.0f;
+            }
+            float f = t >= 0 ? 32768.0f : 0.0f;
+            if (a.grad && t >= 0) f = a.sc->gmax > 0.0f ? 32768.0f * (a.grad[row] / a.sc->gmax) : 0.0f;
+            // stored order inside 16 columns: 0 1 2 3 8 9 10 11 | 4 5 6 7 12 13 14 15 -- what one lane holds, 16 bytes at a time
+            half_t *out = a.g + row * a.ldg + ((int64_t)tv * BM + wm * TM * 32) * (SPLIT ? 2 : 1) + h * 8;
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    half8 hi, lo;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float v = acc[i][j][8 * c + e] * f;
+                        hi[e] = (half_t)v;
+                        if (SPLIT) lo[e] = (half_t)(v - (float)hi[e]);
+                    }
+                    *(half8 *)(out + i * 32 * (SPLIT ? 2 : 1) + c * 16) = hi;
+                    if (SPLIT) *(half8 *)(out + i * 64 + 32 + c * 16) = lo;
+                }
+        }
+    }
+}
+
+// ---- few rows, no gradient: the weight's bytes ------------------------------------------------------------------------------
+// Up to 64 rows.  A wave takes 16 vocabulary entries at a time, operands straight from memory into the matrix instruction's
+// registers (fp32: v_mfma_f32_16x16x4_f32; lane (r, q) loads the 16 bytes k = 4 q .. of row r, element e feeds the e-th
+// instruction for both operands), and keeps the running maximum and sum of every row.
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T, bool VEC> struct ScoreLoad;
+template <bool VEC> struct ScoreLoad<float, VEC> {
+    typedef f32x4 frag;
+    static constexpr int KW = 4;
+    static __device__ __forceinline__ void mma(const frag &a, const frag &b, f32x4 &c) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+    }
+};
+template <bool VEC> struct ScoreLoad<half_t, VEC> {
+    typedef half8 frag;
+    static constexpr int KW = 8;
+    static __device__ __forceinline__ void mma(const frag &a, const frag &b, f32x4 &c) {
+        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+};
+template <bool VEC> struct ScoreLoad<bf16_t, VEC> {
+    typedef bf8 frag;
+    static constexpr int KW = 8;
+    static __device__ __forceinline__ void mma(const frag &a, const frag &b, f32x4 &c) {
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+};
+
+template <typename T, bool VEC>
+__device__ __forceinline__ typename ScoreLoad<T, VEC>::frag score_load(const T *row, int k, int D) {
+    typedef ScoreLoad<T, VEC> L;
+    Pack<T, L::KW> p;
+    if (VEC) {
+        if (k < D) return __builtin_bit_cast(typename L::frag, *(const Pack<T, L::KW> *)(row + k));
+#pragma unroll
+        for (int e = 0; e < L::KW; ++e) p.v[e] = from_f32<T>(0.0f);
+    } else {
+#pragma unroll
+        for (int e = 0; e < L::KW; ++e) p.v[e] = k + e < D ? row[k + e] : from_f32<T>(0.0f);
+    }
+    return __builtin_bit_cast(typename L::frag, p);
+}
+
+template <typename T, bool VEC, int NT>
+__global__ void __launch_bounds__(256) ce_score_kernel(const T *x, int64_t ldx, int M, const T *w, int64_t ldw, int V, int D, const T *bias,
+                                                       const int64_t *target, float2 *part, float *tlogit, CeScalars *sc) {
+    typedef ScoreLoad<T, VEC> L;
+    constexpr int KS = 4 * L::KW, U = NT == 1 ? 4 : 2;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+    if (blockIdx.x == 0 && threadIdx.x == 0) sc->ticket = 0;
+    const T *xr[NT];
+    float m[NT], s[NT];
+    int64_t t[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int i = n * 16 + r < M ? n * 16 + r : M - 1;
+        xr[n] = x + i * ldx;
+        t[n] = n * 16 + r < M ? target[i] : -1;
+        m[n] = CE_NEG_INF;
+        s[n] = 0.0f;
+    }
+    const int groups = (V + 15) / 16;
+    for (int g = blockIdx.x * 4 + wave; g < groups; g += gridDim.x * 4) {
+        const int vr = g * 16 + r < V ? g * 16 + r : V - 1;
+        const T *wr = w + (int64_t)vr * ldw;
+        f32x4 acc[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k = q * L::KW; k < D + q * L::KW; k += U * KS) {
+            typename L::frag fw[U], fx[NT][U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                fw[u] = score_load<T, VEC>(wr, k + u * KS, D);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) fx[n][u] = score_load<T, VEC>(xr[n], k + u * KS, D);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) L::mma(fw[u], fx[n][u], acc[n]);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float l[4], top = m[n];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int v = g * 16 + 4 * q + e;
+                l[e] = v < V ? fmaf(acc[n][e], CE_LOG2E, ce_bias(bias, v)) : CE_NEG_INF;
+                top = fmaxf(top, l[e]);
+                if (t[n] == v) tlogit[n * 16 + r] = l[e];
+            }
+            const float mm = top == CE_NEG_INF ? 0.0f : top;
+            s[n] *= __builtin_amdgcn_exp2f(m[n] - mm);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n] += __builtin_amdgcn_exp2f(l[e] - mm);
+            m[n] = top;
+        }
+    }
+    __shared__ float2 red[4][NT * 16];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        for (int o = 16; o < 64; o <<= 1) {
+            const float mo = __shfl_xor(m[n], o), so = __shfl_xor(s[n], o), top = fmaxf(m[n], mo), mm = top == CE_NEG_INF ? 0.0f : top;
+            s[n] = s[n] * __builtin_amdgcn_exp2f(m[n] - mm) + so * __builtin_amdgcn_exp2f(mo - mm);
+            m[n] = top;
+        }
+        if (q == 0) red[wave][n * 16 + r] = make_float2(m[n], s[n]);
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < NT * 16) {
+        float top = CE_NEG_INF, sum = 0.0f;
+        for (int k = 0; k < 4; ++k) top = fmaxf(top, red[k][threadIdx.x].x);
+        const float mm = top == CE_NEG_INF ? 0.0f : top;
+        for (int k = 0; k < 4; ++k) sum += red[k][threadIdx.x].y * __builtin_amdgcn_exp2f(red[k][threadIdx.x].x - mm);
+        part[(int64_t)blockIdx.x * CE_SCORE_ROWS + threadIdx.x] = make_float2(top, sum);
+    }
+}
+
+// ---- rows: join the tiles' statistics, losses, their sum --------------------------------------------------------------------
+// 2^rsh rows per workgroup, 256 >> rsh threads stride over one row's parts.  The last workgroup to finish adds the workgroups'
+// sums in their order, in fp64.
+__global__ void __launch_bounds__(256) ce_rows_kernel(const float2 *part, int64_t ldp, int parts, const float *tlogit, const int64_t *target,
+                                                      int64_t M, int64_t Mp, int V, int rsh, int reduction, float *lse_out, float *loss,
+                                                      double2 *sums, CeScalars *sc) {
+    __shared__ float2 sh[256];
+    __shared__ double2 tot[256];
+    __shared__ bool last;
+    const int rows = 1 << rsh, segs = 256 >> rsh, r = threadIdx.x & (rows - 1), seg = threadIdx.x >> rsh;
+    const int64_t i = (int64_t)blockIdx.x * rows + r;
+    float m = CE_NEG_INF, s = 0.0f;
+    if (i < M) {
+        constexpr int U = 4;
+        for (int p = seg; p < parts; p += segs * U) {
+            float2 v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u] = p + u * segs < parts ? part[(int64_t)(p + u * segs) * ldp + i] : make_float2(CE_NEG_INF, 0.0f);
+            float top = m;
+#pragma unroll
+            for (int u = 0; u < U; ++u) top = fmaxf(top, v[u].x);
+            const float mm = top == CE_NEG_INF ? 0.0f : top;
+            s *= __builtin_amdgcn_exp2f(m - mm);
+#pragma unroll
+            for (int u = 0; u < U; ++u) s += v[u].y * __builtin_amdgcn_exp2f(v[u].x - mm);
+            m = top;
+        }
+    }
+    sh[threadIdx.x] = make_float2(m, s);
+    __syncthreads();
+    double2 mine = make_double2(0.0, 0.0);
+    if (seg == 0 && i < Mp) {
+        const int64_t t = i < M ? target[i] : -1;
+        float lse = __builtin_inff(), l = 0.0f;
+        if (t >= 0) {
+            float top = CE_NEG_INF, sum = 0.0f;
+            for (int k = 0; k < segs; ++k) top = fmaxf(top, sh[(k << rsh) + r].x);
+            const float mm = top == CE_NEG_INF ? 0.0f : top;
+            for (int k = 0; k < segs; ++k) sum += sh[(k << rsh) + r].y * __builtin_amdgcn_exp2f(sh[(k << rsh) + r].x - mm);
+            const float ls = log2f(sum);
+            lse = t < V ? top + ls : __builtin_nanf("");
+            // (top - target's logit) first: the two are near each other where the loss is small
+            l = t < V ? (float)(((double)(top - tlogit[i]) + (double)ls) * CE_LN2) : __builtin_nanf("");
+            mine = make_double2((double)l, 1.0);
+        }
+        if (lse_out) lse_out[i] = lse;
+        if (reduction == 0 && i < M) loss[i] = l;
+    }
+    if (reduction == 0) return;
+    tot[threadIdx.x] = mine;
+    __syncthreads();
+    for (int o = 128; o; o >>= 1) {
+        if ((int)threadIdx.x < o) { tot[threadIdx.x].x += tot[threadIdx.x + o].x; tot[threadIdx.x].y += tot[threadIdx.x + o].y; }
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+        sums[blockIdx.x] = tot[0];
+        __threadfence();
+        last = atomicAdd(&sc->ticket, 1u) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    mine = make_double2(0.0, 0.0);
+    for (unsigned k = threadIdx.x; k < gridDim.x; k += 256) {
+        const double2 v = make_double2(__hip_atomic_load(&sums[k].x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
+                                       __hip_atomic_load(&sums[k].y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+        mine.x += v.x;
+        mine.y += v.y;
+    }
+    tot[threadIdx.x] = mine;
+    __syncthreads();
+    for (int o = 128; o; o >>= 1) {
+        if ((int)threadIdx.x < o) { tot[threadIdx.x].x += tot[threadIdx.x + o].x; tot[threadIdx.x].y += tot[threadIdx.x + o].y; }
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+        const double n = tot[0].y;
+        loss[0] = (float)(reduction == 1 ? (n > 0.0 ? tot[0].x / n : 0.0) : tot[0].x);
+        sc->count = (float)n;
+        sc->gmax = 1.0f;
+    }
+}
+
+// largest |grad| over the rows that are there (reduction none)
+__global__ void __launch_bounds__(1024) ce_gmax_kernel(const float *grad, const int64_t *target, int64_t M, CeScalars *sc) {
+    __shared__ float sh[16];
+    float a = 0.0f;
+    for (int64_t i = threadIdx.x; i < M; i += 1024)
+        if (target[i] >= 0) {
+            const float g = fabsf(grad[i]);
+            a = g > a || g != g ? g : a;                     // NaN stays
+        }
+    for (int o = 32; o; o >>= 1) {
+        const float b = __shfl_xor(a, o);
+        a = b > a || b != b ? b : a;
+    }
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = a;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int k = 1; k < 16; ++k) a = sh[k] > a || sh[k] != sh[k] ? sh[k] : a;
+        sc->gmax = a;
+    }
+}
+
+// ---- gradient products ------------------------------------------------------------------------------------------------------
+// what takes a sum over G back to the gradient: 2^-15 max g, times the other operand's scale
+__device__ __forceinline__ float ce_unscale(const CeScalars *sc, const float *grad, int reduction, int e) {
+    float g = reduction == 0 ? sc->gmax : reduction == 1 ? grad[0] / fmaxf(sc->count, 1.0f) : grad[0];
+    return ldexpf(g, e - 15);
+}
+
+struct CeGrad {
+    GemmOperand g, o;         // G and the other operand (weight or hidden states)
+    const CeScalars *sc;
+    const float *grad;
+    const int64_t *target;    // dhidden: rows with a negative target are zero
+    int reduction;
+    int64_t rows, out0;       // output rows of this call, the first one's index in the output
+    int D, tiles_r, tiles_d, steps, splits;
+    int64_t ok0;              // first row of the other operand
+    void *out;                // final output (splits == 1, single piece)
+    int64_t ldo;
+    float *part;              // [splits][part_rows][D] sums, or NULL
+    int64_t part_rows;
+    int add;                  // part += (later pieces of the vocabulary)
+};
+
+// WEIGHT: dweight (G read transposed, output rows = vocabulary entries in G's stored column order), else dhidden
+template <typename T, bool SPLIT, bool WEIGHT, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(WM *WN * 64, 2) ce_grad_kernel(CeGrad a) {
+    constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    int tr, td;
+    const int per = (a.tiles_r * a.tiles_d + 7) / 8 * 8, z = blockIdx.x / per;
+    if (!gemm_tile_of(blockIdx.x - z * per, a.tiles_r, a.tiles_d, tr, td)) return;
+    const int64_t r0 = (int64_t)tr * BM;
+    const int d0 = td * BN;
+    const int s0 = (int)((int64_t)a.steps * z / a.splits), s1 = (int)((int64_t)a.steps * (z + 1) / a.splits);
+    f32x16 acc[TM][TN];
+    if (WEIGHT)
+        gemm_tile<SPLIT, true, true, BM, BN, WM, WN>(a.g, a.o, r0, 0, d0, a.ok0, s0, s1, lds, acc);
+    else
+        gemm_tile<SPLIT, false, true, BM, BN, WM, WN>(a.g, a.o, r0, 0, d0, a.ok0, s0, s1, lds, acc);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+    const int wm = wave / WN, wn = wave % WN;
+    const float f = a.part ? 1.0f : ce_unscale(a.sc, a.grad, a.reduction, WEIGHT ? a.sc->ex : a.sc->ew);
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int pos = (e & 3) + 8 * (e >> 2) + 4 * h;
+            const int loc = WEIGHT ? (pos & ~12) | ((pos & 4) << 1) | ((pos & 8) >> 1) : pos;
+            const int64_t row = r0 + wm * TM * 32 + i * 32 + loc;
+            if (row >= a.rows) continue;
+            const bool live = WEIGHT || a.part || a.target[row] >= 0;
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                const int d = d0 + wn * TN * 32 + j * 32 + (lane & 31);
+                if (d >= a.D) continue;
+                const float v = acc[i][j][e];
+                if (a.part) {
+                    float *p = a.part + ((int64_t)z * a.part_rows + row) * a.D + d;
+                    *p = a.add ? *p + v : v;
+                } else {
+                    ((T *)a.out)[(a.out0 + row) * a.ldo + d] = from_f32<T>(live ? v * f : 0.0f);
+                }
+            }
+        }
+}
+
+// out[r][d] = factor * sum over splits of part[s][r][d], the splits in their order
+template <typename T>
+__global__ void __launch_bounds__(256) ce_join_kernel(const float *part, int64_t rows, int64_t part_rows, int splits, int D, const CeScalars *sc,
+                                                      const float *grad, int reduction, int weight, const int64_t *target, T *out,
+                                                      int64_t ldo) {
+    const float f = ce_unscale(sc, grad, reduction, weight ? sc->ex : sc->ew);
+    const int64_t n = rows * D, stride = part_rows * D;
+    for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < n; k += (int64_t)gridDim.x * 256) {
+        const int64_t row = k / D;
+        float v = 0.0f;
+        for (int s = 0; s < splits; ++s) v += part[s * stride + k];
+        out[row * ldo + (k - row * D)] = from_f32<T>(weight || target[row] >= 0 ? v * f : 0.0f);
+    }
+}
+
+// column sums of G (dbias): a lane owns eight stored columns, a workgroup a share of the rows
+__global__ void __launch_bounds__(256) ce_colsum_kernel(const half_t *g, int64_t ldg, int64_t rows, int64_t cols, float *part, int64_t ldp) {
+    __shared__ float sh[3][64][8];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t c = (int64_t)blockIdx.x * 512 + lane * 8;
+    const int64_t per = (rows + gridDim.y - 1) / gridDim.y, r0 = blockIdx.y * per, r1 = r0 + per < rows ? r0 + per : rows;
+    float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (c < cols) {
+        constexpr int U = 4;
+        for (int64_t r = r0 + wave; r < r1; r += 4 * U) {
+            half8 v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (r + 4 * u < r1) v[u] = *(const half8 *)(g + (r + 4 * u) * ldg + c);
+                else
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[u][e] = (half_t)0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[e] += (float)v[u][e];
+        }
+    }
+    if (wave)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sh[wave - 1][lane][e] = s[e];
+    __syncthreads();
+    if (wave == 0 && c < cols)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) part[blockIdx.y * ldp + c + e] = s[e] + sh[0][lane][e] + sh[1][lane][e] + sh[2][lane][e];
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) ce_dbias_kernel(const float *part, int64_t ldp, int shares, int split, int n, const CeScalars *sc,
+                                                       const float *grad, int reduction, T *out) {
+    const int v = blockIdx.x * 256 + threadIdx.x;
+    if (v >= n) return;
+    const int pos = (v & ~12) | ((v & 4) << 1) | ((v & 8) >> 1);
+    float s = 0.0f;
+    for (int k = 0; k < shares; ++k) {
+        const float *p = part + k * ldp;
+        s += split ? p[(pos >> 5) * 64 + (pos & 31)] + p[(pos >> 5) * 64 + (pos & 31) + 32] : p[pos];
+    }
+    out[v] = from_f32<T>(s * ce_unscale(sc, grad, reduction, 0));
+}
+
+// ---- host -------------------------------------------------------------------------------------------------------------------
+static inline size_t ce_up(size_t n) { return (n + 255) & ~(size_t)255; }
+static inline int64_t ce_pad(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
+
+static CeShape ce_shape(const tnp_vocab_ce *p) {
+    CeShape s;
+    s.M = p->M; s.Mp = ce_pad(p->M, CE_ROW_PAD);
+    s.V = p->V; s.Vp = (int)ce_pad(p->V, CE_COL_PAD); s.D = p->D;
+    s.split = p->dtype == TNP_F32;
+    s.ld = s.split ? 2 * ce_pad(p->D, 32) : ce_pad(p->D, 64);
+    s.steps = (int)(s.ld / 64);
+    return s;
+}
+
+struct CeSaved { CeScalars *sc; float *lse; half_t *x, *w; size_t bytes; };
+static CeSaved ce_saved(const CeShape &s, void *base) {
+    CeSaved v;
+    char *p = (char *)base;
+    v.sc = (CeScalars *)p; p += 256;
+    v.lse = (float *)p; p += s.Mp * 4;                 // Mp and Vp are multiples of 256: every part stays aligned
+    v.x = (half_t *)p; p += (size_t)s.Mp * s.ld * 2;
+    v.w = (half_t *)p; p += (size_t)s.Vp * s.ld * 2;
+    v.bytes = (size_t)(p - (char *)base);
+    return v;
+}
+
+static bool ce_scores(const tnp_vocab_ce *p) { return !p->saved && p->M <= CE_SCORE_ROWS; }
+static int ce_score_blocks(int V) {
+    const int g = (V + 63) / 64;
+    return g < 1024 ? g : 1024;
+}
+static int ce_rows_shift(int64_t M) { return M <= CE_SCORE_ROWS ? 2 : 5; }
+
+static bool ce_big(const CeShape &s) { return (s.Mp / 256) * (int64_t)(s.Vp / 256) >= 512; }
+
+struct CeForward { CeSaved saved; float *amax; float2 *part; float *tlogit; double2 *sums; int parts; size_t bytes; };
+static CeForward ce_forward_layout(const tnp_vocab_ce *p, void *ws) {
+    CeForward f;
+    const CeShape s = ce_shape(p);
+    char *w = (char *)ws;
+    f.parts = ce_scores(p) ? ce_score_blocks(p->V) : s.Vp / 256 * (ce_big(s) ? 2 : 4);
+    const int64_t rows = ce_scores(p) ? CE_SCORE_ROWS : s.Mp;
+    f.amax = (float *)w; w += ce_up(2 * CE_AMAX_BLOCKS * 4);
+    f.part = (float2 *)w; w += ce_up((size_t)f.parts * rows * 8);
+    f.tlogit = (float *)w; w += ce_up(rows * 4);
+    f.sums = (double2 *)w; w += ce_up((size_t)((s.Mp >> ce_rows_shift(p->M)) + 1) * 16);
+    f.saved = ce_saved(s, p->saved ? p->saved : w);
+    if (!p->saved) w += ce_scores(p) ? 256 : f.saved.bytes;
+    f.bytes = (size_t)(w - (char *)ws);
+    return f;
+}
+
+// columns of G that are formed at a time, and the splits of the two gradient products
+struct CeBackward {
+    int piece, pieces;
+    int64_t ldg;
+    half_t *g;
+    int big, hidden_bn, splits_x, splits_w;
+    float *part_x, *part_w, *part_b;
+    int shares;
+    size_t bytes;
+};
+static constexpr size_t CE_PIECE_BYTES = (size_t)512 << 20;
+
+static int ce_splits(int64_t tiles, int steps, int target) {
+    int64_t n = target / tiles;
+    if (n > steps / 4) n = steps / 4;
+    return n < 1 ? 1 : (int)n;
+}
+static CeBackward ce_backward_layout(const tnp_vocab_ce *p, void *ws) {
+    CeBackward b;
+    const CeShape s = ce_shape(p);
+    const int planes = s.split ? 2 : 1, ks = s.split ? 32 : 64;
+    int64_t most = (int64_t)(CE_PIECE_BYTES / ((size_t)s.Mp * 2 * planes)) / 256 * 256;
+    if (most < 256) most = 256;
+    b.pieces = (int)((s.Vp + most - 1) / most);
+    b.piece = (int)ce_pad((s.Vp + b.pieces - 1) / b.pieces, 256);
+    b.pieces = (s.Vp + b.piece - 1) / b.piece;
+    b.ldg = (int64_t)b.piece * planes;
+    const int64_t td = (p->D + 127) / 128;
+    b.splits_x = ce_splits(s.Mp / 128 * td, b.piece / ks, 512);
+    b.splits_w = ce_splits((int64_t)b.piece / 128 * td, (int)(s.Mp / ks), 512);
+    b.shares = (int)(s.Mp / 256 < 64 ? s.Mp / 256 : 64);
+    char *w = (char *)ws;
+    b.g = (half_t *)w; w += ce_up((size_t)s.Mp * b.ldg * 2);
+    b.part_x = b.splits_x > 1 || b.pieces > 1 ? (float *)w : nullptr;
+    if (b.part_x) w += ce_up((size_t)b.splits_x * s.Mp * p->D * 4);
+    b.part_w = b.splits_w > 1 ? (float *)w : nullptr;
+    if (b.part_w) w += ce_up((size_t)b.splits_w * b.piece * p->D * 4);
+    b.part_b = p->bias ? (float *)w : nullptr;
+    if (b.part_b) w += ce_up((size_t)b.shares * b.ldg * 4);
+    b.bytes = (size_t)(w - (char *)ws);
+    return b;
+}
+
+static int ce_check(const tnp_vocab_ce *p, const char *who) {
+    if (!p) TNP_FAIL(-1, "%s: NULL arguments", who);
+    if (!dtype_known(p->dtype)) TNP_FAIL(-1, "%s: unknown dtype %d", who, p->dtype);
+    if (p->reduction < 0 || p->reduction > 2) TNP_FAIL(-1, "%s: unknown reduction %d", who, p->reduction);
+    if (p->M < 0 || p->M > (1 << 30)) TNP_FAIL(-1, "%s: %lld rows (0 .. 2^30)", who, (long long)p->M);
+    if (p->V < 1 || p->V > (1 << 28)) TNP_FAIL(-1, "%s: vocabulary of %d (1 .. 2^28)", who, p->V);
+    if (p->D < 1 || p->D > 16384) TNP_FAIL(-1, "%s: %d columns (1 .. 16384)", who, p->D);
+    if (p->ld_hidden < p->D || p->ld_weight < p->D) TNP_FAIL(-1, "%s: a row stride is smaller than the %d columns", who, p->D);
+    return 0;
+}
+
+static int ce_vec(int dtype, int D, int64_t ld, const void *p) {       // elements per load of a row: 16 bytes or one
+    const int ve = 16 / (int)dtype_bytes(dtype);
+    return D % ve == 0 && ld % ve == 0 && (uintptr_t)p % 16 == 0 ? ve : 1;
+}
+
+template <typename KernT>
+static int ce_lds(KernT kern, size_t smem, size_t *done) {             // done: per device
+    int dev = 0;
+    TNP_HIP(hipGetDevice(&dev));
+    if (dev < VOCAB_MAX_DEVICES && done[dev] >= smem) return 0;
+    TNP_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (dev < VOCAB_MAX_DEVICES) done[dev] = smem;
+    return 0;
+}
+
+template <typename T, bool SPLIT, bool BACK, int BM, int BN, int WM, int WN>
+static int ce_launch_logits(CeLogits a, int64_t cols, const T *bias, hipStream_t s) {
+    a.tiles_v = (int)(cols / BM);
+    a.tiles_i = (int)(a.Mp / BN);
+    const size_t smem = 2 * (BM + BN) * 128;
+    static size_t done[VOCAB_MAX_DEVICES] = {0};
+    auto kern = ce_logits_kernel<T, SPLIT, BACK, BM, BN, WM, WN>;
+    if (int rc = ce_lds(kern, smem, done)) return rc;
+    hipLaunchKernelGGL(kern, dim3(gemm_grid((int64_t)a.tiles_v * a.tiles_i)), dim3(WM * WN * 64), smem, s, a, bias);
+    TNP_HIP(hipGetLastError());
+    return 0;
+}
+template <typename T, bool SPLIT, bool BACK>
+static int ce_logits(const CeLogits &a, int64_t cols, bool big, const T *bias, hipStream_t s) {
+    return big ? ce_launch_logits<T, SPLIT, BACK, 256, 256, 2, 4>(a, cols, bias, s) : ce_launch_logits<T, SPLIT, BACK, 128, 128, 2, 2>(a, cols, bias, s);
+}
+
+template <typename T, bool SPLIT, bool WEIGHT>
+static int ce_grad(CeGrad a, hipStream_t s) {
+    constexpr int BM = 128, BN = 128, WM = 2, WN = 2;
+    a.tiles_r = (int)((a.rows + BM - 1) / BM);
+    a.tiles_d = (a.D + BN - 1) / BN;
+    const size_t smem = 2 * (BM + BN) * 128;
+    static size_t done[VOCAB_MAX_DEVICES] = {0};
+    auto kern = ce_grad_kernel<T, SPLIT, WEIGHT, BM, BN, WM, WN>;
+    if (int rc = ce_lds(kern, smem, done)) return rc;
+    hipLaunchKernelGGL(kern, dim3(gemm_grid((int64_t)a.tiles_r * a.tiles_d) * a.splits), dim3(WM * WN * 64), smem, s, a);
+    TNP_HIP(hipGetLastError());
+    return 0;
+}
+
+template <typename T, bool VEC>
+static int ce_score(const tnp_vocab_ce *p, const CeForward &f, hipStream_t s) {
+    const dim3 grid(ce_score_blocks(p->V));
+#define TNP_SCORE(NT)                                                                                                            \
+    hipLaunchKernelGGL((ce_score_kernel<T, VEC, NT>), grid, dim3(256), 0, s, (const T *)p->hidden, p->ld_hidden, (int)p->M,       \
+                       (const T *)p->weight, p->ld_weight, p->V, p->D, (const T *)p->bias, p->target, f.part, f.tlogit, f.saved.sc)
+    switch ((p->M + 15) / 16) {
+        case 1: TNP_SCORE(1); break;
+        case 2: TNP_SCORE(2); break;
+        case 3: TNP_SCORE(3); break;
+        default: TNP_SCORE(4);
+    }
+#undef TNP_SCORE
+    TNP_HIP(hipGetLastError());
+    return 0;
+}
+
+template <typename T, int VX, int VW, bool SPLIT>
+static int ce_pack(const tnp_vocab_ce *p, const CeShape &sh, const CeForward &f, hipStream_t s) {
+    hipLaunchKernelGGL((ce_amax_kernel<T, VX, VW>), dim3(2 * CE_AMAX_BLOCKS), dim3(256), 0, s, (const T *)p->hidden,
+                       p->ld_hidden, p->M, p->target, (const T *)p->weight, p->ld_weight, p->V, p->D, f.amax, f.saved.sc);
+    TNP_HIP(hipGetLastError());
+    const int xb = (int)(sh.Mp / 4 < 1024 ? sh.Mp / 4 : 1024), wb = sh.Vp / 4 < 2048 ? sh.Vp / 4 : 2048;
+    hipLaunchKernelGGL((ce_pack_kernel<T, VX, VW, SPLIT>), dim3(xb + wb), dim3(256), 0, s, (const T *)p->hidden, p->ld_hidden, p->target,
+                       (const T *)p->weight, p->ld_weight, sh, f.amax, f.saved.sc, f.saved.x, f.saved.w, xb);
+    TNP_HIP(hipGetLastError());
+    return 0;
+}
+
+template <typename T, int VE, bool SPLIT>
+static int ce_forward(const tnp_vocab_ce *p, const CeForward &f, float *loss, hipStream_t s) {
+    const CeShape sh = ce_shape(p);
+    const bool vx = ce_vec(p->dtype, p->D, p->ld_hidden, p->hidden) > 1, vw = ce_vec(p->dtype, p->D, p->ld_weight, p->weight) > 1;
+    int rc;
+    if (ce_scores(p)) {
+        rc = vx && vw ? ce_score<T, true>(p, f, s) : ce_score<T, false>(p, f, s);
+        if (rc) return rc;
+    } else {
+        rc = vx && vw ? ce_pack<T, VE, VE, SPLIT>(p, sh, f, s) : vw ? ce_pack<T, 1, VE, SPLIT>(p, sh, f, s)
+             : vx ? ce_pack<T, VE, 1, SPLIT>(p, sh, f, s) : ce_pack<T, 1, 1, SPLIT>(p, sh, f, s);
+        if (rc) return rc;
+        CeLogits a = {};
+        a.w = GemmOperand{f.saved.w, sh.ld, sh.Vp, 0};
+        a.x = GemmOperand{f.saved.x, sh.ld, sh.Mp, 0};
+        a.sc = f.saved.sc; a.target = p->target; a.M = sh.M; a.Mp = sh.Mp; a.V = sh.V; a.v0 = 0; a.steps = sh.steps;
+        a.part = f.part; a.tlogit = f.tlogit;
+        if ((rc = ce_logits<T, SPLIT, false>(a, sh.Vp, ce_big(sh), (const T *)p->bias, s))) return rc;
+    }
+    const int rsh = ce_rows_shift(p->M);
+    const int64_t cover = p->saved ? sh.Mp : p->M;
+    hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)((cover + (1 << rsh) - 1) >> rsh)), dim3(256), 0, s, f.part,
+                       ce_scores(p) ? (int64_t)CE_SCORE_ROWS : sh.Mp, f.parts, f.tlogit, p->target, p->M, cover, p->V, rsh, p->reduction,
+                       p->saved ? f.saved.lse : nullptr, loss, f.sums, f.saved.sc);
+    TNP_HIP(hipGetLastError());
+    return 0;
+}
+
+template <typename T, bool SPLIT>
+static int ce_backward(const tnp_vocab_ce *p, const CeBackward &b, const float *grad, void *dhidden, void *dweight, void *dbias, hipStream_t s) {
+    const CeShape sh = ce_shape(p);
+    const CeSaved sv = ce_saved(sh, p->saved);
+    int rc;
+    if (p->reduction == 0) {
+        hipLaunchKernelGGL(ce_gmax_kernel, dim3(1), dim3(1024), 0, s, grad, p->target, p->M, sv.sc);
+        TNP_HIP(hipGetLastError());
+    }
+    const GemmOperand w{sv.w, sh.ld, sh.Vp, 0}, x{sv.x, sh.ld, sh.Mp, 0};
+    for (int k = 0; k < b.pieces; ++k) {
+        const int v0 = k * b.piece, cols = sh.Vp - v0 < b.piece ? sh.Vp - v0 : b.piece, live = sh.V - v0 < cols ? sh.V - v0 : cols;
+        CeLogits a = {};
+        a.w = w; a.x = x; a.sc = sv.sc; a.target = p->target; a.M = sh.M; a.Mp = sh.Mp; a.V = sh.V; a.v0 = v0; a.steps = sh.steps;
+        a.lse = sv.lse; a.grad = p->reduction == 0 ? grad : nullptr; a.g = b.g; a.ldg = b.ldg;
+        if ((rc = ce_logits<T, SPLIT, true>(a, cols, ce_big(sh), (const T *)p->bias, s))) return rc;
+        CeGrad c = {};
+        c.sc = sv.sc; c.grad = grad; c.target = p->target; c.reduction = p->reduction; c.D = sh.D;
+        if (dhidden) {
+            c.g = GemmOperand{b.g, b.ldg, sh.Mp, 0};
+            c.o = w; c.o.perm = 1; c.ok0 = v0;
+            c.rows = sh.M; c.out0 = 0; c.out = dhidden; c.ldo = sh.D; c.part = b.part_x; c.part_rows = sh.Mp; c.splits = b.splits_x;
+            c.steps = cols / (SPLIT ? 32 : 64); c.add = k > 0;
+            if ((rc = ce_grad<T, SPLIT, false>(c, s))) return rc;
+        }
+        if (dweight) {
+            c.g = GemmOperand{b.g, b.ldg, sh.Mp, 0};
+            c.o = x; c.ok0 = 0;
+            c.rows = live; c.out0 = v0; c.out = dweight; c.ldo = sh.D; c.part = b.part_w; c.part_rows = b.piece; c.splits = b.splits_w;
+            c.steps = (int)(sh.Mp / (SPLIT ? 32 : 64)); c.add = 0;
+            if ((rc = ce_grad<T, SPLIT, true>(c, s))) return rc;
+            if (b.part_w) {
+                const int64_t n = (int64_t)live * sh.D;
+                hipLaunchKernelGGL((ce_join_kernel<T>), dim3((unsigned)(n / 1024 + 1 < 4096 ? n / 1024 + 1 : 4096)), dim3(256), 0, s, b.part_w,
+                                   (int64_t)live, (int64_t)b.piece, b.splits_w, sh.D, sv.sc, grad, p->reduction, 1, p->target,
+                                   (T *)dweight + (int64_t)v0 * sh.D, (int64_t)sh.D);
+                TNP_HIP(hipGetLastError());
+            }
+        }
+        if (dbias) {
+            const int64_t stored = (int64_t)cols * (SPLIT ? 2 : 1);
+            hipLaunchKernelGGL(ce_colsum_kernel, dim3((unsigned)((stored + 511) / 512), b.shares), dim3(256), 0, s, b.g, b.ldg, sh.Mp, stored,
+                               b.part_b, b.ldg);
+            TNP_HIP(hipGetLastError());
+            hipLaunchKernelGGL((ce_dbias_kernel<T>), dim3((live + 255) / 256), dim3(256), 0, s, b.part_b, b.ldg, b.shares, (int)SPLIT, live, sv.sc,
+                               grad, p->reduction, (T *)dbias + v0);
+            TNP_HIP(hipGetLastError());
+        }
+    }
+    if (dhidden && b.part_x) {
+        const int64_t n = sh.M * sh.D;
+        hipLaunchKernelGGL((ce_join_kernel<T>), dim3((unsigned)(n / 1024 + 1 < 4096 ? n / 1024 + 1 : 4096)), dim3(256), 0, s, b.part_x, sh.M, sh.Mp,
+                           b.splits_x, sh.D, sv.sc, grad, p->reduction, 0, p->target, (T *)dhidden, (int64_t)sh.D);
+        TNP_HIP(hipGetLastError());
+    }
+    return 0;
+}
+
+}  // namespace tnp
+
+using namespace tnp;
+
+extern "C" TNP_API size_t tnp_vocab_ce_saved_bytes(const tnp_vocab_ce *args) {
+    if (ce_check(args, "tnp_vocab_ce_saved_bytes")) return 0;
+    return ce_saved(ce_shape(args), nullptr).bytes;
+}
+
+extern "C" TNP_API size_t tnp_vocab_ce_workspace_bytes(const tnp_vocab_ce *args, int backward) {
+    if (ce_check(args, "tnp_vocab_ce_workspace_bytes")) return 0;
+    return backward ? ce_backward_layout(args, nullptr).bytes : ce_forward_layout(args, nullptr).bytes;
+}
+
+extern "C" TNP_API int tnp_vocab_ce_forward(const tnp_vocab_ce *args, float *loss, void *workspace, size_t workspace_bytes, void *stream) {
+    if (int rc = ce_check(args, "tnp_vocab_ce_forward")) return rc;
+    if (args->M == 0) TNP_FAIL(-1, "tnp_vocab_ce_forward: no rows");
+    if (!args->hidden || !args->weight || !args->target || !loss || !workspace) TNP_FAIL(-1, "tnp_vocab_ce_forward: NULL pointer");
+    const CeForward f = ce_forward_layout(args, workspace);
+    if (workspace_bytes < f.bytes) TNP_FAIL(-1, "tnp_vocab_ce_forward: workspace of %zu bytes, %zu needed", workspace_bytes, f.bytes);
+    hipStream_t s = (hipStream_t)stream;
+    if (args->dtype == TNP_F32) return ce_forward<float, 4, true>(args, f, loss, s);
+    if (args->dtype == TNP_BF16) return ce_forward<bf16_t, 8, false>(args, f, loss, s);
+    return ce_forward<half_t, 8, false>(args, f, loss, s);
+}
+
+extern "C" TNP_API int tnp_vocab_ce_backward(const tnp_vocab_ce *args, const float *grad, void *dhidden, void *dweight, void *dbias,
+                                             void *workspace, size_t workspace_bytes, void *stream) {
+    if (int rc = ce_check(args, "tnp_vocab_ce_backward")) return rc;
+    if (args->M == 0) TNP_FAIL(-1, "tnp_vocab_ce_backward: no rows");
+    if (!args->weight || !args->target || !args->saved || !grad || !workspace) TNP_FAIL(-1, "tnp_vocab_ce_backward: NULL pointer");
+    if (dbias && !args->bias) TNP_FAIL(-1, "tnp_vocab_ce_backward: dbias without a bias");
+    const CeBackward b = ce_backward_layout(args, workspace);
+    if (workspace_bytes < b.bytes) TNP_FAIL(-1, "tnp_vocab_ce_backward: workspace of %zu bytes, %zu needed", workspace_bytes, b.bytes);
+    hipStream_t s = (hipStream_t)stream;
+    if (args->dtype == TNP_F32) return ce_backward<float, true>(args, b, grad, dhidden, dweight, dbias, s);
+    if (args->dtype == TNP_BF16) return ce_backward<bf16_t, false>(args, b, grad, dhidden, dweight, dbias, s);
+    return ce_backward<half_t, false>(args, b, grad, dhidden, dweight, dbias, s);
+}

@@ -2,7 +2,7 @@
 batch by csrc/loss.hip: forward values and, on the training path, the analytic backward (tnp_primary_loss_backward)."""
 import torch
 
-from .. import _lib
+from .. import _lib, vocab
 
 
 class _PrimaryLossFn(torch.autograd.Function):
@@ -158,6 +158,21 @@ class L2Loss(torch.nn.Module):
     def forward(self, inputs, targets, batch_split, positions=None):
         loss, col = self.terms(inputs, targets, batch_split, positions)
         return loss if col is None else loss + col
+
+
+class VocabularyLoss(torch.nn.Module):
+    """Output layer and cross entropy of a model whose motions are entries of a vocabulary, in one operator that never stores
+    the logits: ``forward(hidden_state [..., H], target [...])``, a negative target being an absent track.  Stands where
+    Hidden2Normal + PredictionLoss stand for Gaussians; no counterpart in the reference.  The weight may be tied to a
+    TokenEmbedding's (``loss.linear.weight = embedding.weight``)."""
+
+    def __init__(self, hidden_dim, num_tokens, bias=True, reduction='mean'):
+        super(VocabularyLoss, self).__init__()
+        self.reduction = reduction
+        self.linear = torch.nn.Linear(hidden_dim, num_tokens, bias=bias)
+
+    def forward(self, hidden_state, target):
+        return vocab.vocab_cross_entropy(hidden_state, self.linear.weight, target, self.linear.bias, self.reduction)
 
 
 # ---- S-GAN trainer losses (reference lstm/loss.py:165-208, sgan/trainer.py:371-400) ---------------------------

@@ -4,7 +4,7 @@ kernels (csrc/lstm_seq.hip: ``track_prepare_kernel``); the stand-alone forwards 
 their Linear on the fp32 MFMA GEMM."""
 import torch
 
-from .. import _lib
+from .. import _lib, vocab
 
 _N_TAGS = 2   # the two trailing "start of encoder / start of decoder" tag columns of an embedding
 
@@ -57,3 +57,17 @@ class Hidden2Normal(torch.nn.Module):
         raw = _lib.linear_forward(hidden_state, self.linear.weight.detach(), self.linear.bias.detach())
         squashed = torch.sigmoid(raw[:, 2:])
         return torch.cat([raw[:, :2], 0.01 + 0.2 * squashed[:, :2], 0.7 * squashed[:, 2:]], dim=1)
+
+
+class TokenEmbedding(torch.nn.Module):
+    """Input embedding of a model whose motions are entries of a vocabulary (displacement or grid-cell tokens):
+    ``scale * weight[tokens]``, tokens [...] int64 / int32 -> [..., embedding_dim].  A negative token (absent track) embeds to
+    zeros.  No counterpart in the reference, whose InputEmbedding takes velocities."""
+
+    def __init__(self, num_tokens, embedding_dim, scale=1.0):
+        super().__init__()
+        self.num_tokens, self.embedding_dim, self.scale = num_tokens, embedding_dim, scale
+        self.weight = torch.nn.Parameter(torch.randn(num_tokens, embedding_dim) / embedding_dim ** 0.5)
+
+    def forward(self, tokens):
+        return vocab.token_embedding(tokens, self.weight, self.scale)
