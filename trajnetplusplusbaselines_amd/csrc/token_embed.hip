@@ -14,9 +14,9 @@
 namespace tnp {
 
 static constexpr int EMB_CHUNK = 32;          // sorted positions per group of lanes
-static constexpr int EMB_ROWS = 16;           // rows of 64 pairs per wave of the sort
-static constexpr int EMB_SORT_THREADS = 512;  // eight waves: 8192 pairs per workgroup
-static constexpr int EMB_SORT_ITEMS = EMB_SORT_THREADS / 64 * EMB_ROWS * 64;
+static constexpr int EMB_SORT_THREADS = 512;  // eight waves per workgroup of the sort, each with 4 or 16 rows of 64 pairs
+static constexpr int EMB_JOIN_CHUNKS = 32;    // chunks per workgroup of the join
+static constexpr int EMB_JOIN_SHORT = 8;      // parts of a run that one group of lanes adds up by itself
 static constexpr int EMB_MAX_BITS = 10;      // eight waves' counters of 2^10 digits: 32 KB of LDS
 static constexpr int64_t EMB_MAX_TOKENS = 1 << 28;
 
@@ -74,17 +74,17 @@ __device__ __forceinline__ uint64_t same_digit(uint32_t d, int bits, bool live) 
 
 // Ranks of a wave's pairs within (wave, digit), in ascending position, counts left in cnt[] (this wave's counters, zeroed by the
 // caller).  Only the first lane of a digit's group touches the counter, and LDS operations of a wave execute in order.
-template <typename I, bool RANK>
+template <typename I, int ROWS, bool RANK>
 __device__ __forceinline__ void embed_count(const I *tokens, const uint32_t *keys, int64_t base, int64_t N, uint32_t V, int shift,
                                             int bits, uint32_t *cnt, uint32_t *key, uint32_t *rank) {
     const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int r = 0; r < EMB_ROWS; ++r) {
+    for (int r = 0; r < ROWS; ++r) {
         const int64_t i = base + r * 64 + lane;
         key[r] = i < N ? embed_key(tokens, keys, i, V) : 0;
     }
 #pragma unroll
-    for (int r = 0; r < EMB_ROWS; ++r) {
+    for (int r = 0; r < ROWS; ++r) {
         const bool live = base + r * 64 + lane < N;
         const uint32_t d = (key[r] >> shift) & ((1u << bits) - 1);
         const uint64_t m = same_digit(d, bits, live);
@@ -95,23 +95,23 @@ __device__ __forceinline__ void embed_count(const I *tokens, const uint32_t *key
     }
 }
 
-template <typename I>
+template <typename I, int ROWS>
 __global__ void __launch_bounds__(EMB_SORT_THREADS) embed_hist_kernel(const I *tokens, const uint32_t *keys, int64_t N, uint32_t V,
                                                                       int shift, int bits, uint32_t *hist) {
     extern __shared__ uint32_t cnt[];
     const int nb = 1 << bits;
     for (int b = threadIdx.x; b < nb; b += EMB_SORT_THREADS) cnt[b] = 0;
     __syncthreads();
-    uint32_t key[EMB_ROWS];
-    const int64_t base = (int64_t)blockIdx.x * EMB_SORT_ITEMS + (threadIdx.x >> 6) * (EMB_ROWS * 64);
-    embed_count<I, false>(tokens, keys, base, N, V, shift, bits, cnt, key, nullptr);
+    uint32_t key[ROWS];
+    const int64_t base = ((int64_t)blockIdx.x * (EMB_SORT_THREADS / 64) + (threadIdx.x >> 6)) * (ROWS * 64);
+    embed_count<I, ROWS, false>(tokens, keys, base, N, V, shift, bits, cnt, key, nullptr);
     __syncthreads();
     for (int b = threadIdx.x; b < nb; b += EMB_SORT_THREADS) hist[(size_t)blockIdx.x * nb + b] = cnt[b];
 }
 
 // Every workgroup forms its own offsets from the histograms of all of them (nblk * 2^bits counters, L2-resident): one launch less
 // per pass than a scan kernel in between.  nblk == 1 needs no histogram at all.
-template <typename I>
+template <typename I, int ROWS>
 __global__ void __launch_bounds__(EMB_SORT_THREADS) embed_scatter_kernel(const I *tokens, const uint32_t *keys, const uint32_t *idx,
                                                                          int64_t N, uint32_t V, int shift, int bits,
                                                                          const uint32_t *hist, int nblk, uint32_t *keys_out,
@@ -119,13 +119,18 @@ __global__ void __launch_bounds__(EMB_SORT_THREADS) embed_scatter_kernel(const I
     extern __shared__ uint32_t lds[];
     const int nb = 1 << bits, nw = EMB_SORT_THREADS / 64;
     uint32_t *cnt = lds;                // [waves][nb]: counts, then the first position of (wave, digit)
-    uint32_t *part = lds + nw * nb;     // [EMB_SORT_THREADS] partial sums of the scan over digits
+    uint32_t *part = lds + nw * nb;     // [waves] sums of the scan over digits
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     for (int b = tid; b < nw * nb; b += EMB_SORT_THREADS) cnt[b] = 0;
     __syncthreads();
-    uint32_t key[EMB_ROWS], rank[EMB_ROWS];
-    const int64_t base = (int64_t)blockIdx.x * EMB_SORT_ITEMS + wave * (EMB_ROWS * 64);
-    embed_count<I, true>(tokens, keys, base, N, V, shift, bits, cnt + wave * nb, key, rank);
+    uint32_t key[ROWS], rank[ROWS], from[ROWS];
+    const int64_t base = ((int64_t)blockIdx.x * nw + wave) * (ROWS * 64);
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        const int64_t i = base + r * 64 + lane;
+        from[r] = idx && i < N ? idx[i] : (uint32_t)i;
+    }
+    embed_count<I, ROWS, true>(tokens, keys, base, N, V, shift, bits, cnt + wave * nb, key, rank);
     __syncthreads();
     const int per = (nb + EMB_SORT_THREADS - 1) / EMB_SORT_THREADS;       // digits per thread: 1 or 2
     uint32_t total[2] = {0, 0}, before[2] = {0, 0}, sum = 0;
@@ -136,23 +141,29 @@ __global__ void __launch_bounds__(EMB_SORT_THREADS) embed_scatter_kernel(const I
         if (nblk == 1) {
             for (int w = 0; w < nw; ++w) total[j] += cnt[w * nb + b];
         } else {
-            for (int k = 0; k < nblk; ++k) {
-                const uint32_t h = hist[(size_t)k * nb + b];
-                if (k < (int)blockIdx.x) before[j] += h;
-                total[j] += h;
+            constexpr int U = 16;                              // counters in flight
+            for (int k = 0; k < nblk; k += U) {
+                uint32_t h[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) h[u] = k + u < nblk ? hist[(size_t)(k + u) * nb + b] : 0;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    before[j] += k + u < (int)blockIdx.x ? h[u] : 0;
+                    total[j] += h[u];
+                }
             }
         }
         sum += total[j];
     }
-    part[tid] = sum;
-    __syncthreads();
-    for (int off = 1; off < EMB_SORT_THREADS; off <<= 1) {
-        const uint32_t v = tid >= off ? part[tid - off] : 0;
-        __syncthreads();
-        part[tid] += v;
-        __syncthreads();
+    uint32_t incl = sum;                                       // inclusive scan over the wave, then over the waves
+    for (int off = 1; off < 64; off <<= 1) {
+        const uint32_t v = __shfl_up(incl, off);
+        if (lane >= off) incl += v;
     }
-    uint32_t start = part[tid] - sum;
+    if (lane == 63) part[wave] = incl;
+    __syncthreads();
+    uint32_t start = incl - sum;
+    for (int w = 0; w < wave; ++w) start += part[w];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const int b = tid * per + j;
@@ -167,13 +178,13 @@ __global__ void __launch_bounds__(EMB_SORT_THREADS) embed_scatter_kernel(const I
     }
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < EMB_ROWS; ++r) {
+    for (int r = 0; r < ROWS; ++r) {
         const int64_t i = base + r * 64 + lane;
         if (i >= N) continue;
         const uint32_t d = (key[r] >> shift) & (nb - 1);
         const uint32_t at = cnt[wave * nb + d] + rank[r];
         keys_out[at] = key[r];
-        idx_out[at] = idx ? idx[i] : (uint32_t)i;
+        idx_out[at] = from[r];
     }
 }
 
@@ -275,47 +286,92 @@ __global__ void __launch_bounds__(256) embed_reduce_kernel(const uint32_t *keys,
     else finish();
 }
 
-// One workgroup per chunk in which a run starts that goes on: tail[c] + head[c + 1] + ... of that run.  Groups of lanes stride over
-// the parts and meet in LDS in a fixed order.
+// Runs that go on past their chunk: tail[c] + head[c + 1] + ... of the run that starts in chunk c.  A workgroup looks after 32 chunks:
+// first every group of lanes adds up runs of up to eight parts by itself, then all of them together stride over each longer one and
+// meet in LDS.  Every order of addition is fixed by the sizes.
 template <typename T, int VE>
-__global__ void __launch_bounds__(256) embed_join_kernel(const uint32_t *keys, uint32_t N, uint32_t V, int D, int lsh, float scale,
+__global__ void __launch_bounds__(512) embed_join_kernel(const uint32_t *keys, uint32_t N, uint32_t V, int D, int lsh, float scale,
                                                          T *dw, int64_t ldd, const float *head, const float *tail) {
-    extern __shared__ float sums[];                    // [256][VE]
-    const uint32_t chunk = blockIdx.x, a = chunk * EMB_CHUNK, b = a + EMB_CHUNK;
-    if (b >= N) return;
-    const uint32_t k = keys[b - 1];
-    if (k >= V || keys[b] != k || (a > 0 && keys[a - 1] == k)) return;      // uniform: no run starts here and goes on
-    const uint32_t last = (embed_upper(keys, b, N, k) - 1) / EMB_CHUNK;
-    const int lanes = 1 << lsh, groups = 256 >> lsh, grp = threadIdx.x >> lsh;
+    extern __shared__ float sums[];                    // [512][VE]
+    __shared__ uint32_t long_chunk[EMB_JOIN_CHUNKS];
+    __shared__ int longs;
+    const int lanes = 1 << lsh, groups = 512 >> lsh, grp = threadIdx.x >> lsh;
     const int c = (blockIdx.y * lanes + (threadIdx.x & (lanes - 1))) * VE;
-    float acc[VE];
-#pragma unroll
-    for (int e = 0; e < VE; ++e) acc[e] = grp == 0 && c < D ? tail[(size_t)chunk * D + c + e] : 0.0f;
-    if (c < D) {
-        constexpr int U = 4;
-        for (uint32_t j = chunk + 1 + grp; j <= last; j += groups * U) {
-            float h[U][VE];
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int e = 0; e < VE; ++e) h[u][e] = j + u * groups <= last ? head[(size_t)(j + u * groups) * D + c + e] : 0.0f;
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int e = 0; e < VE; ++e) acc[e] += h[u][e];
+    if (threadIdx.x < 64) {                            // the first wave looks for the runs
+        const uint64_t chunk = (uint64_t)blockIdx.x * EMB_JOIN_CHUNKS + threadIdx.x, a = chunk * EMB_CHUNK, b = a + EMB_CHUNK;
+        bool starts = false, more = false;
+        if (threadIdx.x < EMB_JOIN_CHUNKS && b < N) {
+            const uint32_t k = keys[b - 1];
+            starts = k < V && keys[b] == k && !(a > 0 && keys[a - 1] == k);
+            const uint64_t far = b + (uint64_t)EMB_JOIN_SHORT * EMB_CHUNK;
+            more = starts && far < N && keys[far] == k;
+        }
+        const uint64_t m = __ballot(more), s = __ballot(starts);
+        if (threadIdx.x < EMB_JOIN_CHUNKS) {
+            long_chunk[threadIdx.x] = starts ? (more ? 2u : 1u) : 0u;
+            if (threadIdx.x == 0) longs = s ? __popcll(m) : -1;
         }
     }
-#pragma unroll
-    for (int e = 0; e < VE; ++e) sums[threadIdx.x * VE + e] = acc[e];
     __syncthreads();
-    if (grp != 0 || c >= D) return;
-    for (int g = 1; g < groups; ++g)
+    if (longs < 0) return;
+    auto finish = [&](uint32_t k, const float *acc) {
+        Pack<T, VE> o;
 #pragma unroll
-        for (int e = 0; e < VE; ++e) acc[e] += sums[(g * lanes + threadIdx.x) * VE + e];
-    Pack<T, VE> o;
+        for (int e = 0; e < VE; ++e) o.v[e] = from_f32<T>(acc[e] * scale);
+        *(Pack<T, VE> *)(dw + (int64_t)k * ldd + c) = o;
+    };
+    for (int j = grp; j < EMB_JOIN_CHUNKS; j += groups) {
+        if (long_chunk[j] != 1 || c >= D) continue;
+        const uint32_t chunk = blockIdx.x * EMB_JOIN_CHUNKS + j, b = (chunk + 1) * EMB_CHUNK, k = keys[b];
+        float h[EMB_JOIN_SHORT][VE], acc[VE];
+        bool in[EMB_JOIN_SHORT];
 #pragma unroll
-    for (int e = 0; e < VE; ++e) o.v[e] = from_f32<T>(acc[e] * scale);
-    *(Pack<T, VE> *)(dw + (int64_t)k * ldd + c) = o;
+        for (int u = 0; u < EMB_JOIN_SHORT; ++u) in[u] = (uint64_t)b + u * EMB_CHUNK < N && keys[b + u * EMB_CHUNK] == k;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) acc[e] = tail[(size_t)chunk * D + c + e];
+#pragma unroll
+        for (int u = 0; u < EMB_JOIN_SHORT; ++u)
+#pragma unroll
+            for (int e = 0; e < VE; ++e) h[u][e] = in[u] ? head[(size_t)(chunk + 1 + u) * D + c + e] : 0.0f;
+#pragma unroll
+        for (int u = 0; u < EMB_JOIN_SHORT; ++u)
+#pragma unroll
+            for (int e = 0; e < VE; ++e) acc[e] += h[u][e];
+        finish(k, acc);
+    }
+    if (longs == 0) return;
+    for (int j = 0; j < EMB_JOIN_CHUNKS; ++j) {
+        if (long_chunk[j] != 2) continue;              // the same for the whole workgroup
+        const uint32_t chunk = blockIdx.x * EMB_JOIN_CHUNKS + j, b = (chunk + 1) * EMB_CHUNK, k = keys[b];
+        const uint32_t last = (embed_upper(keys, b, N, k) - 1) / EMB_CHUNK;
+        float acc[VE];
+#pragma unroll
+        for (int e = 0; e < VE; ++e) acc[e] = grp == 0 && c < D ? tail[(size_t)chunk * D + c + e] : 0.0f;
+        if (c < D) {
+            constexpr int U = 8;
+            for (uint32_t q = chunk + 1 + grp; q <= last; q += groups * U) {
+                float h[U][VE];
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) h[u][e] = q + u * groups <= last ? head[(size_t)(q + u * groups) * D + c + e] : 0.0f;
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) acc[e] += h[u][e];
+            }
+        }
+        __syncthreads();                               // the sums of the run before have been read
+#pragma unroll
+        for (int e = 0; e < VE; ++e) sums[threadIdx.x * VE + e] = acc[e];
+        __syncthreads();
+        if (grp == 0 && c < D) {
+            for (int g = 1; g < groups; ++g)
+#pragma unroll
+                for (int e = 0; e < VE; ++e) acc[e] += sums[(g * lanes + threadIdx.x) * VE + e];
+            finish(k, acc);
+        }
+    }
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------
@@ -338,14 +394,17 @@ static int lane_shift(int D, int ve, int most) {
     return s;
 }
 
-struct EmbedSort { int bits, passes, nblk; };
+struct EmbedSort { int bits, passes, rows, nblk; };
 static EmbedSort embed_sort_plan(int64_t N, int64_t V) {
     EmbedSort p;
     int need = 1;
     while (((int64_t)1 << need) <= V) ++need;          // keys 0 .. V
     p.passes = (need + EMB_MAX_BITS - 1) / EMB_MAX_BITS;
     p.bits = (need + p.passes - 1) / p.passes;
-    p.nblk = (int)((N + EMB_SORT_ITEMS - 1) / EMB_SORT_ITEMS);
+    // four rows per wave while every workgroup can still read all histograms quickly, sixteen beyond
+    p.rows = N <= (1 << 18) ? 4 : 16;
+    const int64_t items = EMB_SORT_THREADS * p.rows;
+    p.nblk = (int)((N + items - 1) / items);
     return p;
 }
 
@@ -380,23 +439,28 @@ static int embed_forward_typed(const void *tokens, int tb, int64_t N, const void
     return embed_forward_run<T, VE, int32_t>((const int32_t *)tokens, N, (const T *)w, ldw, V, D, scale, (T *)out, ldo, s);
 }
 
-template <typename I>
-static int embed_sort(const I *tokens, int64_t N, uint32_t V, const EmbedSort &p, uint32_t *keys[2], uint32_t *idx[2], uint32_t *hist,
-                      hipStream_t s) {
+template <typename I, int ROWS>
+static int embed_sort_rows(const I *tokens, int64_t N, uint32_t V, const EmbedSort &p, uint32_t *keys[2], uint32_t *idx[2], uint32_t *hist,
+                           hipStream_t s) {
     for (int pass = 0; pass < p.passes; ++pass) {
         const uint32_t *kin = pass ? keys[(pass + 1) & 1] : nullptr, *iin = pass ? idx[(pass + 1) & 1] : nullptr;
         const size_t nb = (size_t)1 << p.bits;
         if (p.nblk > 1) {
-            hipLaunchKernelGGL((embed_hist_kernel<I>), dim3(p.nblk), dim3(EMB_SORT_THREADS), nb * 4, s, tokens, kin, N, V, pass * p.bits, p.bits,
-                               hist);
+            hipLaunchKernelGGL((embed_hist_kernel<I, ROWS>), dim3(p.nblk), dim3(EMB_SORT_THREADS), nb * 4, s, tokens, kin, N, V, pass * p.bits,
+                               p.bits, hist);
             TNP_HIP(hipGetLastError());
         }
-        const size_t smem = (EMB_SORT_THREADS / 64 * nb + EMB_SORT_THREADS) * 4;
-        hipLaunchKernelGGL((embed_scatter_kernel<I>), dim3(p.nblk), dim3(EMB_SORT_THREADS), smem, s, tokens, kin, iin, N, V, pass * p.bits,
+        const size_t smem = (EMB_SORT_THREADS / 64 * nb + EMB_SORT_THREADS / 64) * 4;
+        hipLaunchKernelGGL((embed_scatter_kernel<I, ROWS>), dim3(p.nblk), dim3(EMB_SORT_THREADS), smem, s, tokens, kin, iin, N, V, pass * p.bits,
                            p.bits, hist, p.nblk, keys[pass & 1], idx[pass & 1]);
         TNP_HIP(hipGetLastError());
     }
     return 0;
+}
+template <typename I>
+static int embed_sort(const I *tokens, int64_t N, uint32_t V, const EmbedSort &p, uint32_t *keys[2], uint32_t *idx[2], uint32_t *hist,
+                      hipStream_t s) {
+    return p.rows == 4 ? embed_sort_rows<I, 4>(tokens, N, V, p, keys, idx, hist, s) : embed_sort_rows<I, 16>(tokens, N, V, p, keys, idx, hist, s);
 }
 
 template <typename T, int VE>
@@ -411,8 +475,8 @@ static int embed_sums(const uint32_t *keys, const uint32_t *idx, uint32_t N, uin
                        scale, dw, ldd, head, tail, sum_blocks);
     TNP_HIP(hipGetLastError());
     if (chunks > 1) {
-        hipLaunchKernelGGL((embed_join_kernel<T, VE>), dim3(chunks - 1, cols), dim3(256), 256 * VE * 4, s, keys, N, V, D, lsh, scale, dw, ldd,
-                           head, tail);
+        hipLaunchKernelGGL((embed_join_kernel<T, VE>), dim3((chunks + EMB_JOIN_CHUNKS - 1) / EMB_JOIN_CHUNKS, cols), dim3(512), 512 * VE * 4, s,
+                           keys, N, V, D, lsh, scale, dw, ldd, head, tail);
         TNP_HIP(hipGetLastError());
     }
     return 0;

@@ -433,13 +433,14 @@ __global__ void __launch_bounds__(256) ce_rows_kernel(const float2 *part, int64_
         __syncthreads();
     }
     if (threadIdx.x == 0) {
-        sums[blockIdx.x] = tot[0];
-        __threadfence();
-        last = atomicAdd(&sc->ticket, 1u) == gridDim.x - 1;
+        // written through to where every XCD reads it, and there before the ticket is drawn: no cache has to be flushed
+        __hip_atomic_store(&sums[blockIdx.x].x, tot[0].x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(&sums[blockIdx.x].y, tot[0].y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        last = __hip_atomic_fetch_add(&sc->ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
     }
     __syncthreads();
     if (!last) return;
-    __threadfence();
     mine = make_double2(0.0, 0.0);
     for (unsigned k = threadIdx.x; k < gridDim.x; k += 256) {
         const double2 v = make_double2(__hip_atomic_load(&sums[k].x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
@@ -491,39 +492,41 @@ __device__ __forceinline__ float ce_unscale(const CeScalars *sc, const float *gr
 
 struct CeGrad {
     GemmOperand g, o;         // G and the other operand (weight or hidden states)
-    const CeScalars *sc;
-    const float *grad;
-    const int64_t *target;    // dhidden: rows with a negative target are zero
-    int reduction;
     int64_t rows, out0;       // output rows of this call, the first one's index in the output
-    int D, tiles_r, tiles_d, steps, splits;
+    int tiles_r, tiles_d, steps, splits, blocks;
     int64_t ok0;              // first row of the other operand
-    void *out;                // final output (splits == 1, single piece)
-    int64_t ldo;
+    void *out;                // final output (nothing to add up), [..][D]
     float *part;              // [splits][part_rows][D] sums, or NULL
     int64_t part_rows;
     int add;                  // part += (later pieces of the vocabulary)
 };
+struct CeGrads {
+    CeGrad x, w;              // dhidden, dweight
+    const CeScalars *sc;
+    const float *grad;
+    const int64_t *target;    // dhidden: rows with a negative target are zero
+    int reduction, D;
+    // column sums of G (dbias): 512 stored columns x a share of the rows per workgroup
+    int64_t g_rows, g_cols, ldb;
+    int col_blocks, shares;
+    float *part_b;            // [shares][ldb]
+};
 
 // WEIGHT: dweight (G read transposed, output rows = vocabulary entries in G's stored column order), else dhidden
 template <typename T, bool SPLIT, bool WEIGHT, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(WM *WN * 64, 2) ce_grad_kernel(CeGrad a) {
+__device__ __forceinline__ void ce_grad_tile(const CeGrads &a, const CeGrad &c, int bid, char *lds) {
     constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
-    extern __shared__ __attribute__((aligned(1024))) char lds[];
     int tr, td;
-    const int per = (a.tiles_r * a.tiles_d + 7) / 8 * 8, z = blockIdx.x / per;
-    if (!gemm_tile_of(blockIdx.x - z * per, a.tiles_r, a.tiles_d, tr, td)) return;
+    const int per = (c.tiles_r * c.tiles_d + 7) / 8 * 8, z = bid / per;
+    if (!gemm_tile_of(bid - z * per, c.tiles_r, c.tiles_d, tr, td)) return;
     const int64_t r0 = (int64_t)tr * BM;
     const int d0 = td * BN;
-    const int s0 = (int)((int64_t)a.steps * z / a.splits), s1 = (int)((int64_t)a.steps * (z + 1) / a.splits);
+    const int s0 = (int)((int64_t)c.steps * z / c.splits), s1 = (int)((int64_t)c.steps * (z + 1) / c.splits);
     f32x16 acc[TM][TN];
-    if (WEIGHT)
-        gemm_tile<SPLIT, true, true, BM, BN, WM, WN>(a.g, a.o, r0, 0, d0, a.ok0, s0, s1, lds, acc);
-    else
-        gemm_tile<SPLIT, false, true, BM, BN, WM, WN>(a.g, a.o, r0, 0, d0, a.ok0, s0, s1, lds, acc);
+    gemm_tile<SPLIT, WEIGHT, true, BM, BN, WM, WN>(c.g, c.o, r0, 0, d0, c.ok0, s0, s1, lds, acc);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
     const int wm = wave / WN, wn = wave % WN;
-    const float f = a.part ? 1.0f : ce_unscale(a.sc, a.grad, a.reduction, WEIGHT ? a.sc->ex : a.sc->ew);
+    const float f = c.part ? 1.0f : ce_unscale(a.sc, a.grad, a.reduction, WEIGHT ? a.sc->ex : a.sc->ew);
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -531,52 +534,37 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) ce_grad_kernel(CeGrad a) {
             const int pos = (e & 3) + 8 * (e >> 2) + 4 * h;
             const int loc = WEIGHT ? (pos & ~12) | ((pos & 4) << 1) | ((pos & 8) >> 1) : pos;
             const int64_t row = r0 + wm * TM * 32 + i * 32 + loc;
-            if (row >= a.rows) continue;
-            const bool live = WEIGHT || a.part || a.target[row] >= 0;
+            if (row >= c.rows) continue;
+            const bool live = WEIGHT || c.part || a.target[row] >= 0;
 #pragma unroll
             for (int j = 0; j < TN; ++j) {
                 const int d = d0 + wn * TN * 32 + j * 32 + (lane & 31);
                 if (d >= a.D) continue;
                 const float v = acc[i][j][e];
-                if (a.part) {
-                    float *p = a.part + ((int64_t)z * a.part_rows + row) * a.D + d;
-                    *p = a.add ? *p + v : v;
+                if (c.part) {
+                    float *p = c.part + ((int64_t)z * c.part_rows + row) * a.D + d;
+                    *p = c.add ? *p + v : v;
                 } else {
-                    ((T *)a.out)[(a.out0 + row) * a.ldo + d] = from_f32<T>(live ? v * f : 0.0f);
+                    ((T *)c.out)[(c.out0 + row) * a.D + d] = from_f32<T>(live ? v * f : 0.0f);
                 }
             }
         }
 }
 
-// out[r][d] = factor * sum over splits of part[s][r][d], the splits in their order
-template <typename T>
-__global__ void __launch_bounds__(256) ce_join_kernel(const float *part, int64_t rows, int64_t part_rows, int splits, int D, const CeScalars *sc,
-                                                      const float *grad, int reduction, int weight, const int64_t *target, T *out,
-                                                      int64_t ldo) {
-    const float f = ce_unscale(sc, grad, reduction, weight ? sc->ex : sc->ew);
-    const int64_t n = rows * D, stride = part_rows * D;
-    for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < n; k += (int64_t)gridDim.x * 256) {
-        const int64_t row = k / D;
-        float v = 0.0f;
-        for (int s = 0; s < splits; ++s) v += part[s * stride + k];
-        out[row * ldo + (k - row * D)] = from_f32<T>(weight || target[row] >= 0 ? v * f : 0.0f);
-    }
-}
-
-// column sums of G (dbias): a lane owns eight stored columns, a workgroup a share of the rows
-__global__ void __launch_bounds__(256) ce_colsum_kernel(const half_t *g, int64_t ldg, int64_t rows, int64_t cols, float *part, int64_t ldp) {
-    __shared__ float sh[3][64][8];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t c = (int64_t)blockIdx.x * 512 + lane * 8;
-    const int64_t per = (rows + gridDim.y - 1) / gridDim.y, r0 = blockIdx.y * per, r1 = r0 + per < rows ? r0 + per : rows;
+// a lane owns eight stored columns, the waves of the workgroup share the rows
+template <int NW> __device__ __forceinline__ void ce_colsum(const CeGrads &a, int bid, char *lds) {
+    float(*sh)[64][8] = (float(*)[64][8])lds;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, cb = bid / a.shares, share = bid % a.shares;
+    const int64_t c = (int64_t)cb * 512 + lane * 8;
+    const int64_t per = (a.g_rows + a.shares - 1) / a.shares, r0 = share * per, r1 = r0 + per < a.g_rows ? r0 + per : a.g_rows;
     float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (c < cols) {
-        constexpr int U = 4;
-        for (int64_t r = r0 + wave; r < r1; r += 4 * U) {
+    if (c < a.g_cols) {
+        constexpr int U = 8;
+        for (int64_t r = r0 + wave; r < r1; r += NW * U) {
             half8 v[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (r + 4 * u < r1) v[u] = *(const half8 *)(g + (r + 4 * u) * ldg + c);
+                if (r + NW * u < r1) v[u] = *(const half8 *)(a.x.g.p + (r + NW * u) * a.x.g.ld + c);
                 else
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[u][e] = (half_t)0.0f;
@@ -587,27 +575,80 @@ __global__ void __launch_bounds__(256) ce_colsum_kernel(const half_t *g, int64_t
                 for (int e = 0; e < 8; ++e) s[e] += (float)v[u][e];
         }
     }
-    if (wave)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sh[wave - 1][lane][e] = s[e];
+    for (int e = 0; e < 8; ++e) sh[wave][lane][e] = s[e];
     __syncthreads();
-    if (wave == 0 && c < cols)
+    if (wave == 0 && c < a.g_cols)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) part[blockIdx.y * ldp + c + e] = s[e] + sh[0][lane][e] + sh[1][lane][e] + sh[2][lane][e];
+        for (int e = 0; e < 8; ++e) {
+            float t = sh[0][lane][e];
+            for (int w = 1; w < NW; ++w) t += sh[w][lane][e];
+            a.part_b[share * a.ldb + c + e] = t;
+        }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) ce_dbias_kernel(const float *part, int64_t ldp, int shares, int split, int n, const CeScalars *sc,
-                                                       const float *grad, int reduction, T *out) {
-    const int v = blockIdx.x * 256 + threadIdx.x;
-    if (v >= n) return;
-    const int pos = (v & ~12) | ((v & 4) << 1) | ((v & 8) >> 1);
-    float s = 0.0f;
-    for (int k = 0; k < shares; ++k) {
-        const float *p = part + k * ldp;
-        s += split ? p[(pos >> 5) * 64 + (pos & 31)] + p[(pos >> 5) * 64 + (pos & 31) + 32] : p[pos];
+// Both gradient products and the column sums in one launch: they read the same G, and the workgroups of one fill what the others
+// leave idle.
+template <typename T, bool SPLIT, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(WM *WN * 64, 2) ce_grads_kernel(CeGrads a) {
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    const int bid = blockIdx.x;
+    if (bid < a.x.blocks) ce_grad_tile<T, SPLIT, false, BM, BN, WM, WN>(a, a.x, bid, lds);
+    else if (bid < a.x.blocks + a.w.blocks) ce_grad_tile<T, SPLIT, true, BM, BN, WM, WN>(a, a.w, bid - a.x.blocks, lds);
+    else ce_colsum<WM * WN>(a, bid - a.x.blocks - a.w.blocks, lds);
+}
+
+// out[r][d] = factor * sum over splits of part[s][r][d], the splits in their order; VE elements per thread
+template <typename T, int VE>
+__device__ __forceinline__ void ce_join(const CeGrads &a, const CeGrad &c, bool weight, int bid) {
+    const int64_t n = c.rows * a.D, stride = c.part_rows * a.D, k = ((int64_t)bid * 256 + threadIdx.x) * VE;
+    if (k >= n) return;
+    const int64_t row = k / a.D;
+    float v[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) v[e] = 0.0f;
+    constexpr int U = 8;
+    for (int s = 0; s < c.splits; s += U) {
+        Pack<float, VE> p[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (s + u < c.splits) p[u] = *(const Pack<float, VE> *)(c.part + (s + u) * stride + k);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (s + u < c.splits)
+#pragma unroll
+                for (int e = 0; e < VE; ++e) v[e] += p[u].v[e];
     }
-    out[v] = from_f32<T>(s * ce_unscale(sc, grad, reduction, 0));
+    const float f = ce_unscale(a.sc, a.grad, a.reduction, weight ? a.sc->ex : a.sc->ew);
+    const bool live = weight || a.target[row] >= 0;
+    T *out = (T *)c.out + c.out0 * a.D + k;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) out[e] = from_f32<T>(live ? v[e] * f : 0.0f);
+}
+
+// what is left of a piece in one launch: dhidden and dweight from their partial sums (bx / bw workgroups), dbias
+template <typename T, int VE>
+__global__ void __launch_bounds__(256) ce_join_kernel(CeGrads a, int bx, int bw, int split, int live, T *dbias) {
+    const int bid = blockIdx.x;
+    if (bid < bx) { ce_join<T, VE>(a, a.x, false, bid); return; }
+    if (bid < bx + bw) { ce_join<T, VE>(a, a.w, true, bid - bx); return; }
+    // 32 entries per workgroup, eight threads share the row shares of each
+    __shared__ float sh[8][32];
+    const int seg = threadIdx.x >> 5, v = (bid - bx - bw) * 32 + (threadIdx.x & 31);
+    float s = 0.0f;
+    if (v < live) {
+        const int pos = (v & ~12) | ((v & 4) << 1) | ((v & 8) >> 1);
+        for (int k = seg; k < a.shares; k += 8) {
+            const float *p = a.part_b + k * a.ldb;
+            s += split ? p[(pos >> 5) * 64 + (pos & 31)] + p[(pos >> 5) * 64 + (pos & 31) + 32] : p[pos];
+        }
+    }
+    sh[seg][threadIdx.x & 31] = s;
+    __syncthreads();
+    if (seg == 0 && v < live) {
+        for (int k = 1; k < 8; ++k) s += sh[k][threadIdx.x];
+        dbias[v] = from_f32<T>(s * ce_unscale(a.sc, a.grad, a.reduction, 0));
+    }
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------
@@ -662,23 +703,18 @@ static CeForward ce_forward_layout(const tnp_vocab_ce *p, void *ws) {
     return f;
 }
 
-// columns of G that are formed at a time, and the splits of the two gradient products
+// columns of G that are formed at a time, and the tiles and splits of the two gradient products
 struct CeBackward {
     int piece, pieces;
     int64_t ldg;
     half_t *g;
-    int big, hidden_bn, splits_x, splits_w;
+    int bm, bn, splits_x, splits_w;
     float *part_x, *part_w, *part_b;
     int shares;
     size_t bytes;
 };
 static constexpr size_t CE_PIECE_BYTES = (size_t)512 << 20;
 
-static int ce_splits(int64_t tiles, int steps, int target) {
-    int64_t n = target / tiles;
-    if (n > steps / 4) n = steps / 4;
-    return n < 1 ? 1 : (int)n;
-}
 static CeBackward ce_backward_layout(const tnp_vocab_ce *p, void *ws) {
     CeBackward b;
     const CeShape s = ce_shape(p);
@@ -689,10 +725,20 @@ static CeBackward ce_backward_layout(const tnp_vocab_ce *p, void *ws) {
     b.piece = (int)ce_pad((s.Vp + b.pieces - 1) / b.pieces, 256);
     b.pieces = (s.Vp + b.piece - 1) / b.piece;
     b.ldg = (int64_t)b.piece * planes;
-    const int64_t td = (p->D + 127) / 128;
-    b.splits_x = ce_splits(s.Mp / 128 * td, b.piece / ks, 512);
-    b.splits_w = ce_splits((int64_t)b.piece / 128 * td, (int)(s.Mp / ks), 512);
-    b.shares = (int)(s.Mp / 256 < 64 ? s.Mp / 256 : 64);
+    // tiles of 256 rows once they alone are a round of workgroups, 256 columns where there are as many
+    const int64_t td = (p->D + 127) / 128, small_x = s.Mp / 128 * td, small_w = b.piece / 128 * td;
+    const int sx = b.piece / ks, sw = (int)(s.Mp / ks);
+    const bool big = small_x * sx + small_w * sw >= 65536;
+    b.bm = big ? 256 : 128;
+    b.bn = big && p->D > 128 ? 256 : 128;
+    // both products share a launch: every workgroup gets about the same number of steps, at least 8
+    const int64_t tx = s.Mp / b.bm * ((p->D + b.bn - 1) / b.bn), tw = (b.piece + b.bm - 1) / b.bm * ((p->D + b.bn - 1) / b.bn);
+    int64_t each = (tx * sx + tw * sw) / (b.bm == 256 ? 256 : 512);
+    if (each < 8) each = 8;
+    const int64_t nx = (sx + each / 2) / each, nw = (sw + each / 2) / each;
+    b.splits_x = (int)(nx < 1 ? 1 : nx);
+    b.splits_w = (int)(nw < 1 ? 1 : nw);
+    b.shares = (int)(s.Mp / 128 < 64 ? s.Mp / 128 : 64);
     char *w = (char *)ws;
     b.g = (half_t *)w; w += ce_up((size_t)s.Mp * b.ldg * 2);
     b.part_x = b.splits_x > 1 || b.pieces > 1 ? (float *)w : nullptr;
@@ -748,17 +794,22 @@ static int ce_logits(const CeLogits &a, int64_t cols, bool big, const T *bias, h
     return big ? ce_launch_logits<T, SPLIT, BACK, 256, 256, 2, 4>(a, cols, bias, s) : ce_launch_logits<T, SPLIT, BACK, 128, 128, 2, 2>(a, cols, bias, s);
 }
 
-template <typename T, bool SPLIT, bool WEIGHT>
-static int ce_grad(CeGrad a, hipStream_t s) {
-    constexpr int BM = 128, BN = 128, WM = 2, WN = 2;
-    a.tiles_r = (int)((a.rows + BM - 1) / BM);
-    a.tiles_d = (a.D + BN - 1) / BN;
+template <typename T, bool SPLIT, int BM, int BN, int WM, int WN>
+static int ce_launch_grads(CeGrads &a, hipStream_t s) {
     const size_t smem = 2 * (BM + BN) * 128;
     static size_t done[VOCAB_MAX_DEVICES] = {0};
-    auto kern = ce_grad_kernel<T, SPLIT, WEIGHT, BM, BN, WM, WN>;
+    auto kern = ce_grads_kernel<T, SPLIT, BM, BN, WM, WN>;
     if (int rc = ce_lds(kern, smem, done)) return rc;
-    hipLaunchKernelGGL(kern, dim3(gemm_grid((int64_t)a.tiles_r * a.tiles_d) * a.splits), dim3(WM * WN * 64), smem, s, a);
-    TNP_HIP(hipGetLastError());
+    for (CeGrad *c : {&a.x, &a.w}) {
+        c->tiles_r = (int)((c->rows + BM - 1) / BM);
+        c->tiles_d = (a.D + BN - 1) / BN;
+        c->blocks = c->out ? gemm_grid((int64_t)c->tiles_r * c->tiles_d) * c->splits : 0;
+    }
+    const int blocks = a.x.blocks + a.w.blocks + a.col_blocks * a.shares;
+    if (blocks) {
+        hipLaunchKernelGGL(kern, dim3(blocks), dim3(WM * WN * 64), smem, s, a);
+        TNP_HIP(hipGetLastError());
+    }
     return 0;
 }
 
@@ -835,44 +886,32 @@ static int ce_backward(const tnp_vocab_ce *p, const CeBackward &b, const float *
         a.w = w; a.x = x; a.sc = sv.sc; a.target = p->target; a.M = sh.M; a.Mp = sh.Mp; a.V = sh.V; a.v0 = v0; a.steps = sh.steps;
         a.lse = sv.lse; a.grad = p->reduction == 0 ? grad : nullptr; a.g = b.g; a.ldg = b.ldg;
         if ((rc = ce_logits<T, SPLIT, true>(a, cols, ce_big(sh), (const T *)p->bias, s))) return rc;
-        CeGrad c = {};
+        const bool last = k == b.pieces - 1;
+        const int ks = SPLIT ? 32 : 64;
+        CeGrads c = {};
         c.sc = sv.sc; c.grad = grad; c.target = p->target; c.reduction = p->reduction; c.D = sh.D;
-        if (dhidden) {
-            c.g = GemmOperand{b.g, b.ldg, sh.Mp, 0};
-            c.o = w; c.o.perm = 1; c.ok0 = v0;
-            c.rows = sh.M; c.out0 = 0; c.out = dhidden; c.ldo = sh.D; c.part = b.part_x; c.part_rows = sh.Mp; c.splits = b.splits_x;
-            c.steps = cols / (SPLIT ? 32 : 64); c.add = k > 0;
-            if ((rc = ce_grad<T, SPLIT, false>(c, s))) return rc;
-        }
-        if (dweight) {
-            c.g = GemmOperand{b.g, b.ldg, sh.Mp, 0};
-            c.o = x; c.ok0 = 0;
-            c.rows = live; c.out0 = v0; c.out = dweight; c.ldo = sh.D; c.part = b.part_w; c.part_rows = b.piece; c.splits = b.splits_w;
-            c.steps = (int)(sh.Mp / (SPLIT ? 32 : 64)); c.add = 0;
-            if ((rc = ce_grad<T, SPLIT, true>(c, s))) return rc;
-            if (b.part_w) {
-                const int64_t n = (int64_t)live * sh.D;
-                hipLaunchKernelGGL((ce_join_kernel<T>), dim3((unsigned)(n / 1024 + 1 < 4096 ? n / 1024 + 1 : 4096)), dim3(256), 0, s, b.part_w,
-                                   (int64_t)live, (int64_t)b.piece, b.splits_w, sh.D, sv.sc, grad, p->reduction, 1, p->target,
-                                   (T *)dweight + (int64_t)v0 * sh.D, (int64_t)sh.D);
-                TNP_HIP(hipGetLastError());
-            }
-        }
-        if (dbias) {
-            const int64_t stored = (int64_t)cols * (SPLIT ? 2 : 1);
-            hipLaunchKernelGGL(ce_colsum_kernel, dim3((unsigned)((stored + 511) / 512), b.shares), dim3(256), 0, s, b.g, b.ldg, sh.Mp, stored,
-                               b.part_b, b.ldg);
-            TNP_HIP(hipGetLastError());
-            hipLaunchKernelGGL((ce_dbias_kernel<T>), dim3((live + 255) / 256), dim3(256), 0, s, b.part_b, b.ldg, b.shares, (int)SPLIT, live, sv.sc,
-                               grad, p->reduction, (T *)dbias + v0);
+        c.x.g = c.w.g = GemmOperand{b.g, b.ldg, sh.Mp, 0};
+        c.x.o = w; c.x.o.perm = 1; c.x.ok0 = v0;
+        c.x.rows = sh.M; c.x.out = dhidden; c.x.part = b.part_x; c.x.part_rows = sh.Mp; c.x.splits = b.splits_x;
+        c.x.steps = cols / ks; c.x.add = k > 0;
+        c.w.o = x;
+        c.w.rows = live; c.w.out0 = v0; c.w.out = dweight; c.w.part = b.part_w; c.w.part_rows = b.piece; c.w.splits = b.splits_w;
+        c.w.steps = (int)(sh.Mp / ks);
+        c.shares = b.shares; c.part_b = b.part_b; c.ldb = b.ldg; c.g_rows = sh.Mp; c.g_cols = (int64_t)cols * (SPLIT ? 2 : 1);
+        c.col_blocks = dbias ? (int)((c.g_cols + 511) / 512) : 0;
+        rc = b.bm == 256 ? (b.bn == 256 ? ce_launch_grads<T, SPLIT, 256, 256, 2, 4>(c, s) : ce_launch_grads<T, SPLIT, 256, 128, 4, 2>(c, s))
+                         : ce_launch_grads<T, SPLIT, 128, 128, 2, 2>(c, s);
+        if (rc) return rc;
+        const int ve = sh.D % 4 == 0 ? 4 : 1;
+        const int64_t per = 256 * ve;
+        const int bx = dhidden && b.part_x && last ? (int)((c.x.rows * sh.D + per - 1) / per) : 0;
+        const int bw = dweight && b.part_w ? (int)((c.w.rows * sh.D + per - 1) / per) : 0, bb = dbias ? (live + 31) / 32 : 0;
+        if (bx + bw + bb) {
+            T *db = dbias ? (T *)dbias + v0 : nullptr;
+            if (ve == 4) hipLaunchKernelGGL((ce_join_kernel<T, 4>), dim3(bx + bw + bb), dim3(256), 0, s, c, bx, bw, (int)SPLIT, live, db);
+            else hipLaunchKernelGGL((ce_join_kernel<T, 1>), dim3(bx + bw + bb), dim3(256), 0, s, c, bx, bw, (int)SPLIT, live, db);
             TNP_HIP(hipGetLastError());
         }
-    }
-    if (dhidden && b.part_x) {
-        const int64_t n = sh.M * sh.D;
-        hipLaunchKernelGGL((ce_join_kernel<T>), dim3((unsigned)(n / 1024 + 1 < 4096 ? n / 1024 + 1 : 4096)), dim3(256), 0, s, b.part_x, sh.M, sh.Mp,
-                           b.splits_x, sh.D, sv.sc, grad, p->reduction, 0, p->target, (T *)dhidden, (int64_t)sh.D);
-        TNP_HIP(hipGetLastError());
     }
     return 0;
 }

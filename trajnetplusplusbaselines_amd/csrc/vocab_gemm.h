@@ -13,6 +13,8 @@
 #pragma once
 #include "vocab_types.h"
 
+#include <type_traits>
+
 namespace tnp {
 
 typedef half_t half8 __attribute__((ext_vector_type(8)));
@@ -84,20 +86,64 @@ template <bool KS, bool SPLIT, int BR, int NW> struct TileStage {
             const int r = r0 + (lane & 31), ch = (SPLIT ? plane * 4 : 0) + ss * 2 + (lane >> 5);
             return *(const half8 *)(lds + r * 128 + ((ch ^ ((r >> 1) & 7)) * 16));
         } else {
-            constexpr int CB = BR * 2 * (SPLIT ? 2 : 1);
-            const int g = lane >> 4, j = lane & 15;
-            const int row = ss * 16 + 8 * (g >> 1) + (j >> 2);
-            const int col = (SPLIT ? r0 * 2 + plane * 32 : r0) + 16 * (g & 1) + 4 * (j & 3);
-            const int b0 = row * CB + (((col >> 3) ^ ((row & 3) << 2)) * 16) + (col & 7) * 2;
-            // rows row and row + 4 share (row & 3), hence the swizzle
-            const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((TNP_LDS short4v *)(lds + b0));
-            const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((TNP_LDS short4v *)(lds + b0 + 4 * CB));
-            typedef short short8v __attribute__((ext_vector_type(8)));
-            const short8v v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-            return __builtin_bit_cast(half8, v);
+            return half8{};                                        // KS operands come through ks_frags
         }
     }
+    static constexpr int CB = BR * 2 * (SPLIT ? 2 : 1);            // bytes per k row of a KS tile
+    // KS: LDS byte address of the first value this lane fetches for 32 columns from c (stored), k rows 0 .. 3 of its half.  Rows
+    // row, row + 4, row + 16 share (row & 3), hence the swizzle: further rows are constant offsets.
+    static __device__ __forceinline__ uint32_t ks_addr(const char *lds, int c, int lane) {
+        const int g = lane >> 4, j = lane & 15, row = 8 * (g >> 1) + (j >> 2), col = c + 16 * (g & 1) + 4 * (j & 3);
+        return (uint32_t)(uintptr_t)(TNP_LDS const char *)lds + row * CB + (((col >> 3) ^ ((row & 3) << 2)) * 16) + (col & 7) * 2;
+    }
 };
+
+// Two 32-column blocks of a KS tile, k values 16 ss .. 16 ss + 15 (OFF = 16 ss rows in bytes).  One asm block that ends with its own
+// wait: as builtins these reads would first wait for every global_load_lds in flight, that is for the NEXT step's tile.
+template <int OFF, int CB>
+__device__ __forceinline__ void ks_read2(uint32_t a0, uint32_t a1, half8 &f0, half8 &f1) {
+    typedef int int2v __attribute__((ext_vector_type(2)));
+    typedef int int4v __attribute__((ext_vector_type(4)));
+    int2v p0, q0, p1, q1;
+    asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%c6\n\t"
+                 "ds_read_b64_tr_b16 %1, %4 offset:%c7\n\t"
+                 "ds_read_b64_tr_b16 %2, %5 offset:%c6\n\t"
+                 "ds_read_b64_tr_b16 %3, %5 offset:%c7\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(p0), "=&v"(q0), "=&v"(p1), "=&v"(q1)
+                 : "v"(a0), "v"(a1), "i"(OFF), "i"(OFF + 4 * CB)
+                 : "memory");
+    f0 = __builtin_bit_cast(half8, int4v{p0.x, p0.y, q0.x, q0.y});
+    f1 = __builtin_bit_cast(half8, int4v{p1.x, p1.y, q1.x, q1.y});
+}
+template <int OFF, int CB>
+__device__ __forceinline__ void ks_read4(uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, half8 &f0, half8 &f1, half8 &f2, half8 &f3) {
+    typedef int int2v __attribute__((ext_vector_type(2)));
+    typedef int int4v __attribute__((ext_vector_type(4)));
+    int2v p0, q0, p1, q1, p2, q2, p3, q3;
+    asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%c12\n\t"
+                 "ds_read_b64_tr_b16 %1, %8 offset:%c13\n\t"
+                 "ds_read_b64_tr_b16 %2, %9 offset:%c12\n\t"
+                 "ds_read_b64_tr_b16 %3, %9 offset:%c13\n\t"
+                 "ds_read_b64_tr_b16 %4, %10 offset:%c12\n\t"
+                 "ds_read_b64_tr_b16 %5, %10 offset:%c13\n\t"
+                 "ds_read_b64_tr_b16 %6, %11 offset:%c12\n\t"
+                 "ds_read_b64_tr_b16 %7, %11 offset:%c13\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(p0), "=&v"(q0), "=&v"(p1), "=&v"(q1), "=&v"(p2), "=&v"(q2), "=&v"(p3), "=&v"(q3)
+                 : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "i"(OFF), "i"(OFF + 4 * CB)
+                 : "memory");
+    f0 = __builtin_bit_cast(half8, int4v{p0.x, p0.y, q0.x, q0.y});
+    f1 = __builtin_bit_cast(half8, int4v{p1.x, p1.y, q1.x, q1.y});
+    f2 = __builtin_bit_cast(half8, int4v{p2.x, p2.y, q2.x, q2.y});
+    f3 = __builtin_bit_cast(half8, int4v{p3.x, p3.y, q3.x, q3.y});
+}
+// N = 2 or 4 blocks at the addresses a[0 .. N)
+template <int OFF, int CB, int N> __device__ __forceinline__ void ks_frags(const uint32_t (&a)[N], half8 (&f)[N]) {
+    static_assert(N == 2 || N == 4, "two or four blocks of 32 columns per wave");
+    if constexpr (N == 2) ks_read2<OFF, CB>(a[0], a[1], f[0], f[1]);
+    else ks_read4<OFF, CB>(a[0], a[1], a[2], a[3], f[0], f[1], f[2], f[3]);
+}
 
 // Accumulates steps [s0, s1) of tile (a at row / column a0, b at b0) into acc.  KC operands start at stored column ak0 / bk0, KS
 // operands at row ak0 / bk0.  LDS: 2 * (BM + BN) * 128 bytes.
@@ -130,41 +176,50 @@ __device__ __forceinline__ void gemm_tile(const GemmOperand &a, const GemmOperan
             sb.load(s + 1, nxt + BM * 128, wave, lane);
         }
         const char *la = cur, *lb = cur + BM * 128;
-        if (!SPLIT) {
+        constexpr int P = SPLIT ? 2 : 1, SS = SPLIT ? 2 : 4;
+        uint32_t aa[P][TM], ab[P][TN];                             // KS operands: LDS addresses
+        if (A_KS)
 #pragma unroll
-            for (int ss = 0; ss < 4; ++ss) {
-                half8 fa[TM], fb[TN];
+            for (int p = 0; p < P; ++p)
 #pragma unroll
-                for (int i = 0; i < TM; ++i) fa[i] = SA::frag(la, wm * TM * 32 + i * 32, ss, 0, lane);
+                for (int i = 0; i < TM; ++i) aa[p][i] = SA::ks_addr(la, (wm * TM + i) * 32 * P + p * 32, lane);
+        if (B_KS)
 #pragma unroll
-                for (int j = 0; j < TN; ++j) fb[j] = SB::frag(lb, wn * TN * 32 + j * 32, ss, 0, lane);
+            for (int p = 0; p < P; ++p)
 #pragma unroll
-                for (int i = 0; i < TM; ++i)
+                for (int j = 0; j < TN; ++j) ab[p][j] = SB::ks_addr(lb, (wn * TN + j) * 32 * P + p * 32, lane);
+        auto sub = [&](auto ssc) {
+            constexpr int ss = decltype(ssc)::value;
+            half8 fa[P][TM], fb[P][TN];
 #pragma unroll
-                    for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i], fb[j], acc[i][j], 0, 0, 0);
+            for (int p = 0; p < P; ++p) {
+                if constexpr (A_KS) ks_frags<ss * 16 * SA::CB, SA::CB, TM>(aa[p], fa[p]);
+                else
+#pragma unroll
+                    for (int i = 0; i < TM; ++i) fa[p][i] = SA::frag(la, (wm * TM + i) * 32, ss, p, lane);
+                if constexpr (B_KS) ks_frags<ss * 16 * SB::CB, SB::CB, TN>(ab[p], fb[p]);
+                else
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) fb[p][j] = SB::frag(lb, (wn * TN + j) * 32, ss, p, lane);
             }
-        } else {
 #pragma unroll
-            for (int ss = 0; ss < 2; ++ss) {
-                half8 fa[2][TM], fb[2][TN];
+            for (int i = 0; i < TM; ++i)
 #pragma unroll
-                for (int p = 0; p < 2; ++p) {
-#pragma unroll
-                    for (int i = 0; i < TM; ++i) fa[p][i] = SA::frag(la, wm * TM * 32 + i * 32, ss, p, lane);
-#pragma unroll
-                    for (int j = 0; j < TN; ++j) fb[p][j] = SB::frag(lb, wn * TN * 32 + j * 32, ss, p, lane);
-                }
-                // the small products first: they are not lost against the large ones
-#pragma unroll
-                for (int i = 0; i < TM; ++i)
-#pragma unroll
-                    for (int j = 0; j < TN; ++j) {
+                for (int j = 0; j < TN; ++j) {
+                    if constexpr (SPLIT) {                         // the small products first: they are not lost against the large ones
                         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[1][i], fb[0][j], acc[i][j], 0, 0, 0);
                         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][i], fb[1][j], acc[i][j], 0, 0, 0);
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][i], fb[0][j], acc[i][j], 0, 0, 0);
                     }
-            }
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][i], fb[0][j], acc[i][j], 0, 0, 0);
+                }
+        };
+        sub(std::integral_constant<int, 0>());
+        sub(std::integral_constant<int, 1>());
+        if constexpr (SS == 4) {
+            sub(std::integral_constant<int, 2>());
+            sub(std::integral_constant<int, 3>());
         }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");            // the next step's tile has landed
         __syncthreads();
     }
 }
