@@ -38,8 +38,7 @@ struct CeShape {
     int64_t M, Mp;            // rows, padded to 256
     int V, Vp, D;             // vocabulary, padded to 256
     int split;                // fp32: two planes
-    int64_t ld;               // stored elements per packed row
-    int steps;                // k steps of the logits
+    int panels;               // of 32 columns (16 split ones): k steps of the logits
 };
 
 // ---- scales and packing -----------------------------------------------------------------------------------------------------
@@ -88,36 +87,36 @@ __device__ __forceinline__ int ce_exponent(float a) {
     return e - 15;
 }
 
+// sixteen rows from r0 into panels (vocab_gemm.h): lane = (row, 16-byte chunk), so a panel is written as one contiguous kilobyte
 template <typename T, int VE, bool SPLIT>
-__device__ __forceinline__ void ce_pack_row(const T *src, bool live, int D, int e, half_t *dst, int64_t ld, int lane) {
-    // eight values per lane and trip; split rows hold 32 hi | 32 lo per block
-    const int per = SPLIT ? (int)ld / 2 : (int)ld;
-    for (int c = lane * 8; c < per; c += 512) {
-        float v[8];
+__device__ __forceinline__ void ce_pack_rows(const T *src, int64_t ld, int64_t r0, int64_t rows, const int64_t *target, int D, int e, half_t *dst,
+                                             int64_t panel_rows, int panels, int lane) {
+    constexpr int NV = 8;                                        // values per chunk; a split chunk is the hi or the lo half of eight
+    const int64_t r = r0 + (lane >> 2);
+    const bool live = r < rows && (!target || target[r] >= 0);
+    const int ch = lane & 3, c0 = SPLIT ? (ch & 1) * 8 : ch * 8;
+    half_t *out = dst + r * 32 + ch * 8;
+    for (int p = 0; p < panels; ++p, out += panel_rows * 32) {
+        const int c = p * (SPLIT ? 16 : 32) + c0;
+        float v[NV];
 #pragma unroll
-        for (int k = 0; k < 8; k += VE < 8 ? VE : 8) {
+        for (int k = 0; k < NV; k += VE) {
             if (live && c + k < D) {
-                const Pack<T, (VE < 8 ? VE : 8)> p = *(const Pack<T, (VE < 8 ? VE : 8)> *)(src + c + k);
+                const Pack<T, VE> q = *(const Pack<T, VE> *)(src + r * ld + c + k);
 #pragma unroll
-                for (int q = 0; q < (VE < 8 ? VE : 8); ++q) v[k + q] = ldexpf(to_f32(p.v[q]), -e);
+                for (int m = 0; m < VE; ++m) v[k + m] = ldexpf(to_f32(q.v[m]), -e);
             } else {
 #pragma unroll
-                for (int q = 0; q < (VE < 8 ? VE : 8); ++q) v[k + q] = 0.0f;
+                for (int m = 0; m < VE; ++m) v[k + m] = 0.0f;
             }
         }
-        half8 hi, lo;
+        half8 o;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            hi[k] = (half_t)v[k];
-            lo[k] = fabsf(v[k]) < 65504.0f ? (half_t)(v[k] - (float)hi[k]) : (half_t)0.0f;
+        for (int k = 0; k < NV; ++k) {
+            const half_t hi = (half_t)v[k];
+            o[k] = SPLIT && ch >= 2 ? (fabsf(v[k]) < 65504.0f ? (half_t)(v[k] - (float)hi) : (half_t)0.0f) : hi;
         }
-        if (SPLIT) {
-            half_t *o = dst + (c >> 5) * 64 + (c & 31);
-            *(half8 *)o = hi;
-            *(half8 *)(o + 32) = lo;
-        } else {
-            *(half8 *)(dst + c) = hi;
-        }
+        *(half8 *)out = o;
     }
 }
 
@@ -135,11 +134,11 @@ __global__ void __launch_bounds__(256) ce_pack_kernel(const T *x, int64_t ldx, c
     if (threadIdx.x == 0 && (blockIdx.x == 0 || (int)blockIdx.x == x_blocks)) (is_w ? sc->ew : sc->ex) = e;
     if (is_w) {
         const int blocks = gridDim.x - x_blocks;
-        for (int64_t r = ((int)blockIdx.x - x_blocks) * 4 + wave; r < sh.Vp; r += blocks * 4)
-            ce_pack_row<T, VW, SPLIT>(w + r * ldw, r < sh.V, sh.D, e, wp + r * sh.ld, sh.ld, lane);
+        for (int64_t r = ((int)blockIdx.x - x_blocks) * 64 + wave * 16; r < sh.Vp; r += blocks * 64)
+            ce_pack_rows<T, VW, SPLIT>(w, ldw, r, sh.V, nullptr, sh.D, e, wp, sh.Vp, sh.panels, lane);
     } else {
-        for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < sh.Mp; r += x_blocks * 4)
-            ce_pack_row<T, VX, SPLIT>(x + r * ldx, r < sh.M && target[r] >= 0, sh.D, e, xp + r * sh.ld, sh.ld, lane);
+        for (int64_t r = (int64_t)blockIdx.x * 64 + wave * 16; r < sh.Mp; r += x_blocks * 64)
+            ce_pack_rows<T, VX, SPLIT>(x, ldx, r, sh.M, target, sh.D, e, xp, sh.Mp, sh.panels, lane);
     }
 }
 
@@ -158,13 +157,12 @@ struct CeLogits {
     // backward
     const float *lse;         // [Mp] base 2; +inf: absent, NaN: no such target
     const float *grad;        // reduction none: [M]
-    half_t *g;                // [Mp][ldg], column 0 = vocabulary entry v0
-    int64_t ldg;
+    half_t *g;                // panels of Mp rows, column 0 = vocabulary entry v0
 };
 
 template <typename T> __device__ __forceinline__ float ce_bias(const T *bias, int v) { return bias ? to_f32(bias[v]) * CE_LOG2E : 0.0f; }
 
-template <typename T, bool SPLIT, bool BACK, int BM, int BN, int WM, int WN>
+template <typename T, bool SPLIT, bool BACK, int BM, int BN, int WM, int WN, int NST>
 __global__ void __launch_bounds__(WM *WN * 64, 2) ce_logits_kernel(CeLogits a, const T *bias) {
     constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
@@ -174,7 +172,7 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) ce_logits_kernel(CeLogits a, c
     const int64_t vbase = a.v0 + (int64_t)tv * BM, ibase = (int64_t)ti * BN;
     for (int j = threadIdx.x; j < BM; j += WM * WN * 64) sb[j] = vbase + j < a.V ? ce_bias(bias, (int)vbase + j) : CE_NEG_INF;
     f32x16 acc[TM][TN];
-    gemm_tile<SPLIT, false, false, BM, BN, WM, WN>(a.w, a.x, vbase, 0, ibase, 0, 0, a.steps, lds, acc);
+    gemm_tile<SPLIT, false, false, BM, BN, WM, WN, NST>(a.w, a.x, vbase, 0, 0, ibase, 0, 0, 0, a.steps, lds, acc);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
     const int wm = wave / WN, wn = wave % WN;
     const float scale = ldexpf(CE_LOG2E, a.sc->ex + a.sc->ew);
@@ -237,7 +235,7 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) ce_logits_kernel(CeLogits a, c
             float f = t >= 0 ? 32768.0f : 0.0f;
             if (a.grad && t >= 0) f = a.sc->gmax > 0.0f ? 32768.0f * (a.grad[row] / a.sc->gmax) : 0.0f;
             // stored order inside 16 columns: 0 1 2 3 8 9 10 11 | 4 5 6 7 12 13 14 15 -- what one lane holds, 16 bytes at a time
-            half_t *out = a.g + row * a.ldg + ((int64_t)tv * BM + wm * TM * 32) * (SPLIT ? 2 : 1) + h * 8;
+            half_t *out = a.g + ((int64_t)(tv * BM / 32 + wm * TM) * (SPLIT ? 2 : 1) * a.Mp + row) * 32 + h * 8;
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -249,8 +247,9 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) ce_logits_kernel(CeLogits a, c
                         hi[e] = (half_t)v;
                         if (SPLIT) lo[e] = (half_t)(v - (float)hi[e]);
                     }
-                    *(half8 *)(out + i * 32 * (SPLIT ? 2 : 1) + c * 16) = hi;
-                    if (SPLIT) *(half8 *)(out + i * 64 + 32 + c * 16) = lo;
+                    half_t *o = out + (SPLIT ? (i * 2 + c) * a.Mp * 32 : i * a.Mp * 32 + c * 16);
+                    *(half8 *)o = hi;
+                    if (SPLIT) *(half8 *)(o + 16) = lo;
                 }
         }
     }
@@ -495,6 +494,7 @@ struct CeGrad {
     int64_t rows, out0;       // output rows of this call, the first one's index in the output
     int tiles_r, tiles_d, steps, splits, blocks;
     int64_t ok0;              // first row of the other operand
+    int g_panels, o_panels;
     void *out;                // final output (nothing to add up), [..][D]
     float *part;              // [splits][part_rows][D] sums, or NULL
     int64_t part_rows;
@@ -506,14 +506,14 @@ struct CeGrads {
     const float *grad;
     const int64_t *target;    // dhidden: rows with a negative target are zero
     int reduction, D;
-    // column sums of G (dbias): 512 stored columns x a share of the rows per workgroup
-    int64_t g_rows, g_cols, ldb;
+    // column sums of G (dbias): a panel x a share of the rows per workgroup
+    int64_t g_rows, ldb;
     int col_blocks, shares;
     float *part_b;            // [shares][ldb]
 };
 
 // WEIGHT: dweight (G read transposed, output rows = vocabulary entries in G's stored column order), else dhidden
-template <typename T, bool SPLIT, bool WEIGHT, int BM, int BN, int WM, int WN>
+template <typename T, bool SPLIT, bool WEIGHT, int BM, int BN, int WM, int WN, int NST>
 __device__ __forceinline__ void ce_grad_tile(const CeGrads &a, const CeGrad &c, int bid, char *lds) {
     constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
     int tr, td;
@@ -523,7 +523,10 @@ __device__ __forceinline__ void ce_grad_tile(const CeGrads &a, const CeGrad &c, 
     const int d0 = td * BN;
     const int s0 = (int)((int64_t)c.steps * z / c.splits), s1 = (int)((int64_t)c.steps * (z + 1) / c.splits);
     f32x16 acc[TM][TN];
-    gemm_tile<SPLIT, WEIGHT, true, BM, BN, WM, WN>(c.g, c.o, r0, 0, d0, c.ok0, s0, s1, lds, acc);
+    constexpr int PC = SPLIT ? 16 : 32;                        // columns per panel
+    const int gp = WEIGHT ? (int)(r0 / PC) : 0, op = d0 / PC;
+    gemm_tile<SPLIT, WEIGHT, true, BM, BN, WM, WN, NST>(c.g, c.o, WEIGHT ? 0 : r0, gp, c.g_panels - gp, c.ok0, op, c.o_panels - op, s0, s1, lds,
+                                                        acc);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
     const int wm = wave / WN, wn = wave % WN;
     const float f = c.part ? 1.0f : ce_unscale(a.sc, a.grad, a.reduction, WEIGHT ? a.sc->ex : a.sc->ew);
@@ -551,50 +554,50 @@ __device__ __forceinline__ void ce_grad_tile(const CeGrads &a, const CeGrad &c, 
         }
 }
 
-// a lane owns eight stored columns, the waves of the workgroup share the rows
+// one panel of G per workgroup and share of the rows: lane = (row, chunk of eight columns)
 template <int NW> __device__ __forceinline__ void ce_colsum(const CeGrads &a, int bid, char *lds) {
-    float(*sh)[64][8] = (float(*)[64][8])lds;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, cb = bid / a.shares, share = bid % a.shares;
-    const int64_t c = (int64_t)cb * 512 + lane * 8;
-    const int64_t per = (a.g_rows + a.shares - 1) / a.shares, r0 = share * per, r1 = r0 + per < a.g_rows ? r0 + per : a.g_rows;
+    float(*sh)[4][8] = (float(*)[4][8])lds;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, panel = bid / a.shares, share = bid % a.shares;
+    const int64_t per = (a.g_rows / 16 + a.shares - 1) / a.shares * 16, r0 = share * per, r1 = r0 + per < a.g_rows ? r0 + per : a.g_rows;
+    const half_t *g = a.x.g.p + (int64_t)panel * a.g_rows * 32 + lane * 8;
     float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (c < a.g_cols) {
-        constexpr int U = 8;
-        for (int64_t r = r0 + wave; r < r1; r += NW * U) {
-            half8 v[U];
+    constexpr int U = 8;
+    for (int64_t r = r0 + wave * 16; r < r1; r += NW * 16 * U) {
+        half8 v[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (r + NW * u < r1) v[u] = *(const half8 *)(a.x.g.p + (r + NW * u) * a.x.g.ld + c);
-                else
+        for (int u = 0; u < U; ++u) {
+            if (r + NW * 16 * u < r1) v[u] = *(const half8 *)(g + (r + NW * 16 * u) * 32);
+            else
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[u][e] = (half_t)0.0f;
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) s[e] += (float)v[u][e];
+                for (int e = 0; e < 8; ++e) v[u][e] = (half_t)0.0f;
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e] += (float)v[u][e];
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sh[wave][lane][e] = s[e];
-    __syncthreads();
-    if (wave == 0 && c < a.g_cols)
+    for (int e = 0; e < 8; ++e)
+        for (int o = 4; o < 64; o <<= 1) s[e] += __shfl_xor(s[e], o);
+    if (lane < 4)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float t = sh[0][lane][e];
-            for (int w = 1; w < NW; ++w) t += sh[w][lane][e];
-            a.part_b[share * a.ldb + c + e] = t;
-        }
+        for (int e = 0; e < 8; ++e) sh[wave][lane][e] = s[e];
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        float t = 0.0f;
+        for (int w = 0; w < NW; ++w) t += sh[w][threadIdx.x >> 3][threadIdx.x & 7];
+        a.part_b[share * a.ldb + panel * 32 + threadIdx.x] = t;
+    }
 }
 
 // Both gradient products and the column sums in one launch: they read the same G, and the workgroups of one fill what the others
 // leave idle.
-template <typename T, bool SPLIT, int BM, int BN, int WM, int WN>
+template <typename T, bool SPLIT, int BM, int BN, int WM, int WN, int NST>
 __global__ void __launch_bounds__(WM *WN * 64, 2) ce_grads_kernel(CeGrads a) {
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int bid = blockIdx.x;
-    if (bid < a.x.blocks) ce_grad_tile<T, SPLIT, false, BM, BN, WM, WN>(a, a.x, bid, lds);
-    else if (bid < a.x.blocks + a.w.blocks) ce_grad_tile<T, SPLIT, true, BM, BN, WM, WN>(a, a.w, bid - a.x.blocks, lds);
+    if (bid < a.x.blocks) ce_grad_tile<T, SPLIT, false, BM, BN, WM, WN, NST>(a, a.x, bid, lds);
+    else if (bid < a.x.blocks + a.w.blocks) ce_grad_tile<T, SPLIT, true, BM, BN, WM, WN, NST>(a, a.w, bid - a.x.blocks, lds);
     else ce_colsum<WM * WN>(a, bid - a.x.blocks - a.w.blocks, lds);
 }
 
@@ -640,7 +643,7 @@ __global__ void __launch_bounds__(256) ce_join_kernel(CeGrads a, int bx, int bw,
         const int pos = (v & ~12) | ((v & 4) << 1) | ((v & 8) >> 1);
         for (int k = seg; k < a.shares; k += 8) {
             const float *p = a.part_b + k * a.ldb;
-            s += split ? p[(pos >> 5) * 64 + (pos & 31)] + p[(pos >> 5) * 64 + (pos & 31) + 32] : p[pos];
+            s += split ? p[(pos >> 4) * 32 + (pos & 15)] + p[(pos >> 4) * 32 + (pos & 15) + 16] : p[pos];
         }
     }
     sh[seg][threadIdx.x & 31] = s;
@@ -660,8 +663,7 @@ static CeShape ce_shape(const tnp_vocab_ce *p) {
     s.M = p->M; s.Mp = ce_pad(p->M, CE_ROW_PAD);
     s.V = p->V; s.Vp = (int)ce_pad(p->V, CE_COL_PAD); s.D = p->D;
     s.split = p->dtype == TNP_F32;
-    s.ld = s.split ? 2 * ce_pad(p->D, 32) : ce_pad(p->D, 64);
-    s.steps = (int)(s.ld / 64);
+    s.panels = s.split ? (p->D + 15) / 16 : (p->D + 31) / 32;
     return s;
 }
 
@@ -671,8 +673,8 @@ static CeSaved ce_saved(const CeShape &s, void *base) {
     char *p = (char *)base;
     v.sc = (CeScalars *)p; p += 256;
     v.lse = (float *)p; p += s.Mp * 4;                 // Mp and Vp are multiples of 256: every part stays aligned
-    v.x = (half_t *)p; p += (size_t)s.Mp * s.ld * 2;
-    v.w = (half_t *)p; p += (size_t)s.Vp * s.ld * 2;
+    v.x = (half_t *)p; p += (size_t)s.Mp * s.panels * 64;
+    v.w = (half_t *)p; p += (size_t)s.Vp * s.panels * 64;
     v.bytes = (size_t)(p - (char *)base);
     return v;
 }
@@ -718,7 +720,7 @@ static constexpr size_t CE_PIECE_BYTES = (size_t)512 << 20;
 static CeBackward ce_backward_layout(const tnp_vocab_ce *p, void *ws) {
     CeBackward b;
     const CeShape s = ce_shape(p);
-    const int planes = s.split ? 2 : 1, ks = s.split ? 32 : 64;
+    const int planes = s.split ? 2 : 1, ks = s.split ? 16 : 32;
     int64_t most = (int64_t)(CE_PIECE_BYTES / ((size_t)s.Mp * 2 * planes)) / 256 * 256;
     if (most < 256) most = 256;
     b.pieces = (int)((s.Vp + most - 1) / most);
@@ -728,17 +730,17 @@ static CeBackward ce_backward_layout(const tnp_vocab_ce *p, void *ws) {
     // tiles of 256 rows once they alone are a round of workgroups, 256 columns where there are as many
     const int64_t td = (p->D + 127) / 128, small_x = s.Mp / 128 * td, small_w = b.piece / 128 * td;
     const int sx = b.piece / ks, sw = (int)(s.Mp / ks);
-    const bool big = small_x * sx + small_w * sw >= 65536;
+    const bool big = small_x * sx + small_w * sw >= 131072;
     b.bm = big ? 256 : 128;
     b.bn = big && p->D > 128 ? 256 : 128;
     // both products share a launch: every workgroup gets about the same number of steps, at least 8
     const int64_t tx = s.Mp / b.bm * ((p->D + b.bn - 1) / b.bn), tw = (b.piece + b.bm - 1) / b.bm * ((p->D + b.bn - 1) / b.bn);
-    int64_t each = (tx * sx + tw * sw) / (b.bm == 256 ? 256 : 512);
-    if (each < 8) each = 8;
+    int64_t each = (tx * sx + tw * sw) / (b.bn == 256 ? 256 : 512);
+    if (each < 16) each = 16;
     const int64_t nx = (sx + each / 2) / each, nw = (sw + each / 2) / each;
     b.splits_x = (int)(nx < 1 ? 1 : nx);
     b.splits_w = (int)(nw < 1 ? 1 : nw);
-    b.shares = (int)(s.Mp / 128 < 64 ? s.Mp / 128 : 64);
+    b.shares = (int)(s.Mp / 256 < 16 ? s.Mp / 256 : 16);                   // at least 256 rows of a panel each
     char *w = (char *)ws;
     b.g = (half_t *)w; w += ce_up((size_t)s.Mp * b.ldg * 2);
     b.part_x = b.splits_x > 1 || b.pieces > 1 ? (float *)w : nullptr;
@@ -755,8 +757,8 @@ static int ce_check(const tnp_vocab_ce *p, const char *who) {
     if (!p) TNP_FAIL(-1, "%s: NULL arguments", who);
     if (!dtype_known(p->dtype)) TNP_FAIL(-1, "%s: unknown dtype %d", who, p->dtype);
     if (p->reduction < 0 || p->reduction > 2) TNP_FAIL(-1, "%s: unknown reduction %d", who, p->reduction);
-    if (p->M < 0 || p->M > (1 << 30)) TNP_FAIL(-1, "%s: %lld rows (0 .. 2^30)", who, (long long)p->M);
-    if (p->V < 1 || p->V > (1 << 28)) TNP_FAIL(-1, "%s: vocabulary of %d (1 .. 2^28)", who, p->V);
+    if (p->M < 0 || p->M > (1 << 23)) TNP_FAIL(-1, "%s: %lld rows (0 .. 2^23)", who, (long long)p->M);
+    if (p->V < 1 || p->V > (1 << 23)) TNP_FAIL(-1, "%s: vocabulary of %d (1 .. 2^23)", who, p->V);
     if (p->D < 1 || p->D > 16384) TNP_FAIL(-1, "%s: %d columns (1 .. 16384)", who, p->D);
     if (p->ld_hidden < p->D || p->ld_weight < p->D) TNP_FAIL(-1, "%s: a row stride is smaller than the %d columns", who, p->D);
     return 0;
@@ -777,13 +779,13 @@ static int ce_lds(KernT kern, size_t smem, size_t *done) {             // done: 
     return 0;
 }
 
-template <typename T, bool SPLIT, bool BACK, int BM, int BN, int WM, int WN>
+template <typename T, bool SPLIT, bool BACK, int BM, int BN, int WM, int WN, int NST>
 static int ce_launch_logits(CeLogits a, int64_t cols, const T *bias, hipStream_t s) {
     a.tiles_v = (int)(cols / BM);
     a.tiles_i = (int)(a.Mp / BN);
-    const size_t smem = 2 * (BM + BN) * 128;
+    const size_t smem = NST * (BM + BN) * 64;
     static size_t done[VOCAB_MAX_DEVICES] = {0};
-    auto kern = ce_logits_kernel<T, SPLIT, BACK, BM, BN, WM, WN>;
+    auto kern = ce_logits_kernel<T, SPLIT, BACK, BM, BN, WM, WN, NST>;
     if (int rc = ce_lds(kern, smem, done)) return rc;
     hipLaunchKernelGGL(kern, dim3(gemm_grid((int64_t)a.tiles_v * a.tiles_i)), dim3(WM * WN * 64), smem, s, a, bias);
     TNP_HIP(hipGetLastError());
@@ -791,14 +793,14 @@ static int ce_launch_logits(CeLogits a, int64_t cols, const T *bias, hipStream_t
 }
 template <typename T, bool SPLIT, bool BACK>
 static int ce_logits(const CeLogits &a, int64_t cols, bool big, const T *bias, hipStream_t s) {
-    return big ? ce_launch_logits<T, SPLIT, BACK, 256, 256, 2, 4>(a, cols, bias, s) : ce_launch_logits<T, SPLIT, BACK, 128, 128, 2, 2>(a, cols, bias, s);
+    return big ? ce_launch_logits<T, SPLIT, BACK, 256, 256, 2, 4, 4>(a, cols, bias, s) : ce_launch_logits<T, SPLIT, BACK, 128, 128, 2, 2, 3>(a, cols, bias, s);
 }
 
-template <typename T, bool SPLIT, int BM, int BN, int WM, int WN>
+template <typename T, bool SPLIT, int BM, int BN, int WM, int WN, int NST>
 static int ce_launch_grads(CeGrads &a, hipStream_t s) {
-    const size_t smem = 2 * (BM + BN) * 128;
+    const size_t smem = NST * (BM + BN) * 64;
     static size_t done[VOCAB_MAX_DEVICES] = {0};
-    auto kern = ce_grads_kernel<T, SPLIT, BM, BN, WM, WN>;
+    auto kern = ce_grads_kernel<T, SPLIT, BM, BN, WM, WN, NST>;
     if (int rc = ce_lds(kern, smem, done)) return rc;
     for (CeGrad *c : {&a.x, &a.w}) {
         c->tiles_r = (int)((c->rows + BM - 1) / BM);
@@ -835,7 +837,7 @@ static int ce_pack(const tnp_vocab_ce *p, const CeShape &sh, const CeForward &f,
     hipLaunchKernelGGL((ce_amax_kernel<T, VX, VW>), dim3(2 * CE_AMAX_BLOCKS), dim3(256), 0, s, (const T *)p->hidden,
                        p->ld_hidden, p->M, p->target, (const T *)p->weight, p->ld_weight, p->V, p->D, f.amax, f.saved.sc);
     TNP_HIP(hipGetLastError());
-    const int xb = (int)(sh.Mp / 4 < 1024 ? sh.Mp / 4 : 1024), wb = sh.Vp / 4 < 2048 ? sh.Vp / 4 : 2048;
+    const int xb = (int)(sh.Mp / 64 < 1024 ? sh.Mp / 64 : 1024), wb = sh.Vp / 64 < 2048 ? sh.Vp / 64 : 2048;
     hipLaunchKernelGGL((ce_pack_kernel<T, VX, VW, SPLIT>), dim3(xb + wb), dim3(256), 0, s, (const T *)p->hidden, p->ld_hidden, p->target,
                        (const T *)p->weight, p->ld_weight, sh, f.amax, f.saved.sc, f.saved.x, f.saved.w, xb);
     TNP_HIP(hipGetLastError());
@@ -855,9 +857,9 @@ static int ce_forward(const tnp_vocab_ce *p, const CeForward &f, float *loss, hi
              : vx ? ce_pack<T, VE, 1, SPLIT>(p, sh, f, s) : ce_pack<T, 1, 1, SPLIT>(p, sh, f, s);
         if (rc) return rc;
         CeLogits a = {};
-        a.w = GemmOperand{f.saved.w, sh.ld, sh.Vp, 0};
-        a.x = GemmOperand{f.saved.x, sh.ld, sh.Mp, 0};
-        a.sc = f.saved.sc; a.target = p->target; a.M = sh.M; a.Mp = sh.Mp; a.V = sh.V; a.v0 = 0; a.steps = sh.steps;
+        a.w = GemmOperand{f.saved.w, sh.Vp, 0};
+        a.x = GemmOperand{f.saved.x, sh.Mp, 0};
+        a.sc = f.saved.sc; a.target = p->target; a.M = sh.M; a.Mp = sh.Mp; a.V = sh.V; a.v0 = 0; a.steps = sh.panels;
         a.part = f.part; a.tlogit = f.tlogit;
         if ((rc = ce_logits<T, SPLIT, false>(a, sh.Vp, ce_big(sh), (const T *)p->bias, s))) return rc;
     }
@@ -879,28 +881,29 @@ static int ce_backward(const tnp_vocab_ce *p, const CeBackward &b, const float *
         hipLaunchKernelGGL(ce_gmax_kernel, dim3(1), dim3(1024), 0, s, grad, p->target, p->M, sv.sc);
         TNP_HIP(hipGetLastError());
     }
-    const GemmOperand w{sv.w, sh.ld, sh.Vp, 0}, x{sv.x, sh.ld, sh.Mp, 0};
+    const GemmOperand w{sv.w, sh.Vp, 0}, x{sv.x, sh.Mp, 0};
     for (int k = 0; k < b.pieces; ++k) {
         const int v0 = k * b.piece, cols = sh.Vp - v0 < b.piece ? sh.Vp - v0 : b.piece, live = sh.V - v0 < cols ? sh.V - v0 : cols;
         CeLogits a = {};
-        a.w = w; a.x = x; a.sc = sv.sc; a.target = p->target; a.M = sh.M; a.Mp = sh.Mp; a.V = sh.V; a.v0 = v0; a.steps = sh.steps;
-        a.lse = sv.lse; a.grad = p->reduction == 0 ? grad : nullptr; a.g = b.g; a.ldg = b.ldg;
+        a.w = w; a.x = x; a.sc = sv.sc; a.target = p->target; a.M = sh.M; a.Mp = sh.Mp; a.V = sh.V; a.v0 = v0; a.steps = sh.panels;
+        a.lse = sv.lse; a.grad = p->reduction == 0 ? grad : nullptr; a.g = b.g;
         if ((rc = ce_logits<T, SPLIT, true>(a, cols, ce_big(sh), (const T *)p->bias, s))) return rc;
         const bool last = k == b.pieces - 1;
-        const int ks = SPLIT ? 32 : 64;
+        const int ks = SPLIT ? 16 : 32;
         CeGrads c = {};
         c.sc = sv.sc; c.grad = grad; c.target = p->target; c.reduction = p->reduction; c.D = sh.D;
-        c.x.g = c.w.g = GemmOperand{b.g, b.ldg, sh.Mp, 0};
+        c.x.g = c.w.g = GemmOperand{b.g, sh.Mp, 0};
+        c.x.g_panels = c.w.g_panels = cols / ks; c.x.o_panels = c.w.o_panels = sh.panels;
         c.x.o = w; c.x.o.perm = 1; c.x.ok0 = v0;
         c.x.rows = sh.M; c.x.out = dhidden; c.x.part = b.part_x; c.x.part_rows = sh.Mp; c.x.splits = b.splits_x;
         c.x.steps = cols / ks; c.x.add = k > 0;
         c.w.o = x;
         c.w.rows = live; c.w.out0 = v0; c.w.out = dweight; c.w.part = b.part_w; c.w.part_rows = b.piece; c.w.splits = b.splits_w;
         c.w.steps = (int)(sh.Mp / ks);
-        c.shares = b.shares; c.part_b = b.part_b; c.ldb = b.ldg; c.g_rows = sh.Mp; c.g_cols = (int64_t)cols * (SPLIT ? 2 : 1);
-        c.col_blocks = dbias ? (int)((c.g_cols + 511) / 512) : 0;
-        rc = b.bm == 256 ? (b.bn == 256 ? ce_launch_grads<T, SPLIT, 256, 256, 2, 4>(c, s) : ce_launch_grads<T, SPLIT, 256, 128, 4, 2>(c, s))
-                         : ce_launch_grads<T, SPLIT, 128, 128, 2, 2>(c, s);
+        c.shares = b.shares; c.part_b = b.part_b; c.ldb = b.ldg; c.g_rows = sh.Mp;
+        c.col_blocks = dbias ? cols / ks : 0;
+        rc = b.bm == 256 ? (b.bn == 256 ? ce_launch_grads<T, SPLIT, 256, 256, 2, 4, 4>(c, s) : ce_launch_grads<T, SPLIT, 256, 128, 2, 2, 3>(c, s))
+                         : ce_launch_grads<T, SPLIT, 128, 128, 2, 2, 3>(c, s);
         if (rc) return rc;
         const int ve = sh.D % 4 == 0 ? 4 : 1;
         const int64_t per = 256 * ve;

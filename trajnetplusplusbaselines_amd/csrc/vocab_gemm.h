@@ -1,15 +1,20 @@
-// Matrix products of vocab_ce.hip: C[m, n] = sum_k A[m, k] B[n, k] on v_mfma_f32_32x32x16_f16, both operands fp16 in memory, either
-// with k contiguous in a row ("KC") or with k as the row index ("KS": the transposing LDS read hands the matrix core its layout, so
-// no transposed copy of anything is ever made).
+// Matrix products of vocab_ce.hip: C[m, n] = sum_k A[m, k] B[n, k] on v_mfma_f32_32x32x16_f16.
 //
-// SPLIT operands carry fp32 values as two fp16 numbers, x = hi + lo (22 bits; what is left is below 2^-22 of x), stored as blocks of
-// 32 values: 32 hi | 32 lo.  A product is hi*hi + hi*lo + lo*hi, three matrix instructions into one fp32 accumulator: 2500 / 3
+// Every matrix lies in memory as PANELS: 32 columns of all rows, 64 bytes per row, row after row; panel after panel.  A tile of rows
+// is then one contiguous piece per panel, whichever way it is used: with the columns as k ("KC", one panel per step) or with the
+// rows as k ("KS", 32 rows of several panels per step; the transposing LDS read hands the matrix core its layout, so no transposed
+// copy of anything is ever made).  Row-major rows of 64 bytes per step were half cache lines: 4.0e8 instead of 2.0e8 L2 requests for
+// 16384 x 65536 x 1024.  Row counts are multiples of 256, so nothing is clamped.
+//
+// SPLIT matrices carry fp32 values as two fp16 numbers, x = hi + lo (22 bits; what is left is below 2^-22 of x); a panel is 16 columns,
+// a row of it 16 hi | 16 lo.  A product is hi*hi + hi*lo + lo*hi, three matrix instructions into one fp32 accumulator: 2500 / 3
 // TFLOP/s of matrix rate where v_mfma_f32_* has 157.
 //
-// A step stages 128 bytes per tile row (64 values, or 32 split ones) by global_load_lds into one of two LDS buffers while the other
-// is multiplied.  global_load_lds writes linearly, so the bank swizzle is applied to the global address: KC rows of 128 bytes put
-// chunk c (16 bytes) at c ^ ((row >> 1) & 7): sixteen consecutive rows cover all 64 banks; KS rows put 64-byte unit u at
-// u ^ (row & 3): the four k rows of a transposing read cover all 64 banks.
+// A step (32 k values, 16 split ones: 64 bytes per tile row) is staged by global_load_lds into a ring of LDS buffers, several steps
+// ahead of the one that is multiplied; one barrier per step.  global_load_lds writes linearly, so bank swizzles are applied to the
+// global address: KC rows put chunk c (16 bytes) at c ^ ((row >> 2) & 3): sixteen consecutive rows cover all 64 banks.  The four k rows
+// of a transposing read are 256 contiguous bytes as they are; split ones take 32 of every 64 bytes from two panels, so odd panels
+// change their halves.
 #pragma once
 #include "vocab_types.h"
 
@@ -25,140 +30,188 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 #define TNP_GLB __attribute__((address_space(1)))
 
 struct GemmOperand {
-    const half_t *p;     // first element of the matrix
-    int64_t ld;          // stored elements per row (a multiple of 64)
-    int64_t rows;        // rows that may be read: a row index beyond is clamped to the last
-    int perm;            // KS: bits 2 and 3 of the row index change places (the order in which the G kernel stores its columns)
+    const half_t *p;     // panel 0, row 0
+    int64_t rows;        // rows of a panel (a multiple of 256)
+    int perm;            // KS: bits 2 and 3 of the row index change places (the order in which G's columns are stored)
 };
 
 // One operand's tile of BR rows (KC) / BR columns (KS).
 template <bool KS, bool SPLIT, int BR, int NW> struct TileStage {
-    static constexpr int INSTR = BR / 8 / NW;                      // 1 KB wave instructions per wave and step
-    static_assert(BR / 8 % NW == 0, "tile rows must spread evenly over the waves");
-    static constexpr int KSTEP = SPLIT ? 32 : 64;
+    static constexpr int INSTR = BR / 16 / NW;                     // 1 KB wave instructions per wave and step: 16 rows of a panel each
+    static_assert(BR / 16 % NW == 0, "tile rows must spread evenly over the waves");
+    static constexpr int KSTEP = SPLIT ? 16 : 32;                  // k values per step = columns per panel
     const half_t *base;
-    int64_t ld, rows, row0;
+    int64_t advance;                                               // elements per step
     uint32_t off[INSTR];
-    int perm;
 
-    // KC: tile rows [r0, r0 + BR), k from stored column c0.  KS: tile columns (stored) from c0, k from row r0.
-    __device__ __forceinline__ void init(const GemmOperand &o, int64_t r0, int64_t c0, int wave, int lane) {
-        ld = o.ld; rows = o.rows; perm = o.perm; row0 = r0;
-        if (!KS) {
-            base = o.p + r0 * ld + c0;
-#pragma unroll
-            for (int j = 0; j < INSTR; ++j) {
-                const int r = (wave + j * NW) * 8 + (lane >> 3);
-                const int64_t row = r0 + r < rows ? r : rows - 1 - r0;
-                off[j] = (uint32_t)(row * ld) + ((lane & 7) ^ ((r >> 1) & 7)) * 8;
-            }
-        } else {
-            base = o.p;
-            constexpr int CB = BR * 2 * (SPLIT ? 2 : 1);           // bytes per k row
-#pragma unroll
-            for (int j = 0; j < INSTR; ++j) {
-                const int byte = (wave + j * NW) * 1024 + lane * 16, r = byte / CB, ch = byte % CB / 16;
-                const int64_t col = c0 + (ch ^ ((r & 3) << 2)) * 8;
-                off[j] = (uint32_t)(col < ld - 8 ? col : ld - 8);
-            }
-        }
-    }
-    __device__ __forceinline__ void load(int step, char *lds, int wave, int lane) const {
+    // KC: tile rows [r0, r0 + BR), k from panel k0.  KS: tile columns from panel c0 (the last of `panels` again beyond), k from row k0.
+    __device__ __forceinline__ void init(const GemmOperand &o, int64_t r0, int64_t panel, int panels_left, int wave, int lane) {
+        base = o.p + (panel * o.rows + r0) * 32;
+        advance = KS ? KSTEP * 32 : o.rows * 32;
 #pragma unroll
         for (int j = 0; j < INSTR; ++j) {
-            const half_t *src;
+            const int q = wave + j * NW;
             if (!KS) {
-                src = base + (int64_t)step * 64 + off[j];
+                const int r = q * 16 + (lane >> 2);
+                off[j] = r * 32 + ((lane & 3) ^ ((r >> 2) & 3)) * 8;
             } else {
-                constexpr int CB = BR * 2 * (SPLIT ? 2 : 1);
-                int r = ((wave + j * NW) * 1024 + lane * 16) / CB;
-                if (perm) r = (r & ~12) | ((r & 4) << 1) | ((r & 8) >> 1);
-                int64_t row = row0 + (int64_t)step * KSTEP + r;
-                row = row < rows ? row : rows - 1;
-                src = base + row * ld + off[j];
+                int pan = SPLIT ? q : q >> 1, r = (SPLIT ? 0 : (q & 1) * 16) + (lane >> 2), ch = lane & 3;
+                if (SPLIT) ch ^= (pan & 1) << 1;
+                if (o.perm) r = (r & ~12) | ((r & 4) << 1) | ((r & 8) >> 1);
+                pan = pan < panels_left ? pan : panels_left - 1;
+                off[j] = (uint32_t)(pan * o.rows * 32) + r * 32 + ch * 8;
             }
-            __builtin_amdgcn_global_load_lds((const TNP_GLB void *)src, (TNP_LDS void *)(lds + (wave + j * NW) * 1024), 16, 0, 0);
         }
     }
-    // operand of one 32-row block at tile row r0, sub-step ss of 16 values, plane 0 = hi / 1 = lo (SPLIT)
+    __device__ __forceinline__ void load(int step, char *lds, int wave) const {
+        const half_t *b = base + step * advance;
+#pragma unroll
+        for (int j = 0; j < INSTR; ++j)
+            __builtin_amdgcn_global_load_lds((const TNP_GLB void *)(b + off[j]), (TNP_LDS void *)(lds + (wave + j * NW) * 1024), 16, 0, 0);
+    }
+    // KC: operand of one 32-row block at tile row r0, sub-step ss of 16 values, plane 0 = hi / 1 = lo (SPLIT)
     static __device__ __forceinline__ half8 frag(const char *lds, int r0, int ss, int plane, int lane) {
-        if (!KS) {
-            const int r = r0 + (lane & 31), ch = (SPLIT ? plane * 4 : 0) + ss * 2 + (lane >> 5);
-            return *(const half8 *)(lds + r * 128 + ((ch ^ ((r >> 1) & 7)) * 16));
-        } else {
-            return half8{};                                        // KS operands come through ks_frags
-        }
+        const int r = r0 + (lane & 31), ch = (SPLIT ? plane : ss) * 2 + (lane >> 5);
+        return *(const half8 *)(lds + r * 64 + ((ch ^ ((r >> 2) & 3)) * 16));
     }
-    static constexpr int CB = BR * 2 * (SPLIT ? 2 : 1);            // bytes per k row of a KS tile
-    // KS: LDS byte address of the first value this lane fetches for 32 columns from c (stored), k rows 0 .. 3 of its half.  Rows
-    // row, row + 4, row + 16 share (row & 3), hence the swizzle: further rows are constant offsets.
-    static __device__ __forceinline__ uint32_t ks_addr(const char *lds, int c, int lane) {
-        const int g = lane >> 4, j = lane & 15, row = 8 * (g >> 1) + (j >> 2), col = c + 16 * (g & 1) + 4 * (j & 3);
-        return (uint32_t)(uintptr_t)(TNP_LDS const char *)lds + row * CB + (((col >> 3) ^ ((row & 3) << 2)) * 16) + (col & 7) * 2;
+    // KS: LDS byte address of the first value this lane fetches for 32 columns from c, k rows 0 .. 3 of its half; rows row + 4 and row + 16
+    // are constant offsets
+    static constexpr int ROW4 = 4 * 64, ROW16 = 16 * 64;
+    static __device__ __forceinline__ uint32_t ks_addr(const char *lds, int c, int plane, int lane) {
+        const int g = lane >> 4, j = lane & 15, row = 8 * (g >> 1) + (j >> 2);
+        int at;
+        if (SPLIT) at = ((c >> 4) + (g & 1)) * 1024 + row * 64 + (plane ^ (g & 1)) * 32 + (j & 3) * 8;      // c is a multiple of 32
+        else at = (c >> 5) * 2048 + row * 64 + (g & 1) * 32 + (j & 3) * 8;
+        return (uint32_t)(uintptr_t)(TNP_LDS const char *)lds + at;
     }
 };
 
-// Two 32-column blocks of a KS tile, k values 16 ss .. 16 ss + 15 (OFF = 16 ss rows in bytes).  One asm block that ends with its own
-// wait: as builtins these reads would first wait for every global_load_lds in flight, that is for the NEXT step's tile.
-template <int OFF, int CB>
-__device__ __forceinline__ void ks_read2(uint32_t a0, uint32_t a1, half8 &f0, half8 &f1) {
-    typedef int int2v __attribute__((ext_vector_type(2)));
-    typedef int int4v __attribute__((ext_vector_type(4)));
-    int2v p0, q0, p1, q1;
-    asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%c6\n\t"
-                 "ds_read_b64_tr_b16 %1, %4 offset:%c7\n\t"
-                 "ds_read_b64_tr_b16 %2, %5 offset:%c6\n\t"
-                 "ds_read_b64_tr_b16 %3, %5 offset:%c7\n\t"
+// 32-column blocks of KS tiles at the LDS addresses a[], k rows 0 .. 3 and (R4 bytes on) 4 .. 7 of every half.  One asm block that ends
+// with its own wait: as builtins these reads would first wait for every global_load_lds in flight, that is for the tiles of the
+// next steps.
+typedef int int2v __attribute__((ext_vector_type(2)));
+typedef int int4v __attribute__((ext_vector_type(4)));
+template <int R4> __device__ __forceinline__ void ks_read(const uint32_t (&a)[2], half8 (&f)[2]) {
+    int2v r[4];
+    asm volatile(
+                 "ds_read_b64_tr_b16 %0, %4\n\t"
+                 "ds_read_b64_tr_b16 %1, %4 offset:%c6\n\t"
+                 "ds_read_b64_tr_b16 %2, %5\n\t"
+                 "ds_read_b64_tr_b16 %3, %5 offset:%c6\n\t"
                  "s_waitcnt lgkmcnt(0)"
-                 : "=&v"(p0), "=&v"(q0), "=&v"(p1), "=&v"(q1)
-                 : "v"(a0), "v"(a1), "i"(OFF), "i"(OFF + 4 * CB)
+                 : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
+                 : "v"(a[0]), "v"(a[1]), "i"(R4)
                  : "memory");
-    f0 = __builtin_bit_cast(half8, int4v{p0.x, p0.y, q0.x, q0.y});
-    f1 = __builtin_bit_cast(half8, int4v{p1.x, p1.y, q1.x, q1.y});
+#pragma unroll
+    for (int k = 0; k < 2; ++k) f[k] = __builtin_bit_cast(half8, int4v{r[2 * k].x, r[2 * k].y, r[2 * k + 1].x, r[2 * k + 1].y});
 }
-template <int OFF, int CB>
-__device__ __forceinline__ void ks_read4(uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, half8 &f0, half8 &f1, half8 &f2, half8 &f3) {
-    typedef int int2v __attribute__((ext_vector_type(2)));
-    typedef int int4v __attribute__((ext_vector_type(4)));
-    int2v p0, q0, p1, q1, p2, q2, p3, q3;
-    asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%c12\n\t"
-                 "ds_read_b64_tr_b16 %1, %8 offset:%c13\n\t"
-                 "ds_read_b64_tr_b16 %2, %9 offset:%c12\n\t"
-                 "ds_read_b64_tr_b16 %3, %9 offset:%c13\n\t"
-                 "ds_read_b64_tr_b16 %4, %10 offset:%c12\n\t"
-                 "ds_read_b64_tr_b16 %5, %10 offset:%c13\n\t"
-                 "ds_read_b64_tr_b16 %6, %11 offset:%c12\n\t"
-                 "ds_read_b64_tr_b16 %7, %11 offset:%c13\n\t"
+template <int R4> __device__ __forceinline__ void ks_read(const uint32_t (&a)[4], half8 (&f)[4]) {
+    int2v r[8];
+    asm volatile(
+                 "ds_read_b64_tr_b16 %0, %8\n\t"
+                 "ds_read_b64_tr_b16 %1, %8 offset:%c12\n\t"
+                 "ds_read_b64_tr_b16 %2, %9\n\t"
+                 "ds_read_b64_tr_b16 %3, %9 offset:%c12\n\t"
+                 "ds_read_b64_tr_b16 %4, %10\n\t"
+                 "ds_read_b64_tr_b16 %5, %10 offset:%c12\n\t"
+                 "ds_read_b64_tr_b16 %6, %11\n\t"
+                 "ds_read_b64_tr_b16 %7, %11 offset:%c12\n\t"
                  "s_waitcnt lgkmcnt(0)"
-                 : "=&v"(p0), "=&v"(q0), "=&v"(p1), "=&v"(q1), "=&v"(p2), "=&v"(q2), "=&v"(p3), "=&v"(q3)
-                 : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "i"(OFF), "i"(OFF + 4 * CB)
+                 : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "i"(R4)
                  : "memory");
-    f0 = __builtin_bit_cast(half8, int4v{p0.x, p0.y, q0.x, q0.y});
-    f1 = __builtin_bit_cast(half8, int4v{p1.x, p1.y, q1.x, q1.y});
-    f2 = __builtin_bit_cast(half8, int4v{p2.x, p2.y, q2.x, q2.y});
-    f3 = __builtin_bit_cast(half8, int4v{p3.x, p3.y, q3.x, q3.y});
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f[k] = __builtin_bit_cast(half8, int4v{r[2 * k].x, r[2 * k].y, r[2 * k + 1].x, r[2 * k + 1].y});
 }
-// N = 2 or 4 blocks at the addresses a[0 .. N)
-template <int OFF, int CB, int N> __device__ __forceinline__ void ks_frags(const uint32_t (&a)[N], half8 (&f)[N]) {
-    static_assert(N == 2 || N == 4, "two or four blocks of 32 columns per wave");
-    if constexpr (N == 2) ks_read2<OFF, CB>(a[0], a[1], f[0], f[1]);
-    else ks_read4<OFF, CB>(a[0], a[1], a[2], a[3], f[0], f[1], f[2], f[3]);
+template <int R4> __device__ __forceinline__ void ks_read(const uint32_t (&a)[8], half8 (&f)[8]) {
+    int2v r[16];
+    asm volatile(
+                 "ds_read_b64_tr_b16 %0, %16\n\t"
+                 "ds_read_b64_tr_b16 %1, %16 offset:%c24\n\t"
+                 "ds_read_b64_tr_b16 %2, %17\n\t"
+                 "ds_read_b64_tr_b16 %3, %17 offset:%c24\n\t"
+                 "ds_read_b64_tr_b16 %4, %18\n\t"
+                 "ds_read_b64_tr_b16 %5, %18 offset:%c24\n\t"
+                 "ds_read_b64_tr_b16 %6, %19\n\t"
+                 "ds_read_b64_tr_b16 %7, %19 offset:%c24\n\t"
+                 "ds_read_b64_tr_b16 %8, %20\n\t"
+                 "ds_read_b64_tr_b16 %9, %20 offset:%c24\n\t"
+                 "ds_read_b64_tr_b16 %10, %21\n\t"
+                 "ds_read_b64_tr_b16 %11, %21 offset:%c24\n\t"
+                 "ds_read_b64_tr_b16 %12, %22\n\t"
+                 "ds_read_b64_tr_b16 %13, %22 offset:%c24\n\t"
+                 "ds_read_b64_tr_b16 %14, %23\n\t"
+                 "ds_read_b64_tr_b16 %15, %23 offset:%c24\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7]), "=&v"(r[8]), "=&v"(r[9]), "=&v"(r[10]), "=&v"(r[11]), "=&v"(r[12]), "=&v"(r[13]), "=&v"(r[14]), "=&v"(r[15])
+                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(a[4]), "v"(a[5]), "v"(a[6]), "v"(a[7]), "i"(R4)
+                 : "memory");
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = __builtin_bit_cast(half8, int4v{r[2 * k].x, r[2 * k].y, r[2 * k + 1].x, r[2 * k + 1].y});
 }
 
-// Accumulates steps [s0, s1) of tile (a at row / column a0, b at b0) into acc.  KC operands start at stored column ak0 / bk0, KS
-// operands at row ak0 / bk0.  LDS: 2 * (BM + BN) * 128 bytes.
-template <bool SPLIT, bool A_KS, bool B_KS, int BM, int BN, int WM, int WN>
-__device__ __forceinline__ void gemm_tile(const GemmOperand &a, const GemmOperand &b, int64_t a0, int64_t ak0, int64_t b0, int64_t bk0, int s0,
-                                          int s1, char *lds, f32x16 (&acc)[BM / WM / 32][BN / WN / 32]) {
-    constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, STAGE = (BM + BN) * 128;
+// Waits until at most N of this wave's loads are in flight and all its LDS reads are done, then meets the other waves.
+template <int N> __device__ __forceinline__ void stage_barrier() {
+    asm volatile("s_waitcnt vmcnt(%c0) lgkmcnt(0)\n\ts_barrier" ::"i"(N) : "memory");
+}
+
+__device__ __forceinline__ void stage_barrier_only() { asm volatile("s_barrier" ::: "memory"); }
+
+// All of a wave's operand blocks of one step: NB blocks of 32 rows (KC) / columns (KS) from c, each with two 8-value registers (the two
+// sub-steps of 16 values, or the hi and lo planes of a split step): f[2 * block + which].
+template <typename ST, bool KS, bool SPLIT, int NB>
+__device__ __forceinline__ void step_frags(const char *lds, int c, int lane, half8 (&f)[2 * NB]) {
+    if constexpr (KS) {
+        uint32_t a[2 * NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int w = 0; w < 2; ++w) a[2 * b + w] = ST::ks_addr(lds, c + b * 32, SPLIT ? w : 0, lane) + (SPLIT ? 0 : w * ST::ROW16);
+        ks_read<ST::ROW4>(a, f);
+    } else {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int w = 0; w < 2; ++w) f[2 * b + w] = ST::frag(lds, c + b * 32, w, w, lane);
+    }
+}
+
+template <bool SPLIT, int TM, int TN>
+__device__ __forceinline__ void step_mfma(const half8 (&fa)[2 * TM], const half8 (&fb)[2 * TN], f32x16 (&acc)[TM][TN]) {
+    // products per block pair: the two sub-steps, or lo * hi, hi * lo, hi * hi (the small ones are not lost against the large)
+    constexpr int N = SPLIT ? 3 : 2;
+    constexpr int wa[3] = {SPLIT ? 1 : 0, SPLIT ? 0 : 1, 0}, wb[3] = {0, 1, 0};
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[2 * i + wa[k]], fb[2 * j + wb[k]], acc[i][j], 0, 0, 0);
+}
+
+// Accumulates steps [s0, s1) of the tile at (row ar, panel ap) of a and (br, bp) of b into acc; al / bl: panels from there to the last
+// (KS).  LDS: NST * (BM + BN) * 64 bytes.
+//
+// Eight waves (two per SIMD) take turns: while one half of the workgroup fetches the operands of a step into registers, the other
+// half multiplies the step it has fetched; a barrier per turn keeps them half a step apart.  In lockstep both waves of a SIMD would
+// fetch at the same time and leave the matrix cores idle meanwhile (2150 cycles per step of 1024 cycles of matrix work).  With
+// four waves the other workgroup on the CU fills that time.
+template <bool SPLIT, bool A_KS, bool B_KS, int BM, int BN, int WM, int WN, int NST>
+__device__ __forceinline__ void gemm_tile(const GemmOperand &a, const GemmOperand &b, int64_t ar, int64_t ap, int al, int64_t br, int64_t bp, int bl,
+                                          int s0, int s1, char *lds, f32x16 (&acc)[BM / WM / 32][BN / WN / 32]) {
+    constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, STAGE = (BM + BN) * 64;
+    constexpr bool TURNS = NW == 8;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
     typedef TileStage<A_KS, SPLIT, BM, NW> SA;
     typedef TileStage<B_KS, SPLIT, BN, NW> SB;
+    constexpr int LOADS = SA::INSTR + SB::INSTR;                   // per wave and step
+    static_assert(NST >= 3, "the tile after next is in flight while one is read");
     SA sa;
     SB sb;
-    if (A_KS) sa.init(a, ak0, a0 * (SPLIT ? 2 : 1), wave, lane); else sa.init(a, a0, ak0, wave, lane);
-    if (B_KS) sb.init(b, bk0, b0 * (SPLIT ? 2 : 1), wave, lane); else sb.init(b, b0, bk0, wave, lane);
+    sa.init(a, ar, ap, al, wave, lane);
+    sb.init(b, br, bp, bl, wave, lane);
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -166,62 +219,48 @@ __device__ __forceinline__ void gemm_tile(const GemmOperand &a, const GemmOperan
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
     if (s0 >= s1) return;
-    sa.load(s0, lds, wave, lane);
-    sb.load(s0, lds + BM * 128, wave, lane);
-    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < NST - 1; ++k)
+        if (s0 + k < s1) {
+            sa.load(s0 + k, lds + k * STAGE, wave);
+            sb.load(s0 + k, lds + k * STAGE + BM * 64, wave);
+        }
+    // the tile of the step that has `left` steps behind it has landed in every wave (those in flight: at most NST - 2)
+    auto landed = [&](int left) {
+        if (NST >= 4 && left >= 2) stage_barrier<(NST >= 4 ? 2 : 0) * LOADS>();
+        else if (left >= 1) stage_barrier<LOADS>();
+        else stage_barrier<0>();
+    };
+    landed(s1 - 1 - s0);
+    if (TURNS && wave >= 4) stage_barrier_only();
+    int cur = 0;
+    half8 fa[2 * TM], fb[2 * TN];
     for (int s = s0; s < s1; ++s) {
-        char *cur = lds + ((s - s0) & 1) * STAGE, *nxt = lds + ((s - s0 + 1) & 1) * STAGE;
-        if (s + 1 < s1) {
-            sa.load(s + 1, nxt, wave, lane);
-            sb.load(s + 1, nxt + BM * 128, wave, lane);
+        const char *la = lds + cur * STAGE, *lb = la + BM * 64;
+        step_frags<SB, B_KS, SPLIT, TN>(lb, wn * TN * 32, lane, fb);
+        step_frags<SA, A_KS, SPLIT, TM>(la, wm * TM * 32, lane, fa);
+        if (s + NST - 1 < s1) {                                    // into the buffer that every wave was done with one barrier ago
+            const int nxt = cur == 0 ? NST - 1 : cur - 1;
+            sa.load(s + NST - 1, lds + nxt * STAGE, wave);
+            sb.load(s + NST - 1, lds + nxt * STAGE + BM * 64, wave);
         }
-        const char *la = cur, *lb = cur + BM * 128;
-        constexpr int P = SPLIT ? 2 : 1, SS = SPLIT ? 2 : 4;
-        uint32_t aa[P][TM], ab[P][TN];                             // KS operands: LDS addresses
-        if (A_KS)
-#pragma unroll
-            for (int p = 0; p < P; ++p)
-#pragma unroll
-                for (int i = 0; i < TM; ++i) aa[p][i] = SA::ks_addr(la, (wm * TM + i) * 32 * P + p * 32, lane);
-        if (B_KS)
-#pragma unroll
-            for (int p = 0; p < P; ++p)
-#pragma unroll
-                for (int j = 0; j < TN; ++j) ab[p][j] = SB::ks_addr(lb, (wn * TN + j) * 32 * P + p * 32, lane);
-        auto sub = [&](auto ssc) {
-            constexpr int ss = decltype(ssc)::value;
-            half8 fa[P][TM], fb[P][TN];
-#pragma unroll
-            for (int p = 0; p < P; ++p) {
-                if constexpr (A_KS) ks_frags<ss * 16 * SA::CB, SA::CB, TM>(aa[p], fa[p]);
-                else
-#pragma unroll
-                    for (int i = 0; i < TM; ++i) fa[p][i] = SA::frag(la, (wm * TM + i) * 32, ss, p, lane);
-                if constexpr (B_KS) ks_frags<ss * 16 * SB::CB, SB::CB, TN>(ab[p], fb[p]);
-                else
-#pragma unroll
-                    for (int j = 0; j < TN; ++j) fb[p][j] = SB::frag(lb, (wn * TN + j) * 32, ss, p, lane);
-            }
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TN; ++j) {
-                    if constexpr (SPLIT) {                         // the small products first: they are not lost against the large ones
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[1][i], fb[0][j], acc[i][j], 0, 0, 0);
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][i], fb[1][j], acc[i][j], 0, 0, 0);
-                    }
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][i], fb[0][j], acc[i][j], 0, 0, 0);
-                }
-        };
-        sub(std::integral_constant<int, 0>());
-        sub(std::integral_constant<int, 1>());
-        if constexpr (SS == 4) {
-            sub(std::integral_constant<int, 2>());
-            sub(std::integral_constant<int, 3>());
+        cur = cur + 1 == NST ? 0 : cur + 1;
+        if (TURNS) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (s + 1 < s1) landed(s1 - 2 - s); else stage_barrier<0>();
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(1);
+            step_mfma<SPLIT, TM, TN>(fa, fb, acc);
+            __builtin_amdgcn_s_setprio(0);
+            __builtin_amdgcn_sched_barrier(0);
+            stage_barrier_only();
+            __builtin_amdgcn_sched_barrier(0);
+        } else {
+            step_mfma<SPLIT, TM, TN>(fa, fb, acc);
+            if (s + 1 < s1) landed(s1 - 2 - s);
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");            // the next step's tile has landed
-        __syncthreads();
     }
+    if (TURNS && wave < 4) stage_barrier_only();
 }
 
 // Workgroup -> tile: the eight XCDs take the workgroups in turn, so each gets a contiguous share of the tiles, walked in groups of
