@@ -5,23 +5,24 @@
 // fault), nothing backward.
 //
 // Forward: one pass, bound by memory.  Backward: the tokens are sorted (a stable radix sort of (token, i) pairs, digits of up to
-// 10 bits), so that all rows of one token are neighbours; chunks of 32 sorted positions are summed by one group of lanes each,
-// whatever the distribution of the tokens -- a table row that owns half of the batch is split over thousands of chunks and joined.
+// 10 bits), so that all rows of one token are neighbours; chunks of 8, 16 or 32 sorted positions are summed by one group of lanes each,
+// whatever the distribution of the tokens -- a table row that owns half of the batch is split over many chunks and joined.
 // Every gradient row is read once and every table row written once; table rows without a token are zeroed by their own workgroups,
 // which find them by binary search in the sorted tokens.
 #include "vocab_types.h"
 
 namespace tnp {
 
-static constexpr int EMB_CHUNK = 32;          // sorted positions per group of lanes
 static constexpr int EMB_SORT_THREADS = 512;  // eight waves per workgroup of the sort, each with 4 or 16 rows of 64 pairs
+static constexpr int EMB_COUNT_ALL = 8;       // workgroups of the sort up to which each counts all keys
 static constexpr int EMB_JOIN_CHUNKS = 32;    // chunks per workgroup of the join
 static constexpr int EMB_JOIN_SHORT = 8;      // parts of a run that one group of lanes adds up by itself
 static constexpr int EMB_MAX_BITS = 10;      // eight waves' counters of 2^10 digits: 32 KB of LDS
 static constexpr int64_t EMB_MAX_TOKENS = 1 << 28;
 
 // ---- forward ----------------------------------------------------------------------------------------------------------------
-// 2^lsh lanes per row; U rows per lane whose loads are in flight together.
+// 2^lsh lanes per row; U rows per lane whose loads are in flight together (a token without a row loads row 0 and drops it: loads
+// under a condition would wait for each other).
 template <typename T, int VE, typename I, int U>
 __global__ void __launch_bounds__(256) embed_forward_kernel(const I *tokens, int64_t N, const T *weight, int64_t ldw, int64_t V,
                                                             int D, int lsh, float scale, T *out, int64_t ldo) {
@@ -33,20 +34,13 @@ __global__ void __launch_bounds__(256) embed_forward_kernel(const I *tokens, int
     for (int c = (threadIdx.x & (lanes - 1)) * VE; c < D; c += lanes * VE) {
         Pack<T, VE> w[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (tok[u] >= 0 && tok[u] < V) {
-                w[u] = *(const Pack<T, VE> *)(weight + tok[u] * ldw + c);
-            } else {
-                const T fill = from_f32<T>(tok[u] < 0 ? 0.0f : __builtin_nanf(""));
-#pragma unroll
-                for (int e = 0; e < VE; ++e) w[u].v[e] = fill;
-            }
-        }
+        for (int u = 0; u < U; ++u) w[u] = *(const Pack<T, VE> *)(weight + (tok[u] >= 0 && tok[u] < V ? tok[u] : 0) * ldw + c);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (i0 + u * rows >= N) continue;
 #pragma unroll
-            for (int e = 0; e < VE; ++e) w[u].v[e] = tok[u] < 0 ? from_f32<T>(0.0f) : from_f32<T>(to_f32(w[u].v[e]) * scale);
+            for (int e = 0; e < VE; ++e)
+                w[u].v[e] = from_f32<T>(tok[u] < 0 ? 0.0f : tok[u] < V ? to_f32(w[u].v[e]) * scale : __builtin_nanf(""));
             *(Pack<T, VE> *)(out + (i0 + u * rows) * ldo + c) = w[u];
         }
     }
@@ -110,7 +104,7 @@ __global__ void __launch_bounds__(EMB_SORT_THREADS) embed_hist_kernel(const I *t
 }
 
 // Every workgroup forms its own offsets from the histograms of all of them (nblk * 2^bits counters, L2-resident): one launch less
-// per pass than a scan kernel in between.  nblk == 1 needs no histogram at all.
+// per pass than a scan kernel in between.  Up to eight workgroups (hist == NULL) count all the keys themselves, another launch less.
 template <typename I, int ROWS>
 __global__ void __launch_bounds__(EMB_SORT_THREADS) embed_scatter_kernel(const I *tokens, const uint32_t *keys, const uint32_t *idx,
                                                                          int64_t N, uint32_t V, int shift, int bits,
@@ -120,9 +114,29 @@ __global__ void __launch_bounds__(EMB_SORT_THREADS) embed_scatter_kernel(const I
     const int nb = 1 << bits, nw = EMB_SORT_THREADS / 64;
     uint32_t *cnt = lds;                // [waves][nb]: counts, then the first position of (wave, digit)
     uint32_t *part = lds + nw * nb;     // [waves] sums of the scan over digits
+    uint32_t *all = part + nw;          // [2][nb] without histograms: keys of the digit, those of them before this workgroup's
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     for (int b = tid; b < nw * nb; b += EMB_SORT_THREADS) cnt[b] = 0;
+    const bool count_all = nblk > 1 && !hist;
+    if (count_all)
+        for (int b = tid; b < 2 * nb; b += EMB_SORT_THREADS) all[b] = 0;
     __syncthreads();
+    if (count_all) {
+        const int64_t mine = (int64_t)blockIdx.x * nw * ROWS * 64;
+        constexpr int U = 8;
+        for (int64_t i = tid; i < N; i += EMB_SORT_THREADS * U) {
+            uint32_t k[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) k[u] = i + u * EMB_SORT_THREADS < N ? embed_key(tokens, keys, i + u * EMB_SORT_THREADS, V) : 0;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (i + u * EMB_SORT_THREADS >= N) continue;
+                const uint32_t d = (k[u] >> shift) & (nb - 1);
+                atomicAdd(&all[d], 1u);
+                if (i + u * EMB_SORT_THREADS < mine) atomicAdd(&all[nb + d], 1u);
+            }
+        }
+    }
     uint32_t key[ROWS], rank[ROWS], from[ROWS];
     const int64_t base = ((int64_t)blockIdx.x * nw + wave) * (ROWS * 64);
 #pragma unroll
@@ -140,6 +154,9 @@ __global__ void __launch_bounds__(EMB_SORT_THREADS) embed_scatter_kernel(const I
         if (j >= per || b >= nb) continue;
         if (nblk == 1) {
             for (int w = 0; w < nw; ++w) total[j] += cnt[w * nb + b];
+        } else if (count_all) {
+            total[j] = all[b];
+            before[j] = all[nb + b];
         } else {
             constexpr int U = 16;                              // counters in flight
             for (int k = 0; k < nblk; k += U) {
@@ -198,12 +215,12 @@ __device__ __forceinline__ uint32_t embed_upper(const uint32_t *keys, uint32_t l
     return lo;
 }
 
-// Chunk c = sorted positions [32 c, 32 c + 32), 2^lsh lanes, fp32 sums.  A run (one token) inside the chunk is finished here; the
+// Chunk c = sorted positions [c << csh, (c + 1) << csh), 2^lsh lanes, fp32 sums.  A run (one token) inside the chunk is finished here; the
 // part of a run that came in from the chunk before goes to head[c], the first part of a run that goes on into the next to tail[c]
 // (embed_join_kernel adds those).  Workgroups from `sum_blocks` on zero the table rows that no token names.
 template <typename T, int VE>
 __global__ void __launch_bounds__(256) embed_reduce_kernel(const uint32_t *keys, const uint32_t *idx, uint32_t N, uint32_t V,
-                                                           const T *grad, int64_t ldg, int D, int lsh, float scale, T *dw,
+                                                           const T *grad, int64_t ldg, int D, int lsh, int csh, float scale, T *dw,
                                                            int64_t ldd, float *head, float *tail, uint32_t sum_blocks) {
     const int lanes = 1 << lsh;
     if (blockIdx.x >= sum_blocks) {                    // 64 table rows per wave
@@ -235,9 +252,9 @@ __global__ void __launch_bounds__(256) embed_reduce_kernel(const uint32_t *keys,
         return;
     }
     const uint32_t chunk = blockIdx.x * (256u >> lsh) + (threadIdx.x >> lsh);
-    const uint64_t a64 = (uint64_t)chunk * EMB_CHUNK;
+    const uint64_t a64 = (uint64_t)chunk << csh;
     if (a64 >= N) return;
-    const uint32_t a = (uint32_t)a64, b = min(a + EMB_CHUNK, N);
+    const uint32_t a = (uint32_t)a64, b = min(a + (1u << csh), N);
     const int c = (blockIdx.y * lanes + (threadIdx.x & (lanes - 1))) * VE;
     if (c >= D) return;
     uint32_t cur = keys[a];
@@ -260,10 +277,11 @@ __global__ void __launch_bounds__(256) embed_reduce_kernel(const uint32_t *keys,
         uint32_t k[U];
         Pack<T, VE> g[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) k[u] = p + u < b ? keys[p + u] : V;
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (k[u] < V) g[u] = *(const Pack<T, VE> *)(grad + (int64_t)idx[p + u] * ldg + c);
+        for (int u = 0; u < U; ++u) {                  // behind the chunk: its last row again, not added
+            const uint32_t at = p + u < b ? p + u : b - 1;
+            k[u] = keys[at];
+            g[u] = *(const Pack<T, VE> *)(grad + (int64_t)idx[at] * ldg + c);
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (p + u >= b) break;
@@ -286,11 +304,20 @@ __global__ void __launch_bounds__(256) embed_reduce_kernel(const uint32_t *keys,
     else finish();
 }
 
+// VE partial sums (rows of D floats, D a multiple of VE)
+template <int VE> struct Parts { Pack<float, (VE < 4 ? VE : 4)> p[VE < 4 ? 1 : VE / 4]; };
+template <int VE> __device__ __forceinline__ Parts<VE> load_parts(const float *at) {
+    Parts<VE> r;
+#pragma unroll
+    for (int k = 0; k < (VE < 4 ? 1 : VE / 4); ++k) r.p[k] = *(const Pack<float, (VE < 4 ? VE : 4)> *)(at + 4 * k);
+    return r;
+}
+
 // Runs that go on past their chunk: tail[c] + head[c + 1] + ... of the run that starts in chunk c.  A workgroup looks after 32 chunks:
 // first every group of lanes adds up runs of up to eight parts by itself, then all of them together stride over each longer one and
 // meet in LDS.  Every order of addition is fixed by the sizes.
 template <typename T, int VE>
-__global__ void __launch_bounds__(512) embed_join_kernel(const uint32_t *keys, uint32_t N, uint32_t V, int D, int lsh, float scale,
+__global__ void __launch_bounds__(512) embed_join_kernel(const uint32_t *keys, uint32_t N, uint32_t V, int D, int lsh, int csh, float scale,
                                                          T *dw, int64_t ldd, const float *head, const float *tail) {
     extern __shared__ float sums[];                    // [512][VE]
     __shared__ uint32_t long_chunk[EMB_JOIN_CHUNKS];
@@ -298,12 +325,12 @@ __global__ void __launch_bounds__(512) embed_join_kernel(const uint32_t *keys, u
     const int lanes = 1 << lsh, groups = 512 >> lsh, grp = threadIdx.x >> lsh;
     const int c = (blockIdx.y * lanes + (threadIdx.x & (lanes - 1))) * VE;
     if (threadIdx.x < 64) {                            // the first wave looks for the runs
-        const uint64_t chunk = (uint64_t)blockIdx.x * EMB_JOIN_CHUNKS + threadIdx.x, a = chunk * EMB_CHUNK, b = a + EMB_CHUNK;
+        const uint64_t chunk = (uint64_t)blockIdx.x * EMB_JOIN_CHUNKS + threadIdx.x, a = chunk << csh, b = (chunk + 1) << csh;
         bool starts = false, more = false;
         if (threadIdx.x < EMB_JOIN_CHUNKS && b < N) {
             const uint32_t k = keys[b - 1];
             starts = k < V && keys[b] == k && !(a > 0 && keys[a - 1] == k);
-            const uint64_t far = b + (uint64_t)EMB_JOIN_SHORT * EMB_CHUNK;
+            const uint64_t far = b + ((uint64_t)EMB_JOIN_SHORT << csh);
             more = starts && far < N && keys[far] == k;
         }
         const uint64_t m = __ballot(more), s = __ballot(starts);
@@ -322,43 +349,53 @@ __global__ void __launch_bounds__(512) embed_join_kernel(const uint32_t *keys, u
     };
     for (int j = grp; j < EMB_JOIN_CHUNKS; j += groups) {
         if (long_chunk[j] != 1 || c >= D) continue;
-        const uint32_t chunk = blockIdx.x * EMB_JOIN_CHUNKS + j, b = (chunk + 1) * EMB_CHUNK, k = keys[b];
-        float h[EMB_JOIN_SHORT][VE], acc[VE];
-        bool in[EMB_JOIN_SHORT];
+        const uint32_t chunk = blockIdx.x * EMB_JOIN_CHUNKS + j, b = (chunk + 1) << csh, k = keys[b];
+        // parts behind the run's end: the run's first part again, not added -- loads under a condition wait for each other
+        uint32_t first[EMB_JOIN_SHORT];
+        Parts<VE> h[EMB_JOIN_SHORT];
 #pragma unroll
-        for (int u = 0; u < EMB_JOIN_SHORT; ++u) in[u] = (uint64_t)b + u * EMB_CHUNK < N && keys[b + u * EMB_CHUNK] == k;
+        for (int u = 0; u < EMB_JOIN_SHORT; ++u) first[u] = keys[(uint64_t)b + (u << csh) < N ? b + (u << csh) : b - 1];
+        int parts = 0;
 #pragma unroll
-        for (int e = 0; e < VE; ++e) acc[e] = tail[(size_t)chunk * D + c + e];
+        for (int u = 0; u < EMB_JOIN_SHORT; ++u) parts += (uint64_t)b + (u << csh) < N && first[u] == k;
+        const Parts<VE> t = load_parts<VE>(tail + (size_t)chunk * D + c);
 #pragma unroll
-        for (int u = 0; u < EMB_JOIN_SHORT; ++u)
+        for (int u = 0; u < EMB_JOIN_SHORT; ++u) h[u] = load_parts<VE>(head + (size_t)(chunk + 1 + (u < parts ? u : 0)) * D + c);
+        float acc[VE];
 #pragma unroll
-            for (int e = 0; e < VE; ++e) h[u][e] = in[u] ? head[(size_t)(chunk + 1 + u) * D + c + e] : 0.0f;
+        for (int e = 0; e < VE; ++e) {
+            acc[e] = t.p[e / 4].v[e % 4];
 #pragma unroll
-        for (int u = 0; u < EMB_JOIN_SHORT; ++u)
-#pragma unroll
-            for (int e = 0; e < VE; ++e) acc[e] += h[u][e];
+            for (int u = 0; u < EMB_JOIN_SHORT; ++u) acc[e] += u < parts ? h[u].p[e / 4].v[e % 4] : 0.0f;
+        }
         finish(k, acc);
     }
     if (longs == 0) return;
     for (int j = 0; j < EMB_JOIN_CHUNKS; ++j) {
         if (long_chunk[j] != 2) continue;              // the same for the whole workgroup
-        const uint32_t chunk = blockIdx.x * EMB_JOIN_CHUNKS + j, b = (chunk + 1) * EMB_CHUNK, k = keys[b];
-        const uint32_t last = (embed_upper(keys, b, N, k) - 1) / EMB_CHUNK;
+        const uint32_t chunk = blockIdx.x * EMB_JOIN_CHUNKS + j, k = keys[(chunk + 1) << csh];
+        // last chunk that the run enters: it begins with k (monotone in the chunk), 512 probes at a time
+        uint32_t last = chunk + 1 + EMB_JOIN_SHORT, end = (N + (1u << csh) - 1) >> csh;
+        while (end - last > 1) {
+            const uint32_t step = (end - last + 511) / 512;
+            const uint64_t at = last + (uint64_t)(threadIdx.x + 1) * step;
+            const uint32_t hit = (uint32_t)__syncthreads_count(at < end && keys[at << csh] == k);
+            last += hit * step;
+            end = min(last + step, end);
+        }
         float acc[VE];
 #pragma unroll
         for (int e = 0; e < VE; ++e) acc[e] = grp == 0 && c < D ? tail[(size_t)chunk * D + c + e] : 0.0f;
         if (c < D) {
             constexpr int U = 8;
             for (uint32_t q = chunk + 1 + grp; q <= last; q += groups * U) {
-                float h[U][VE];
+                Parts<VE> h[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) h[u] = load_parts<VE>(head + (size_t)(q + u * groups <= last ? q + u * groups : q) * D + c);
 #pragma unroll
                 for (int u = 0; u < U; ++u)
 #pragma unroll
-                    for (int e = 0; e < VE; ++e) h[u][e] = q + u * groups <= last ? head[(size_t)(q + u * groups) * D + c + e] : 0.0f;
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-#pragma unroll
-                    for (int e = 0; e < VE; ++e) acc[e] += h[u][e];
+                    for (int e = 0; e < VE; ++e) acc[e] += q + u * groups <= last ? h[u].p[e / 4].v[e % 4] : 0.0f;
             }
         }
         __syncthreads();                               // the sums of the run before have been read
@@ -396,7 +433,7 @@ static int lane_shift(int D, int ve, int most) {
 
 struct EmbedSort { int bits, passes, rows, nblk; };
 static EmbedSort embed_sort_plan(int64_t N, int64_t V) {
-    EmbedSort p;
+    EmbedSort p = {};
     int need = 1;
     while (((int64_t)1 << need) <= V) ++need;          // keys 0 .. V
     p.passes = (need + EMB_MAX_BITS - 1) / EMB_MAX_BITS;
@@ -406,6 +443,12 @@ static EmbedSort embed_sort_plan(int64_t N, int64_t V) {
     const int64_t items = EMB_SORT_THREADS * p.rows;
     p.nblk = (int)((N + items - 1) / items);
     return p;
+}
+
+// rows of head / tail: chunks are shorter than 32 positions only where there are fewer than 1024 * 64 of the shorter ones
+static size_t embed_parts(int64_t N) {
+    const size_t most = (size_t)((N + 31) / 32), short_ones = (size_t)((N + 7) / 8);
+    return most > 131072 ? most : short_ones < 131072 ? short_ones : 131072;
 }
 
 static inline size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -445,14 +488,15 @@ static int embed_sort_rows(const I *tokens, int64_t N, uint32_t V, const EmbedSo
     for (int pass = 0; pass < p.passes; ++pass) {
         const uint32_t *kin = pass ? keys[(pass + 1) & 1] : nullptr, *iin = pass ? idx[(pass + 1) & 1] : nullptr;
         const size_t nb = (size_t)1 << p.bits;
-        if (p.nblk > 1) {
+        const bool count_all = p.nblk <= EMB_COUNT_ALL;
+        if (!count_all) {
             hipLaunchKernelGGL((embed_hist_kernel<I, ROWS>), dim3(p.nblk), dim3(EMB_SORT_THREADS), nb * 4, s, tokens, kin, N, V, pass * p.bits,
                                p.bits, hist);
             TNP_HIP(hipGetLastError());
         }
-        const size_t smem = (EMB_SORT_THREADS / 64 * nb + EMB_SORT_THREADS / 64) * 4;
+        const size_t smem = (EMB_SORT_THREADS / 64 * nb + EMB_SORT_THREADS / 64 + (count_all ? 2 * nb : 0)) * 4;
         hipLaunchKernelGGL((embed_scatter_kernel<I, ROWS>), dim3(p.nblk), dim3(EMB_SORT_THREADS), smem, s, tokens, kin, iin, N, V, pass * p.bits,
-                           p.bits, hist, p.nblk, keys[pass & 1], idx[pass & 1]);
+                           p.bits, count_all ? nullptr : hist, p.nblk, keys[pass & 1], idx[pass & 1]);
         TNP_HIP(hipGetLastError());
     }
     return 0;
@@ -468,15 +512,19 @@ static int embed_sums(const uint32_t *keys, const uint32_t *idx, uint32_t N, uin
                       int64_t ldd, float *head, float *tail, hipStream_t s) {
     const int lsh = lane_shift(D, VE, 6);
     const unsigned cols = (unsigned)((D + (VE << lsh) - 1) / (VE << lsh));
-    const unsigned chunks = (unsigned)(((uint64_t)N + EMB_CHUNK - 1) / EMB_CHUNK);
+    // 32 positions per chunk where that already is a wave per SIMD; shorter chunks shorten the chain of dependent loads of a small
+    // batch (43008 x 64: 16 us at 32 positions, see the table of measurements)
+    int csh = 5;
+    while (csh > 3 && (((uint64_t)N >> csh << lsh) >> 6) * cols < 1024) --csh;
+    const unsigned chunks = (unsigned)(((uint64_t)N + (1u << csh) - 1) >> csh);
     const unsigned sum_blocks = (unsigned)(((uint64_t)chunks + (256u >> lsh) - 1) / (256u >> lsh));
     const unsigned zero_blocks = (unsigned)(((uint64_t)V + 255) / 256);
     hipLaunchKernelGGL((embed_reduce_kernel<T, VE>), dim3(sum_blocks + zero_blocks, cols), dim3(256), 0, s, keys, idx, N, V, grad, ldg, D, lsh,
-                       scale, dw, ldd, head, tail, sum_blocks);
+                       csh, scale, dw, ldd, head, tail, sum_blocks);
     TNP_HIP(hipGetLastError());
     if (chunks > 1) {
         hipLaunchKernelGGL((embed_join_kernel<T, VE>), dim3((chunks + EMB_JOIN_CHUNKS - 1) / EMB_JOIN_CHUNKS, cols), dim3(512), 512 * VE * 4, s,
-                           keys, N, V, D, lsh, scale, dw, ldd, head, tail);
+                           keys, N, V, D, lsh, csh, scale, dw, ldd, head, tail);
         TNP_HIP(hipGetLastError());
     }
     return 0;
@@ -512,7 +560,7 @@ extern "C" TNP_API int tnp_token_embedding_forward(const void *tokens, int token
 extern "C" TNP_API size_t tnp_token_embedding_backward_workspace_bytes(int64_t N, int64_t V, int D) {
     if (N <= 0 || V < 1 || D < 1) return 0;
     const EmbedSort p = embed_sort_plan(N, V);
-    const size_t chunks = (size_t)((N + EMB_CHUNK - 1) / EMB_CHUNK);
+    const size_t chunks = embed_parts(N);
     return 4 * up256((size_t)N * 4) + up256((size_t)p.nblk * 4 << p.bits) + 2 * up256(chunks * (size_t)D * 4);
 }
 
@@ -542,7 +590,7 @@ extern "C" TNP_API int tnp_token_embedding_backward(const void *tokens, int toke
         uint32_t *hist = (uint32_t *)w;
         w += up256((size_t)p.nblk * 4 << p.bits);
         head = (float *)w;
-        tail = (float *)(w + up256((size_t)((N + EMB_CHUNK - 1) / EMB_CHUNK) * D * 4));
+        tail = (float *)(w + up256(embed_parts(N) * D * 4));
         const int rc = token_bytes == 8 ? embed_sort((const int64_t *)tokens, N, (uint32_t)V, p, keys, idx, hist, s)
                                         : embed_sort((const int32_t *)tokens, N, (uint32_t)V, p, keys, idx, hist, s);
         if (rc) return rc;

@@ -22,7 +22,7 @@ namespace tnp {
 static constexpr float CE_LOG2E = 1.4426950408889634f;
 static constexpr double CE_LN2 = 0.6931471805599453;
 static constexpr float CE_NEG_INF = -__builtin_inff();
-static constexpr int CE_AMAX_BLOCKS = 256;            // per tensor
+static constexpr int CE_AMAX_BLOCKS = 512;            // per tensor
 static constexpr int CE_ROW_PAD = 256, CE_COL_PAD = 256;
 static constexpr int CE_SCORE_ROWS = 64;              // rows up to which scoring reads the inputs in place
 
@@ -42,16 +42,29 @@ struct CeShape {
 };
 
 // ---- scales and packing -----------------------------------------------------------------------------------------------------
+// largest finite |element| of rows [r0, r1): the rows' accesses one after the other, four in flight per lane
 template <typename T, int VE>
-__device__ __forceinline__ float ce_row_amax(const T *row, int D, int lane) {
+__device__ __forceinline__ float ce_rows_amax(const T *x, int64_t ld, int64_t r0, int64_t r1, const int64_t *target, int D) {
+    const uint32_t per = (uint32_t)D / VE, n = (uint32_t)(r1 - r0) * per;
     float a = 0.0f;
-    for (int c = lane * VE; c < D; c += 64 * VE) {
-        const Pack<T, VE> p = *(const Pack<T, VE> *)(row + c);
+    constexpr int U = 4;
+    for (uint32_t k = threadIdx.x; k < n; k += 256 * U) {
+        Pack<T, VE> p[U];
+        bool in[U];
 #pragma unroll
-        for (int e = 0; e < VE; ++e) {
-            const float v = fabsf(to_f32(p.v[e]));
-            if (v < __builtin_inff()) a = fmaxf(a, v);           // infinities and NaN do not set the scale
+        for (int u = 0; u < U; ++u) {
+            const uint32_t q = k + u * 256, row = q / per, c = q - row * per;
+            in[u] = q < n && (!target || target[r0 + row] >= 0);
+            if (in[u]) p[u] = *(const Pack<T, VE> *)(x + (r0 + row) * ld + c * VE);
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (in[u])
+#pragma unroll
+                for (int e = 0; e < VE; ++e) {
+                    const float v = fabsf(to_f32(p[u].v[e]));
+                    if (v < __builtin_inff()) a = fmaxf(a, v);       // infinities and NaN do not set the scale
+                }
     }
     return a;
 }
@@ -61,14 +74,9 @@ __global__ void __launch_bounds__(256) ce_amax_kernel(const T *x, int64_t ldx, i
                                                       int D, float *part, CeScalars *sc) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const bool is_w = blockIdx.x >= CE_AMAX_BLOCKS;
-    const int bid = is_w ? blockIdx.x - CE_AMAX_BLOCKS : blockIdx.x;
-    float a = 0.0f;
-    if (is_w) {
-        for (int64_t r = bid * 4 + wave; r < V; r += CE_AMAX_BLOCKS * 4) a = fmaxf(a, ce_row_amax<T, VW>(w + r * ldw, D, lane));
-    } else {
-        for (int64_t r = bid * 4 + wave; r < M; r += CE_AMAX_BLOCKS * 4)
-            if (target[r] >= 0) a = fmaxf(a, ce_row_amax<T, VX>(x + r * ldx, D, lane));
-    }
+    const int64_t bid = is_w ? blockIdx.x - CE_AMAX_BLOCKS : blockIdx.x, rows = is_w ? V : M;
+    const int64_t r0 = rows * bid / CE_AMAX_BLOCKS, r1 = rows * (bid + 1) / CE_AMAX_BLOCKS;
+    float a = is_w ? ce_rows_amax<T, VW>(w, ldw, r0, r1, nullptr, D) : ce_rows_amax<T, VX>(x, ldx, r0, r1, target, D);
     __shared__ float sh[4];
     for (int o = 32; o; o >>= 1) a = fmaxf(a, __shfl_xor(a, o));
     if (lane == 0) sh[wave] = a;
@@ -95,28 +103,32 @@ __device__ __forceinline__ void ce_pack_rows(const T *src, int64_t ld, int64_t r
     const int64_t r = r0 + (lane >> 2);
     const bool live = r < rows && (!target || target[r] >= 0);
     const int ch = lane & 3, c0 = SPLIT ? (ch & 1) * 8 : ch * 8;
+    constexpr int U = 4;                                         // panels in flight
     half_t *out = dst + r * 32 + ch * 8;
-    for (int p = 0; p < panels; ++p, out += panel_rows * 32) {
-        const int c = p * (SPLIT ? 16 : 32) + c0;
-        float v[NV];
+    for (int p = 0; p < panels; p += U) {
+        Pack<T, VE> q[U][NV / VE];
 #pragma unroll
-        for (int k = 0; k < NV; k += VE) {
-            if (live && c + k < D) {
-                const Pack<T, VE> q = *(const Pack<T, VE> *)(src + r * ld + c + k);
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int m = 0; m < VE; ++m) v[k + m] = ldexpf(to_f32(q.v[m]), -e);
-            } else {
+            for (int k = 0; k < NV / VE; ++k) {
+                const int c = (p + u) * (SPLIT ? 16 : 32) + c0 + k * VE;
+                if (live && p + u < panels && c < D) q[u][k] = *(const Pack<T, VE> *)(src + r * ld + c);
+                else
 #pragma unroll
-                for (int m = 0; m < VE; ++m) v[k + m] = 0.0f;
+                    for (int m = 0; m < VE; ++m) q[u][k].v[m] = from_f32<T>(0.0f);
             }
-        }
-        half8 o;
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const half_t hi = (half_t)v[k];
-            o[k] = SPLIT && ch >= 2 ? (fabsf(v[k]) < 65504.0f ? (half_t)(v[k] - (float)hi) : (half_t)0.0f) : hi;
+        for (int u = 0; u < U; ++u) {
+            if (p + u >= panels) break;
+            half8 o;
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const float v = ldexpf(to_f32(q[u][k / VE].v[k % VE]), -e);
+                const half_t hi = (half_t)v;
+                o[k] = SPLIT && ch >= 2 ? (fabsf(v) < 65504.0f ? (half_t)(v - (float)hi) : (half_t)0.0f) : hi;
+            }
+            *(half8 *)(out + (p + u) * panel_rows * 32) = o;
         }
-        *(half8 *)out = o;
     }
 }
 
@@ -126,7 +138,7 @@ __global__ void __launch_bounds__(256) ce_pack_kernel(const T *x, int64_t ldx, c
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const bool is_w = (int)blockIdx.x >= x_blocks;
     __shared__ float red[4];
-    float a = part[(is_w ? CE_AMAX_BLOCKS : 0) + threadIdx.x];
+    float a = fmaxf(part[(is_w ? CE_AMAX_BLOCKS : 0) + threadIdx.x], part[(is_w ? CE_AMAX_BLOCKS : 0) + 256 + threadIdx.x]);
     for (int o = 32; o; o >>= 1) a = fmaxf(a, __shfl_xor(a, o));
     if (lane == 0) red[wave] = a;
     __syncthreads();
