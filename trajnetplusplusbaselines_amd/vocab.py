@@ -9,7 +9,6 @@ Both are differentiable, run on the current stream of the tensors' device withou
 and refuse host tensors.  A negative token or target is an absent track (zero row, no loss, no gradient); one past the end of the
 vocabulary gives NaN, since the host does not look at device data.
 """
-import contextlib
 import ctypes
 
 import torch
@@ -20,31 +19,34 @@ _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _l
 _REDUCTIONS = {'none': 0, 'mean': 1, 'sum': 2}
 
 
-def _on(device):
-    """The device's own context when it is not the current one (the native calls take the CURRENT device's stream)."""
-    if device.index is None or device.index == torch._C._cuda_getDevice():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+_current = torch._C._cuda_getDevice
+
+
+class _On(object):
+    """The device's own context where it is not the current one (the native calls take the CURRENT device's stream)."""
+    __slots__ = ('ctx',)
+
+    def __init__(self, device):
+        self.ctx = None if device.index is None or device.index == _current() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.ctx is not None:
+            self.ctx.__enter__()
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
 
 
 def _rows(t):
-    """[n, D] with unit column stride; a copy only where the layout asks for one"""
-    if t.stride(-1) == 1 or t.shape[-1] == 1:
-        if t.dim() == 2:
-            if t.shape[0] <= 1 or t.stride(0) >= t.shape[1]:
-                return t if t.stride(-1) == 1 else t.contiguous()
-        elif t.is_contiguous():
-            return t.reshape(-1, t.shape[-1])
-    return t.contiguous().reshape(-1, t.shape[-1])
-
-
-def _ld(t):
-    """elements per row (a single row's stride is whatever torch left there)"""
-    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
-
-
-def _workspace(nbytes, device):
-    return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+    """(t, elements per row) with unit column stride and rows that do not overlap; a copy only where the layout asks for one.  t of
+    more than two dimensions has to be, or is made, contiguous."""
+    d = t.shape[-1]
+    if t.is_contiguous():
+        return t, d
+    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= d:
+        return t, t.stride(0)
+    return t.contiguous(), d
 
 
 def _check_table(weight, what):
@@ -56,31 +58,29 @@ def _check_table(weight, what):
 
 # ---- token embedding ---------------------------------------------------------------------------------------------------------
 def _embedding_forward(tokens, weight, scale):
-    w = _rows(weight)
-    tok = tokens.reshape(-1)                                   # a view where it can be
-    if not tok.is_contiguous():
-        tok = tok.contiguous()
-    n, d = tok.shape[0], w.shape[1]
-    out = torch.empty(tokens.shape + (d,), dtype=w.dtype, device=w.device)
-    with _on(w.device):
+    w, ld = _rows(weight)
+    tok = tokens if tokens.is_contiguous() else tokens.contiguous()
+    v, d = w.shape
+    dev = w.device
+    with _On(dev):
+        out = torch.empty(tokens.shape + (d,), dtype=w.dtype, device=dev)
         _lib.check(_lib.lib().tnp_token_embedding_forward(
-            tok.data_ptr(), tok.element_size(), n, w.data_ptr(), _ld(w), w.shape[0], d, _DTYPES[w.dtype], scale, out.data_ptr(), d,
-            _lib.raw_stream()), 'tnp_token_embedding_forward')
+            tok.data_ptr(), 8 if tok.dtype == torch.int64 else 4, tok.numel(), w.data_ptr(), ld, v, d, _DTYPES[w.dtype], scale,
+            out.data_ptr(), d, _lib.raw_stream()), 'tnp_token_embedding_forward')
     return out
 
 
 def _embedding_backward(grad, tokens, vocab, scale):
-    d = grad.shape[-1]
-    tok = tokens.reshape(-1).contiguous()
-    g = _rows(grad) if grad.numel() else grad.reshape(0, d)
-    n = tok.shape[0]
-    dw = torch.empty(vocab, d, dtype=grad.dtype, device=grad.device)
+    g, ld = _rows(grad)
+    tok = tokens if tokens.is_contiguous() else tokens.contiguous()
+    n, d, dev = tok.numel(), g.shape[-1], g.device
     L = _lib.lib()
-    with _on(grad.device):
+    with _On(dev):
+        dw = torch.empty((vocab, d), dtype=g.dtype, device=dev)
         need = L.tnp_token_embedding_backward_workspace_bytes(n, vocab, d)
-        ws = _workspace(need, grad.device)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
         _lib.check(L.tnp_token_embedding_backward(
-            tok.data_ptr(), tok.element_size(), n, g.data_ptr(), _ld(g) if n else d, vocab, d, _DTYPES[grad.dtype], scale, dw.data_ptr(),
+            tok.data_ptr(), 8 if tok.dtype == torch.int64 else 4, n, g.data_ptr(), ld, vocab, d, _DTYPES[g.dtype], scale, dw.data_ptr(),
             d, ws.data_ptr(), need, _lib.raw_stream()), 'tnp_token_embedding_backward')
     return dw
 
@@ -90,13 +90,12 @@ class _TokenEmbeddingFn(torch.autograd.Function):
     def forward(ctx, tokens, weight, scale):
         ctx.save_for_backward(tokens)
         ctx.args = (weight.shape[0], scale)
-        return _embedding_forward(tokens, weight.detach(), scale)
+        return _embedding_forward(tokens, weight, scale)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        tokens, = ctx.saved_tensors
-        return None, _embedding_backward(grad, tokens, *ctx.args), None
+        return None, _embedding_backward(grad, ctx.saved_tensors[0], *ctx.args), None
 
 
 def check_embedding(tokens, weight, scale):
@@ -129,50 +128,49 @@ class VocabCe(ctypes.Structure):
                 ('ld_weight', ctypes.c_int64), ('bias', ctypes.c_void_p), ('target', ctypes.c_void_p), ('saved', ctypes.c_void_p)]
 
 
-def _ce_args(hidden, weight, bias, target, reduction):
-    a = VocabCe()
-    a.dtype, a.reduction = _DTYPES[weight.dtype], reduction
-    a.M, a.V, a.D = hidden.shape[0], weight.shape[0], weight.shape[1]
-    a.hidden, a.ld_hidden = hidden.data_ptr(), _ld(hidden)
-    a.weight, a.ld_weight = weight.data_ptr(), _ld(weight)
-    a.bias = bias.data_ptr() if bias is not None else None
-    a.target = target.data_ptr()
-    return a
+def _ce_args(hidden, weight, bias, target, reduction, saved):
+    """(struct, the tensors in kernel layout that it points to)"""
+    x, ldx = _rows(hidden)
+    w, ldw = _rows(weight)
+    t = target if target.dtype == torch.int64 and target.is_contiguous() else target.to(torch.int64).contiguous()
+    b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
+    v, d = w.shape
+    return VocabCe(_DTYPES[w.dtype], reduction, t.numel(), v, d, x.data_ptr(), ldx, w.data_ptr(), ldw, None if b is None else b.data_ptr(),
+                   t.data_ptr(), None if saved is None else saved.data_ptr()), (x, w, t, b)
 
 
 def _ce_forward(hidden, weight, bias, target, reduction, train):
-    """(loss [M] or [1], what the backward pass reads or None); every operand already in kernel layout, M >= 1"""
+    """(loss, what the backward pass reads or None); at least one row"""
     dev = weight.device
     L = _lib.lib()
-    a = _ce_args(hidden, weight, bias, target, reduction)
-    saved = None
-    with _on(dev):
+    with _On(dev):
+        a, held = _ce_args(hidden, weight, bias, target, reduction, None)
+        ref = ctypes.byref(a)
+        saved = None
         if train:
-            saved = _workspace(L.tnp_vocab_ce_saved_bytes(ctypes.byref(a)), dev)
+            saved = torch.empty(L.tnp_vocab_ce_saved_bytes(ref), dtype=torch.uint8, device=dev)
             a.saved = saved.data_ptr()
-        need = L.tnp_vocab_ce_workspace_bytes(ctypes.byref(a), 0)
-        ws = _workspace(need, dev)
-        loss = torch.empty(hidden.shape[0] if reduction == 0 else 1, dtype=torch.float32, device=dev)
-        _lib.check(L.tnp_vocab_ce_forward(ctypes.byref(a), loss.data_ptr(), ws.data_ptr(), need, _lib.raw_stream()),
-                   'tnp_vocab_ce_forward')
+        need = L.tnp_vocab_ce_workspace_bytes(ref, 0)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        loss = torch.empty(target.shape if reduction == 0 else (), dtype=torch.float32, device=dev)
+        _lib.check(L.tnp_vocab_ce_forward(ref, loss.data_ptr(), ws.data_ptr(), need, _lib.raw_stream()), 'tnp_vocab_ce_forward')
     return loss, saved
 
 
 def _ce_backward(grad, hidden, weight, bias, target, saved, reduction, needs):
     dev = weight.device
     L = _lib.lib()
-    a = _ce_args(hidden, weight, bias, target, reduction)
-    a.saved = saved.data_ptr()
-    with _on(dev):
-        g = grad.detach().reshape(-1).float().contiguous()
+    with _On(dev):
+        a, held = _ce_args(hidden, weight, bias, target, reduction, saved)
+        ref = ctypes.byref(a)
+        g = grad if grad.dtype == torch.float32 and grad.is_contiguous() else grad.float().contiguous()
         dx = torch.empty(hidden.shape, dtype=hidden.dtype, device=dev) if needs[0] else None
         dw = torch.empty(weight.shape, dtype=weight.dtype, device=dev) if needs[1] else None
-        db = torch.empty(weight.shape[0], dtype=weight.dtype, device=dev) if needs[2] else None
-        need = L.tnp_vocab_ce_workspace_bytes(ctypes.byref(a), 1)
-        ws = _workspace(need, dev)
-        p = lambda t: None if t is None else t.data_ptr()
-        _lib.check(L.tnp_vocab_ce_backward(ctypes.byref(a), g.data_ptr(), p(dx), p(dw), p(db), ws.data_ptr(), need, _lib.raw_stream()),
-                   'tnp_vocab_ce_backward')
+        db = torch.empty(bias.shape, dtype=bias.dtype, device=dev) if needs[2] else None
+        need = L.tnp_vocab_ce_workspace_bytes(ref, 1)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        _lib.check(L.tnp_vocab_ce_backward(ref, g.data_ptr(), _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db), ws.data_ptr(), need,
+                                           _lib.raw_stream()), 'tnp_vocab_ce_backward')
     return dx, dw, db
 
 
@@ -188,9 +186,7 @@ class _VocabCeFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         hidden, weight, bias, target, saved = ctx.saved_tensors
-        n = ctx.needs_input_grad
-        return _ce_backward(grad, hidden, weight, bias, target, saved, ctx.reduction,
-                            (n[0], n[1], n[2] and bias is not None)) + (None, None)
+        return _ce_backward(grad, hidden, weight, bias, target, saved, ctx.reduction, ctx.needs_input_grad) + (None, None)
 
 
 def check_cross_entropy(hidden, weight, target, bias, reduction):
@@ -228,21 +224,9 @@ def vocab_cross_entropy(hidden, weight, target, bias=None, reduction='mean'):
     NaN."""
     check_cross_entropy(hidden, weight, target, bias, reduction)
     red = _REDUCTIONS[reduction]
-    shape = target.shape
-    t = target.reshape(-1)
-    if t.dtype != torch.int64 or not t.is_contiguous():
-        t = t.to(torch.int64).contiguous()
-    x, w = hidden.reshape(-1, hidden.shape[-1]) if hidden.dim() != 2 else hidden, weight
-    if x.shape[0] == 0:                                                       # no rows: an empty / zero loss with zero gradients
+    if target.numel() == 0:                                              # no rows: an empty / zero loss with zero gradients
         zero = hidden.float().sum() + weight[:0].float().sum() + (bias[:0].float().sum() if bias is not None else 0.0)
-        return zero.expand(shape) if red == 0 else zero
-    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
-        x = x.contiguous()
-    if w.stride(1) != 1 or (w.shape[0] > 1 and w.stride(0) < w.shape[1]):
-        w = w.contiguous()
-    b = bias.contiguous() if bias is not None else None
-    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or (b is not None and b.requires_grad)):
-        loss = _VocabCeFn.apply(x, w, b, t, red)
-    else:
-        loss, _ = _ce_forward(x, w, b, t, red, False)
-    return loss.reshape(shape) if red == 0 else loss[0]
+        return zero.expand(target.shape) if red == 0 else zero
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        return _VocabCeFn.apply(hidden, weight, bias, target, red)
+    return _ce_forward(hidden, weight, bias, target, red, False)[0]
