@@ -54,17 +54,18 @@ __device__ __forceinline__ float ce_rows_amax(const T *x, int64_t ld, int64_t r0
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const uint32_t q = k + u * 256, row = q / per, c = q - row * per;
-            in[u] = q < n && (!target || target[r0 + row] >= 0);
-            if (in[u]) p[u] = *(const Pack<T, VE> *)(x + (r0 + row) * ld + c * VE);
+            in[u] = q < n;                                       // behind the end: the first row again, loads under a condition wait
+            const int64_t r = r0 + (in[u] ? row : 0);            // for each other
+            if (target) in[u] = in[u] && target[r] >= 0;
+            p[u] = *(const Pack<T, VE> *)(x + r * ld + (q < n ? c * VE : 0));
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (in[u])
 #pragma unroll
-                for (int e = 0; e < VE; ++e) {
-                    const float v = fabsf(to_f32(p[u].v[e]));
-                    if (v < __builtin_inff()) a = fmaxf(a, v);       // infinities and NaN do not set the scale
-                }
+            for (int e = 0; e < VE; ++e) {
+                const float v = fabsf(to_f32(p[u].v[e]));
+                a = fmaxf(a, in[u] && v < __builtin_inff() ? v : 0.0f);      // infinities and NaN do not set the scale
+            }
     }
     return a;
 }
@@ -104,6 +105,7 @@ __device__ __forceinline__ void ce_pack_rows(const T *src, int64_t ld, int64_t r
     const bool live = r < rows && (!target || target[r] >= 0);
     const int ch = lane & 3, c0 = SPLIT ? (ch & 1) * 8 : ch * 8;
     constexpr int U = 4;                                         // panels in flight
+    const T *from = src + (live ? r : 0) * ld;                   // rows and columns that are not there: row 0, column 0, not used
     half_t *out = dst + r * 32 + ch * 8;
     for (int p = 0; p < panels; p += U) {
         Pack<T, VE> q[U][NV / VE];
@@ -112,10 +114,7 @@ __device__ __forceinline__ void ce_pack_rows(const T *src, int64_t ld, int64_t r
 #pragma unroll
             for (int k = 0; k < NV / VE; ++k) {
                 const int c = (p + u) * (SPLIT ? 16 : 32) + c0 + k * VE;
-                if (live && p + u < panels && c < D) q[u][k] = *(const Pack<T, VE> *)(src + r * ld + c);
-                else
-#pragma unroll
-                    for (int m = 0; m < VE; ++m) q[u][k].v[m] = from_f32<T>(0.0f);
+                q[u][k] = *(const Pack<T, VE> *)(from + (c < D ? c : 0));
             }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -123,7 +122,8 @@ __device__ __forceinline__ void ce_pack_rows(const T *src, int64_t ld, int64_t r
             half8 o;
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                const float v = ldexpf(to_f32(q[u][k / VE].v[k % VE]), -e);
+                const bool there = live && (p + u) * (SPLIT ? 16 : 32) + c0 + k < D;
+                const float v = there ? ldexpf(to_f32(q[u][k / VE].v[k % VE]), -e) : 0.0f;
                 const half_t hi = (half_t)v;
                 o[k] = SPLIT && ch >= 2 ? (fabsf(v) < 65504.0f ? (half_t)(v - (float)hi) : (half_t)0.0f) : hi;
             }
@@ -184,7 +184,8 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) ce_logits_kernel(CeLogits a, c
     const int64_t vbase = a.v0 + (int64_t)tv * BM, ibase = (int64_t)ti * BN;
     for (int j = threadIdx.x; j < BM; j += WM * WN * 64) sb[j] = vbase + j < a.V ? ce_bias(bias, (int)vbase + j) : CE_NEG_INF;
     f32x16 acc[TM][TN];
-    gemm_tile<SPLIT, false, false, BM, BN, WM, WN, NST>(a.w, a.x, vbase, 0, 0, ibase, 0, 0, 0, a.steps, lds, acc);
+    float none[TM];
+    gemm_tile<SPLIT, false, false, BM, BN, WM, WN, NST, false>(a.w, a.x, vbase, 0, 0, ibase, 0, 0, 0, a.steps, lds, acc, false, none);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
     const int wm = wave / WN, wn = wave % WN;
     const float scale = ldexpf(CE_LOG2E, a.sc->ex + a.sc->ew);
@@ -518,10 +519,8 @@ struct CeGrads {
     const float *grad;
     const int64_t *target;    // dhidden: rows with a negative target are zero
     int reduction, D;
-    // column sums of G (dbias): a panel x a share of the rows per workgroup
-    int64_t g_rows, ldb;
-    int col_blocks, shares;
-    float *part_b;            // [shares][ldb]
+    float *part_b;            // dbias: [w.splits][ldb] sums in G's stored column order, or NULL
+    int64_t ldb;
 };
 
 // WEIGHT: dweight (G read transposed, output rows = vocabulary entries in G's stored column order), else dhidden
@@ -537,10 +536,23 @@ __device__ __forceinline__ void ce_grad_tile(const CeGrads &a, const CeGrad &c, 
     f32x16 acc[TM][TN];
     constexpr int PC = SPLIT ? 16 : 32;                        // columns per panel
     const int gp = WEIGHT ? (int)(r0 / PC) : 0, op = d0 / PC;
-    gemm_tile<SPLIT, WEIGHT, true, BM, BN, WM, WN, NST>(c.g, c.o, WEIGHT ? 0 : r0, gp, c.g_panels - gp, c.ok0, op, c.o_panels - op, s0, s1, lds,
-                                                        acc);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
     const int wm = wave / WN, wn = wave % WN;
+    // dbias: the sums over k of G^T, which the first column of waves of the first column of tiles has in registers anyway
+    const bool sums = WEIGHT && a.part_b && td == 0 && wn == 0;
+    float asum[TM];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) asum[i] = 0.0f;
+    gemm_tile<SPLIT, WEIGHT, true, BM, BN, WM, WN, NST, WEIGHT>(c.g, c.o, WEIGHT ? 0 : r0, gp, c.g_panels - gp, c.ok0, op, c.o_panels - op, s0, s1,
+                                                                lds, acc, sums, asum);
+    if (sums) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            const float t = asum[i] + __shfl_xor(asum[i], 32);
+            if (h == 0) a.part_b[z * a.ldb + r0 + wm * TM * 32 + i * 32 + lane] = t;
+        }
+    }
+    if (!c.out) return;                                        // only dbias is asked for
     const float f = c.part ? 1.0f : ce_unscale(a.sc, a.grad, a.reduction, WEIGHT ? a.sc->ex : a.sc->ew);
 #pragma unroll
     for (int i = 0; i < TM; ++i)
@@ -566,51 +578,13 @@ __device__ __forceinline__ void ce_grad_tile(const CeGrads &a, const CeGrad &c, 
         }
 }
 
-// one panel of G per workgroup and share of the rows: lane = (row, chunk of eight columns)
-template <int NW> __device__ __forceinline__ void ce_colsum(const CeGrads &a, int bid, char *lds) {
-    float(*sh)[4][8] = (float(*)[4][8])lds;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, panel = bid / a.shares, share = bid % a.shares;
-    const int64_t per = (a.g_rows / 16 + a.shares - 1) / a.shares * 16, r0 = share * per, r1 = r0 + per < a.g_rows ? r0 + per : a.g_rows;
-    const half_t *g = a.x.g.p + (int64_t)panel * a.g_rows * 32 + lane * 8;
-    float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    constexpr int U = 8;
-    for (int64_t r = r0 + wave * 16; r < r1; r += NW * 16 * U) {
-        half8 v[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (r + NW * 16 * u < r1) v[u] = *(const half8 *)(g + (r + NW * 16 * u) * 32);
-            else
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[u][e] = (half_t)0.0f;
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) s[e] += (float)v[u][e];
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-        for (int o = 4; o < 64; o <<= 1) s[e] += __shfl_xor(s[e], o);
-    if (lane < 4)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sh[wave][lane][e] = s[e];
-    __syncthreads();
-    if (threadIdx.x < 32) {
-        float t = 0.0f;
-        for (int w = 0; w < NW; ++w) t += sh[w][threadIdx.x >> 3][threadIdx.x & 7];
-        a.part_b[share * a.ldb + panel * 32 + threadIdx.x] = t;
-    }
-}
-
-// Both gradient products and the column sums in one launch: they read the same G, and the workgroups of one fill what the others
-// leave idle.
+// Both gradient products in one launch: they read the same G, and the workgroups of one fill what the other's leave idle.
 template <typename T, bool SPLIT, int BM, int BN, int WM, int WN, int NST>
 __global__ void __launch_bounds__(WM *WN * 64, 2) ce_grads_kernel(CeGrads a) {
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int bid = blockIdx.x;
     if (bid < a.x.blocks) ce_grad_tile<T, SPLIT, false, BM, BN, WM, WN, NST>(a, a.x, bid, lds);
-    else if (bid < a.x.blocks + a.w.blocks) ce_grad_tile<T, SPLIT, true, BM, BN, WM, WN, NST>(a, a.w, bid - a.x.blocks, lds);
-    else ce_colsum<WM * WN>(a, bid - a.x.blocks - a.w.blocks, lds);
+    else ce_grad_tile<T, SPLIT, true, BM, BN, WM, WN, NST>(a, a.w, bid - a.x.blocks, lds);
 }
 
 // out[r][d] = factor * sum over splits of part[s][r][d], the splits in their order; VE elements per thread
@@ -643,27 +617,16 @@ __device__ __forceinline__ void ce_join(const CeGrads &a, const CeGrad &c, bool 
 
 // what is left of a piece in one launch: dhidden and dweight from their partial sums (bx / bw workgroups), dbias
 template <typename T, int VE>
-__global__ void __launch_bounds__(256) ce_join_kernel(CeGrads a, int bx, int bw, int split, int live, T *dbias) {
+__global__ void __launch_bounds__(256) ce_join_kernel(CeGrads a, int bx, int bw, int live, T *dbias) {
     const int bid = blockIdx.x;
     if (bid < bx) { ce_join<T, VE>(a, a.x, false, bid); return; }
     if (bid < bx + bw) { ce_join<T, VE>(a, a.w, true, bid - bx); return; }
-    // 32 entries per workgroup, eight threads share the row shares of each
-    __shared__ float sh[8][32];
-    const int seg = threadIdx.x >> 5, v = (bid - bx - bw) * 32 + (threadIdx.x & 31);
+    const int v = (bid - bx - bw) * 256 + threadIdx.x;
+    if (v >= live) return;
+    const int pos = (v & ~12) | ((v & 4) << 1) | ((v & 8) >> 1);
     float s = 0.0f;
-    if (v < live) {
-        const int pos = (v & ~12) | ((v & 4) << 1) | ((v & 8) >> 1);
-        for (int k = seg; k < a.shares; k += 8) {
-            const float *p = a.part_b + k * a.ldb;
-            s += split ? p[(pos >> 4) * 32 + (pos & 15)] + p[(pos >> 4) * 32 + (pos & 15) + 16] : p[pos];
-        }
-    }
-    sh[seg][threadIdx.x & 31] = s;
-    __syncthreads();
-    if (seg == 0 && v < live) {
-        for (int k = 1; k < 8; ++k) s += sh[k][threadIdx.x];
-        dbias[v] = from_f32<T>(s * ce_unscale(a.sc, a.grad, a.reduction, 0));
-    }
+    for (int k = 0; k < a.w.splits; ++k) s += a.part_b[k * a.ldb + pos];
+    dbias[v] = from_f32<T>(s * ce_unscale(a.sc, a.grad, a.reduction, 0));
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------
@@ -696,7 +659,9 @@ static int ce_score_blocks(int V) {
     const int g = (V + 63) / 64;
     return g < 1024 ? g : 1024;
 }
-static int ce_rows_shift(int64_t M) { return M <= CE_SCORE_ROWS ? 2 : 5; }
+// rows per workgroup of the join: few rows share the threads, many rows with few parts keep the workgroups few (each draws a ticket:
+// 24576 rows of 16 parts 14 us at 32 rows, 7 at 128; 16384 rows of 512 parts 20 us at 32 rows, 37 at 128)
+static int ce_rows_shift(int64_t M, int parts) { return M <= CE_SCORE_ROWS ? 2 : M >= 8192 && parts <= 32 ? 7 : 5; }
 
 static bool ce_big(const CeShape &s) { return (s.Mp / 256) * (int64_t)(s.Vp / 256) >= 512; }
 
@@ -710,7 +675,7 @@ static CeForward ce_forward_layout(const tnp_vocab_ce *p, void *ws) {
     f.amax = (float *)w; w += ce_up(2 * CE_AMAX_BLOCKS * 4);
     f.part = (float2 *)w; w += ce_up((size_t)f.parts * rows * 8);
     f.tlogit = (float *)w; w += ce_up(rows * 4);
-    f.sums = (double2 *)w; w += ce_up((size_t)((s.Mp >> ce_rows_shift(p->M)) + 1) * 16);
+    f.sums = (double2 *)w; w += ce_up((size_t)((s.Mp >> ce_rows_shift(p->M, f.parts)) + 1) * 16);
     f.saved = ce_saved(s, p->saved ? p->saved : w);
     if (!p->saved) w += ce_scores(p) ? 256 : f.saved.bytes;
     f.bytes = (size_t)(w - (char *)ws);
@@ -724,7 +689,6 @@ struct CeBackward {
     half_t *g;
     int bm, bn, splits_x, splits_w;
     float *part_x, *part_w, *part_b;
-    int shares;
     size_t bytes;
 };
 static constexpr size_t CE_PIECE_BYTES = (size_t)512 << 20;
@@ -752,7 +716,6 @@ static CeBackward ce_backward_layout(const tnp_vocab_ce *p, void *ws) {
     const int64_t nx = (sx + each / 2) / each, nw = (sw + each / 2) / each;
     b.splits_x = (int)(nx < 1 ? 1 : nx);
     b.splits_w = (int)(nw < 1 ? 1 : nw);
-    b.shares = (int)(s.Mp / 256 < 16 ? s.Mp / 256 : 16);                   // at least 256 rows of a panel each
     char *w = (char *)ws;
     b.g = (half_t *)w; w += ce_up((size_t)s.Mp * b.ldg * 2);
     b.part_x = b.splits_x > 1 || b.pieces > 1 ? (float *)w : nullptr;
@@ -760,7 +723,7 @@ static CeBackward ce_backward_layout(const tnp_vocab_ce *p, void *ws) {
     b.part_w = b.splits_w > 1 ? (float *)w : nullptr;
     if (b.part_w) w += ce_up((size_t)b.splits_w * b.piece * p->D * 4);
     b.part_b = p->bias ? (float *)w : nullptr;
-    if (b.part_b) w += ce_up((size_t)b.shares * b.ldg * 4);
+    if (b.part_b) w += ce_up((size_t)b.splits_w * b.piece * 4);
     b.bytes = (size_t)(w - (char *)ws);
     return b;
 }
@@ -817,9 +780,10 @@ static int ce_launch_grads(CeGrads &a, hipStream_t s) {
     for (CeGrad *c : {&a.x, &a.w}) {
         c->tiles_r = (int)((c->rows + BM - 1) / BM);
         c->tiles_d = (a.D + BN - 1) / BN;
-        c->blocks = c->out ? gemm_grid((int64_t)c->tiles_r * c->tiles_d) * c->splits : 0;
+        if (!c->out) c->tiles_d = 1;
+        c->blocks = c->out || (c == &a.w && a.part_b) ? gemm_grid((int64_t)c->tiles_r * c->tiles_d) * c->splits : 0;
     }
-    const int blocks = a.x.blocks + a.w.blocks + a.col_blocks * a.shares;
+    const int blocks = a.x.blocks + a.w.blocks;
     if (blocks) {
         hipLaunchKernelGGL(kern, dim3(blocks), dim3(WM * WN * 64), smem, s, a);
         TNP_HIP(hipGetLastError());
@@ -875,7 +839,7 @@ static int ce_forward(const tnp_vocab_ce *p, const CeForward &f, float *loss, hi
         a.part = f.part; a.tlogit = f.tlogit;
         if ((rc = ce_logits<T, SPLIT, false>(a, sh.Vp, ce_big(sh), (const T *)p->bias, s))) return rc;
     }
-    const int rsh = ce_rows_shift(p->M);
+    const int rsh = ce_rows_shift(p->M, f.parts);
     const int64_t cover = p->saved ? sh.Mp : p->M;
     hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)((cover + (1 << rsh) - 1) >> rsh)), dim3(256), 0, s, f.part,
                        ce_scores(p) ? (int64_t)CE_SCORE_ROWS : sh.Mp, f.parts, f.tlogit, p->target, p->M, cover, p->V, rsh, p->reduction,
@@ -912,19 +876,18 @@ static int ce_backward(const tnp_vocab_ce *p, const CeBackward &b, const float *
         c.w.o = x;
         c.w.rows = live; c.w.out0 = v0; c.w.out = dweight; c.w.part = b.part_w; c.w.part_rows = b.piece; c.w.splits = b.splits_w;
         c.w.steps = (int)(sh.Mp / ks);
-        c.shares = b.shares; c.part_b = b.part_b; c.ldb = b.ldg; c.g_rows = sh.Mp;
-        c.col_blocks = dbias ? cols / ks : 0;
+        c.part_b = dbias ? b.part_b : nullptr; c.ldb = b.piece;
         rc = b.bm == 256 ? (b.bn == 256 ? ce_launch_grads<T, SPLIT, 256, 256, 2, 4, 4>(c, s) : ce_launch_grads<T, SPLIT, 256, 128, 2, 2, 3>(c, s))
-                         : ce_launch_grads<T, SPLIT, 128, 128, 2, 2, 3>(c, s);
+                         : ce_launch_grads<T, SPLIT, 128, 128, 2, 2, 4>(c, s);
         if (rc) return rc;
         const int ve = sh.D % 4 == 0 ? 4 : 1;
         const int64_t per = 256 * ve;
         const int bx = dhidden && b.part_x && last ? (int)((c.x.rows * sh.D + per - 1) / per) : 0;
-        const int bw = dweight && b.part_w ? (int)((c.w.rows * sh.D + per - 1) / per) : 0, bb = dbias ? (live + 31) / 32 : 0;
+        const int bw = dweight && b.part_w ? (int)((c.w.rows * sh.D + per - 1) / per) : 0, bb = dbias ? (live + 255) / 256 : 0;
         if (bx + bw + bb) {
             T *db = dbias ? (T *)dbias + v0 : nullptr;
-            if (ve == 4) hipLaunchKernelGGL((ce_join_kernel<T, 4>), dim3(bx + bw + bb), dim3(256), 0, s, c, bx, bw, (int)SPLIT, live, db);
-            else hipLaunchKernelGGL((ce_join_kernel<T, 1>), dim3(bx + bw + bb), dim3(256), 0, s, c, bx, bw, (int)SPLIT, live, db);
+            if (ve == 4) hipLaunchKernelGGL((ce_join_kernel<T, 4>), dim3(bx + bw + bb), dim3(256), 0, s, c, bx, bw, live, db);
+            else hipLaunchKernelGGL((ce_join_kernel<T, 1>), dim3(bx + bw + bb), dim3(256), 0, s, c, bx, bw, live, db);
             TNP_HIP(hipGetLastError());
         }
     }

@@ -190,6 +190,20 @@ __device__ __forceinline__ void step_mfma(const half8 (&fa)[2 * TM], const half8
                 acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[2 * i + wa[k]], fb[2 * j + wb[k]], acc[i][j], 0, 0, 0);
 }
 
+// sums over k of an operand's values, per row of the block: asum[i] += what this lane holds of block i (half of the k values; the
+// other half of the wave holds the rest)
+template <int TM> __device__ __forceinline__ void step_row_sums(const half8 (&fa)[2 * TM], float (&asum)[TM]) {
+    typedef half_t half2v __attribute__((ext_vector_type(2)));
+    const half2v one = {(half_t)1.0f, (half_t)1.0f};
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                asum[i] = __builtin_amdgcn_fdot2(half2v{fa[2 * i + w][2 * e], fa[2 * i + w][2 * e + 1]}, one, asum[i], false);
+}
+
 // Accumulates steps [s0, s1) of the tile at (row ar, panel ap) of a and (br, bp) of b into acc; al / bl: panels from there to the last
 // (KS).  LDS: NST * (BM + BN) * 64 bytes.
 //
@@ -197,9 +211,11 @@ __device__ __forceinline__ void step_mfma(const half8 (&fa)[2 * TM], const half8
 // half multiplies the step it has fetched; a barrier per turn keeps them half a step apart.  In lockstep both waves of a SIMD would
 // fetch at the same time and leave the matrix cores idle meanwhile (2150 cycles per step of 1024 cycles of matrix work).  With
 // four waves the other workgroup on the CU fills that time.
-template <bool SPLIT, bool A_KS, bool B_KS, int BM, int BN, int WM, int WN, int NST>
+// SUMS: with `sums` (the same for the wave), asum[] gathers the row sums of a as well (step_row_sums).
+template <bool SPLIT, bool A_KS, bool B_KS, int BM, int BN, int WM, int WN, int NST, bool SUMS>
 __device__ __forceinline__ void gemm_tile(const GemmOperand &a, const GemmOperand &b, int64_t ar, int64_t ap, int al, int64_t br, int64_t bp, int bl,
-                                          int s0, int s1, char *lds, f32x16 (&acc)[BM / WM / 32][BN / WN / 32]) {
+                                          int s0, int s1, char *lds, f32x16 (&acc)[BM / WM / 32][BN / WN / 32], bool sums,
+                                          float (&asum)[BM / WM / 32]) {
     constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, STAGE = (BM + BN) * 64;
     constexpr bool TURNS = NW == 8;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -251,12 +267,14 @@ __device__ __forceinline__ void gemm_tile(const GemmOperand &a, const GemmOperan
             __builtin_amdgcn_sched_barrier(0);
             __builtin_amdgcn_s_setprio(1);
             step_mfma<SPLIT, TM, TN>(fa, fb, acc);
+            if (SUMS && sums) step_row_sums<TM>(fa, asum);
             __builtin_amdgcn_s_setprio(0);
             __builtin_amdgcn_sched_barrier(0);
             stage_barrier_only();
             __builtin_amdgcn_sched_barrier(0);
         } else {
             step_mfma<SPLIT, TM, TN>(fa, fb, acc);
+            if (SUMS && sums) step_row_sums<TM>(fa, asum);
             if (s + 1 < s1) landed(s1 - 2 - s);
         }
     }
