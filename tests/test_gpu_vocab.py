@@ -310,6 +310,38 @@ def test_no_row_is_there(m, dtype):
     assert vocab.vocab_cross_entropy(x[:0], w, gone[:0], reduction='none').shape == (0,)
 
 
+@pytest.mark.parametrize('pattern', ['first', 'last', 'one', 'blocks', 'alternate'])
+@pytest.mark.parametrize('m', [70, 3000])
+def test_where_the_absent_rows_are(m, pattern):
+    x, w, b, t = _case(m, 270, 24, torch.bfloat16, 35)
+    i = torch.arange(m, device='cuda')
+    gone = {'first': i < m - 3, 'last': i > 2, 'one': i != m // 2, 'blocks': (i // 16) % 3 != 1, 'alternate': i % 2 == 0}[pattern]
+    t = torch.where(gone, -1, t)
+    with torch.no_grad():
+        x[gone] = float('nan')
+    up = torch.randn(m, device='cuda', generator=_gen(36))
+    loss, bound, want, bounds = _formula(x, w, b, t, up)
+    out = vocab.vocab_cross_entropy(x, w, t, bias=b, reduction='none')
+    _within(out.detach(), loss, bound)
+    for a, e, lim in zip(torch.autograd.grad(out, (x, w, b), up), want, bounds):
+        _within(a, e, lim)
+
+
+def test_many_rows_with_a_small_vocabulary():
+    """more rows than 256 per packing workgroup, and shares of the rows that are absent altogether"""
+    m = 140001
+    x, w, b, t = _case(m, 9, 5, torch.float32, 37, absent=0.3)
+    t[1000:3000] = -1
+    t[-700:] = -1
+    loss, bound, want, bounds = _formula(x, w, b, t, torch.ones(m, device='cuda'))
+    out = vocab.vocab_cross_entropy(x, w, t, bias=b, reduction='sum')
+    _within(out.detach(), loss.sum(), bound.sum() + 2.0 ** -23 * loss.sum())
+    for a, e, lim in zip(torch.autograd.grad(out, (x, w, b)), want, bounds):
+        _within(a, e, lim)
+    with torch.no_grad():
+        _within(vocab.vocab_cross_entropy(x, w, t, bias=b, reduction='none'), loss, bound)
+
+
 @pytest.mark.parametrize('m', [9, 150])
 def test_targets_past_the_vocabulary_show(m):
     x, w, b, t = _case(m, 90, 16, torch.float32, 41)
