@@ -482,3 +482,60 @@ def test_token_model_trains_a_run_of_the_operators():
     assert abs(float(loss) - float(ref)) < lim * float(ref)
     for a, c in zip(got, want):
         assert float((a.double() - c).abs().max()) < lim * max(0.1, float(c.abs().max()))
+
+
+def test_registered_operators():
+    """torch.ops.trajnet.*: the eager calls' bits, schema and fake tensors, and a compiled step without a graph break"""
+    from trajnetplusplusbaselines_amd import ops  # noqa: F401
+    x, w, b, t = _case(90, 70, 24, torch.float32, 110, absent=0.1)
+    with torch.no_grad():
+        x.nan_to_num_()
+    tok = torch.randint(-1, 70, (9, 10), device='cuda', generator=_gen(111))
+    out = torch.ops.trajnet.token_embedding(tok, w, 3.0)
+    assert torch.equal(out, vocab.token_embedding(tok, w, 3.0))
+    up = torch.randn(out.shape, device='cuda', generator=_gen(112))
+    assert torch.equal(torch.autograd.grad(out, w, up)[0], torch.autograd.grad(vocab.token_embedding(tok, w, 3.0), w, up)[0])
+    for bias in (b, None):
+        leaves = (x, w) if bias is None else (x, w, b)
+        for red in ('mean', 'none'):
+            loss = torch.ops.trajnet.vocab_cross_entropy(x, w, t, bias, red)[0]
+            ref = vocab.vocab_cross_entropy(x, w, t, bias=bias, reduction=red)
+            assert torch.equal(loss, ref)
+            g = torch.ones_like(loss)
+            assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(loss, leaves, g), torch.autograd.grad(ref, leaves, g)))
+    tests = ('test_schema', 'test_faketensor')
+    torch.library.opcheck(torch.ops.trajnet.token_embedding, (tok, w, 3.0), test_utils=tests)
+    torch.library.opcheck(torch.ops.trajnet.vocab_cross_entropy, (x.detach(), w.detach(), t, b.detach(), 'mean'), test_utils='test_schema')
+
+    def step(x, w, b, t, tok):
+        return vocab.vocab_cross_entropy(x, w, t, bias=b) + vocab.token_embedding(tok, w, 2.0).square().mean()
+
+    want = torch.autograd.grad(step(x, w, b, t, tok), (x, w, b))
+    got = torch.autograd.grad(torch.compile(step, fullgraph=True, backend='aot_eager')(x, w, b, t, tok), (x, w, b))
+    # the compiled graph may sum the two gradients of w in the other order: one rounding
+    assert all(torch.allclose(p, q, rtol=2.0 ** -22, atol=0.0) for p, q in zip(got, want))
+
+
+def test_a_weight_that_changes_before_the_backward_pass_is_noticed():
+    x, w, b, t = _case(70, 50, 16, torch.float32, 120)
+    loss = vocab.vocab_cross_entropy(x, w, t, bias=b)
+    with torch.no_grad():
+        w.mul_(2.0)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        torch.autograd.grad(loss, w)
+
+
+def test_no_gradient_of_a_gradient():
+    x, w, b, t = _case(70, 50, 16, torch.float32, 121)
+    g, = torch.autograd.grad(vocab.vocab_cross_entropy(x, w, t, bias=b), w, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), w)
+
+
+def test_backward_twice_and_broadcast_gradient():
+    x, w, b, t = _case(80, 60, 16, torch.bfloat16, 122, absent=0.2)
+    out = vocab.vocab_cross_entropy(x, w, t, bias=b, reduction='none')
+    one = torch.ones((), device='cuda').expand(80)                       # stride 0
+    first = torch.autograd.grad(out, (x, w, b), one, retain_graph=True)
+    second = torch.autograd.grad(out, (x, w, b), torch.ones(80, device='cuda'))
+    assert all(torch.equal(p, q) for p, q in zip(first, second))

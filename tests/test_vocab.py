@@ -79,3 +79,23 @@ def test_c_entries_refuse_on_the_host():
 
 def test_struct_mirror():
     assert _lib.lib().tnp_abi_sizeof(8) == ctypes.sizeof(vocab.VocabCe)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+def test_saved_bytes_from_the_sizes(dtype):
+    for m, v, d in ((1, 1, 1), (256, 256, 16), (257, 300, 33), (5000, 70000, 200)):
+        a = vocab.VocabCe(dtype=vocab._DTYPES[dtype], M=m, V=v, D=d, ld_hidden=d, ld_weight=d)
+        assert _lib.lib().tnp_vocab_ce_saved_bytes(ctypes.byref(a)) == vocab.saved_bytes(m, v, d, dtype)
+
+
+def test_fake_implementations():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from trajnetplusplusbaselines_amd import ops  # noqa: F401
+    with FakeTensorMode():
+        w = torch.empty(30, 8, dtype=torch.bfloat16)
+        tok = torch.empty(5, 7, dtype=torch.int64)
+        out = torch.ops.trajnet.token_embedding(tok, w, 2.0)
+        assert out.shape == (5, 7, 8) and out.dtype == torch.bfloat16
+        loss, saved = torch.ops.trajnet.vocab_cross_entropy(out, w, tok, None, 'mean')
+        assert loss.shape == () and loss.dtype == torch.float32 and saved.dtype == torch.uint8
+        assert torch.ops.trajnet.vocab_cross_entropy(out, w, tok, torch.empty(30, dtype=torch.bfloat16), 'none')[0].shape == (5, 7)

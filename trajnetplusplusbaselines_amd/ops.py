@@ -18,6 +18,8 @@ tensor raises, as everywhere in this package.
     pool_embed_sparse(winners, values, scene_start, weight, bias?, relu)                -> fp32 [M, N1]
     constant_velocity(last, prev, n_predict)                                            -> fp64 [n_predict, N, 2]
     sf_rollout(state, scene_start, n_max, n_predict, v0, sigma, tau)                    -> fp64 [n_predict, M, 2]
+    token_embedding(tokens, weight, scale)                                              -> weight dtype [..., D]           (+ autograd)
+    vocab_cross_entropy(hidden, weight, target, bias?, reduction)                       -> (fp32 loss, uint8 saved)        (+ autograd)
     lstm_sequence(observed, goals?, batch_split, truth?, t_dec, pad_to, model, params)  -> (fp32 [S, M, 5], fp32 [S', M, 2])
     lstm_sequence_train(same arguments)             -> (fp32 [S, M, 5], fp32 [S', M, 2], fp32 [M, H], int64 handle)   (+ autograd)
     lstm_sequence_backward(handle, d_rel, d_pred, d_hlast, params)                      -> list of parameter gradients
@@ -29,7 +31,7 @@ from typing import List, Optional, Tuple
 
 import torch
 
-from . import _lib
+from . import _lib, vocab
 
 _POOL = {'occupancy': _lib.POOL_OCCUPANCY, 'directional': _lib.POOL_DIRECTIONAL, 'social': _lib.POOL_SOCIAL}
 
@@ -133,6 +135,92 @@ def _linear_backward(ctx, grad):
 
 
 linear.register_autograd(_linear_backward, setup_context=_linear_setup)
+
+
+@torch.library.custom_op('trajnet::token_embedding', mutates_args=())
+def token_embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float) -> torch.Tensor:
+    """scale * weight[tokens], a zero row for a negative token (vocab.token_embedding, tnp_token_embedding_forward)."""
+    return vocab._embedding_forward(tokens, weight, vocab.check_embedding(tokens, weight, scale))
+
+
+@token_embedding.register_fake
+def _(tokens, weight, scale):
+    return weight.new_empty(tuple(tokens.shape) + (weight.shape[1],))
+
+
+@torch.library.custom_op('trajnet::token_embedding_backward', mutates_args=())
+def token_embedding_backward(grad: torch.Tensor, tokens: torch.Tensor, vocab_size: int, scale: float) -> torch.Tensor:
+    """dense gradient of the table (tnp_token_embedding_backward)"""
+    _dev(grad, 'grad')
+    return vocab._embedding_backward(grad, tokens, vocab_size, scale)
+
+
+@token_embedding_backward.register_fake
+def _(grad, tokens, vocab_size, scale):
+    return grad.new_empty((vocab_size, grad.shape[-1]))
+
+
+def _token_embedding_setup(ctx, inputs, output):
+    tokens, weight, ctx.scale = inputs
+    ctx.vocab_size = weight.shape[0]
+    ctx.save_for_backward(tokens)
+
+
+def _token_embedding_backward(ctx, grad):
+    return None, torch.ops.trajnet.token_embedding_backward(grad, ctx.saved_tensors[0], ctx.vocab_size, ctx.scale), None
+
+
+token_embedding.register_autograd(_token_embedding_backward, setup_context=_token_embedding_setup)
+
+
+@torch.library.custom_op('trajnet::vocab_cross_entropy', mutates_args=())
+def vocab_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, bias: Optional[torch.Tensor],
+                        reduction: str) -> Tuple[torch.Tensor, torch.Tensor]:
+    """vocab.vocab_cross_entropy; the second output is what the backward pass reads (tnp_vocab_ce.saved)."""
+    vocab.check_cross_entropy(hidden, weight, target, bias, reduction)
+    if target.numel() == 0:
+        loss = hidden.new_zeros(target.shape if reduction == 'none' else (), dtype=torch.float32)
+        return loss, hidden.new_empty(vocab.saved_bytes(0, weight.shape[0], weight.shape[1], weight.dtype), dtype=torch.uint8)
+    return vocab._ce_forward(hidden, weight, bias, target, vocab._REDUCTIONS[reduction], True)
+
+
+@vocab_cross_entropy.register_fake
+def _(hidden, weight, target, bias, reduction):
+    loss = hidden.new_empty(target.shape if reduction == 'none' else (), dtype=torch.float32)
+    return loss, hidden.new_empty(vocab.saved_bytes(target.numel(), weight.shape[0], weight.shape[1], weight.dtype), dtype=torch.uint8)
+
+
+@torch.library.custom_op('trajnet::vocab_cross_entropy_backward', mutates_args=())
+def vocab_cross_entropy_backward(grad: torch.Tensor, hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor,
+                                 bias: Optional[torch.Tensor], saved: torch.Tensor,
+                                 reduction: str) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """gradients of hidden, weight and bias (without a bias the third is empty)"""
+    _dev(grad, 'grad')
+    if target.numel() == 0:
+        return torch.zeros_like(hidden), torch.zeros_like(weight), torch.zeros_like(bias) if bias is not None else weight.new_zeros(0)
+    dx, dw, db = vocab._ce_backward(grad, hidden, weight, bias, target, saved, vocab._REDUCTIONS[reduction], (True, True, bias is not None))
+    return dx, dw, db if db is not None else weight.new_empty(0)
+
+
+@vocab_cross_entropy_backward.register_fake
+def _(grad, hidden, weight, target, bias, saved, reduction):
+    return (hidden.new_empty(hidden.shape), weight.new_empty(weight.shape),
+            weight.new_empty(0) if bias is None else weight.new_empty(bias.shape))
+
+
+def _vocab_ce_setup(ctx, inputs, output):
+    hidden, weight, target, bias, ctx.reduction = inputs
+    ctx.save_for_backward(hidden, weight, target, bias, output[1])
+    ctx.mark_non_differentiable(output[1])
+
+
+def _vocab_ce_backward(ctx, grad, _):
+    hidden, weight, target, bias, saved = ctx.saved_tensors
+    dx, dw, db = torch.ops.trajnet.vocab_cross_entropy_backward(grad, hidden, weight, target, bias, saved, ctx.reduction)
+    return dx, dw, None, db if bias is not None else None, None
+
+
+vocab_cross_entropy.register_autograd(_vocab_ce_backward, setup_context=_vocab_ce_setup)
 
 
 @torch.library.custom_op('trajnet::pool_embed_sparse', mutates_args=())

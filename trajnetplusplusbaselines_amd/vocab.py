@@ -114,6 +114,9 @@ def token_embedding(tokens, weight, scale=1.0):
     """``scale * weight[tokens]``: tokens int64 / int32 of any shape, weight [V, D] -> tokens.shape + (D,) in weight's dtype, rounded
     once.  tokens < 0 (absent track): a row of zeros; tokens >= V: a row of NaN.  The gradient of ``weight`` is dense, summed in fp32
     in a fixed order (two calls give the same bits)."""
+    if torch.compiler.is_compiling():
+        from . import ops  # noqa: F401  (registers the operators)
+        return torch.ops.trajnet.token_embedding(tokens, weight, float(scale))
     scale = check_embedding(tokens, weight, scale)
     if weight.requires_grad and torch.is_grad_enabled():
         return _TokenEmbeddingFn.apply(tokens, weight, scale)
@@ -126,6 +129,13 @@ class VocabCe(ctypes.Structure):
     _fields_ = [('dtype', ctypes.c_int32), ('reduction', ctypes.c_int32), ('M', ctypes.c_int64), ('V', ctypes.c_int32),
                 ('D', ctypes.c_int32), ('hidden', ctypes.c_void_p), ('ld_hidden', ctypes.c_int64), ('weight', ctypes.c_void_p),
                 ('ld_weight', ctypes.c_int64), ('bias', ctypes.c_void_p), ('target', ctypes.c_void_p), ('saved', ctypes.c_void_p)]
+
+
+def saved_bytes(rows, entries, columns, dtype):
+    """tnp_vocab_ce_saved_bytes() from the sizes alone (they may be symbolic while a graph is traced)"""
+    panels = (columns + 15) // 16 if dtype == torch.float32 else (columns + 31) // 32
+    up = lambda n: (n + 255) // 256 * 256
+    return 256 + 12 * up(rows) + 64 * panels * (up(rows) + up(entries))
 
 
 def _ce_args(hidden, weight, bias, target, reduction, saved):
@@ -222,6 +232,9 @@ def vocab_cross_entropy(hidden, weight, target, bias=None, reduction='mean'):
     fp32 operands are multiplied as two fp16 numbers each, scaled by the largest finite element of their tensor: an element below
     2^-16 of that one loses relative precision (2^-40 of the largest remains), a row of valid targets that holds an infinity gives
     NaN."""
+    if torch.compiler.is_compiling():
+        from . import ops  # noqa: F401  (registers the operators)
+        return torch.ops.trajnet.vocab_cross_entropy(hidden, weight, target, bias, reduction)[0]
     check_cross_entropy(hidden, weight, target, bias, reduction)
     red = _REDUCTIONS[reduction]
     if target.numel() == 0:                                              # no rows: an empty / zero loss with zero gradients
