@@ -121,6 +121,21 @@ def test_embedding_tokens_outside_the_table():
     assert bool((vocab.token_embedding(torch.tensor([-1], device='cuda'), nan) == 0).all())
 
 
+def test_embedding_rows_behind_four_gigabytes():
+    """row offsets that pass 32 bits, in bytes and in elements (a table and a gradient of 9 GB)"""
+    v, d = 4400000, 512
+    w = torch.empty(v, d, dtype=torch.float32, device='cuda')
+    at = [0, 1, v // 2, v - 2, v - 1]
+    rows = torch.randn(5, d, device='cuda', generator=_gen(4))
+    w[at] = rows
+    w.requires_grad_()
+    tok = torch.tensor(at + [v - 1], device='cuda')
+    out = vocab.token_embedding(tok, w)
+    assert torch.equal(out[:5], rows) and torch.equal(out[5], rows[4])
+    dw, = torch.autograd.grad(out, w, torch.ones_like(out))
+    assert dw[at, 0].tolist() == [1.0, 1.0, 1.0, 1.0, 2.0] and int((dw != 0).any(1).sum()) == 5
+
+
 def test_embedding_half_rows_that_are_not_sixteen_bytes():
     """every width of access: row lengths and base addresses of 2, 4 and 16 bytes"""
     g = _gen(3)
@@ -291,6 +306,49 @@ def test_masked_entries_and_rows(m):
         assert torch.equal(torch.isinf(got), t == hit)
         none = vocab.vocab_cross_entropy(x, w, t, bias=torch.full_like(b3, float('-inf')), reduction='none')
         assert torch.equal(torch.isnan(none), t >= 0) and bool((none[t < 0] == 0).all())
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('m', [6, 130])
+def test_every_entry_at_the_lowest_finite_value(m, dtype):
+    """a mask of the type's lowest value over the whole vocabulary: all entries alike, loss log V, p = 1 / V"""
+    x, w, b, t = _case(m, 300, 16, dtype, 23)
+    low = torch.full_like(b, torch.finfo(dtype).min).requires_grad_()
+    out = vocab.vocab_cross_entropy(x, w, t, bias=low, reduction='none')
+    assert float((out.detach() - math.log(300.0)).abs().max()) < 1e-5
+    with torch.no_grad():
+        assert float((vocab.vocab_cross_entropy(x, w, t, bias=low, reduction='none') - math.log(300.0)).abs().max()) < 1e-5
+    db, = torch.autograd.grad(out.sum(), low)
+    want = m / 300.0 - torch.bincount(t, minlength=300)
+    assert float((db.double() - want).abs().max()) < m * 2.0 ** -11 + _u(dtype) * float(want.abs().max())
+
+
+@pytest.mark.parametrize('size', [30.0, 1e4])
+def test_large_logits_keep_the_gradients_precision(size):
+    """p = 2^(l - top) / sum: near the largest logit its error does not grow with the logits' size (a bias common to all entries)"""
+    x, w, b, t = _case(200, 300, 16, torch.float32, 24)
+    with torch.no_grad():
+        b.add_(size)
+        b.copy_(torch.round(b * 64) / 64)                                # exact in the sum with `size`
+    _, _, want, bounds = _formula(x, w, b.detach() - size, t, torch.ones(200, device='cuda'))
+    got = torch.autograd.grad(vocab.vocab_cross_entropy(x, w, t, bias=b, reduction='sum'), (x, w, b))
+    # a logit is rounded at `size`: 2^-24 size twice (product times scale plus bias, base 2), p by as much
+    extra = 4 * 2.0 ** -24 * 1.5 * size
+    for a, e, lim in zip(got, want, bounds):
+        _within(a, e, lim + extra * 200)
+
+
+def test_one_row_without_a_leading_dimension():
+    x, w, b, t = _case(3, 40, 16, torch.float32, 25)
+    whole = torch.autograd.grad(vocab.vocab_cross_entropy(x, w, t, bias=b, reduction='none')[1], x)[0][1]
+    row = x.detach()[1].requires_grad_()
+    out = vocab.vocab_cross_entropy(row, w, t[1], bias=b, reduction='none')
+    assert out.shape == ()
+    assert float((torch.autograd.grad(out, row)[0] - whole).abs().max()) < 1e-6
+    wide = torch.zeros(32, device='cuda')
+    wide[::2] = row.detach()
+    with torch.no_grad():
+        assert abs(float(vocab.vocab_cross_entropy(wide[::2], w, t[1], bias=b)) - float(out)) < 1e-5
 
 
 @pytest.mark.parametrize('m', [8, 300])

@@ -32,7 +32,6 @@ struct CeScalars {            // head of the saved area
     int ex, ew;               // packed = value * 2^-e
     uint32_t ticket;          // last-workgroup counter of the loss sum
     int live;                 // rows that are there
-    float gmax;               // largest |grad| (reduction none), else 1
 };
 __device__ __forceinline__ int ce_padded(int live) { return (live + 255) & ~255; }
 
@@ -223,12 +222,17 @@ struct CeLogits {
     float2 *part;             // [wave tile along V][Mp]: (max, sum of 2^(l - max)), base 2
     float *tlogit;            // [Mp] target's logit, base 2
     // backward
-    const float *lse;         // [Mp] base 2; +inf: padding, NaN: no such target
-    const float *grad;        // reduction none: [M]
+    const float2 *stat;       // [Mp] (largest logit, base 2; 1 / sum of 2^(l - largest)), padding (+inf, 0), no such target (.., NaN)
+    const float *grad, *gmax; // reduction none: [M], largest |grad|
     half_t *g;                // panels of Mp rows, column 0 = vocabulary entry v0
 };
 
-template <typename T> __device__ __forceinline__ float ce_bias(const T *bias, int v) { return bias ? to_f32(bias[v]) * CE_LOG2E : 0.0f; }
+// bias in base 2; a finite one stays finite (the lowest value of fp32 as a mask: where it masks a whole row, all entries are alike)
+template <typename T> __device__ __forceinline__ float ce_bias(const T *bias, int v) {
+    if (!bias) return 0.0f;
+    const float b = to_f32(bias[v]), l = b * CE_LOG2E;
+    return fabsf(b) < __builtin_inff() ? fminf(fmaxf(l, -3.402823466e38f), 3.402823466e38f) : l;
+}
 
 template <typename T, bool SPLIT, bool BACK, int BM, int BN, int WM, int WN, int NST>
 __global__ void __launch_bounds__(WM *WN * 64, 2) ce_logits_kernel(CeLogits a, const T *bias) {
@@ -291,20 +295,21 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) ce_logits_kernel(CeLogits a, c
                 if (mine) a.tlogit[row] = l;
             }
         } else {
-            const float lse = a.lse[row];
+            const float2 st = a.stat[row];
+            float f = t >= 0 ? 32768.0f : 0.0f;
+            if (a.grad && t >= 0) f = *a.gmax > 0.0f ? 32768.0f * (a.grad[a.orig[row]] / *a.gmax) : 0.0f;
+            const float pf = st.y * f;                           // f (p - y) = 2^(l - top) (f / sum) - f y
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_amdgcn_exp2f(acc[i][j][e] - lse);
+                for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_amdgcn_exp2f(acc[i][j][e] - st.x) * pf;
             if (__any(mine)) {
 #pragma unroll
                 for (int i = 0; i < TM; ++i)
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
-                        if (mine && off == 32 * i + 8 * (e >> 2) + (e & 3)) acc[i][j][e] -= 1.0f;
+                        if (mine && off == 32 * i + 8 * (e >> 2) + (e & 3)) acc[i][j][e] -= f;
             }
-            float f = t >= 0 ? 32768.0f : 0.0f;
-            if (a.grad && t >= 0) f = a.sc->gmax > 0.0f ? 32768.0f * (a.grad[a.orig[row]] / a.sc->gmax) : 0.0f;
             // stored order inside 16 columns: 0 1 2 3 8 9 10 11 | 4 5 6 7 12 13 14 15 -- what one lane holds, 16 bytes at a time
             half_t *out = a.g + ((int64_t)(tv * BM / 32 + wm * TM) * (SPLIT ? 2 : 1) * a.Mp + row) * 32 + h * 8;
 #pragma unroll
@@ -314,7 +319,7 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) ce_logits_kernel(CeLogits a, c
                     half8 hi, lo;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const float v = acc[i][j][8 * c + e] * f;
+                        const float v = acc[i][j][8 * c + e];
                         hi[e] = (half_t)v;
                         if (SPLIT) lo[e] = (half_t)(v - (float)hi[e]);
                     }
@@ -459,7 +464,8 @@ struct CeRows {
     const int32_t *tc, *orig;
     int64_t M;
     int V, rsh, reduction;
-    float *lse, *loss;
+    float2 *stat;
+    float *loss;
     double2 *sums;
     CeScalars *sc;
 };
@@ -491,19 +497,21 @@ template <bool PACKED> __global__ void __launch_bounds__(256) ce_rows_kernel(CeR
     double2 mine = make_double2(0.0, 0.0);
     if (seg == 0) {
         const int64_t t = i < n ? (PACKED ? (int64_t)a.tc[i] : a.target[i]) : -1;
-        float lse = __builtin_inff(), l = 0.0f;
+        float2 stat = make_float2(__builtin_inff(), 0.0f);
+        float l = 0.0f;
         if (t >= 0) {
             float top = CE_NEG_INF, sum = 0.0f;
             for (int k = 0; k < segs; ++k) top = fmaxf(top, sh[(k << a.rsh) + r].x);
             const float mm = top == CE_NEG_INF ? 0.0f : top;
             for (int k = 0; k < segs; ++k) sum += sh[(k << a.rsh) + r].y * __builtin_amdgcn_exp2f(sh[(k << a.rsh) + r].x - mm);
             const float ls = log2f(sum);
-            lse = t < a.V ? top + ls : __builtin_nanf("");
+            // kept apart: the backward pass forms 2^(l - top) / sum, which keeps its precision however large the logits are
+            stat = make_float2(top, t < a.V ? 1.0f / sum : __builtin_nanf(""));
             // (top - target's logit) first: the two are near each other where the loss is small
             l = t < a.V ? (float)(((double)(top - a.tlogit[i]) + (double)ls) * CE_LN2) : __builtin_nanf("");
             mine = make_double2((double)l, 1.0);
         }
-        if (PACKED && a.lse && i < ce_padded((int)n)) a.lse[i] = lse;
+        if (PACKED && a.stat && i < ce_padded((int)n)) a.stat[i] = stat;
         if (a.reduction == 0) {
             if (!PACKED && i < a.M) a.loss[i] = l;
             if (PACKED && i < n) a.loss[a.orig[i]] = l;
@@ -540,12 +548,11 @@ template <bool PACKED> __global__ void __launch_bounds__(256) ce_rows_kernel(CeR
     if (threadIdx.x == 0) {
         const double c = tot[0].y;
         a.loss[0] = (float)(a.reduction == 1 ? (c > 0.0 ? tot[0].x / c : 0.0) : tot[0].x);
-        a.sc->gmax = 1.0f;
     }
 }
 
 // largest |grad| over the rows that are there (reduction none)
-__global__ void __launch_bounds__(1024) ce_gmax_kernel(const float *grad, const int64_t *target, int64_t M, CeScalars *sc) {
+__global__ void __launch_bounds__(1024) ce_gmax_kernel(const float *grad, const int64_t *target, int64_t M, float *gmax) {
     __shared__ float sh[16];
     float a = 0.0f;
     for (int64_t i = threadIdx.x; i < M; i += 1024)
@@ -561,14 +568,14 @@ __global__ void __launch_bounds__(1024) ce_gmax_kernel(const float *grad, const 
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int k = 1; k < 16; ++k) a = sh[k] > a || sh[k] != sh[k] ? sh[k] : a;
-        sc->gmax = a;
+        *gmax = a;
     }
 }
 
 // ---- gradient products ------------------------------------------------------------------------------------------------------
 // what takes a sum over G back to the gradient: 2^-15 max g, times the other operand's scale
-__device__ __forceinline__ float ce_unscale(const CeScalars *sc, const float *grad, int reduction, int e) {
-    float g = reduction == 0 ? sc->gmax : reduction == 1 ? grad[0] / (float)(sc->live > 0 ? sc->live : 1) : grad[0];
+__device__ __forceinline__ float ce_unscale(const CeScalars *sc, const float *grad, const float *gmax, int reduction, int e) {
+    const float g = reduction == 0 ? *gmax : reduction == 1 ? grad[0] / (float)(sc->live > 0 ? sc->live : 1) : grad[0];
     return ldexpf(g, e - 15);
 }
 
@@ -586,7 +593,7 @@ struct CeGrad {
 struct CeGrads {
     CeGrad x, w;              // dhidden, dweight
     const CeScalars *sc;
-    const float *grad;
+    const float *grad, *gmax;
     const int64_t *target;
     const int32_t *orig;      // dhidden: the caller's row of a row that is there
     int64_t M;
@@ -628,7 +635,7 @@ __device__ __forceinline__ void ce_grad_tile(const CeGrads &a, const CeGrad &c, 
         }
     }
     if (!c.out) return;                                        // only dbias is asked for
-    const float f = c.part ? 1.0f : ce_unscale(a.sc, a.grad, a.reduction, WEIGHT ? a.sc->ex : a.sc->ew);
+    const float f = c.part ? 1.0f : ce_unscale(a.sc, a.grad, a.gmax, a.reduction, WEIGHT ? a.sc->ex : a.sc->ew);
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -690,7 +697,7 @@ __device__ __forceinline__ void ce_join(const CeGrads &a, const CeGrad &c, bool 
 #pragma unroll
                 for (int e = 0; e < VE; ++e) v[e] += p[u].v[e];
     }
-    const float f = ce_unscale(a.sc, a.grad, a.reduction, weight ? a.sc->ex : a.sc->ew);
+    const float f = ce_unscale(a.sc, a.grad, a.gmax, a.reduction, weight ? a.sc->ex : a.sc->ew);
     T *out = (T *)c.out + (weight ? c.out0 + row : (int64_t)a.orig[row]) * a.D + (k - row * a.D);
 #pragma unroll
     for (int e = 0; e < VE; ++e) out[e] = from_f32<T>(v[e] * f);
@@ -707,7 +714,7 @@ __global__ void __launch_bounds__(256) ce_join_kernel(CeGrads a, int bx, int bw,
     const int pos = (v & ~12) | ((v & 4) << 1) | ((v & 8) >> 1);
     float s = 0.0f;
     for (int k = 0; k < a.w.splits; ++k) s += a.part_b[k * a.ldb + pos];
-    dbias[v] = from_f32<T>(s * ce_unscale(a.sc, a.grad, a.reduction, 0));
+    dbias[v] = from_f32<T>(s * ce_unscale(a.sc, a.grad, a.gmax, a.reduction, 0));
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------
@@ -723,12 +730,12 @@ static CeShape ce_shape(const tnp_vocab_ce *p) {
     return s;
 }
 
-struct CeSaved { CeScalars *sc; float *lse; int32_t *tc, *orig; half_t *x, *w; size_t bytes; };
+struct CeSaved { CeScalars *sc; float2 *stat; int32_t *tc, *orig; half_t *x, *w; size_t bytes; };
 static CeSaved ce_saved(const CeShape &s, void *base) {
     CeSaved v;
     char *p = (char *)base;
     v.sc = (CeScalars *)p; p += 256;
-    v.lse = (float *)p; p += s.Mp * 4;                 // Mp and Vp are multiples of 256: every part stays aligned
+    v.stat = (float2 *)p; p += s.Mp * 8;               // Mp and Vp are multiples of 256: every part stays aligned
     v.tc = (int32_t *)p; p += s.Mp * 4;
     v.orig = (int32_t *)p; p += s.Mp * 4;
     v.x = (half_t *)p; p += (size_t)s.Mp * s.panels * 64;
@@ -777,7 +784,7 @@ struct CeBackward {
     int64_t ldg;
     half_t *g;
     int tile, splits_x, splits_w;
-    float *part_x, *part_w, *part_b;
+    float *gmax, *part_x, *part_w, *part_b;
     size_t bytes;
 };
 static constexpr size_t CE_PIECE_BYTES = (size_t)512 << 20;
@@ -805,6 +812,7 @@ static CeBackward ce_backward_layout(const tnp_vocab_ce *p, void *ws) {
     b.splits_x = (int)(nx < 1 ? 1 : nx);
     b.splits_w = (int)(nw < 1 ? 1 : nw);
     char *w = (char *)ws;
+    b.gmax = (float *)w; w += 256;
     b.g = (half_t *)w; w += ce_up((size_t)s.Mp * b.ldg * 2);
     b.part_x = b.splits_x > 1 || b.pieces > 1 ? (float *)w : nullptr;
     if (b.part_x) w += ce_up((size_t)b.splits_x * s.Mp * p->D * 4);
@@ -930,7 +938,7 @@ static int ce_forward(const tnp_vocab_ce *p, const CeForward &f, float *loss, hi
     CeRows r = {};
     r.part = f.part; r.ldp = ce_scores(p) ? (int64_t)CE_SCORE_ROWS : sh.Mp; r.parts = f.parts; r.tlogit = f.tlogit; r.target = p->target;
     r.tc = f.saved.tc; r.orig = f.saved.orig; r.M = p->M; r.V = p->V; r.rsh = ce_rows_shift(p->M, f.parts); r.reduction = p->reduction;
-    r.lse = p->saved ? f.saved.lse : nullptr; r.loss = loss; r.sums = f.sums; r.sc = f.saved.sc;
+    r.stat = p->saved ? f.saved.stat : nullptr; r.loss = loss; r.sums = f.sums; r.sc = f.saved.sc;
     const int64_t cover = ce_scores(p) ? p->M : sh.Mp;
     const dim3 grid((unsigned)((cover + (1 << r.rsh) - 1) >> r.rsh));
     if (ce_scores(p)) hipLaunchKernelGGL((ce_rows_kernel<false>), grid, dim3(256), 0, s, r);
@@ -945,7 +953,7 @@ static int ce_backward(const tnp_vocab_ce *p, const CeBackward &b, const float *
     const CeSaved sv = ce_saved(sh, p->saved);
     int rc;
     if (p->reduction == 0) {
-        hipLaunchKernelGGL(ce_gmax_kernel, dim3(1), dim3(1024), 0, s, grad, p->target, p->M, sv.sc);
+        hipLaunchKernelGGL(ce_gmax_kernel, dim3(1), dim3(1024), 0, s, grad, p->target, p->M, b.gmax);
         TNP_HIP(hipGetLastError());
     }
     const GemmOperand w{sv.w, sh.Vp, 0}, x{sv.x, sh.Mp, 0};
@@ -953,12 +961,12 @@ static int ce_backward(const tnp_vocab_ce *p, const CeBackward &b, const float *
         const int v0 = k * b.piece, cols = sh.Vp - v0 < b.piece ? sh.Vp - v0 : b.piece, live = sh.V - v0 < cols ? sh.V - v0 : cols;
         CeLogits a = {};
         a.w = w; a.x = x; a.sc = sv.sc; a.tc = sv.tc; a.orig = sv.orig; a.Mp = sh.Mp; a.V = sh.V; a.v0 = v0; a.steps = sh.panels;
-        a.lse = sv.lse; a.grad = p->reduction == 0 ? grad : nullptr; a.g = b.g;
+        a.stat = sv.stat; a.grad = p->reduction == 0 ? grad : nullptr; a.gmax = b.gmax; a.g = b.g;
         if ((rc = ce_logits<T, SPLIT, true>(a, cols, ce_big(sh), (const T *)p->bias, s))) return rc;
         const bool last = k == b.pieces - 1;
         const int ks = SPLIT ? 16 : 32;
         CeGrads c = {};
-        c.sc = sv.sc; c.grad = grad; c.target = p->target; c.orig = sv.orig; c.M = sh.M; c.reduction = p->reduction; c.D = sh.D;
+        c.sc = sv.sc; c.grad = grad; c.gmax = b.gmax; c.target = p->target; c.orig = sv.orig; c.M = sh.M; c.reduction = p->reduction; c.D = sh.D;
         c.zero_blocks = dhidden && k == 0 ? (int)(sh.Mp / 64 < 512 ? sh.Mp / 64 : 512) : 0;
         c.x.g = c.w.g = GemmOperand{b.g, sh.Mp, 0};
         c.x.g_panels = c.w.g_panels = cols / ks; c.x.o_panels = c.w.o_panels = sh.panels;

@@ -135,7 +135,7 @@ def saved_bytes(rows, entries, columns, dtype):
     """tnp_vocab_ce_saved_bytes() from the sizes alone (they may be symbolic while a graph is traced)"""
     panels = (columns + 15) // 16 if dtype == torch.float32 else (columns + 31) // 32
     up = lambda n: (n + 255) // 256 * 256
-    return 256 + 12 * up(rows) + 64 * panels * (up(rows) + up(entries))
+    return 256 + 16 * up(rows) + 64 * panels * (up(rows) + up(entries))
 
 
 def _ce_args(hidden, weight, bias, target, reduction, saved):
