@@ -217,9 +217,9 @@ struct CeLogits {
     const CeScalars *sc;
     const int32_t *tc, *orig; // of the rows that are there: target (V: none such), row of the caller
     int64_t Mp;
-    int V, v0, tiles_v, tiles_i, steps;
+    int V, v0, tiles_v, v_shares, steps;
     // forward
-    float2 *part;             // [wave tile along V][Mp]: (max, sum of 2^(l - max)), base 2
+    float2 *part;             // [vocabulary share, wave row][Mp]: (max, sum of 2^(l - max)), base 2
     float *tlogit;            // [Mp] target's logit, base 2
     // backward
     const float2 *stat;       // [Mp] (largest logit, base 2; 1 / sum of 2^(l - largest)), padding (+inf, 0), no such target (.., NaN)
@@ -234,99 +234,138 @@ template <typename T> __device__ __forceinline__ float ce_bias(const T *bias, in
     return fabsf(b) < __builtin_inff() ? fminf(fmaxf(l, -3.402823466e38f), 3.402823466e38f) : l;
 }
 
+// A workgroup keeps its BN hidden rows and walks over a share of the vocabulary's tiles, the next tile's first steps in flight while it
+// works on this one's logits (86 -> LOGITS_FWD us for 8192 x 16384 x 128 bf16 with one tile per workgroup); the running maximum and sum stay
+// in each lane until the last tile.
 template <typename T, bool SPLIT, bool BACK, int BM, int BN, int WM, int WN, int NST>
 __global__ void __launch_bounds__(WM *WN * 64, 2) ce_logits_kernel(CeLogits a, const T *bias) {
-    constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
+    typedef TileGemm<SPLIT, false, false, BM, BN, WM, WN, NST> Gemm;
+    constexpr int TM = Gemm::TM, TN = Gemm::TN, NT = WM * WN * 64;
+    static_assert(BM <= NT, "one thread per bias entry of a tile");
     extern __shared__ __attribute__((aligned(1024))) char lds[];
-    __shared__ __attribute__((aligned(16))) float sb[BM];
-    int tv, ti;
+    __shared__ __attribute__((aligned(16))) float sb[2][BM];
+    int ti, vs;
     const int live = a.sc->live;
-    if (!gemm_tile_of(blockIdx.x, a.tiles_v, ce_padded(live) / BN, tv, ti)) return;
-    const int64_t vbase = a.v0 + (int64_t)tv * BM, ibase = (int64_t)ti * BN;
-    for (int j = threadIdx.x; j < BM; j += WM * WN * 64) sb[j] = vbase + j < a.V ? ce_bias(bias, (int)vbase + j) : CE_NEG_INF;
-    f32x16 acc[TM][TN];
-    float none[TM];
-    gemm_tile<SPLIT, false, false, BM, BN, WM, WN, NST, false>(a.w, a.x, vbase, 0, 0, ibase, 0, 0, 0, a.steps, lds, acc, false, none);
+    if (!gemm_tile_of(blockIdx.x, ce_padded(live) / BN, a.v_shares, ti, vs)) return;
+    const int tv0 = (int)((int64_t)a.tiles_v * vs / a.v_shares), tv1 = (int)((int64_t)a.tiles_v * (vs + 1) / a.v_shares);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
     const int wm = wave / WN, wn = wave % WN;
     const float scale = ldexpf(CE_LOG2E, a.sc->ex + a.sc->ew);
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const float4 b = *(const float4 *)(sb + wm * TM * 32 + i * 32 + 8 * q + 4 * h);
-#pragma unroll
-            for (int j = 0; j < TN; ++j) {
-                acc[i][j][4 * q + 0] = fmaf(acc[i][j][4 * q + 0], scale, b.x);
-                acc[i][j][4 * q + 1] = fmaf(acc[i][j][4 * q + 1], scale, b.y);
-                acc[i][j][4 * q + 2] = fmaf(acc[i][j][4 * q + 2], scale, b.z);
-                acc[i][j][4 * q + 3] = fmaf(acc[i][j][4 * q + 3], scale, b.w);
-            }
-        }
+    // this lane's rows
+    int64_t row[TN];
+    int tc[TN];
+    float m[TN], s[TN], pf[TN], f[TN];                           // running statistics; backward: top, -, 2^15 r / sum, 2^15 r
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-        const int64_t row = ibase + wn * TN * 32 + j * 32 + (lane & 31);
-        // the target's place in this lane's part of the wave tile: local - 4 h = 32 i + 8 q + e
-        const int t = row < live ? a.tc[row] : -1;
-        const int64_t off = t - vbase - wm * TM * 32 - 4 * h;
-        const bool mine = t >= 0 && off >= 0 && off < TM * 32 && (off & 4) == 0;
-        if (!BACK) {
-            float m = CE_NEG_INF;
+        row[j] = (int64_t)ti * BN + wn * TN * 32 + j * 32 + (lane & 31);
+        tc[j] = row[j] < live ? a.tc[row[j]] : -1;
+        m[j] = CE_NEG_INF;
+        s[j] = 0.0f;
+        if (BACK) {
+            const float2 st = a.stat[row[j]];
+            f[j] = tc[j] >= 0 ? 32768.0f : 0.0f;
+            if (a.grad && tc[j] >= 0) f[j] = *a.gmax > 0.0f ? 32768.0f * (a.grad[a.orig[row[j]]] / *a.gmax) : 0.0f;
+            m[j] = st.x;
+            pf[j] = st.y * f[j];                                 // f (p - y) = 2^(l - top) (f / sum) - f y
+        }
+    }
+    auto next_bias = [&](int tv) {
+        const int v = a.v0 + tv * BM + (int)threadIdx.x;
+        return (int)threadIdx.x < BM && v < a.V ? ce_bias(bias, v) : CE_NEG_INF;
+    };
+    float b_next = next_bias(tv0);
+    Gemm g;
+    g.init(a.w, a.x, a.v0 + (int64_t)tv0 * BM, 0, 0, (int64_t)ti * BN, 0, 0, lds);
+    g.first(0, a.steps);
+    for (int tv = tv0; tv < tv1; ++tv) {
+        float *tb = sb[tv & 1];
+        if ((int)threadIdx.x < BM) tb[threadIdx.x] = b_next;     // read behind the barriers of run(); the other half is still being read
+        f32x16 acc[TM][TN];
+        float none[TM];
+        g.template run<false>(0, a.steps, acc, false, none);
+        if (tv + 1 < tv1) {
+            b_next = next_bias(tv + 1);
+            g.a_rows(BM);
+            g.first(0, a.steps);
+        }
 #pragma unroll
-            for (int i = 0; i < TM; ++i)
+        for (int i = 0; i < TM; ++i)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) m = fmaxf(m, acc[i][j][e]);
-            m = fmaxf(m, __shfl_xor(m, 32));
-            const float mm = m == CE_NEG_INF ? 0.0f : m;         // nothing but masked entries: a sum of zeros, not of NaN
-            float s = 0.0f;
+            for (int q = 0; q < 4; ++q) {
+                const float4 b = *(const float4 *)(tb + wm * TM * 32 + i * 32 + 8 * q + 4 * h);
 #pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) s += __builtin_amdgcn_exp2f(acc[i][j][e] - mm);
-            s += __shfl_xor(s, 32);
-            if (h == 0) a.part[(int64_t)(tv * WM + wm) * a.Mp + row] = make_float2(m, s);
-            if (__any(mine)) {
-                float l = 0.0f;
-#pragma unroll
-                for (int i = 0; i < TM; ++i)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        if (off == 32 * i + 8 * (e >> 2) + (e & 3)) l = acc[i][j][e];
-                if (mine) a.tlogit[row] = l;
-            }
-        } else {
-            const float2 st = a.stat[row];
-            float f = t >= 0 ? 32768.0f : 0.0f;
-            if (a.grad && t >= 0) f = *a.gmax > 0.0f ? 32768.0f * (a.grad[a.orig[row]] / *a.gmax) : 0.0f;
-            const float pf = st.y * f;                           // f (p - y) = 2^(l - top) (f / sum) - f y
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_amdgcn_exp2f(acc[i][j][e] - st.x) * pf;
-            if (__any(mine)) {
-#pragma unroll
-                for (int i = 0; i < TM; ++i)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        if (mine && off == 32 * i + 8 * (e >> 2) + (e & 3)) acc[i][j][e] -= f;
-            }
-            // stored order inside 16 columns: 0 1 2 3 8 9 10 11 | 4 5 6 7 12 13 14 15 -- what one lane holds, 16 bytes at a time
-            half_t *out = a.g + ((int64_t)(tv * BM / 32 + wm * TM) * (SPLIT ? 2 : 1) * a.Mp + row) * 32 + h * 8;
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    half8 hi, lo;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float v = acc[i][j][8 * c + e];
-                        hi[e] = (half_t)v;
-                        if (SPLIT) lo[e] = (half_t)(v - (float)hi[e]);
-                    }
-                    half_t *o = out + (SPLIT ? (i * 2 + c) * a.Mp * 32 : i * a.Mp * 32 + c * 16);
-                    *(half8 *)o = hi;
-                    if (SPLIT) *(half8 *)(o + 16) = lo;
+                for (int j = 0; j < TN; ++j) {
+                    acc[i][j][4 * q + 0] = fmaf(acc[i][j][4 * q + 0], scale, b.x);
+                    acc[i][j][4 * q + 1] = fmaf(acc[i][j][4 * q + 1], scale, b.y);
+                    acc[i][j][4 * q + 2] = fmaf(acc[i][j][4 * q + 2], scale, b.z);
+                    acc[i][j][4 * q + 3] = fmaf(acc[i][j][4 * q + 3], scale, b.w);
                 }
+            }
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            // the target's place in this lane's part of the wave tile: 32 i + 8 q + e
+            const int off = tc[j] - (a.v0 + tv * BM) - wm * TM * 32 - 4 * h;
+            const bool mine = tc[j] >= 0 && off >= 0 && off < TM * 32 && (off & 4) == 0;
+            if (!BACK) {
+                float top = m[j];
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) top = fmaxf(top, acc[i][j][e]);
+                const float mm = top == CE_NEG_INF ? 0.0f : top; // nothing but masked entries: a sum of zeros, not of NaN
+                s[j] *= __builtin_amdgcn_exp2f(m[j] - mm);
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[j] += __builtin_amdgcn_exp2f(acc[i][j][e] - mm);
+                m[j] = top;
+                if (__any(mine)) {
+                    float l = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < TM; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if (off == 32 * i + 8 * (e >> 2) + (e & 3)) l = acc[i][j][e];
+                    if (mine) a.tlogit[row[j]] = l;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_amdgcn_exp2f(acc[i][j][e] - m[j]) * pf[j];
+                if (__any(mine)) {
+#pragma unroll
+                    for (int i = 0; i < TM; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if (mine && off == 32 * i + 8 * (e >> 2) + (e & 3)) acc[i][j][e] -= f[j];
+                }
+                // stored order inside 16 columns: 0 1 2 3 8 9 10 11 | 4 5 6 7 12 13 14 15 -- what one lane holds, 16 bytes at a time
+                half_t *out = a.g + ((int64_t)(tv * BM / 32 + wm * TM) * (SPLIT ? 2 : 1) * a.Mp + row[j]) * 32 + h * 8;
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        half8 hi, lo;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const float v = acc[i][j][8 * c + e];
+                            hi[e] = (half_t)v;
+                            if (SPLIT) lo[e] = (half_t)(v - (float)hi[e]);
+                        }
+                        half_t *o = out + (SPLIT ? (i * 2 + c) * a.Mp * 32 : i * a.Mp * 32 + c * 16);
+                        *(half8 *)o = hi;
+                        if (SPLIT) *(half8 *)(o + 16) = lo;
+                    }
+            }
+        }
+    }
+    if (!BACK) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            const float mo = __shfl_xor(m[j], 32), so = __shfl_xor(s[j], 32), top = fmaxf(m[j], mo), mm = top == CE_NEG_INF ? 0.0f : top;
+            const float sum = s[j] * __builtin_amdgcn_exp2f(m[j] - mm) + so * __builtin_amdgcn_exp2f(mo - mm);
+            if (h == 0) a.part[(int64_t)(vs * WM + wm) * a.Mp + row[j]] = make_float2(top, sum);
         }
     }
 }
@@ -625,8 +664,10 @@ __device__ __forceinline__ void ce_grad_tile(const CeGrads &a, const CeGrad &c, 
     float asum[TM];
 #pragma unroll
     for (int i = 0; i < TM; ++i) asum[i] = 0.0f;
-    gemm_tile<SPLIT, WEIGHT, true, BM, BN, WM, WN, NST, WEIGHT>(c.g, c.o, WEIGHT ? 0 : r0, gp, c.g_panels - gp, c.ok0, op, c.o_panels - op, s0, s1,
-                                                                lds, acc, sums, asum);
+    TileGemm<SPLIT, WEIGHT, true, BM, BN, WM, WN, NST> g;
+    g.init(c.g, c.o, WEIGHT ? 0 : r0, gp, c.g_panels - gp, c.ok0, op, c.o_panels - op, lds);
+    g.first(s0, s1);
+    g.template run<WEIGHT>(s0, s1, acc, sums, asum);
     if (sums) {
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
@@ -758,6 +799,24 @@ static int ce_x_blocks(int64_t M) { return (int)((M + 7) / 8 < CE_AMAX_BLOCKS ? 
 
 // 256 x 256 tiles of logits (eight waves) from two rounds of workgroups and eight steps on: 4096 x 16384 x 1024 fp32 forward 381 us
 // against 437, 8192 x 16384 x 128 bf16 (four steps) 95 against 86
+// Shares that the `tiles_v` vocabulary tiles are split into for each of `tiles_i` row tiles, `slots` workgroups running at a time: the
+// fewest rounds of workgroups times tiles per workgroup, and of those the fewest shares.
+static int ce_shares(int64_t tiles_i, int tiles_v, int slots) {
+    int best = 1;
+    int64_t cost = INT64_MAX;
+    for (int n = 1; n <= tiles_v && n <= 64; ++n) {
+        const int64_t rounds = (tiles_i * n + slots - 1) / slots, c = rounds * ((tiles_v + n - 1) / n);
+        if (c < cost) { cost = c; best = n; }
+        if (tiles_i * n >= 2 * slots) break;
+    }
+    return best;
+}
+static bool ce_big(const CeShape &s);
+// slots: one workgroup of the 256 tiles per CU, three of the 128 ones
+static int ce_logit_shares(const CeShape &s, int64_t cols) {
+    return ce_big(s) ? ce_shares(s.Mp / 256, (int)(cols / 256), 256) : ce_shares(s.Mp / 128, (int)(cols / 128), 768);
+}
+
 static bool ce_big(const CeShape &s) { return (s.Mp / 256) * (int64_t)(s.Vp / 256) >= 512 && s.panels >= 8; }
 
 struct CeForward { CeSaved saved; float *amax; int *count; float2 *part; float *tlogit; double2 *sums; int parts; size_t bytes; };
@@ -765,7 +824,7 @@ static CeForward ce_forward_layout(const tnp_vocab_ce *p, void *ws) {
     CeForward f;
     const CeShape s = ce_shape(p);
     char *w = (char *)ws;
-    f.parts = ce_scores(p) ? ce_score_blocks(p->V) : s.Vp / 256 * (ce_big(s) ? 2 : 4);
+    f.parts = ce_scores(p) ? ce_score_blocks(p->V) : 2 * ce_logit_shares(s, s.Vp);
     const int64_t rows = ce_scores(p) ? CE_SCORE_ROWS : s.Mp;
     f.amax = (float *)w; w += ce_up(2 * CE_AMAX_BLOCKS * 4);
     f.count = (int *)w; w += ce_up(CE_AMAX_BLOCKS * 4);
@@ -853,12 +912,11 @@ static int ce_lds(KernT kern, size_t smem, size_t *done) {             // done: 
 template <typename T, bool SPLIT, bool BACK, int BM, int BN, int WM, int WN, int NST>
 static int ce_launch_logits(CeLogits a, int64_t cols, const T *bias, hipStream_t s) {
     a.tiles_v = (int)(cols / BM);
-    a.tiles_i = (int)(a.Mp / BN);
     const size_t smem = NST * (BM + BN) * 64;
     static size_t done[VOCAB_MAX_DEVICES] = {0};
     auto kern = ce_logits_kernel<T, SPLIT, BACK, BM, BN, WM, WN, NST>;
     if (int rc = ce_lds(kern, smem, done)) return rc;
-    hipLaunchKernelGGL(kern, dim3(gemm_grid((int64_t)a.tiles_v * a.tiles_i)), dim3(WM * WN * 64), smem, s, a, bias);
+    hipLaunchKernelGGL(kern, dim3(gemm_grid(a.Mp / BN * a.v_shares)), dim3(WM * WN * 64), smem, s, a, bias);
     TNP_HIP(hipGetLastError());
     return 0;
 }
@@ -932,7 +990,7 @@ static int ce_forward(const tnp_vocab_ce *p, const CeForward &f, float *loss, hi
         a.w = GemmOperand{f.saved.w, sh.Vp, 0};
         a.x = GemmOperand{f.saved.x, sh.Mp, 0};
         a.sc = f.saved.sc; a.tc = f.saved.tc; a.orig = f.saved.orig; a.Mp = sh.Mp; a.V = sh.V; a.v0 = 0; a.steps = sh.panels;
-        a.part = f.part; a.tlogit = f.tlogit;
+            a.part = f.part; a.tlogit = f.tlogit; a.v_shares = ce_logit_shares(sh, sh.Vp);
         if ((rc = ce_logits<T, SPLIT, false>(a, sh.Vp, ce_big(sh), (const T *)p->bias, s))) return rc;
     }
     CeRows r = {};
@@ -961,7 +1019,7 @@ static int ce_backward(const tnp_vocab_ce *p, const CeBackward &b, const float *
         const int v0 = k * b.piece, cols = sh.Vp - v0 < b.piece ? sh.Vp - v0 : b.piece, live = sh.V - v0 < cols ? sh.V - v0 : cols;
         CeLogits a = {};
         a.w = w; a.x = x; a.sc = sv.sc; a.tc = sv.tc; a.orig = sv.orig; a.Mp = sh.Mp; a.V = sh.V; a.v0 = v0; a.steps = sh.panels;
-        a.stat = sv.stat; a.grad = p->reduction == 0 ? grad : nullptr; a.gmax = b.gmax; a.g = b.g;
+        a.stat = sv.stat; a.grad = p->reduction == 0 ? grad : nullptr; a.gmax = b.gmax; a.g = b.g; a.v_shares = ce_logit_shares(sh, cols);
         if ((rc = ce_logits<T, SPLIT, true>(a, cols, ce_big(sh), (const T *)p->bias, s))) return rc;
         const bool last = k == b.pieces - 1;
         const int ks = SPLIT ? 16 : 32;

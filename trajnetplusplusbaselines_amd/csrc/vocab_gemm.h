@@ -204,82 +204,92 @@ template <int TM> __device__ __forceinline__ void step_row_sums(const half8 (&fa
                 asum[i] = __builtin_amdgcn_fdot2(half2v{fa[2 * i + w][2 * e], fa[2 * i + w][2 * e + 1]}, one, asum[i], false);
 }
 
-// Accumulates steps [s0, s1) of the tile at (row ar, panel ap) of a and (br, bp) of b into acc; al / bl: panels from there to the last
-// (KS).  LDS: NST * (BM + BN) * 64 bytes.
+// One workgroup's products: init() takes the tile at (row ar, panel ap) of a and (br, bp) of b (al / bl: panels from there to the last,
+// KS), first() starts to fetch its steps [s0, s1), run() accumulates them into acc.  After run() the ring is free: first() of the next
+// tile (a_rows() moves a KC operand a on by whole rows) can be called before this one's results are used, which hides its latency.
+// LDS: NST * (BM + BN) * 64 bytes.
 //
 // Eight waves (two per SIMD) take turns: while one half of the workgroup fetches the operands of a step into registers, the other
 // half multiplies the step it has fetched; a barrier per turn keeps them half a step apart.  In lockstep both waves of a SIMD would
 // fetch at the same time and leave the matrix cores idle meanwhile (2150 cycles per step of 1024 cycles of matrix work).  With
-// four waves the other workgroup on the CU fills that time.
+// four waves the other workgroups on the CU fill that time.
+//
 // SUMS: with `sums` (the same for the wave), asum[] gathers the row sums of a as well (step_row_sums).
-template <bool SPLIT, bool A_KS, bool B_KS, int BM, int BN, int WM, int WN, int NST, bool SUMS>
-__device__ __forceinline__ void gemm_tile(const GemmOperand &a, const GemmOperand &b, int64_t ar, int64_t ap, int al, int64_t br, int64_t bp, int bl,
-                                          int s0, int s1, char *lds, f32x16 (&acc)[BM / WM / 32][BN / WN / 32], bool sums,
-                                          float (&asum)[BM / WM / 32]) {
-    constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, STAGE = (BM + BN) * 64;
-    constexpr bool TURNS = NW == 8;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave / WN, wn = wave % WN;
+template <bool SPLIT, bool A_KS, bool B_KS, int BM, int BN, int WM, int WN, int NST> struct TileGemm {
+    static constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, STAGE = (BM + BN) * 64;
+    static constexpr bool TURNS = NW == 8;
     typedef TileStage<A_KS, SPLIT, BM, NW> SA;
     typedef TileStage<B_KS, SPLIT, BN, NW> SB;
-    constexpr int LOADS = SA::INSTR + SB::INSTR;                   // per wave and step
+    static constexpr int LOADS = SA::INSTR + SB::INSTR;            // per wave and step
     static_assert(NST >= 3, "the tile after next is in flight while one is read");
     SA sa;
     SB sb;
-    sa.init(a, ar, ap, al, wave, lane);
-    sb.init(b, br, bp, bl, wave, lane);
+    char *lds;
+    int lane, wave;
+
+    __device__ __forceinline__ void init(const GemmOperand &a, const GemmOperand &b, int64_t ar, int64_t ap, int al, int64_t br, int64_t bp, int bl,
+                                         char *lds_) {
+        lds = lds_;
+        lane = threadIdx.x & 63;
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        sa.init(a, ar, ap, al, wave, lane);
+        sb.init(b, br, bp, bl, wave, lane);
+    }
+    __device__ __forceinline__ void a_rows(int rows) { sa.base += (int64_t)rows * 32; }
+    __device__ __forceinline__ void load(int s, int stage) {
+        sa.load(s, lds + stage * STAGE, wave);
+        sb.load(s, lds + stage * STAGE + BM * 64, wave);
+    }
+    __device__ __forceinline__ void first(int s0, int s1) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < TN; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
-    if (s0 >= s1) return;
-#pragma unroll
-    for (int k = 0; k < NST - 1; ++k)
-        if (s0 + k < s1) {
-            sa.load(s0 + k, lds + k * STAGE, wave);
-            sb.load(s0 + k, lds + k * STAGE + BM * 64, wave);
-        }
-    // the tile of the step that has `left` steps behind it has landed in every wave (those in flight: at most NST - 2)
-    auto landed = [&](int left) {
+        for (int k = 0; k < NST - 1; ++k)
+            if (s0 + k < s1) load(s0 + k, k);
+    }
+    // the step that has `left` steps behind it has landed in every wave (those in flight: at most NST - 2)
+    static __device__ __forceinline__ void landed(int left) {
         if (NST >= 4 && left >= 2) stage_barrier<(NST >= 4 ? 2 : 0) * LOADS>();
         else if (left >= 1) stage_barrier<LOADS>();
         else stage_barrier<0>();
-    };
-    landed(s1 - 1 - s0);
-    if (TURNS && wave >= 4) stage_barrier_only();
-    int cur = 0;
-    half8 fa[2 * TM], fb[2 * TN];
-    for (int s = s0; s < s1; ++s) {
-        const char *la = lds + cur * STAGE, *lb = la + BM * 64;
-        step_frags<SB, B_KS, SPLIT, TN>(lb, wn * TN * 32, lane, fb);
-        step_frags<SA, A_KS, SPLIT, TM>(la, wm * TM * 32, lane, fa);
-        if (s + NST - 1 < s1) {                                    // into the buffer that every wave was done with one barrier ago
-            const int nxt = cur == 0 ? NST - 1 : cur - 1;
-            sa.load(s + NST - 1, lds + nxt * STAGE, wave);
-            sb.load(s + NST - 1, lds + nxt * STAGE + BM * 64, wave);
-        }
-        cur = cur + 1 == NST ? 0 : cur + 1;
-        if (TURNS) {
-            __builtin_amdgcn_sched_barrier(0);
-            if (s + 1 < s1) landed(s1 - 2 - s); else stage_barrier<0>();
-            __builtin_amdgcn_sched_barrier(0);
-            __builtin_amdgcn_s_setprio(1);
-            step_mfma<SPLIT, TM, TN>(fa, fb, acc);
-            if (SUMS && sums) step_row_sums<TM>(fa, asum);
-            __builtin_amdgcn_s_setprio(0);
-            __builtin_amdgcn_sched_barrier(0);
-            stage_barrier_only();
-            __builtin_amdgcn_sched_barrier(0);
-        } else {
-            step_mfma<SPLIT, TM, TN>(fa, fb, acc);
-            if (SUMS && sums) step_row_sums<TM>(fa, asum);
-            if (s + 1 < s1) landed(s1 - 2 - s);
-        }
     }
-    if (TURNS && wave < 4) stage_barrier_only();
-}
+    template <bool SUMS> __device__ __forceinline__ void run(int s0, int s1, f32x16 (&acc)[TM][TN], bool sums, float (&asum)[TM]) {
+        const int wm = wave / WN, wn = wave % WN;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+        if (s0 >= s1) return;
+        landed(s1 - 1 - s0);
+        if (TURNS && wave >= 4) stage_barrier_only();
+        int cur = 0;
+        half8 fa[2 * TM], fb[2 * TN];
+        for (int s = s0; s < s1; ++s) {
+            const char *la = lds + cur * STAGE, *lb = la + BM * 64;
+            step_frags<SB, B_KS, SPLIT, TN>(lb, wn * TN * 32, lane, fb);
+            step_frags<SA, A_KS, SPLIT, TM>(la, wm * TM * 32, lane, fa);
+            if (s + NST - 1 < s1) load(s + NST - 1, cur == 0 ? NST - 1 : cur - 1);   // the buffer that every wave left one barrier ago
+            cur = cur + 1 == NST ? 0 : cur + 1;
+            if (TURNS) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (s + 1 < s1) landed(s1 - 2 - s); else stage_barrier<0>();
+                __builtin_amdgcn_sched_barrier(0);
+                __builtin_amdgcn_s_setprio(1);
+                step_mfma<SPLIT, TM, TN>(fa, fb, acc);
+                if (SUMS && sums) step_row_sums<TM>(fa, asum);
+                __builtin_amdgcn_s_setprio(0);
+                __builtin_amdgcn_sched_barrier(0);
+                stage_barrier_only();
+                __builtin_amdgcn_sched_barrier(0);
+            } else {
+                step_mfma<SPLIT, TM, TN>(fa, fb, acc);
+                if (SUMS && sums) step_row_sums<TM>(fa, asum);
+                landed(s1 - 2 - s);                                // after the last step: every wave is done with the ring
+            }
+        }
+        if (TURNS && wave < 4) stage_barrier_only();
+    }
+};
 
 // Workgroup -> tile: the eight XCDs take the workgroups in turn, so each gets a contiguous share of the tiles, walked in groups of
 // eight tile rows; the panels of a group stay in the XCD's own L2.  Returns false for the workgroups behind the last tile.
