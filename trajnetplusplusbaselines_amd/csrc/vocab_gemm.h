@@ -245,11 +245,14 @@ template <bool SPLIT, bool A_KS, bool B_KS, int BM, int BN, int WM, int WN, int 
         for (int k = 0; k < NST - 1; ++k)
             if (s0 + k < s1) load(s0 + k, k);
     }
-    // the step that has `left` steps behind it has landed in every wave (those in flight: at most NST - 2)
-    static __device__ __forceinline__ void landed(int left) {
-        if (NST >= 4 && left >= 2) stage_barrier<(NST >= 4 ? 2 : 0) * LOADS>();
-        else if (left >= 1) stage_barrier<LOADS>();
-        else stage_barrier<0>();
+    // the step that has `left` steps behind it has landed in every wave: at most NST - 2 steps' loads are still in flight
+    template <int N = NST - 2> static __device__ __forceinline__ void landed(int left) {
+        if constexpr (N > 0) {
+            if (left >= N) stage_barrier<N * LOADS>();
+            else landed<N - 1>(left);
+        } else {
+            stage_barrier<0>();
+        }
     }
     template <bool SUMS> __device__ __forceinline__ void run(int s0, int s1, f32x16 (&acc)[TM][TN], bool sums, float (&asum)[TM]) {
         const int wm = wave / WN, wn = wave % WN;
