@@ -19,6 +19,8 @@
 
 #include <math.h>
 
+#include <algorithm>
+
 namespace tnp {
 
 static constexpr float CE_LOG2E = 1.4426950408889634f;
@@ -26,7 +28,9 @@ static constexpr double CE_LN2 = 0.6931471805599453;
 static constexpr float CE_NEG_INF = -__builtin_inff();
 static constexpr int CE_AMAX_BLOCKS = 512;            // per tensor, the hidden states in as many shares of rows as they are packed in
 static constexpr int CE_ROW_PAD = 256, CE_COL_PAD = 256;
-static constexpr int CE_SCORE_ROWS = 64;              // rows up to which scoring reads the inputs in place
+static constexpr int CE_JOIN_BLOCKS = 1 << 20;         // a grid holds fewer than 2^32 threads
+// rows up to which scoring reads the inputs in place: 64 x 65536 x 512 bf16 48 us against 62 packed, fp32 89 against 127
+static constexpr int CE_SCORE_ROWS = 64;
 
 struct CeScalars {            // head of the saved area
     int ex, ew;               // packed = value * 2^-e
@@ -235,7 +239,7 @@ template <typename T> __device__ __forceinline__ float ce_bias(const T *bias, in
 }
 
 // A workgroup keeps its BN hidden rows and walks over a share of the vocabulary's tiles, the next tile's first steps in flight while it
-// works on this one's logits (86 -> LOGITS_FWD us for 8192 x 16384 x 128 bf16 with one tile per workgroup); the running maximum and sum stay
+// works on this one's logits (forward pass of 8192 x 16384 x 128 bf16: 81 us, 90 with one tile per workgroup); the running maximum and sum stay
 // in each lane until the last tile.
 template <typename T, bool SPLIT, bool BACK, int BM, int BN, int WM, int WN, int NST>
 __global__ void __launch_bounds__(WM *WN * 64, 2) ce_logits_kernel(CeLogits a, const T *bias) {
@@ -717,39 +721,40 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) ce_grads_kernel(CeGrads a) {
     }
 }
 
-// out[r][d] = factor * sum over splits of part[s][r][d], the splits in their order; VE elements per thread
+// out[r][d] = factor * sum over splits of part[s][r][d], the splits in their order; VE elements per thread and trip
 template <typename T, int VE>
-__device__ __forceinline__ void ce_join(const CeGrads &a, const CeGrad &c, bool weight, int bid) {
-    const int64_t n = (weight ? c.rows : (int64_t)a.sc->live) * a.D, stride = c.part_rows * a.D, k = ((int64_t)bid * 256 + threadIdx.x) * VE;
-    if (k >= n) return;
-    const int64_t row = k / a.D;
-    float v[VE];
-#pragma unroll
-    for (int e = 0; e < VE; ++e) v[e] = 0.0f;
-    constexpr int U = 8;
-    for (int s = 0; s < c.splits; s += U) {
-        Pack<float, VE> p[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            p[u] = *(const Pack<float, VE> *)(c.part + (s + u < c.splits ? s + u : s) * stride + k);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (s + u < c.splits)
-#pragma unroll
-                for (int e = 0; e < VE; ++e) v[e] += p[u].v[e];
-    }
+__device__ __forceinline__ void ce_join(const CeGrads &a, const CeGrad &c, bool weight, int bid, int blocks) {
+    const int64_t n = (weight ? c.rows : (int64_t)a.sc->live) * a.D, stride = c.part_rows * a.D;
     const float f = ce_unscale(a.sc, a.grad, a.gmax, a.reduction, weight ? a.sc->ex : a.sc->ew);
-    T *out = (T *)c.out + (weight ? c.out0 + row : (int64_t)a.orig[row]) * a.D + (k - row * a.D);
+    for (int64_t k = ((int64_t)bid * 256 + threadIdx.x) * VE; k < n; k += (int64_t)blocks * 256 * VE) {
+        const int64_t row = k / a.D;
+        float v[VE];
 #pragma unroll
-    for (int e = 0; e < VE; ++e) out[e] = from_f32<T>(v[e] * f);
+        for (int e = 0; e < VE; ++e) v[e] = 0.0f;
+        constexpr int U = 8;
+        for (int s = 0; s < c.splits; s += U) {
+            Pack<float, VE> p[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                p[u] = *(const Pack<float, VE> *)(c.part + (s + u < c.splits ? s + u : s) * stride + k);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (s + u < c.splits)
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) v[e] += p[u].v[e];
+        }
+        T *out = (T *)c.out + (weight ? c.out0 + row : (int64_t)a.orig[row]) * a.D + (k - row * a.D);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) out[e] = from_f32<T>(v[e] * f);
+    }
 }
 
 // what is left of a piece in one launch: dhidden and dweight from their partial sums (bx / bw workgroups), dbias
 template <typename T, int VE>
 __global__ void __launch_bounds__(256) ce_join_kernel(CeGrads a, int bx, int bw, int live, T *dbias) {
     const int bid = blockIdx.x;
-    if (bid < bx) { ce_join<T, VE>(a, a.x, false, bid); return; }
-    if (bid < bx + bw) { ce_join<T, VE>(a, a.w, true, bid - bx); return; }
+    if (bid < bx) { ce_join<T, VE>(a, a.x, false, bid, bx); return; }
+    if (bid < bx + bw) { ce_join<T, VE>(a, a.w, true, bid - bx, bw); return; }
     const int v = (bid - bx - bw) * 256 + threadIdx.x;
     if (v >= live) return;
     const int pos = (v & ~12) | ((v & 4) << 1) | ((v & 8) >> 1);
@@ -990,7 +995,7 @@ static int ce_forward(const tnp_vocab_ce *p, const CeForward &f, float *loss, hi
         a.w = GemmOperand{f.saved.w, sh.Vp, 0};
         a.x = GemmOperand{f.saved.x, sh.Mp, 0};
         a.sc = f.saved.sc; a.tc = f.saved.tc; a.orig = f.saved.orig; a.Mp = sh.Mp; a.V = sh.V; a.v0 = 0; a.steps = sh.panels;
-            a.part = f.part; a.tlogit = f.tlogit; a.v_shares = ce_logit_shares(sh, sh.Vp);
+        a.part = f.part; a.tlogit = f.tlogit; a.v_shares = ce_logit_shares(sh, sh.Vp);
         if ((rc = ce_logits<T, SPLIT, false>(a, sh.Vp, ce_big(sh), (const T *)p->bias, s))) return rc;
     }
     CeRows r = {};
@@ -1037,9 +1042,9 @@ static int ce_backward(const tnp_vocab_ce *p, const CeBackward &b, const float *
         rc = b.tile == 256 ? ce_launch_grads<T, SPLIT, 256, 256, 2, 4, 4>(c, s) : ce_launch_grads<T, SPLIT, 128, 128, 2, 2, 4>(c, s);
         if (rc) return rc;
         const int ve = sh.D % 4 == 0 ? 4 : 1;
-        const int64_t per = 256 * ve;
-        const int bx = dhidden && b.part_x && last ? (int)((sh.M * sh.D + per - 1) / per) : 0;
-        const int bw = dweight && b.part_w ? (int)((c.w.rows * sh.D + per - 1) / per) : 0, bb = dbias ? (live + 255) / 256 : 0;
+        auto join_blocks = [&](int64_t n) { return (int)std::min<int64_t>((n + 256 * ve - 1) / (256 * ve), CE_JOIN_BLOCKS); };
+        const int bx = dhidden && b.part_x && last ? join_blocks(sh.M * sh.D) : 0;
+        const int bw = dweight && b.part_w ? join_blocks(c.w.rows * sh.D) : 0, bb = dbias ? (live + 255) / 256 : 0;
         if (bx + bw + bb) {
             T *db = dbias ? (T *)dbias + v0 : nullptr;
             if (ve == 4) hipLaunchKernelGGL((ce_join_kernel<T, 4>), dim3(bx + bw + bb), dim3(256), 0, s, c, bx, bw, live, db);
