@@ -45,6 +45,27 @@ def test_cross_entropy_arguments(kw, error):
         _ce(**kw)
 
 
+def test_registered_backward_operators_refuse():
+    """called by hand with tensors that do not belong together"""
+    from trajnetplusplusbaselines_amd import ops  # noqa: F401
+    i = lambda *s: torch.zeros(*s, dtype=torch.int64)
+    emb = torch.ops.trajnet.token_embedding_backward
+    for grad, tok, v, error in ((torch.zeros(3, 8), i(4), 5, ValueError), (torch.zeros(3, 8), i(3), 0, ValueError),
+                                (torch.zeros(3, 8), torch.zeros(3), 5, TypeError), (torch.zeros(3, 8).double(), i(3), 5, TypeError),
+                                (torch.zeros(3, 8), i(3), 5, RuntimeError)):
+        with pytest.raises(error):
+            emb(grad, tok, v, 1.0)
+    ce = torch.ops.trajnet.vocab_cross_entropy_backward
+    x, w, t, b = torch.zeros(3, 8), torch.zeros(4, 8), i(3), torch.zeros(4)
+    saved = torch.zeros(vocab.saved_bytes(3, 4, 8, torch.float32), dtype=torch.uint8)
+    for args, error in (((torch.zeros(3), x, w, t, b, saved, 'mean'), ValueError), ((torch.zeros(()), x, w, t, b, saved, 'none'), ValueError),
+                        ((torch.zeros(()), x, w, t, b, saved[1:], 'mean'), ValueError), ((torch.zeros(()), x, w, t, b, saved.char(), 'mean'), ValueError),
+                        ((torch.zeros(()), x, w, i(2), b, saved, 'sum'), ValueError), ((torch.zeros(()), x, w, t, b[:3], saved, 'sum'), ValueError),
+                        ((torch.zeros(()), x, w, t, b, saved, 'mean'), RuntimeError)):
+        with pytest.raises(error):
+            ce(*args)
+
+
 def test_c_entries_refuse_on_the_host():
     L = _lib.lib()
     p = ctypes.c_void_p(1 << 20)        # never followed: every call below is refused first
@@ -55,9 +76,10 @@ def test_c_entries_refuse_on_the_host():
         assert fwd(**bad) == -1
         assert b'tnp_token_embedding_forward' in L.tnp_last_error()
     assert fwd(N=0, tokens=None) == 0
-    need = L.tnp_token_embedding_backward_workspace_bytes(100, 50, 8)
+    assert L.tnp_token_embedding_backward_workspace_bytes(100, 50, 8) == 0          # few tokens are not sorted
+    need = L.tnp_token_embedding_backward_workspace_bytes(10000, 50, 8)
     assert need > 0
-    args = [p, 8, 100, p, 8, 50, 8, 0, 1.0, p, 8, p, need - 1, None]
+    args = [p, 8, 10000, p, 8, 50, 8, 0, 1.0, p, 8, p, need - 1, None]
     assert L.tnp_token_embedding_backward(*args) == -1 and b'workspace' in L.tnp_last_error()
     a = vocab.VocabCe(dtype=0, reduction=1, M=10, V=20, D=8, hidden=1 << 20, ld_hidden=8, weight=1 << 20, ld_weight=8, target=1 << 20)
     ref = ctypes.byref(a)

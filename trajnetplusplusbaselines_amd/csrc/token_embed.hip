@@ -1,10 +1,11 @@
 // Token embedding (gfx950): out[i] = scale * weight[token[i]], and the gradient of the table,
 //     dweight[v] = scale * sum over { i : token[i] == v } of grad[i]
-// summed in ascending i within fixed chunks, so that two calls on the same inputs give the same bits.  A negative token is an
+// summed in an order that the sizes and tokens fix, so that two calls on the same inputs give the same bits.  A negative token is an
 // absent track: a zero row forward, nothing backward.  A token >= V has no row: NaN forward (an error that shows and cannot
 // fault), nothing backward.
 //
-// Forward: one pass, bound by memory.  Backward: the tokens are sorted (a stable radix sort of (token, i) pairs, digits of up to
+// Forward: one pass, bound by memory.  Backward of few tokens: every token's workgroup looks for its like (embed_small_kernel).  Of more:
+// the tokens are sorted (a stable radix sort of (token, i) pairs, digits of up to
 // 10 bits), so that all rows of one token are neighbours; chunks of 8, 16 or 32 sorted positions are summed by one group of lanes each,
 // whatever the distribution of the tokens -- a table row that owns half of the batch is split over many chunks and joined.
 // Every gradient row is read once and every table row written once; table rows without a token are zeroed by their own workgroups,
@@ -13,10 +14,17 @@
 
 namespace tnp {
 
-static constexpr int EMB_SORT_THREADS = 512;  // eight waves per workgroup of the sort, each with 4 or 16 rows of 64 pairs
-static constexpr int EMB_COUNT_ALL = 8;       // workgroups of the sort up to which each counts all keys
+static constexpr int EMB_SORT_THREADS = 512, EMB_SORT_ROWS = 4;      // eight waves per workgroup of the sort, each with four rows of 64 pairs
+static constexpr int EMB_COUNT_ALL = 4;       // workgroups of the sort up to which each counts all keys: 6000 x 64 19 us against 21, 16000 x 64 28 against 26
+// workgroups of the sort from which on their histograms are summed by segments: 524288 x 64 56 us against 64, 1310720 x 64 163 against 226,
+// 16777216 x 16 1.17 ms against 10.7; 128 workgroups (262144 x 64) 48 against 48
+static constexpr int EMB_SEGMENTS_FROM = 256;
+// Tokens, and elements of the gradient, up to which nothing is sorted.  Tables of 300 rows, all tokens alike / spread, against the sort:
+// 36 x 64 9 / 9 us against 16 / 16, 4096 x 64 34 / 10 against 26 / 18, 1024 x 512 17 / 15 against 23 / 17; beyond it: 8192 x 64 spread 24
+// against 19, 1024 x 1024 24 / 25 against 22 / 17, 4096 x 512 71 / 55 against 33 / 21.
+static constexpr int64_t EMB_SMALL_TOKENS = 4096, EMB_SMALL_ELEMENTS = 1 << 19;
 static constexpr int EMB_JOIN_CHUNKS = 32;    // chunks per workgroup of the join
-static constexpr int EMB_JOIN_SHORT = 8;      // parts of a run that one group of lanes adds up by itself
+static constexpr int EMB_JOIN_SHORT = 32;     // parts of a run that one group of lanes adds up by itself
 static constexpr int EMB_MAX_BITS = 10;      // eight waves' counters of 2^10 digits: 32 KB of LDS
 static constexpr int64_t EMB_MAX_TOKENS = 1 << 28;
 
@@ -68,17 +76,17 @@ __device__ __forceinline__ uint64_t same_digit(uint32_t d, int bits, bool live) 
 
 // Ranks of a wave's pairs within (wave, digit), in ascending position, counts left in cnt[] (this wave's counters, zeroed by the
 // caller).  Only the first lane of a digit's group touches the counter, and LDS operations of a wave execute in order.
-template <typename I, int ROWS, bool RANK>
+template <typename I, bool RANK>
 __device__ __forceinline__ void embed_count(const I *tokens, const uint32_t *keys, int64_t base, int64_t N, uint32_t V, int shift,
                                             int bits, uint32_t *cnt, uint32_t *key, uint32_t *rank) {
     const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
+    for (int r = 0; r < EMB_SORT_ROWS; ++r) {
         const int64_t i = base + r * 64 + lane;
         key[r] = i < N ? embed_key(tokens, keys, i, V) : 0;
     }
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
+    for (int r = 0; r < EMB_SORT_ROWS; ++r) {
         const bool live = base + r * 64 + lane < N;
         const uint32_t d = (key[r] >> shift) & ((1u << bits) - 1);
         const uint64_t m = same_digit(d, bits, live);
@@ -89,27 +97,44 @@ __device__ __forceinline__ void embed_count(const I *tokens, const uint32_t *key
     }
 }
 
-template <typename I, int ROWS>
+template <typename I>
 __global__ void __launch_bounds__(EMB_SORT_THREADS) embed_hist_kernel(const I *tokens, const uint32_t *keys, int64_t N, uint32_t V,
                                                                       int shift, int bits, uint32_t *hist) {
     extern __shared__ uint32_t cnt[];
     const int nb = 1 << bits;
     for (int b = threadIdx.x; b < nb; b += EMB_SORT_THREADS) cnt[b] = 0;
     __syncthreads();
-    uint32_t key[ROWS];
-    const int64_t base = ((int64_t)blockIdx.x * (EMB_SORT_THREADS / 64) + (threadIdx.x >> 6)) * (ROWS * 64);
-    embed_count<I, ROWS, false>(tokens, keys, base, N, V, shift, bits, cnt, key, nullptr);
+    uint32_t key[EMB_SORT_ROWS];
+    const int64_t base = ((int64_t)blockIdx.x * (EMB_SORT_THREADS / 64) + (threadIdx.x >> 6)) * (EMB_SORT_ROWS * 64);
+    embed_count<I, false>(tokens, keys, base, N, V, shift, bits, cnt, key, nullptr);
     __syncthreads();
     for (int b = threadIdx.x; b < nb; b += EMB_SORT_THREADS) hist[(size_t)blockIdx.x * nb + b] = cnt[b];
 }
 
+// sums of 2^sl histograms each
+__global__ void __launch_bounds__(256) embed_segments_kernel(const uint32_t *hist, int nblk, int nb, int sl, uint32_t *seg) {
+    const int b = blockIdx.y * 256 + threadIdx.x, k0 = blockIdx.x << sl, k1 = min(k0 + (1 << sl), nblk);
+    if (b >= nb) return;
+    constexpr int U = 16;
+    uint32_t sum = 0;
+    for (int k = k0; k < k1; k += U) {
+        uint32_t h[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) h[u] = hist[(size_t)(k + u < k1 ? k + u : k) * nb + b];
+#pragma unroll
+        for (int u = 0; u < U; ++u) sum += k + u < k1 ? h[u] : 0;
+    }
+    seg[(size_t)blockIdx.x * nb + b] = sum;
+}
+
 // Every workgroup forms its own offsets from the histograms of all of them (nblk * 2^bits counters, L2-resident): one launch less
 // per pass than a scan kernel in between.  Up to eight workgroups (hist == NULL) count all the keys themselves, another launch less.
-template <typename I, int ROWS>
+// From 256 on the histograms are summed by segments first (seg): what all workgroups read together would grow with their square.
+template <typename I>
 __global__ void __launch_bounds__(EMB_SORT_THREADS) embed_scatter_kernel(const I *tokens, const uint32_t *keys, const uint32_t *idx,
                                                                          int64_t N, uint32_t V, int shift, int bits,
-                                                                         const uint32_t *hist, int nblk, uint32_t *keys_out,
-                                                                         uint32_t *idx_out) {
+                                                                         const uint32_t *hist, const uint32_t *seg, int sl, int nblk,
+                                                                         uint32_t *keys_out, uint32_t *idx_out) {
     extern __shared__ uint32_t lds[];
     const int nb = 1 << bits, nw = EMB_SORT_THREADS / 64;
     uint32_t *cnt = lds;                // [waves][nb]: counts, then the first position of (wave, digit)
@@ -122,7 +147,7 @@ __global__ void __launch_bounds__(EMB_SORT_THREADS) embed_scatter_kernel(const I
         for (int b = tid; b < 2 * nb; b += EMB_SORT_THREADS) all[b] = 0;
     __syncthreads();
     if (count_all) {
-        const int64_t mine = (int64_t)blockIdx.x * nw * ROWS * 64;
+        const int64_t mine = (int64_t)blockIdx.x * nw * EMB_SORT_ROWS * 64;
         constexpr int U = 8;
         for (int64_t i = tid; i < N; i += EMB_SORT_THREADS * U) {
             uint32_t k[U];
@@ -137,14 +162,14 @@ __global__ void __launch_bounds__(EMB_SORT_THREADS) embed_scatter_kernel(const I
             }
         }
     }
-    uint32_t key[ROWS], rank[ROWS], from[ROWS];
-    const int64_t base = ((int64_t)blockIdx.x * nw + wave) * (ROWS * 64);
+    uint32_t key[EMB_SORT_ROWS], rank[EMB_SORT_ROWS], from[EMB_SORT_ROWS];
+    const int64_t base = ((int64_t)blockIdx.x * nw + wave) * (EMB_SORT_ROWS * 64);
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
+    for (int r = 0; r < EMB_SORT_ROWS; ++r) {
         const int64_t i = base + r * 64 + lane;
         from[r] = idx && i < N ? idx[i] : (uint32_t)i;
     }
-    embed_count<I, ROWS, true>(tokens, keys, base, N, V, shift, bits, cnt + wave * nb, key, rank);
+    embed_count<I, true>(tokens, keys, base, N, V, shift, bits, cnt + wave * nb, key, rank);
     __syncthreads();
     const int per = (nb + EMB_SORT_THREADS - 1) / EMB_SORT_THREADS;       // digits per thread: 1 or 2
     uint32_t total[2] = {0, 0}, before[2] = {0, 0}, sum = 0;
@@ -159,15 +184,25 @@ __global__ void __launch_bounds__(EMB_SORT_THREADS) embed_scatter_kernel(const I
             before[j] = all[nb + b];
         } else {
             constexpr int U = 16;                              // counters in flight
-            for (int k = 0; k < nblk; k += U) {
-                uint32_t h[U];
+            auto add = [&](const uint32_t *from, int k0, int k1, int mine) {      // total += all of them, before += those below mine
+                for (int k = k0; k < k1; k += U) {
+                    uint32_t h[U];
 #pragma unroll
-                for (int u = 0; u < U; ++u) h[u] = k + u < nblk ? hist[(size_t)(k + u) * nb + b] : 0;
+                    for (int u = 0; u < U; ++u) h[u] = k + u < k1 ? from[(size_t)(k + u) * nb + b] : 0;
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    before[j] += k + u < (int)blockIdx.x ? h[u] : 0;
-                    total[j] += h[u];
+                    for (int u = 0; u < U; ++u) {
+                        before[j] += k + u < mine ? h[u] : 0;
+                        total[j] += h[u];
+                    }
                 }
+            };
+            if (!seg) {
+                add(hist, 0, nblk, blockIdx.x);
+            } else {
+                const int s = blockIdx.x >> sl;
+                add(hist, s << sl, blockIdx.x, blockIdx.x);
+                total[j] = 0;
+                add(seg, 0, (nblk + (1 << sl) - 1) >> sl, s);
             }
         }
         sum += total[j];
@@ -195,7 +230,7 @@ __global__ void __launch_bounds__(EMB_SORT_THREADS) embed_scatter_kernel(const I
     }
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
+    for (int r = 0; r < EMB_SORT_ROWS; ++r) {
         const int64_t i = base + r * 64 + lane;
         if (i >= N) continue;
         const uint32_t d = (key[r] >> shift) & (nb - 1);
@@ -226,7 +261,7 @@ __global__ void __launch_bounds__(256) embed_reduce_kernel(const uint32_t *keys,
     if (blockIdx.x >= sum_blocks) {                    // 64 table rows per wave
         const uint32_t v0 = ((blockIdx.x - sum_blocks) * 4 + (threadIdx.x >> 6)) * 64, v = v0 + (threadIdx.x & 63);
         bool none = v < V;
-        if (none && N > 0) {
+        if (none) {
             const uint32_t at = v == 0 ? 0 : embed_upper(keys, 0, N, v - 1);
             none = at >= N || keys[at] != v;
         }
@@ -314,7 +349,7 @@ template <int VE> __device__ __forceinline__ Parts<VE> load_parts(const float *a
 }
 
 // Runs that go on past their chunk: tail[c] + head[c + 1] + ... of the run that starts in chunk c.  A workgroup looks after 32 chunks:
-// first every group of lanes adds up runs of up to eight parts by itself, then all of them together stride over each longer one and
+// first every group of lanes adds up runs of up to 32 parts by itself, then all of them together stride over each longer one and
 // meet in LDS.  Every order of addition is fixed by the sizes.
 template <typename T, int VE>
 __global__ void __launch_bounds__(512) embed_join_kernel(const uint32_t *keys, uint32_t N, uint32_t V, int D, int lsh, int csh, float scale,
@@ -351,22 +386,28 @@ __global__ void __launch_bounds__(512) embed_join_kernel(const uint32_t *keys, u
         if (long_chunk[j] != 1 || c >= D) continue;
         const uint32_t chunk = blockIdx.x * EMB_JOIN_CHUNKS + j, b = (chunk + 1) << csh, k = keys[b];
         // parts behind the run's end: the run's first part again, not added -- loads under a condition wait for each other
-        uint32_t first[EMB_JOIN_SHORT];
-        Parts<VE> h[EMB_JOIN_SHORT];
-#pragma unroll
-        for (int u = 0; u < EMB_JOIN_SHORT; ++u) first[u] = keys[(uint64_t)b + (u << csh) < N ? b + (u << csh) : b - 1];
-        int parts = 0;
-#pragma unroll
-        for (int u = 0; u < EMB_JOIN_SHORT; ++u) parts += (uint64_t)b + (u << csh) < N && first[u] == k;
         const Parts<VE> t = load_parts<VE>(tail + (size_t)chunk * D + c);
-#pragma unroll
-        for (int u = 0; u < EMB_JOIN_SHORT; ++u) h[u] = load_parts<VE>(head + (size_t)(chunk + 1 + (u < parts ? u : 0)) * D + c);
         float acc[VE];
 #pragma unroll
-        for (int e = 0; e < VE; ++e) {
-            acc[e] = t.p[e / 4].v[e % 4];
+        for (int e = 0; e < VE; ++e) acc[e] = t.p[e / 4].v[e % 4];
+        constexpr int P = 16, U = 8;                   // keys looked at and parts fetched at a time
+        for (int q0 = 0, parts = P; q0 < EMB_JOIN_SHORT && parts == P; q0 += P) {
+            const uint64_t b0 = (uint64_t)b + ((uint64_t)q0 << csh);
+            uint32_t first[P];
 #pragma unroll
-            for (int u = 0; u < EMB_JOIN_SHORT; ++u) acc[e] += u < parts ? h[u].p[e / 4].v[e % 4] : 0.0f;
+            for (int u = 0; u < P; ++u) first[u] = keys[b0 + (u << csh) < N ? b0 + (u << csh) : b - 1];
+            parts = 0;
+#pragma unroll
+            for (int u = 0; u < P; ++u) parts += b0 + (u << csh) < N && first[u] == k;
+            for (int q = 0; q < parts; q += U) {
+                Parts<VE> h[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) h[u] = load_parts<VE>(head + (size_t)(chunk + 1 + (q + u < parts ? q0 + q + u : 0)) * D + c);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) acc[e] += q + u < parts ? h[u].p[e / 4].v[e % 4] : 0.0f;
+            }
         }
         finish(k, acc);
     }
@@ -411,6 +452,101 @@ __global__ void __launch_bounds__(512) embed_join_kernel(const uint32_t *keys, u
     }
 }
 
+// ---- few tokens: no sort ----------------------------------------------------------------------------------------------------
+// One launch: workgroup (i < N, 64 columns) owns token i's row if no earlier position names it, lists the positions that do (every wave
+// compacts its quarter of them in order) and adds their gradient rows, groups of lanes striding over the list; the workgroups behind
+// zero 256 table rows each, less those named.  N^2 comparisons from the L2 instead of four to six dependent launches.
+template <typename T, int VE, typename I>
+__global__ void __launch_bounds__(256) embed_small_kernel(const I *tokens, int N, int64_t V, const T *grad, int64_t ldg, int D, float scale,
+                                                          T *dw, int64_t ldd) {
+    constexpr int LANES = 64 / VE, GROUPS = 256 / LANES, U = 8;
+    __shared__ uint16_t list[4][EMB_SMALL_TOKENS / 4];
+    __shared__ int count[4];
+    __shared__ float sums[256 * VE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, grp = tid / LANES;
+    const int c = ((int)blockIdx.y * LANES + tid % LANES) * VE;
+    if ((int)blockIdx.x >= N) {
+        uint8_t *named = (uint8_t *)list;
+        const int64_t v0 = (int64_t)(blockIdx.x - N) * 256;
+        named[tid] = 0;
+        __syncthreads();
+        for (int j = tid; j < N; j += 256 * U) {
+            int64_t t[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) t[u] = tokens[j + u * 256 < N ? j + u * 256 : j];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (t[u] >= v0 && t[u] < v0 + 256) named[t[u] - v0] = 1;
+        }
+        __syncthreads();
+        if (c >= D) return;
+        Pack<T, VE> z;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) z.v[e] = from_f32<T>(0.0f);
+        for (int r = grp; r < 256 && v0 + r < V; r += GROUPS)
+            if (!named[r]) *(Pack<T, VE> *)(dw + (v0 + r) * ldd + c) = z;
+        return;
+    }
+    const int i = blockIdx.x;
+    const int64_t t = tokens[i];
+    if (t < 0 || t >= V) return;                       // uniform
+    bool before = false;
+    for (int j = tid; j < i; j += 256 * U) {
+        int64_t o[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) o[u] = tokens[j + u * 256 < i ? j + u * 256 : j];
+#pragma unroll
+        for (int u = 0; u < U; ++u) before = before || o[u] == t;
+    }
+    if (__syncthreads_or(before)) return;
+    const int quarter = (N - i + 3) / 4, j0 = i + wave * quarter, j1 = j0 + quarter < N ? j0 + quarter : N;
+    int n = 0;
+    for (int j = j0; j < j1; j += 64 * U) {
+        int64_t o[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) o[u] = tokens[j + u * 64 + lane < j1 ? j + u * 64 + lane : i];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool hit = j + u * 64 + lane < j1 && o[u] == t;
+            const uint64_t m = __ballot(hit);
+            if (hit) list[wave][n + __popcll(m & ((1ull << lane) - 1))] = (uint16_t)(j + u * 64 + lane);
+            n += __popcll(m);
+        }
+    }
+    if (lane == 0) count[wave] = n;
+    __syncthreads();
+    const int n1 = count[0], n2 = n1 + count[1], n3 = n2 + count[2], all = n3 + count[3];
+    auto at = [&](int k) -> int64_t { return k < n1 ? list[0][k] : k < n2 ? list[1][k - n1] : k < n3 ? list[2][k - n2] : list[3][k - n3]; };
+    float acc[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) acc[e] = 0.0f;
+    if (c < D)
+        for (int k = grp; k < all; k += GROUPS * U) {
+            Pack<T, VE> g[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) g[u] = *(const Pack<T, VE> *)(grad + at(k + u * GROUPS < all ? k + u * GROUPS : k) * ldg + c);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < VE; ++e) acc[e] += k + u * GROUPS < all ? to_f32(g[u].v[e]) : 0.0f;
+        }
+    const int used = all < GROUPS ? all : GROUPS;      // groups that have a row
+    if (used > 1) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) sums[tid * VE + e] = acc[e];
+        __syncthreads();
+    }
+    if (grp == 0 && c < D) {
+        for (int g = 1; g < used; ++g)
+#pragma unroll
+            for (int e = 0; e < VE; ++e) acc[e] += sums[(g * LANES + tid) * VE + e];
+        Pack<T, VE> o;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) o.v[e] = from_f32<T>(acc[e] * scale);
+        *(Pack<T, VE> *)(dw + t * ldd + c) = o;
+    }
+}
+
 // ---- host -------------------------------------------------------------------------------------------------------------------
 // elements per lane: 16 bytes where rows and pointers allow it, else 4, else one element
 static int embed_width(int dtype, int D, std::initializer_list<int64_t> lds, std::initializer_list<const void *> ptrs) {
@@ -431,19 +567,22 @@ static int lane_shift(int D, int ve, int most) {
     return s;
 }
 
-struct EmbedSort { int bits, passes, rows, nblk; };
+struct EmbedSort { int bits, passes, nblk, sl, nseg; };  // nseg sums of 2^sl histograms, or 0
 static EmbedSort embed_sort_plan(int64_t N, int64_t V) {
     EmbedSort p = {};
     int need = 1;
     while (((int64_t)1 << need) <= V) ++need;          // keys 0 .. V
     p.passes = (need + EMB_MAX_BITS - 1) / EMB_MAX_BITS;
     p.bits = (need + p.passes - 1) / p.passes;
-    // four rows per wave while every workgroup can still read all histograms quickly, sixteen beyond
-    p.rows = N <= (1 << 18) ? 4 : 16;
-    const int64_t items = EMB_SORT_THREADS * p.rows;
+    const int64_t items = EMB_SORT_THREADS * EMB_SORT_ROWS;
     p.nblk = (int)((N + items - 1) / items);
+    p.sl = 6;                                          // about as many sums as histograms in one
+    while (((int64_t)1 << 2 * p.sl) < p.nblk) ++p.sl;
+    p.nseg = p.nblk >= EMB_SEGMENTS_FROM ? (p.nblk + (1 << p.sl) - 1) >> p.sl : 0;
     return p;
 }
+
+static bool embed_small(int64_t N, int D) { return N <= EMB_SMALL_TOKENS && N * D <= EMB_SMALL_ELEMENTS; }
 
 // rows of head / tail: chunks are shorter than 32 positions only where there are fewer than 1024 * 64 of the shorter ones
 static size_t embed_parts(int64_t N) {
@@ -482,29 +621,30 @@ static int embed_forward_typed(const void *tokens, int tb, int64_t N, const void
     return embed_forward_run<T, VE, int32_t>((const int32_t *)tokens, N, (const T *)w, ldw, V, D, scale, (T *)out, ldo, s);
 }
 
-template <typename I, int ROWS>
-static int embed_sort_rows(const I *tokens, int64_t N, uint32_t V, const EmbedSort &p, uint32_t *keys[2], uint32_t *idx[2], uint32_t *hist,
-                           hipStream_t s) {
+template <typename I>
+static int embed_sort(const I *tokens, int64_t N, uint32_t V, const EmbedSort &p, uint32_t *keys[2], uint32_t *idx[2], uint32_t *hist,
+                      hipStream_t s) {
     for (int pass = 0; pass < p.passes; ++pass) {
         const uint32_t *kin = pass ? keys[(pass + 1) & 1] : nullptr, *iin = pass ? idx[(pass + 1) & 1] : nullptr;
         const size_t nb = (size_t)1 << p.bits;
         const bool count_all = p.nblk <= EMB_COUNT_ALL;
         if (!count_all) {
-            hipLaunchKernelGGL((embed_hist_kernel<I, ROWS>), dim3(p.nblk), dim3(EMB_SORT_THREADS), nb * 4, s, tokens, kin, N, V, pass * p.bits,
+            hipLaunchKernelGGL((embed_hist_kernel<I>), dim3(p.nblk), dim3(EMB_SORT_THREADS), nb * 4, s, tokens, kin, N, V, pass * p.bits,
                                p.bits, hist);
             TNP_HIP(hipGetLastError());
         }
+        uint32_t *seg = p.nseg ? hist + (size_t)p.nblk * nb : nullptr;
+        if (seg) {
+            hipLaunchKernelGGL(embed_segments_kernel, dim3(p.nseg, (unsigned)((nb + 255) / 256)), dim3(256), 0, s, hist, p.nblk, (int)nb, p.sl,
+                               seg);
+            TNP_HIP(hipGetLastError());
+        }
         const size_t smem = (EMB_SORT_THREADS / 64 * nb + EMB_SORT_THREADS / 64 + (count_all ? 2 * nb : 0)) * 4;
-        hipLaunchKernelGGL((embed_scatter_kernel<I, ROWS>), dim3(p.nblk), dim3(EMB_SORT_THREADS), smem, s, tokens, kin, iin, N, V, pass * p.bits,
-                           p.bits, count_all ? nullptr : hist, p.nblk, keys[pass & 1], idx[pass & 1]);
+        hipLaunchKernelGGL((embed_scatter_kernel<I>), dim3(p.nblk), dim3(EMB_SORT_THREADS), smem, s, tokens, kin, iin, N, V, pass * p.bits,
+                           p.bits, count_all ? nullptr : hist, seg, p.sl, p.nblk, keys[pass & 1], idx[pass & 1]);
         TNP_HIP(hipGetLastError());
     }
     return 0;
-}
-template <typename I>
-static int embed_sort(const I *tokens, int64_t N, uint32_t V, const EmbedSort &p, uint32_t *keys[2], uint32_t *idx[2], uint32_t *hist,
-                      hipStream_t s) {
-    return p.rows == 4 ? embed_sort_rows<I, 4>(tokens, N, V, p, keys, idx, hist, s) : embed_sort_rows<I, 16>(tokens, N, V, p, keys, idx, hist, s);
 }
 
 template <typename T, int VE>
@@ -513,7 +653,7 @@ static int embed_sums(const uint32_t *keys, const uint32_t *idx, uint32_t N, uin
     const int lsh = lane_shift(D, VE, 6);
     const unsigned cols = (unsigned)((D + (VE << lsh) - 1) / (VE << lsh));
     // 32 positions per chunk where that already is a wave per SIMD; shorter chunks shorten the chain of dependent loads of a small
-    // batch (43008 x 64: 16 us at 32 positions, see the table of measurements)
+    // batch (43008 x 64: 6 us at 8 positions, 16 at 32)
     int csh = 5;
     while (csh > 3 && (((uint64_t)N >> csh << lsh) >> 6) * cols < 1024) --csh;
     const unsigned chunks = (unsigned)(((uint64_t)N + (1u << csh) - 1) >> csh);
@@ -558,10 +698,10 @@ extern "C" TNP_API int tnp_token_embedding_forward(const void *tokens, int token
 }
 
 extern "C" TNP_API size_t tnp_token_embedding_backward_workspace_bytes(int64_t N, int64_t V, int D) {
-    if (N <= 0 || V < 1 || D < 1) return 0;
+    if (V < 1 || D < 1 || embed_small(N, D)) return 0;
     const EmbedSort p = embed_sort_plan(N, V);
     const size_t chunks = embed_parts(N);
-    return 4 * up256((size_t)N * 4) + up256((size_t)p.nblk * 4 << p.bits) + 2 * up256(chunks * (size_t)D * 4);
+    return 4 * up256((size_t)N * 4) + up256((size_t)(p.nblk + p.nseg) * 4 << p.bits) + 2 * up256(chunks * (size_t)D * 4);
 }
 
 namespace tnp {
@@ -570,32 +710,40 @@ static int embed_backward_typed(const uint32_t *keys, const uint32_t *idx, int64
                                 void *dw, int64_t ldd, float *head, float *tail, hipStream_t s) {
     return embed_sums<T, VE>(keys, idx, (uint32_t)N, (uint32_t)V, (const T *)grad, ldg, D, scale, (T *)dw, ldd, head, tail, s);
 }
+template <typename T, int VE>
+static int embed_small_typed(const void *tokens, int tb, int64_t N, int64_t V, const void *grad, int64_t ldg, int D, float scale, void *dw,
+                             int64_t ldd, hipStream_t s) {
+    const dim3 grid((unsigned)(N + (V + 255) / 256), (unsigned)((D + 63) / 64));
+    if (tb == 8) hipLaunchKernelGGL((embed_small_kernel<T, VE, int64_t>), grid, dim3(256), 0, s, (const int64_t *)tokens, (int)N, V,
+                                    (const T *)grad, ldg, D, scale, (T *)dw, ldd);
+    else hipLaunchKernelGGL((embed_small_kernel<T, VE, int32_t>), grid, dim3(256), 0, s, (const int32_t *)tokens, (int)N, V, (const T *)grad, ldg,
+                            D, scale, (T *)dw, ldd);
+    TNP_HIP(hipGetLastError());
+    return 0;
+}
 }  // namespace tnp
 
 extern "C" TNP_API int tnp_token_embedding_backward(const void *tokens, int token_bytes, int64_t N, const void *grad, int64_t ldg, int64_t V,
                                                     int D, int dtype, float scale, void *dweight, int64_t ldd, void *workspace,
                                                     size_t workspace_bytes, void *stream) {
     if (int rc = embed_check("tnp_token_embedding_backward", token_bytes, N, V, D, dtype, ldg, ldd)) return rc;
-    if (!dweight || (N > 0 && (!tokens || !grad || !workspace))) TNP_FAIL(-1, "tnp_token_embedding_backward: NULL pointer");
-    const size_t need = tnp_token_embedding_backward_workspace_bytes(N, V, D);
-    if (workspace_bytes < need) TNP_FAIL(-1, "tnp_token_embedding_backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    if (!dweight || (N > 0 && (!tokens || !grad))) TNP_FAIL(-1, "tnp_token_embedding_backward: NULL pointer");
     hipStream_t s = (hipStream_t)stream;
-    uint32_t *keys[2] = {nullptr, nullptr}, *idx[2] = {nullptr, nullptr};
-    float *head = nullptr, *tail = nullptr;
-    int at = 0;
-    if (N > 0) {
-        const EmbedSort p = embed_sort_plan(N, V);
-        char *w = (char *)workspace;
-        for (int k = 0; k < 2; ++k) { keys[k] = (uint32_t *)w; w += up256((size_t)N * 4); idx[k] = (uint32_t *)w; w += up256((size_t)N * 4); }
-        uint32_t *hist = (uint32_t *)w;
-        w += up256((size_t)p.nblk * 4 << p.bits);
-        head = (float *)w;
-        tail = (float *)(w + up256(embed_parts(N) * D * 4));
-        const int rc = token_bytes == 8 ? embed_sort((const int64_t *)tokens, N, (uint32_t)V, p, keys, idx, hist, s)
-                                        : embed_sort((const int32_t *)tokens, N, (uint32_t)V, p, keys, idx, hist, s);
-        if (rc) return rc;
-        at = (p.passes - 1) & 1;
-    }
     const int ve = embed_width(dtype, D, {ldg, ldd}, {grad, dweight});
+    if (embed_small(N, D))
+        return TNP_BY_WIDTH(embed_small_typed, ve, dtype, tokens, token_bytes, N, V, grad, ldg, D, scale, dweight, ldd, s);
+    const size_t need = tnp_token_embedding_backward_workspace_bytes(N, V, D);
+    if (!workspace || workspace_bytes < need) TNP_FAIL(-1, "tnp_token_embedding_backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    uint32_t *keys[2], *idx[2];
+    const EmbedSort p = embed_sort_plan(N, V);
+    char *w = (char *)workspace;
+    for (int k = 0; k < 2; ++k) { keys[k] = (uint32_t *)w; w += up256((size_t)N * 4); idx[k] = (uint32_t *)w; w += up256((size_t)N * 4); }
+    uint32_t *hist = (uint32_t *)w;
+    w += up256((size_t)(p.nblk + p.nseg) * 4 << p.bits);
+    float *head = (float *)w, *tail = (float *)(w + up256(embed_parts(N) * D * 4));
+    const int rc = token_bytes == 8 ? embed_sort((const int64_t *)tokens, N, (uint32_t)V, p, keys, idx, hist, s)
+                                    : embed_sort((const int32_t *)tokens, N, (uint32_t)V, p, keys, idx, hist, s);
+    if (rc) return rc;
+    const int at = (p.passes - 1) & 1;
     return TNP_BY_WIDTH(embed_backward_typed, ve, dtype, keys[at], idx[at], N, V, grad, ldg, D, scale, dweight, ldd, head, tail, s);
 }

@@ -151,7 +151,7 @@ def _(tokens, weight, scale):
 @torch.library.custom_op('trajnet::token_embedding_backward', mutates_args=())
 def token_embedding_backward(grad: torch.Tensor, tokens: torch.Tensor, vocab_size: int, scale: float) -> torch.Tensor:
     """dense gradient of the table (tnp_token_embedding_backward)"""
-    _dev(grad, 'grad')
+    vocab.check_embedding_backward(grad, tokens, vocab_size)
     return vocab._embedding_backward(grad, tokens, vocab_size, scale)
 
 
@@ -194,8 +194,8 @@ def _(hidden, weight, target, bias, reduction):
 def vocab_cross_entropy_backward(grad: torch.Tensor, hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor,
                                  bias: Optional[torch.Tensor], saved: torch.Tensor,
                                  reduction: str) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """gradients of hidden, weight and bias (without a bias the third is empty)"""
-    _dev(grad, 'grad')
+    """gradients of hidden, weight and bias (without a bias the third is empty); saved: the forward operator's second output"""
+    vocab.check_cross_entropy_backward(grad, hidden, weight, target, bias, saved, reduction)
     if target.numel() == 0:
         return torch.zeros_like(hidden), torch.zeros_like(weight), torch.zeros_like(bias) if bias is not None else weight.new_zeros(0)
     dx, dw, db = vocab._ce_backward(grad, hidden, weight, bias, target, saved, vocab._REDUCTIONS[reduction], (True, True, bias is not None))

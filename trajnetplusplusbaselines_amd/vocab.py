@@ -78,10 +78,10 @@ def _embedding_backward(grad, tokens, vocab, scale):
     with _On(dev):
         dw = torch.empty((vocab, d), dtype=g.dtype, device=dev)
         need = L.tnp_token_embedding_backward_workspace_bytes(n, vocab, d)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         _lib.check(L.tnp_token_embedding_backward(
             tok.data_ptr(), 8 if tok.dtype == torch.int64 else 4, n, g.data_ptr(), ld, vocab, d, _DTYPES[g.dtype], scale, dw.data_ptr(),
-            d, ws.data_ptr(), need, _lib.raw_stream()), 'tnp_token_embedding_backward')
+            d, None if ws is None else ws.data_ptr(), need, _lib.raw_stream()), 'tnp_token_embedding_backward')
     return dw
 
 
@@ -108,6 +108,16 @@ def check_embedding(tokens, weight, scale):
     if tokens.device != weight.device:
         raise RuntimeError('token_embedding: tokens on %s, weight on %s' % (tokens.device, weight.device))
     return float(scale)
+
+
+def check_embedding_backward(grad, tokens, entries):
+    if grad.dtype not in _DTYPES or tokens.dtype not in (torch.int64, torch.int32):
+        raise TypeError('token_embedding_backward: gradient of %s for tokens of %s' % (grad.dtype, tokens.dtype))
+    if grad.dim() < 1 or grad.shape[:-1] != tokens.shape or grad.shape[-1] < 1 or entries < 1:
+        raise ValueError('token_embedding_backward: gradient %s, tokens %s, %d entries' % (tuple(grad.shape), tuple(tokens.shape), entries))
+    _lib.require_device(grad, 'token_embedding_backward: grad')
+    if tokens.device != grad.device:
+        raise RuntimeError('token_embedding_backward: tokens on %s, gradient on %s' % (tokens.device, grad.device))
 
 
 def token_embedding(tokens, weight, scale=1.0):
@@ -220,6 +230,19 @@ def check_cross_entropy(hidden, weight, target, bias, reduction):
     for name, t in (('hidden', hidden), ('target', target), ('bias', bias)):
         if t is not None and t.device != weight.device:
             raise RuntimeError('vocab_cross_entropy: %s on %s, weight on %s' % (name, t.device, weight.device))
+
+
+def check_cross_entropy_backward(grad, hidden, weight, target, bias, saved, reduction):
+    if grad.shape != (target.shape if reduction == 'none' else ()):
+        raise ValueError('vocab_cross_entropy_backward: gradient %s of a loss with reduction %r, target %s'
+                         % (tuple(grad.shape), reduction, tuple(target.shape)))
+    if saved.dtype != torch.uint8 or saved.numel() != saved_bytes(target.numel(), weight.shape[0], weight.shape[-1], weight.dtype) \
+            or not saved.is_contiguous():
+        raise ValueError('vocab_cross_entropy_backward: saved is not the second output of this vocab_cross_entropy')
+    check_cross_entropy(hidden, weight, target, bias, reduction)
+    for name, t in (('grad', grad), ('saved', saved)):
+        if t.device != weight.device:
+            raise RuntimeError('vocab_cross_entropy_backward: %s on %s, weight on %s' % (name, t.device, weight.device))
 
 
 def vocab_cross_entropy(hidden, weight, target, bias=None, reduction='mean'):
