@@ -586,10 +586,35 @@ def test_a_weight_that_changes_before_the_backward_pass_is_noticed():
 
 
 def test_no_gradient_of_a_gradient():
+    """raises, also where the rest of what is differentiated has a gradient"""
     x, w, b, t = _case(70, 50, 16, torch.float32, 121)
     g, = torch.autograd.grad(vocab.vocab_cross_entropy(x, w, t, bias=b), w, create_graph=True)
-    with pytest.raises(RuntimeError):
-        torch.autograd.grad(g.sum(), w)
+    e, = torch.autograd.grad(vocab.token_embedding(t, w, 2.0).square().sum(), w, create_graph=True)
+    for z in (g, e):
+        with pytest.raises(RuntimeError, match='has no gradient'):
+            torch.autograd.grad(z.sum(), w, retain_graph=True)
+        with pytest.raises(RuntimeError, match='has no gradient'):
+            torch.autograd.grad((z * w).sum(), w, retain_graph=True)
+        with pytest.raises(RuntimeError, match='has no gradient'):
+            (z * w).sum().backward()
+    e, = torch.autograd.grad(vocab.token_embedding(t, w, 2.0).sum(), w, create_graph=True)       # of a constant: no part of it is w's
+    assert torch.equal(torch.autograd.grad((e * w).sum(), w)[0], e)
+
+
+def test_backward_accumulates_and_hooks_see_it():
+    """.backward() accumulates, twice; a hook sees the gradient; a weight that needs none gets none"""
+    x, w, b, t = _case(90, 60, 16, torch.float32, 123)
+    seen = []
+    w.register_hook(lambda g: seen.append(g.clone()))
+    for _ in range(2):
+        (vocab.vocab_cross_entropy(x, w, t, bias=b) + vocab.token_embedding(t, w).sum()).backward()
+    assert len(seen) == 2 and torch.equal(seen[0], seen[1]) and torch.equal(w.grad, 2 * seen[0])
+    fixed = w.detach()
+    loss = vocab.vocab_cross_entropy(x, fixed, t, bias=b)
+    gx, gb = torch.autograd.grad(loss, (x, b))
+    assert torch.equal(gx, x.grad / 2) and torch.equal(gb, b.grad / 2) and not vocab.token_embedding(t, fixed).requires_grad
+    with torch.no_grad():
+        assert not vocab.vocab_cross_entropy(x, w, t, bias=b).requires_grad
 
 
 def test_backward_twice_and_broadcast_gradient():

@@ -9,6 +9,13 @@ from trajnetplusplusbaselines_amd import _lib, vocab
 from trajnetplusplusbaselines_amd.lstm import TokenEmbedding, VocabularyLoss
 
 
+class VocabCe(ctypes.Structure):
+    """struct tnp_vocab_ce of include/trajnet_hip.h"""
+    _fields_ = [('dtype', ctypes.c_int32), ('reduction', ctypes.c_int32), ('M', ctypes.c_int64), ('V', ctypes.c_int32),
+                ('D', ctypes.c_int32), ('hidden', ctypes.c_void_p), ('ld_hidden', ctypes.c_int64), ('weight', ctypes.c_void_p),
+                ('ld_weight', ctypes.c_int64), ('bias', ctypes.c_void_p), ('target', ctypes.c_void_p), ('saved', ctypes.c_void_p)]
+
+
 def test_host_tensors_are_refused():
     with pytest.raises(RuntimeError, match='no CPU fallback'):
         vocab.token_embedding(torch.zeros(3, dtype=torch.int64), torch.zeros(4, 8))
@@ -81,7 +88,7 @@ def test_c_entries_refuse_on_the_host():
     assert need > 0
     args = [p, 8, 10000, p, 8, 50, 8, 0, 1.0, p, 8, p, need - 1, None]
     assert L.tnp_token_embedding_backward(*args) == -1 and b'workspace' in L.tnp_last_error()
-    a = vocab.VocabCe(dtype=0, reduction=1, M=10, V=20, D=8, hidden=1 << 20, ld_hidden=8, weight=1 << 20, ld_weight=8, target=1 << 20)
+    a = VocabCe(dtype=0, reduction=1, M=10, V=20, D=8, hidden=1 << 20, ld_hidden=8, weight=1 << 20, ld_weight=8, target=1 << 20)
     ref = ctypes.byref(a)
     assert L.tnp_vocab_ce_saved_bytes(ref) > 0
     need = L.tnp_vocab_ce_workspace_bytes(ref, 0)
@@ -90,7 +97,7 @@ def test_c_entries_refuse_on_the_host():
     a.saved = 1 << 20
     assert L.tnp_vocab_ce_backward(ref, p, p, p, p, p, 1 << 40, None) == -1 and b'bias' in L.tnp_last_error()
     for field, value in (('dtype', 3), ('reduction', 3), ('V', 0), ('D', 0), ('D', 20000), ('M', -1), ('ld_hidden', 7), ('ld_weight', 7)):
-        b = vocab.VocabCe.from_buffer_copy(a)
+        b = VocabCe.from_buffer_copy(a)
         setattr(b, field, value)
         assert L.tnp_vocab_ce_saved_bytes(ctypes.byref(b)) == 0
         assert L.tnp_vocab_ce_workspace_bytes(ctypes.byref(b), 1) == 0
@@ -100,13 +107,13 @@ def test_c_entries_refuse_on_the_host():
 
 
 def test_struct_mirror():
-    assert _lib.lib().tnp_abi_sizeof(8) == ctypes.sizeof(vocab.VocabCe)
+    assert _lib.lib().tnp_abi_sizeof(8) == ctypes.sizeof(VocabCe)
 
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
 def test_saved_bytes_from_the_sizes(dtype):
     for m, v, d in ((1, 1, 1), (256, 256, 16), (257, 300, 33), (5000, 70000, 200)):
-        a = vocab.VocabCe(dtype=vocab._DTYPES[dtype], M=m, V=v, D=d, ld_hidden=d, ld_weight=d)
+        a = VocabCe(dtype=(torch.float32, torch.bfloat16, torch.float16).index(dtype), M=m, V=v, D=d, ld_hidden=d, ld_weight=d)
         assert _lib.lib().tnp_vocab_ce_saved_bytes(ctypes.byref(a)) == vocab.saved_bytes(m, v, d, dtype)
 
 

@@ -140,7 +140,7 @@ linear.register_autograd(_linear_backward, setup_context=_linear_setup)
 @torch.library.custom_op('trajnet::token_embedding', mutates_args=())
 def token_embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float) -> torch.Tensor:
     """scale * weight[tokens], a zero row for a negative token (vocab.token_embedding, tnp_token_embedding_forward)."""
-    return vocab._embedding_forward(tokens, weight, vocab.check_embedding(tokens, weight, scale))
+    return vocab.native().embedding_forward(tokens, weight, vocab.check_embedding(tokens, weight, scale))
 
 
 @token_embedding.register_fake
@@ -152,7 +152,7 @@ def _(tokens, weight, scale):
 def token_embedding_backward(grad: torch.Tensor, tokens: torch.Tensor, vocab_size: int, scale: float) -> torch.Tensor:
     """dense gradient of the table (tnp_token_embedding_backward)"""
     vocab.check_embedding_backward(grad, tokens, vocab_size)
-    return vocab._embedding_backward(grad, tokens, vocab_size, scale)
+    return vocab.native().embedding_backward(grad, tokens, vocab_size, scale)
 
 
 @token_embedding_backward.register_fake
@@ -181,7 +181,7 @@ def vocab_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: torc
     if target.numel() == 0:
         loss = hidden.new_zeros(target.shape if reduction == 'none' else (), dtype=torch.float32)
         return loss, hidden.new_empty(vocab.saved_bytes(0, weight.shape[0], weight.shape[1], weight.dtype), dtype=torch.uint8)
-    return vocab._ce_forward(hidden, weight, bias, target, vocab._REDUCTIONS[reduction], True)
+    return vocab.native().ce_forward(hidden, weight, target, bias, vocab._REDUCTIONS[reduction])
 
 
 @vocab_cross_entropy.register_fake
@@ -198,7 +198,7 @@ def vocab_cross_entropy_backward(grad: torch.Tensor, hidden: torch.Tensor, weigh
     vocab.check_cross_entropy_backward(grad, hidden, weight, target, bias, saved, reduction)
     if target.numel() == 0:
         return torch.zeros_like(hidden), torch.zeros_like(weight), torch.zeros_like(bias) if bias is not None else weight.new_zeros(0)
-    dx, dw, db = vocab._ce_backward(grad, hidden, weight, bias, target, saved, vocab._REDUCTIONS[reduction], (True, True, bias is not None))
+    dx, dw, db = vocab.native().ce_backward(grad, hidden, weight, target, bias, saved, vocab._REDUCTIONS[reduction])
     return dx, dw, db if db is not None else weight.new_empty(0)
 
 

@@ -1,5 +1,5 @@
 """Motions as tokens: the two operators that a model over a vocabulary of displacements or grid cells needs beside the ones for
-continuous positions, on the kernels of csrc/token_embed.hip and csrc/vocab_ce.hip.
+continuous positions, on the kernels of csrc/token_embed.hip and csrc/vocab_ce.hip (autograd nodes: csrc/vocab_torch.cpp).
 
     token_embedding(tokens, weight, scale)               scale * weight[tokens]           (module: lstm.TokenEmbedding)
     vocab_cross_entropy(hidden, weight, target, bias)    cross entropy of the output layer hidden @ weight.T + bias against
@@ -10,43 +10,34 @@ and refuse host tensors.  A negative token or target is an absent track (zero ro
 vocabulary gives NaN, since the host does not look at device data.
 """
 import ctypes
+import importlib.util
+import os
 
 import torch
 
 from . import _lib
 
-_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _REDUCTIONS = {'none': 0, 'mean': 1, 'sum': 2}
+_ENTRIES = ('tnp_last_error', 'tnp_token_embedding_forward', 'tnp_token_embedding_backward_workspace_bytes', 'tnp_token_embedding_backward',
+            'tnp_vocab_ce_saved_bytes', 'tnp_vocab_ce_workspace_bytes', 'tnp_vocab_ce_forward', 'tnp_vocab_ce_backward')
+_NATIVE = None
 
 
-_current = torch._C._cuda_getDevice
-
-
-class _On(object):
-    """The device's own context where it is not the current one (the native calls take the CURRENT device's stream)."""
-    __slots__ = ('ctx',)
-
-    def __init__(self, device):
-        self.ctx = None if device.index is None or device.index == _current() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
-
-    def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
-
-
-def _rows(t):
-    """(t, elements per row) with unit column stride and rows that do not overlap; a copy only where the layout asks for one.  t of
-    more than two dimensions has to be, or is made, contiguous."""
-    d = t.shape[-1]
-    if t.is_contiguous():
-        return t, d
-    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= d:
-        return t, t.stride(0)
-    return t.contiguous(), d
+def native():
+    """csrc/vocab_torch.cpp, bound to the loaded library's entries (once)"""
+    global _NATIVE
+    if _NATIVE is None:
+        L = _lib.lib()
+        path = os.path.join(os.path.dirname(os.path.abspath(__file__)), 'lib', '_trajnet_torch.so')
+        if not os.path.exists(path):
+            raise RuntimeError('%s not found: build it with `python -c "import __graft_entry__ as g; g.build()"`' % path)
+        spec = importlib.util.spec_from_file_location('_trajnet_torch', path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind([ctypes.cast(getattr(L, e), ctypes.c_void_p).value for e in _ENTRIES])
+        _NATIVE = module
+    return _NATIVE
 
 
 def _check_table(weight, what):
@@ -57,47 +48,6 @@ def _check_table(weight, what):
 
 
 # ---- token embedding ---------------------------------------------------------------------------------------------------------
-def _embedding_forward(tokens, weight, scale):
-    w, ld = _rows(weight)
-    tok = tokens if tokens.is_contiguous() else tokens.contiguous()
-    v, d = w.shape
-    dev = w.device
-    with _On(dev):
-        out = torch.empty(tokens.shape + (d,), dtype=w.dtype, device=dev)
-        _lib.check(_lib.lib().tnp_token_embedding_forward(
-            tok.data_ptr(), 8 if tok.dtype == torch.int64 else 4, tok.numel(), w.data_ptr(), ld, v, d, _DTYPES[w.dtype], scale,
-            out.data_ptr(), d, _lib.raw_stream()), 'tnp_token_embedding_forward')
-    return out
-
-
-def _embedding_backward(grad, tokens, vocab, scale):
-    g, ld = _rows(grad)
-    tok = tokens if tokens.is_contiguous() else tokens.contiguous()
-    n, d, dev = tok.numel(), g.shape[-1], g.device
-    L = _lib.lib()
-    with _On(dev):
-        dw = torch.empty((vocab, d), dtype=g.dtype, device=dev)
-        need = L.tnp_token_embedding_backward_workspace_bytes(n, vocab, d)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        _lib.check(L.tnp_token_embedding_backward(
-            tok.data_ptr(), 8 if tok.dtype == torch.int64 else 4, n, g.data_ptr(), ld, vocab, d, _DTYPES[g.dtype], scale, dw.data_ptr(),
-            d, None if ws is None else ws.data_ptr(), need, _lib.raw_stream()), 'tnp_token_embedding_backward')
-    return dw
-
-
-class _TokenEmbeddingFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, tokens, weight, scale):
-        ctx.save_for_backward(tokens)
-        ctx.args = (weight.shape[0], scale)
-        return _embedding_forward(tokens, weight, scale)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        return None, _embedding_backward(grad, ctx.saved_tensors[0], *ctx.args), None
-
-
 def check_embedding(tokens, weight, scale):
     if not isinstance(tokens, torch.Tensor) or not isinstance(weight, torch.Tensor):
         raise TypeError('token_embedding: tokens and weight are tensors')
@@ -127,86 +77,15 @@ def token_embedding(tokens, weight, scale=1.0):
     if torch.compiler.is_compiling():
         from . import ops  # noqa: F401  (registers the operators)
         return torch.ops.trajnet.token_embedding(tokens, weight, float(scale))
-    scale = check_embedding(tokens, weight, scale)
-    if weight.requires_grad and torch.is_grad_enabled():
-        return _TokenEmbeddingFn.apply(tokens, weight, scale)
-    return _embedding_forward(tokens, weight, scale)
+    return native().token_embedding(tokens, weight, check_embedding(tokens, weight, scale))
 
 
 # ---- cross entropy over a vocabulary -----------------------------------------------------------------------------------------
-class VocabCe(ctypes.Structure):
-    """mirror of ``struct tnp_vocab_ce`` (include/trajnet_hip.h)"""
-    _fields_ = [('dtype', ctypes.c_int32), ('reduction', ctypes.c_int32), ('M', ctypes.c_int64), ('V', ctypes.c_int32),
-                ('D', ctypes.c_int32), ('hidden', ctypes.c_void_p), ('ld_hidden', ctypes.c_int64), ('weight', ctypes.c_void_p),
-                ('ld_weight', ctypes.c_int64), ('bias', ctypes.c_void_p), ('target', ctypes.c_void_p), ('saved', ctypes.c_void_p)]
-
-
 def saved_bytes(rows, entries, columns, dtype):
     """tnp_vocab_ce_saved_bytes() from the sizes alone (they may be symbolic while a graph is traced)"""
     panels = (columns + 15) // 16 if dtype == torch.float32 else (columns + 31) // 32
     up = lambda n: (n + 255) // 256 * 256
     return 256 + 16 * up(rows) + 64 * panels * (up(rows) + up(entries))
-
-
-def _ce_args(hidden, weight, bias, target, reduction, saved):
-    """(struct, the tensors in kernel layout that it points to)"""
-    x, ldx = _rows(hidden)
-    w, ldw = _rows(weight)
-    t = target if target.dtype == torch.int64 and target.is_contiguous() else target.to(torch.int64).contiguous()
-    b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
-    v, d = w.shape
-    return VocabCe(_DTYPES[w.dtype], reduction, t.numel(), v, d, x.data_ptr(), ldx, w.data_ptr(), ldw, None if b is None else b.data_ptr(),
-                   t.data_ptr(), None if saved is None else saved.data_ptr()), (x, w, t, b)
-
-
-def _ce_forward(hidden, weight, bias, target, reduction, train):
-    """(loss, what the backward pass reads or None); at least one row"""
-    dev = weight.device
-    L = _lib.lib()
-    with _On(dev):
-        a, held = _ce_args(hidden, weight, bias, target, reduction, None)
-        ref = ctypes.byref(a)
-        saved = None
-        if train:
-            saved = torch.empty(L.tnp_vocab_ce_saved_bytes(ref), dtype=torch.uint8, device=dev)
-            a.saved = saved.data_ptr()
-        need = L.tnp_vocab_ce_workspace_bytes(ref, 0)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        loss = torch.empty(target.shape if reduction == 0 else (), dtype=torch.float32, device=dev)
-        _lib.check(L.tnp_vocab_ce_forward(ref, loss.data_ptr(), ws.data_ptr(), need, _lib.raw_stream()), 'tnp_vocab_ce_forward')
-    return loss, saved
-
-
-def _ce_backward(grad, hidden, weight, bias, target, saved, reduction, needs):
-    dev = weight.device
-    L = _lib.lib()
-    with _On(dev):
-        a, held = _ce_args(hidden, weight, bias, target, reduction, saved)
-        ref = ctypes.byref(a)
-        g = grad if grad.dtype == torch.float32 and grad.is_contiguous() else grad.float().contiguous()
-        dx = torch.empty(hidden.shape, dtype=hidden.dtype, device=dev) if needs[0] else None
-        dw = torch.empty(weight.shape, dtype=weight.dtype, device=dev) if needs[1] else None
-        db = torch.empty(bias.shape, dtype=bias.dtype, device=dev) if needs[2] else None
-        need = L.tnp_vocab_ce_workspace_bytes(ref, 1)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        _lib.check(L.tnp_vocab_ce_backward(ref, g.data_ptr(), _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db), ws.data_ptr(), need,
-                                           _lib.raw_stream()), 'tnp_vocab_ce_backward')
-    return dx, dw, db
-
-
-class _VocabCeFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, hidden, weight, bias, target, reduction):
-        loss, saved = _ce_forward(hidden, weight, bias, target, reduction, True)
-        ctx.save_for_backward(hidden, weight, bias, target, saved)
-        ctx.reduction = reduction
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        hidden, weight, bias, target, saved = ctx.saved_tensors
-        return _ce_backward(grad, hidden, weight, bias, target, saved, ctx.reduction, ctx.needs_input_grad) + (None, None)
 
 
 def check_cross_entropy(hidden, weight, target, bias, reduction):
@@ -263,6 +142,4 @@ def vocab_cross_entropy(hidden, weight, target, bias=None, reduction='mean'):
     if target.numel() == 0:                                              # no rows: an empty / zero loss with zero gradients
         zero = hidden.float().sum() + weight[:0].float().sum() + (bias[:0].float().sum() if bias is not None else 0.0)
         return zero.expand(target.shape) if red == 0 else zero
-    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
-        return _VocabCeFn.apply(hidden, weight, bias, target, red)
-    return _ce_forward(hidden, weight, bias, target, red, False)[0]
+    return native().vocab_cross_entropy(hidden, weight, target, bias, red)
