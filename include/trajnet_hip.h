@@ -403,7 +403,8 @@ typedef struct tnp_bwd_sweep {
     float *at_posrec_all;            /* TNP_POOL_ATTNMLP, optional out: [S,M,n_max,4] per-pair position-gradient records, or NULL */
 } tnp_bwd_sweep;
 /* sizeof() of the structs of this header as the library was compiled (which: 0 tnp_lstm_model, 1 tnp_lstm_extras,
- * 2 tnp_step_saves, 3 tnp_train_saves, 4 tnp_bwd_sweep; 0 for any other value) -- lets a binding check its mirrors */
+ * 2 tnp_step_saves, 3 tnp_train_saves, 4 tnp_bwd_sweep, 5 tnp_wgrad_problem, 6 tnp_adam_tensor, 7 tnp_transpose_problem,
+ * 8 tnp_vocab_ce; 0 for any other value) -- lets a binding check its mirrors */
 TNP_API size_t tnp_abi_sizeof(int which);
 TNP_API size_t tnp_lstm_backward_scratch_bytes(const tnp_bwd_sweep *sweep);
 TNP_API int tnp_lstm_backward_sweep(const tnp_bwd_sweep *sweep, int s_hi, int s_lo, void *scratch, size_t scratch_bytes,
@@ -691,7 +692,7 @@ typedef struct tnp_vocab_ce {
     int64_t ld_weight;
     const void *bias;           /* [V] or NULL */
     const int64_t *target;      /* [M] */
-    void *saved;                /* tnp_vocab_ce_saved_bytes() bytes that the forward pass fills for the backward pass (which
+    void *saved;                /* 256-byte aligned, like the workspaces: tnp_vocab_ce_saved_bytes() bytes that the forward pass fills for the backward pass (which
                                    reads them, weight, bias and target); NULL: no backward pass will follow */
 } tnp_vocab_ce;
 TNP_API size_t tnp_vocab_ce_saved_bytes(const tnp_vocab_ce *args);

@@ -30,7 +30,8 @@ static constexpr int64_t EMB_MAX_TOKENS = 1 << 28;
 
 // ---- forward ----------------------------------------------------------------------------------------------------------------
 // 2^lsh lanes per row; U rows per lane whose loads are in flight together (a token without a row loads row 0 and drops it: loads
-// under a condition would wait for each other).
+// under a condition would wait for each other).  43008 x 512 bf16 13.5 us, 4.5 TB/s of tokens, table rows and output (a copy of a GB:
+// 5.1); 262144 x 256 bf16 41 us.
 template <typename T, int VE, typename I, int U>
 __global__ void __launch_bounds__(256) embed_forward_kernel(const I *tokens, int64_t N, const T *weight, int64_t ldw, int64_t V,
                                                             int D, int lsh, float scale, T *out, int64_t ldo) {
@@ -55,7 +56,8 @@ __global__ void __launch_bounds__(256) embed_forward_kernel(const I *tokens, int
 }
 
 // ---- stable radix sort of (token, i) ----------------------------------------------------------------------------------------
-// Keys: the token, or V for a token outside the table (sorted behind everything, skipped by the sums).
+// Keys: the token, or V for a token outside the table (sorted behind everything, skipped by the sums).  Bound by latency, not bytes: a
+// pass over 43008 tokens takes 5.3 us of counting and 9.6 of scattering, over 262144 (17-bit keys, two passes) 4.8 and 16.
 template <typename I>
 __device__ __forceinline__ uint32_t embed_key(const I *tokens, const uint32_t *keys, int64_t i, uint32_t V) {
     if (keys) return keys[i];
@@ -252,7 +254,8 @@ __device__ __forceinline__ uint32_t embed_upper(const uint32_t *keys, uint32_t l
 
 // Chunk c = sorted positions [c << csh, (c + 1) << csh), 2^lsh lanes, fp32 sums.  A run (one token) inside the chunk is finished here; the
 // part of a run that came in from the chunk before goes to head[c], the first part of a run that goes on into the next to tail[c]
-// (embed_join_kernel adds those).  Workgroups from `sum_blocks` on zero the table rows that no token names.
+// (embed_join_kernel adds those).  Workgroups from `sum_blocks` on zero the table rows that no token names.  262144 x 256 bf16 into 65536
+// rows 46 us, 3.6 TB/s: the gradient's rows are read in the tokens' order, 512 bytes at a time.
 template <typename T, int VE>
 __global__ void __launch_bounds__(256) embed_reduce_kernel(const uint32_t *keys, const uint32_t *idx, uint32_t N, uint32_t V,
                                                            const T *grad, int64_t ldg, int D, int lsh, int csh, float scale, T *dw,
@@ -350,7 +353,8 @@ template <int VE> __device__ __forceinline__ Parts<VE> load_parts(const float *a
 
 // Runs that go on past their chunk: tail[c] + head[c + 1] + ... of the run that starts in chunk c.  A workgroup looks after 32 chunks:
 // first every group of lanes adds up runs of up to 32 parts by itself, then all of them together stride over each longer one and
-// meet in LDS.  Every order of addition is fixed by the sizes.
+// meet in LDS.  Every order of addition is fixed by the sizes.  262144 x 256 bf16, tokens ~ u^6: 23 us (the longest run has 41000 rows);
+// 43008 x 64 into 257 rows 9.6 us.
 template <typename T, int VE>
 __global__ void __launch_bounds__(512) embed_join_kernel(const uint32_t *keys, uint32_t N, uint32_t V, int D, int lsh, int csh, float scale,
                                                          T *dw, int64_t ldd, const float *head, const float *tail) {
@@ -455,7 +459,8 @@ __global__ void __launch_bounds__(512) embed_join_kernel(const uint32_t *keys, u
 // ---- few tokens: no sort ----------------------------------------------------------------------------------------------------
 // One launch: workgroup (i < N, 64 columns) owns token i's row if no earlier position names it, lists the positions that do (every wave
 // compacts its quarter of them in order) and adds their gradient rows, groups of lanes striding over the list; the workgroups behind
-// zero 256 table rows each, less those named.  N^2 comparisons from the L2 instead of four to six dependent launches.
+// zero 256 table rows each, less those named.  N^2 comparisons from the L2 instead of four to six dependent launches.  Bound by the
+// token whose list is longest, which is why a workgroup takes 64 columns only.
 template <typename T, int VE, typename I>
 __global__ void __launch_bounds__(256) embed_small_kernel(const I *tokens, int N, int64_t V, const T *grad, int64_t ldg, int D, float scale,
                                                           T *dw, int64_t ldd) {
@@ -597,7 +602,8 @@ static int embed_forward_run(const I *tokens, int64_t N, const T *w, int64_t ldw
                              hipStream_t s) {
     const int lsh = lane_shift(D, VE, 8);
     const int64_t rows = 256 >> lsh;
-    // four rows per lane once one row per lane would be several rounds of workgroups
+    // four rows per lane once one row per lane would be several rounds of workgroups: 1048576 x 64 fp32 75 us against 86, 16384 x 64 9.8
+    // against 8.9
     const bool four = N / rows >= 4096;
     const int64_t most = rows << 22;                   // rows per launch: a grid holds fewer than 2^32 threads
     for (int64_t i = 0; i < N; i += most) {
