@@ -693,7 +693,7 @@ typedef struct tnp_vocab_ce {
     const void *bias;           /* [V] or NULL */
     const int64_t *target;      /* [M] */
     void *saved;                /* 256-byte aligned, like the workspaces: tnp_vocab_ce_saved_bytes() bytes that the forward pass fills for the backward pass (which
-                                   reads them, weight, bias and target); NULL: no backward pass will follow */
+                                   reads them, bias and target; not hidden, not weight); NULL: no backward pass will follow */
 } tnp_vocab_ce;
 TNP_API size_t tnp_vocab_ce_saved_bytes(const tnp_vocab_ce *args);
 TNP_API size_t tnp_vocab_ce_workspace_bytes(const tnp_vocab_ce *args, int backward);

@@ -138,6 +138,20 @@ def test_embedding_rows_behind_four_gigabytes():
     assert dw[at, 0].tolist() == [1.0, 1.0, 1.0, 1.0, 2.0] and int((dw != 0).any(1).sum()) == 5
 
 
+@pytest.mark.parametrize('n', [500, 5000])
+def test_embedding_largest_vocabulary(n):
+    """2^30 entries: keys of 31 bits"""
+    v = 1 << 30
+    tok = torch.randint(v, (n,), device='cuda', generator=_gen(7))
+    tok[:4] = torch.tensor([0, v - 1, v - 1, v], device='cuda')
+    w = torch.zeros(v, 1, dtype=torch.bfloat16, device='cuda').requires_grad_()
+    out = vocab.token_embedding(tok, w)
+    assert torch.isnan(out[3]).all() and int((out != 0).sum()) == 1
+    dw, = torch.autograd.grad(out, w, torch.ones_like(out))
+    at, count = tok[tok < v].unique(return_counts=True)
+    assert torch.equal(dw[at, 0].double(), count.double()) and int(torch.count_nonzero(dw)) == at.numel()
+
+
 def test_embedding_half_rows_that_are_not_sixteen_bytes():
     """every width of access: row lengths and base addresses of 2, 4 and 16 bytes"""
     g = _gen(3)
@@ -583,6 +597,36 @@ def test_a_weight_that_changes_before_the_backward_pass_is_noticed():
         w.mul_(2.0)
     with pytest.raises(RuntimeError, match='modified by an inplace operation'):
         torch.autograd.grad(loss, w)
+
+
+def test_derivatives_that_are_not_offered_raise():
+    from torch.autograd import forward_ad
+    x, w, b, t = (z.detach() for z in _case(70, 50, 16, torch.float32, 124))
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(w, w)
+        with pytest.raises(RuntimeError, match='forward-mode'):
+            vocab.token_embedding(t, dual)
+        with pytest.raises(RuntimeError, match='forward-mode'):
+            vocab.vocab_cross_entropy(x, dual, t, bias=b)
+    for f in (lambda z: vocab.token_embedding(t, z).sum(), lambda z: vocab.vocab_cross_entropy(x, z, t, bias=b)):
+        with pytest.raises(RuntimeError):
+            torch.func.grad(f)(w)
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(f)(torch.stack([w, w]))
+
+
+@pytest.mark.parametrize('m,v,d', [(1 << 23, 5, 8), (3, 1 << 23, 8), (300, 500, 16384), (40, 70, 16384)])
+def test_largest_sizes(m, v, d):
+    dtype = torch.bfloat16
+    x, w, b, t = _case(m, v, d, dtype, 125, absent=0.1)
+    out = vocab.vocab_cross_entropy(x, w, t, bias=b, reduction='sum')
+    grads = torch.autograd.grad(out, (x, w, b))
+    want, bound, dwant, dbound = _formula(x, w, b, t, torch.ones(m, device='cuda'))
+    _within(out, want.sum(), bound.sum() + want.sum().abs() * 2.0 ** -23)
+    for got, val, lim in zip(grads, dwant, dbound):
+        _within(got, val, lim)
+    with torch.no_grad():
+        _within(vocab.vocab_cross_entropy(x, w, t, bias=b, reduction='none'), want, bound)
 
 
 def test_no_gradient_of_a_gradient():

@@ -808,27 +808,26 @@ static int ce_rows_shift(int64_t M, int parts) { return M <= CE_SCORE_ROWS ? 2 :
 // shares of the hidden states' rows: at least eight rows each
 static int ce_x_blocks(int64_t M) { return (int)((M + 7) / 8 < CE_AMAX_BLOCKS ? (M + 7) / 8 : CE_AMAX_BLOCKS); }
 
-// 256 x 256 tiles of logits (eight waves) from two rounds of workgroups and eight steps on: 4096 x 16384 x 1024 fp32 forward 381 us
-// against 437, 8192 x 16384 x 128 bf16 (four steps) 95 against 86
 // Shares that the `tiles_v` vocabulary tiles are split into for each of `tiles_i` row tiles, `slots` workgroups running at a time: the
-// fewest rounds of workgroups times tiles per workgroup, and of those the fewest shares.
+// fewest rounds of workgroups times tiles per workgroup, and of those the fewest shares.  No bound on the shares: 200 x 65536 x 512 bf16 forward
+// 72 us, 97 with at most 64 of them.
 static int ce_shares(int64_t tiles_i, int tiles_v, int slots) {
     int best = 1;
     int64_t cost = INT64_MAX;
-    for (int n = 1; n <= tiles_v && n <= 64; ++n) {
+    for (int n = 1; n <= tiles_v; ++n) {
         const int64_t rounds = (tiles_i * n + slots - 1) / slots, c = rounds * ((tiles_v + n - 1) / n);
         if (c < cost) { cost = c; best = n; }
         if (tiles_i * n >= 2 * slots) break;
     }
     return best;
 }
-static bool ce_big(const CeShape &s);
+// 256 x 256 tiles of logits (eight waves) from two rounds of workgroups and eight steps on: 4096 x 16384 x 1024 fp32 forward 381 us
+// against 437, 8192 x 16384 x 128 bf16 (four steps) 95 against 86
+static bool ce_big(const CeShape &s) { return (s.Mp / 256) * (int64_t)(s.Vp / 256) >= 512 && s.panels >= 8; }
 // slots: one workgroup of the 256 tiles per CU, three of the 128 ones
 static int ce_logit_shares(const CeShape &s, int64_t cols) {
     return ce_big(s) ? ce_shares(s.Mp / 256, (int)(cols / 256), 256) : ce_shares(s.Mp / 128, (int)(cols / 128), 768);
 }
-
-static bool ce_big(const CeShape &s) { return (s.Mp / 256) * (int64_t)(s.Vp / 256) >= 512 && s.panels >= 8; }
 
 struct CeForward { CeSaved saved; float *amax; int *count; float2 *part; float *tlogit; double2 *sums; int parts; size_t bytes; };
 static CeForward ce_forward_layout(const tnp_vocab_ce *p, void *ws) {
@@ -1091,7 +1090,7 @@ extern "C" TNP_API int tnp_vocab_ce_backward(const tnp_vocab_ce *args, const flo
                                              void *workspace, size_t workspace_bytes, void *stream) {
     if (int rc = ce_check(args, "tnp_vocab_ce_backward")) return rc;
     if (args->M == 0) TNP_FAIL(-1, "tnp_vocab_ce_backward: no rows");
-    if (!args->weight || !args->target || !args->saved || !grad || !workspace) TNP_FAIL(-1, "tnp_vocab_ce_backward: NULL pointer");
+    if (!args->target || !args->saved || !grad || !workspace) TNP_FAIL(-1, "tnp_vocab_ce_backward: NULL pointer");
     if (dbias && !args->bias) TNP_FAIL(-1, "tnp_vocab_ce_backward: dbias without a bias");
     const CeBackward b = ce_backward_layout(args, workspace);
     if (workspace_bytes < b.bytes) TNP_FAIL(-1, "tnp_vocab_ce_backward: workspace of %zu bytes, %zu needed", workspace_bytes, b.bytes);

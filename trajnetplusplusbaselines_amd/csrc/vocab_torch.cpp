@@ -48,6 +48,9 @@ int dtype_of(const Tensor &t) {
 Tensor workspace(size_t bytes, const Tensor &like) { return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)); }
 void *data(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 
+// a tangent would be dropped in silence
+void no_tangent(const Tensor &t) { TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "the vocabulary operators have no forward-mode derivative"); }
+
 // rows with unit column stride that do not overlap; a copy only where the layout asks for one
 struct Rows {
     Tensor t;
@@ -118,27 +121,24 @@ struct EmbeddingNode : torch::autograd::Function<EmbeddingNode> {
 };
 
 Tensor token_embedding(const Tensor &tokens, const Tensor &weight, double scale) {
+    no_tangent(weight);
     if (weight.requires_grad() && at::GradMode::is_enabled()) return EmbeddingNode::apply(tokens, weight, scale);
     return embedding_forward(tokens, weight, scale);
 }
 
 // ---- cross entropy over a vocabulary ------------------------------------------------------------------------------------------
 struct CeArgs {
-    Rows x, w;
     Tensor t, b;
     tnp_vocab_ce c = {};
-    CeArgs(const Tensor &hidden, const Tensor &weight, const Tensor &target, const Tensor &bias, int64_t reduction)
-        : x(hidden), w(weight), t(target.to(at::kLong).contiguous()), b(bias.defined() ? bias.contiguous() : bias) {
+    CeArgs(const Tensor &weight, const Tensor &target, const Tensor &bias, int64_t reduction)
+        : t(target.to(at::kLong).contiguous()), b(bias.defined() ? bias.contiguous() : bias) {
         c.dtype = dtype_of(weight);
         c.reduction = (int32_t)reduction;
         c.M = t.numel();
         // too many for the entries' 32 bits: refused there
         c.V = (int32_t)std::min<int64_t>(weight.size(0), INT32_MAX);
         c.D = (int32_t)std::min<int64_t>(weight.size(1), INT32_MAX);
-        c.hidden = x.t.data_ptr();
-        c.ld_hidden = x.ld;
-        c.weight = w.t.data_ptr();
-        c.ld_weight = w.ld;
+        c.ld_hidden = c.ld_weight = weight.size(1);
         c.bias = data(b);
         c.target = t.data_ptr<int64_t>();
     }
@@ -148,7 +148,12 @@ struct CeArgs {
 std::pair<Tensor, Tensor> ce_forward(const Tensor &hidden, const Tensor &weight, const Tensor &target, const Tensor &bias, int64_t reduction,
                                      bool train) {
     const c10::DeviceGuard guard(weight.device());
-    CeArgs a(hidden, weight, target, bias, reduction);
+    CeArgs a(weight, target, bias, reduction);
+    const Rows x(hidden), w(weight);
+    a.c.hidden = x.t.data_ptr();
+    a.c.ld_hidden = x.ld;
+    a.c.weight = w.t.data_ptr();
+    a.c.ld_weight = w.ld;
     Tensor saved;
     if (train) {
         saved = workspace(entry.ce_saved(&a.c), weight);
@@ -164,7 +169,7 @@ std::pair<Tensor, Tensor> ce_forward(const Tensor &hidden, const Tensor &weight,
 variable_list ce_backward(const Tensor &grad, const Tensor &hidden, const Tensor &weight, const Tensor &target, const Tensor &bias,
                           const Tensor &saved, int64_t reduction, bool need_x, bool need_w, bool need_b) {
     const c10::DeviceGuard guard(weight.device());
-    CeArgs a(hidden, weight, target, bias, reduction);
+    CeArgs a(weight, target, bias, reduction);                  // hidden states and weight are read from what was saved
     a.c.saved = saved.data_ptr();
     const Tensor g = grad.to(at::kFloat).contiguous();
     Tensor dx, dw, db;
@@ -201,6 +206,7 @@ struct CeNode : torch::autograd::Function<CeNode> {
 Tensor vocab_cross_entropy(const Tensor &hidden, const Tensor &weight, const Tensor &target, const std::optional<Tensor> &bias,
                            int64_t reduction) {
     const Tensor b = or_undefined(bias);
+    for (const Tensor &t : {hidden, weight, b}) no_tangent(t);
     if (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad() || (b.defined() && b.requires_grad())))
         return CeNode::apply(hidden, weight, bias, target, reduction);
     return ce_forward(hidden, weight, target, b, reduction, false).first;
