@@ -225,7 +225,7 @@ SHAPES = [(1, 1, 1), (1, 300, 64), (2, 17, 3), (16, 255, 8), (17, 257, 33), (64,
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
-@pytest.mark.parametrize('m,v,d', SHAPES)
+@pytest.mark.parametrize('m,v,d', SHAPES + [(20, 20479, 40), (20, 20480, 40), (33, 30001, 24), (64, 70003, 33)])
 def test_scoring_without_gradient(dtype, m, v, d):
     x, w, b, t = _case(m, v, d, dtype, 1000 * m + v, absent=0.3 if m > 4 else 0.0)
     loss, bound, _, _ = _formula(x, w, b, t, torch.ones(m, device='cuda'))

@@ -28,8 +28,11 @@ static constexpr double CE_LN2 = 0.6931471805599453;
 static constexpr float CE_NEG_INF = -__builtin_inff();
 static constexpr int CE_AMAX_BLOCKS = 512;            // per tensor, the hidden states in as many shares of rows as they are packed in
 static constexpr int CE_ROW_PAD = 256, CE_COL_PAD = 256;
+// Groups of 16 entries that a wave scores at a time for more than 16 rows, from this vocabulary on (more than one wave per SIMD with one):
+// 64 x 65536 x 512 bf16 37 us against 48, 64 x 20480 x 512 bf16 25 against 29; 64 x 16384 x 128 fp32 21 against 16
+static constexpr int CE_SCORE_GROUPS = 2, CE_SCORE_GROUPS_FROM = 20480;
 static constexpr int CE_JOIN_BLOCKS = 1 << 20;         // a grid holds fewer than 2^32 threads
-// rows up to which scoring reads the inputs in place: 64 x 65536 x 512 bf16 48 us against 62 packed, fp32 89 against 127
+// rows up to which scoring reads the inputs in place: 64 x 65536 x 512 bf16 37 us against 62 packed, fp32 74 against 127
 static constexpr int CE_SCORE_ROWS = 64;
 
 struct CeScalars {            // head of the saved area
@@ -424,11 +427,12 @@ __device__ __forceinline__ typename ScoreLoad<T, VEC>::frag score_load(const T *
     return __builtin_bit_cast(typename L::frag, p);
 }
 
-template <typename T, bool VEC, int NT>
+// G groups of 16 entries at a time: the hidden states' operands, read from the caches, serve all of them.
+template <typename T, bool VEC, int NT, int G>
 __global__ void __launch_bounds__(256) ce_score_kernel(const T *x, int64_t ldx, int M, const T *w, int64_t ldw, int V, int D, const T *bias,
                                                        const int64_t *target, float2 *part, float *tlogit, CeScalars *sc) {
     typedef ScoreLoad<T, VEC> L;
-    constexpr int KS = 4 * L::KW, U = NT == 1 ? 4 : 2;
+    constexpr int KS = 4 * L::KW, U = NT == 1 && G == 1 ? 4 : 2;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
     if (blockIdx.x == 0 && threadIdx.x == 0) sc->ticket = 0;
     const T *xr[NT];
@@ -443,39 +447,50 @@ __global__ void __launch_bounds__(256) ce_score_kernel(const T *x, int64_t ldx, 
         s[n] = 0.0f;
     }
     const int groups = (V + 15) / 16;
-    for (int g = blockIdx.x * 4 + wave; g < groups; g += gridDim.x * 4) {
-        const int vr = g * 16 + r < V ? g * 16 + r : V - 1;
-        const T *wr = w + (int64_t)vr * ldw;
-        f32x4 acc[NT];
+    for (int g0 = (blockIdx.x * 4 + wave) * G; g0 < groups; g0 += gridDim.x * 4 * G) {
+        const T *wr[G];
+        f32x4 acc[G][NT];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) acc[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int g = 0; g < G; ++g) {
+            const int v = (g0 + g) * 16 + r;
+            wr[g] = w + (int64_t)(v < V ? v : V - 1) * ldw;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[g][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
         for (int k = q * L::KW; k < D + q * L::KW; k += U * KS) {
-            typename L::frag fw[U], fx[NT][U];
+            typename L::frag fw[G][U], fx[NT][U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                fw[u] = score_load<T, VEC>(wr, k + u * KS, D);
+#pragma unroll
+                for (int g = 0; g < G; ++g) fw[g][u] = score_load<T, VEC>(wr[g], k + u * KS, D);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) fx[n][u] = score_load<T, VEC>(xr[n], k + u * KS, D);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) L::mma(fw[u], fx[n][u], acc[n]);
+                for (int g = 0; g < G; ++g)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) L::mma(fw[g][u], fx[n][u], acc[g][n]);
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            float l[4], top = m[n];
+            float l[G][4], top = m[n];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int v = g * 16 + 4 * q + e;
-                l[e] = v < V ? fmaf(acc[n][e], CE_LOG2E, ce_bias(bias, v)) : CE_NEG_INF;
-                top = fmaxf(top, l[e]);
-                if (t[n] == v) tlogit[n * 16 + r] = l[e];
-            }
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int v = (g0 + g) * 16 + 4 * q + e;
+                    l[g][e] = v < V ? fmaf(acc[g][n][e], CE_LOG2E, ce_bias(bias, v)) : CE_NEG_INF;
+                    top = fmaxf(top, l[g][e]);
+                    if (t[n] == v) tlogit[n * 16 + r] = l[g][e];
+                }
             const float mm = top == CE_NEG_INF ? 0.0f : top;
             s[n] *= __builtin_amdgcn_exp2f(m[n] - mm);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[n] += __builtin_amdgcn_exp2f(l[e] - mm);
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n] += __builtin_amdgcn_exp2f(l[g][e] - mm);
             m[n] = top;
         }
     }
@@ -797,8 +812,9 @@ static CeSaved ce_saved(const CeShape &s, void *base) {
 }
 
 static bool ce_scores(const tnp_vocab_ce *p) { return !p->saved && p->M <= CE_SCORE_ROWS; }
-static int ce_score_blocks(int V) {
-    const int g = (V + 63) / 64;
+static int ce_score_groups(const tnp_vocab_ce *p) { return p->M > 16 && p->V >= CE_SCORE_GROUPS_FROM ? CE_SCORE_GROUPS : 1; }
+static int ce_score_blocks(const tnp_vocab_ce *p) {
+    const int each = 64 * ce_score_groups(p), g = (p->V + each - 1) / each;
     return g < 1024 ? g : 1024;
 }
 // rows per workgroup of the join: few rows share the threads, many rows with few parts keep the workgroups few (each draws a ticket:
@@ -834,7 +850,7 @@ static CeForward ce_forward_layout(const tnp_vocab_ce *p, void *ws) {
     CeForward f;
     const CeShape s = ce_shape(p);
     char *w = (char *)ws;
-    f.parts = ce_scores(p) ? ce_score_blocks(p->V) : 2 * ce_logit_shares(s, s.Vp);
+    f.parts = ce_scores(p) ? ce_score_blocks(p) : 2 * ce_logit_shares(s, s.Vp);
     const int64_t rows = ce_scores(p) ? CE_SCORE_ROWS : s.Mp;
     f.amax = (float *)w; w += ce_up(2 * CE_AMAX_BLOCKS * 4);
     f.count = (int *)w; w += ce_up(CE_AMAX_BLOCKS * 4);
@@ -954,21 +970,22 @@ static int ce_launch_grads(CeGrads &a, hipStream_t s) {
     return 0;
 }
 
-template <typename T, bool VEC>
-static int ce_score(const tnp_vocab_ce *p, const CeForward &f, hipStream_t s) {
-    const dim3 grid(ce_score_blocks(p->V));
-#define TNP_SCORE(NT)                                                                                                            \
-    hipLaunchKernelGGL((ce_score_kernel<T, VEC, NT>), grid, dim3(256), 0, s, (const T *)p->hidden, p->ld_hidden, (int)p->M,       \
-                       (const T *)p->weight, p->ld_weight, p->V, p->D, (const T *)p->bias, p->target, f.part, f.tlogit, f.saved.sc)
-    switch ((p->M + 15) / 16) {
-        case 1: TNP_SCORE(1); break;
-        case 2: TNP_SCORE(2); break;
-        case 3: TNP_SCORE(3); break;
-        default: TNP_SCORE(4);
-    }
-#undef TNP_SCORE
+template <typename T, bool VEC, int NT, int G>
+static int ce_score_run(const tnp_vocab_ce *p, const CeForward &f, hipStream_t s) {
+    hipLaunchKernelGGL((ce_score_kernel<T, VEC, NT, G>), dim3(ce_score_blocks(p)), dim3(256), 0, s, (const T *)p->hidden, p->ld_hidden, (int)p->M,
+                       (const T *)p->weight, p->ld_weight, p->V, p->D, (const T *)p->bias, p->target, f.part, f.tlogit, f.saved.sc);
     TNP_HIP(hipGetLastError());
     return 0;
+}
+template <typename T, bool VEC>
+static int ce_score(const tnp_vocab_ce *p, const CeForward &f, hipStream_t s) {
+    const bool one = ce_score_groups(p) == 1;
+    switch ((p->M + 15) / 16) {
+        case 1: return ce_score_run<T, VEC, 1, 1>(p, f, s);
+        case 2: return one ? ce_score_run<T, VEC, 2, 1>(p, f, s) : ce_score_run<T, VEC, 2, CE_SCORE_GROUPS>(p, f, s);
+        case 3: return one ? ce_score_run<T, VEC, 3, 1>(p, f, s) : ce_score_run<T, VEC, 3, CE_SCORE_GROUPS>(p, f, s);
+        default: return one ? ce_score_run<T, VEC, 4, 1>(p, f, s) : ce_score_run<T, VEC, 4, CE_SCORE_GROUPS>(p, f, s);
+    }
 }
 
 template <typename T, int VX, int VW, bool SPLIT>
