@@ -629,6 +629,24 @@ def test_largest_sizes(m, v, d):
         _within(vocab.vocab_cross_entropy(x, w, t, bias=b, reduction='none'), want, bound)
 
 
+@pytest.mark.parametrize('v,d', [(2, (1 << 20) + 1), (1, (1 << 32) + 8), ((1 << 30) + 1, 1)])
+def test_embedding_sizes_past_the_limits_are_refused(v, d):
+    w = torch.empty(v, d, dtype=torch.bfloat16, device='cuda', requires_grad=True)
+    tok = torch.zeros(1, dtype=torch.int64, device='cuda')
+    with pytest.raises(RuntimeError, match='table of'):
+        vocab.token_embedding(tok, w)
+
+
+@pytest.mark.parametrize('m,v,d', [((1 << 23) + 1, 2, 1), (2, (1 << 23) + 1, 1), (2, 2, 16385), (1, 1, (1 << 32) + 8)])
+def test_cross_entropy_sizes_past_the_limits_are_refused(m, v, d):
+    x, w = (torch.empty(k, d, dtype=torch.bfloat16, device='cuda', requires_grad=True) for k in (m, v))
+    t = torch.zeros(m, dtype=torch.int64, device='cuda')
+    with pytest.raises(RuntimeError, match='tnp_vocab_ce_forward failed'):
+        vocab.vocab_cross_entropy(x, w, t)
+    with torch.no_grad(), pytest.raises(RuntimeError, match='tnp_vocab_ce_forward failed'):
+        vocab.vocab_cross_entropy(x, w, t)
+
+
 def test_no_gradient_of_a_gradient():
     """raises, also where the rest of what is differentiated has a gradient"""
     x, w, b, t = _case(70, 50, 16, torch.float32, 121)

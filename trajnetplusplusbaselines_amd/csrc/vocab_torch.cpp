@@ -48,6 +48,9 @@ int dtype_of(const Tensor &t) {
 Tensor workspace(size_t bytes, const Tensor &like) { return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)); }
 void *data(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 
+// sizes that the entries take as 32 bits: one that does not fit is refused there
+int32_t narrow(int64_t n) { return (int32_t)std::min<int64_t>(n, INT32_MAX); }
+
 // a tangent would be dropped in silence
 void no_tangent(const Tensor &t) { TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "the vocabulary operators have no forward-mode derivative"); }
 
@@ -71,7 +74,7 @@ Tensor embedding_forward(const Tensor &tokens, const Tensor &weight, double scal
     std::vector<int64_t> shape = tokens.sizes().vec();
     shape.push_back(d);
     Tensor out = at::empty(shape, weight.options());
-    check(entry.embed_forward(tok.data_ptr(), (int)tok.element_size(), tok.numel(), w.t.data_ptr(), w.ld, v, (int)d, dtype_of(weight),
+    check(entry.embed_forward(tok.data_ptr(), (int)tok.element_size(), tok.numel(), w.t.data_ptr(), w.ld, v, narrow(d), dtype_of(weight),
                               (float)scale, out.data_ptr(), d, stream_of(weight)), "tnp_token_embedding_forward");
     return out;
 }
@@ -82,9 +85,9 @@ Tensor embedding_backward(const Tensor &grad, const Tensor &tokens, int64_t entr
     const Tensor tok = tokens.contiguous();
     const int64_t n = tok.numel(), d = grad.size(-1);
     Tensor dw = at::empty({entries, d}, grad.options()), ws;
-    const size_t need = entry.embed_workspace(n, entries, (int)d);
+    const size_t need = entry.embed_workspace(n, entries, narrow(d));
     if (need) ws = workspace(need, grad);
-    check(entry.embed_backward(tok.data_ptr(), (int)tok.element_size(), n, g.t.data_ptr(), g.ld, entries, (int)d, dtype_of(grad), (float)scale,
+    check(entry.embed_backward(tok.data_ptr(), (int)tok.element_size(), n, g.t.data_ptr(), g.ld, entries, narrow(d), dtype_of(grad), (float)scale,
                                dw.data_ptr(), d, data(ws), need, stream_of(grad)), "tnp_token_embedding_backward");
     return dw;
 }
@@ -135,9 +138,8 @@ struct CeArgs {
         c.dtype = dtype_of(weight);
         c.reduction = (int32_t)reduction;
         c.M = t.numel();
-        // too many for the entries' 32 bits: refused there
-        c.V = (int32_t)std::min<int64_t>(weight.size(0), INT32_MAX);
-        c.D = (int32_t)std::min<int64_t>(weight.size(1), INT32_MAX);
+        c.V = narrow(weight.size(0));
+        c.D = narrow(weight.size(1));
         c.ld_hidden = c.ld_weight = weight.size(1);
         c.bias = data(b);
         c.target = t.data_ptr<int64_t>();
