@@ -60,7 +60,7 @@ def _tokens(n, vocab_size, kind, g):
 @pytest.mark.parametrize('n,v,d,kind', [
     (1, 1, 1, 'one'), (1, 7, 64, 'even'), (36, 256, 64, 'skew'), (31, 5, 3, 'one'), (33, 5, 8, 'one'), (65, 3, 17, 'absent'),
     (1000, 1023, 33, 'even'), (1000, 1024, 128, 'skew'), (5000, 2, 100, 'skew'), (4096, 300, 16, 'one'), (4097, 300, 16, 'one'), (4096, 70000, 8, 'absent'), (3000, 40, 1030, 'skew'), (4200, 5, 3, 'absent'), (6000, 9, 24, 'none'),
-    (8192, 300, 16, 'one'), (8193, 300, 16, 'one'), (9000, 1300000, 4, 'even'), (6000, 50, 1030, 'skew'), (5000, 1025, 17, 'skew'),
+    (8192, 300, 16, 'one'), (8193, 300, 16, 'one'), (12288, 4099, 7, 'skew'), (12289, 4099, 7, 'skew'), (9000, 1300000, 4, 'even'), (6000, 50, 1030, 'skew'), (5000, 1025, 17, 'skew'),
     (20011, 70001, 12, 'even'), (2200003, 70001, 3, 'even'), (500, 50, 1030, 'skew'), (4096, 300, 128, 'skew'), (4096, 300, 129, 'skew'),
     (2048, 7, 256, 'one'), (40000, 257, 64, 'absent'), (100, 1300000, 4, 'even'), (777, 50, 1030, 'skew'), (50, 9, 24, 'none')])
 def test_embedding_lookup_and_gradient(dtype, n, v, d, kind):

@@ -15,7 +15,8 @@
 namespace tnp {
 
 static constexpr int EMB_SORT_THREADS = 512, EMB_SORT_ROWS = 4;      // eight waves per workgroup of the sort, each with four rows of 64 pairs
-static constexpr int EMB_COUNT_ALL = 4;       // workgroups of the sort up to which each counts all keys: 6000 x 64 19 us against 21, 16000 x 64 28 against 26
+static constexpr int EMB_COUNT_ALL = 6;       // workgroups of the sort up to which each counts all keys: 5000 x 64 18.5 us against 20.5, 12000 x 64 22 against 22
+                                              // (and a launch less), 16000 x 64 24 against 22
 // workgroups of the sort from which on their histograms are summed by segments: 524288 x 64 56 us against 64, 1310720 x 64 163 against 226,
 // 16777216 x 16 1.17 ms against 10.7; 128 workgroups (262144 x 64) 48 against 48
 static constexpr int EMB_SEGMENTS_FROM = 256;
@@ -130,7 +131,7 @@ __global__ void __launch_bounds__(256) embed_segments_kernel(const uint32_t *his
 }
 
 // Every workgroup forms its own offsets from the histograms of all of them (nblk * 2^bits counters, L2-resident): one launch less
-// per pass than a scan kernel in between.  Up to eight workgroups (hist == NULL) count all the keys themselves, another launch less.
+// per pass than a scan kernel in between.  Up to six workgroups (hist == NULL) count all the keys themselves, another launch less.
 // From 256 on the histograms are summed by segments first (seg): what all workgroups read together would grow with their square.
 template <typename I>
 __global__ void __launch_bounds__(EMB_SORT_THREADS) embed_scatter_kernel(const I *tokens, const uint32_t *keys, const uint32_t *idx,
