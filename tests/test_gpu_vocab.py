@@ -354,6 +354,18 @@ def test_large_logits_keep_the_gradients_precision(size):
         _within(a, e, lim + extra * 200)
 
 
+@pytest.mark.parametrize('reduction', ['mean', 'sum', 'none'])
+def test_small_upstream_gradients_keep_their_precision(reduction):
+    """a gradient 2^-100 times as large is the same numbers 2^-100 times as large (2^-149: what is left below the normal numbers)"""
+    x, w, b, t = _case(300, 200, 48, torch.float32, 126)
+    out = vocab.vocab_cross_entropy(x, w, t, bias=b, reduction=reduction)
+    up = torch.full(out.shape, 1.1, device='cuda')
+    one = torch.autograd.grad(out, (x, w, b), up, retain_graph=True)
+    small = torch.autograd.grad(out, (x, w, b), up * 2.0 ** -100)
+    for p, q in zip(one, small):
+        _within(q.double() * 2.0 ** 100, p, p.double().abs() * 2.0 ** -23 + 2.0 ** -48)
+
+
 def test_one_row_without_a_leading_dimension():
     x, w, b, t = _case(3, 40, 16, torch.float32, 25)
     whole = torch.autograd.grad(vocab.vocab_cross_entropy(x, w, t, bias=b, reduction='none')[1], x)[0][1]

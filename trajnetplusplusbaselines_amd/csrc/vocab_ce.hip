@@ -635,10 +635,12 @@ __global__ void __launch_bounds__(1024) ce_gmax_kernel(const float *grad, const 
 }
 
 // ---- gradient products ------------------------------------------------------------------------------------------------------
-// what takes a sum over G back to the gradient: 2^-15 max g, times the other operand's scale
-__device__ __forceinline__ float ce_unscale(const CeScalars *sc, const float *grad, const float *gmax, int reduction, int e) {
+// what takes a sum over G back to the gradient: 2^-15 times the other operand's scale, a power of two, and then max g (in one factor a
+// small max g would lose bits below the smallest normal number)
+struct CeFactor { float two, g; };
+__device__ __forceinline__ CeFactor ce_unscale(const CeScalars *sc, const float *grad, const float *gmax, int reduction, int e) {
     const float g = reduction == 0 ? *gmax : reduction == 1 ? grad[0] / (float)(sc->live > 0 ? sc->live : 1) : grad[0];
-    return ldexpf(g, e - 15);
+    return CeFactor{ldexpf(1.0f, e - 15), g};
 }
 
 struct CeGrad {
@@ -699,7 +701,7 @@ __device__ __forceinline__ void ce_grad_tile(const CeGrads &a, const CeGrad &c, 
         }
     }
     if (!c.out) return;                                        // only dbias is asked for
-    const float f = c.part ? 1.0f : ce_unscale(a.sc, a.grad, a.gmax, a.reduction, WEIGHT ? a.sc->ex : a.sc->ew);
+    const CeFactor f = ce_unscale(a.sc, a.grad, a.gmax, a.reduction, WEIGHT ? a.sc->ex : a.sc->ew);
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -718,7 +720,7 @@ __device__ __forceinline__ void ce_grad_tile(const CeGrads &a, const CeGrad &c, 
                     float *p = c.part + ((int64_t)z * c.part_rows + row) * a.D + d;
                     *p = c.add ? *p + v : v;
                 } else {
-                    ((T *)c.out)[to * a.D + d] = from_f32<T>(v * f);
+                    ((T *)c.out)[to * a.D + d] = from_f32<T>(v * f.two * f.g);
                 }
             }
         }
@@ -746,7 +748,7 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) ce_grads_kernel(CeGrads a) {
 template <typename T, int VE>
 __device__ __forceinline__ void ce_join(const CeGrads &a, const CeGrad &c, bool weight, int bid, int blocks) {
     const int64_t n = (weight ? c.rows : (int64_t)a.sc->live) * a.D, stride = c.part_rows * a.D;
-    const float f = ce_unscale(a.sc, a.grad, a.gmax, a.reduction, weight ? a.sc->ex : a.sc->ew);
+    const CeFactor f = ce_unscale(a.sc, a.grad, a.gmax, a.reduction, weight ? a.sc->ex : a.sc->ew);
     for (int64_t k = ((int64_t)bid * 256 + threadIdx.x) * VE; k < n; k += (int64_t)blocks * 256 * VE) {
         const int64_t row = k / a.D;
         float v[VE];
@@ -766,7 +768,7 @@ __device__ __forceinline__ void ce_join(const CeGrads &a, const CeGrad &c, bool 
         }
         T *out = (T *)c.out + (weight ? c.out0 + row : (int64_t)a.orig[row]) * a.D + (k - row * a.D);
 #pragma unroll
-        for (int e = 0; e < VE; ++e) out[e] = from_f32<T>(v[e] * f);
+        for (int e = 0; e < VE; ++e) out[e] = from_f32<T>(v[e] * f.two * f.g);
     }
 }
 
@@ -781,7 +783,8 @@ __global__ void __launch_bounds__(256) ce_join_kernel(CeGrads a, int bx, int bw,
     const int pos = (v & ~12) | ((v & 4) << 1) | ((v & 8) >> 1);
     float s = 0.0f;
     for (int k = 0; k < a.w.splits; ++k) s += a.part_b[k * a.ldb + pos];
-    dbias[v] = from_f32<T>(s * ce_unscale(a.sc, a.grad, a.gmax, a.reduction, 0));
+    const CeFactor f = ce_unscale(a.sc, a.grad, a.gmax, a.reduction, 0);
+    dbias[v] = from_f32<T>(s * f.two * f.g);
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------
