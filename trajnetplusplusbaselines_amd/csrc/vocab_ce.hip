@@ -262,13 +262,13 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) ce_logits_kernel(CeLogits a, c
     const int wm = wave / WN, wn = wave % WN;
     const float scale = ldexpf(CE_LOG2E, a.sc->ex + a.sc->ew);
     // this lane's rows
-    int64_t row[TN];
+    uint32_t row[TN];
     int tc[TN];
     float m[TN], s[TN], pf[TN], f[TN];                           // running statistics; backward: top, -, 2^15 r / sum, 2^15 r
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-        row[j] = (int64_t)ti * BN + wn * TN * 32 + j * 32 + (lane & 31);
-        tc[j] = row[j] < live ? a.tc[row[j]] : -1;
+        row[j] = (uint32_t)(ti * BN + wn * TN * 32 + j * 32 + (lane & 31));
+        tc[j] = (int)row[j] < live ? a.tc[row[j]] : -1;
         m[j] = CE_NEG_INF;
         s[j] = 0.0f;
         if (BACK) {
@@ -339,21 +339,22 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) ce_logits_kernel(CeLogits a, c
                     if (mine) a.tlogit[row[j]] = l;
                 }
             } else {
+                const bool any = __any(mine);
+                // stored order inside 16 columns: 0 1 2 3 8 9 10 11 | 4 5 6 7 12 13 14 15 -- what one lane holds, 16 bytes at a time, at a
+                // wave's base and a lane's offset of 32 bits
+                half_t *out = a.g + (int64_t)(tv * BM / 32 + wm * TM) * (SPLIT ? 2 : 1) * a.Mp * 32;
+                const uint32_t at = row[j] * 32 + h * 8;
 #pragma unroll
-                for (int i = 0; i < TM; ++i)
+                for (int i = 0; i < TM; ++i) {
+                    __builtin_amdgcn_sched_barrier(0);           // one block after the other: all together spill 34 registers (8192 x 16384 x
+                                                                 // 128 fp32 backward 493 us against 458)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_amdgcn_exp2f(acc[i][j][e] - m[j]) * pf[j];
-                if (__any(mine)) {
-#pragma unroll
-                    for (int i = 0; i < TM; ++i)
+                    if (any) {
 #pragma unroll
                         for (int e = 0; e < 16; ++e)
-                            if (mine && off == 32 * i + 8 * (e >> 2) + (e & 3)) acc[i][j][e] -= f[j];
-                }
-                // stored order inside 16 columns: 0 1 2 3 8 9 10 11 | 4 5 6 7 12 13 14 15 -- what one lane holds, 16 bytes at a time
-                half_t *out = a.g + ((int64_t)(tv * BM / 32 + wm * TM) * (SPLIT ? 2 : 1) * a.Mp + row[j]) * 32 + h * 8;
-#pragma unroll
-                for (int i = 0; i < TM; ++i)
+                            acc[i][j][e] -= mine && off == 32 * i + 8 * (e >> 2) + (e & 3) ? f[j] : 0.0f;
+                    }
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         half8 hi, lo;
@@ -363,10 +364,11 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) ce_logits_kernel(CeLogits a, c
                             hi[e] = (half_t)v;
                             if (SPLIT) lo[e] = (half_t)(v - (float)hi[e]);
                         }
-                        half_t *o = out + (SPLIT ? (i * 2 + c) * a.Mp * 32 : i * a.Mp * 32 + c * 16);
+                        half_t *o = out + (SPLIT ? (i * 2 + c) * a.Mp * 32 : i * a.Mp * 32 + c * 16) + at;
                         *(half8 *)o = hi;
                         if (SPLIT) *(half8 *)(o + 16) = lo;
                     }
+                }
             }
         }
     }
