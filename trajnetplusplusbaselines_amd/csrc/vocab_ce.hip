@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(256) ce_pack_kernel(const T *x, int64_t ldx, c
 // ---- logits: statistics forward, G backward ---------------------------------------------------------------------------------
 // The vocabulary runs over the rows of the matrix instruction, so a lane holds 16 logits of ONE hidden row per 32 x 32 block and
 // maxima, sums and exponentials stay inside the lane; the two halves of a wave meet once per share of the vocabulary.  16384 x 65536 x 1024
-// bf16: 2.15 ms of statistics (1.02 PFLOP/s), 2.29 with G written (2 GB); 4096 x 16384 x 512 fp32: 185 and 228 us (372 and 301 TFLOP/s; a
+// bf16: 2.16 ms of statistics (1.02 PFLOP/s), 2.26 with G written (2 GB); 4096 x 16384 x 512 fp32: 182 and 212 us (377 and 324 TFLOP/s; a
 // library product in fp32: 138).  Bound by the matrix cores' rate under load, the exponentials of a tile come on top.
 struct CeLogits {
     GemmOperand w, x;
@@ -729,8 +729,8 @@ __device__ __forceinline__ void ce_grad_tile(const CeGrads &a, const CeGrad &c, 
 }
 
 // Both gradient products in one launch: they read the same G, and the workgroups of one fill what the other's leave idle.  The last
-// workgroups zero dhidden of the absent rows.  16384 x 65536 x 1024 bf16 2 x 1.99 ms: 1.10 PFLOP/s (library products of these sizes 1.14 and
-// 1.51); 4096 x 16384 x 512 fp32 362 us: 380 TFLOP/s; 19700 x 1024 x 128 fp32 50 us: 207.  This loop with the operands left in place
+// workgroups zero dhidden of the absent rows.  16384 x 65536 x 1024 bf16 2 x 1.98 ms: 1.11 PFLOP/s (library products of these sizes 1.14 and
+// 1.51); 4096 x 16384 x 512 fp32 360 us: 382 TFLOP/s; 19700 x 1024 x 128 fp32 51 us: 203.  This loop with the operands left in place
 // reaches 1.3 PFLOP/s, which is the matrix cores' power.
 template <typename T, bool SPLIT, int BM, int BN, int WM, int WN, int NST>
 __global__ void __launch_bounds__(WM *WN * 64, 2) ce_grads_kernel(CeGrads a) {
