@@ -509,7 +509,42 @@ def test_other_stream_and_two_calls_at_once():
         assert all(torch.equal(p, q) for p, q in zip(got, want)) and all(torch.equal(p, q) for p, q in zip(got2, want2))
 
 
-@pytest.mark.parametrize('m', [20, 400])
+@pytest.mark.parametrize('n', [300, 9000, 600000])
+def test_embedding_on_two_streams_and_in_two_graphs(n):
+    """two gradients at once, eagerly and from two captured graphs that are replayed in turn and side by side"""
+    v, d = 700, 24
+    tok = [_tokens(n, v, kind, _gen(130)) for kind in ('skew', 'absent')]
+    w = torch.randn(v, d, device='cuda', generator=_gen(131)).requires_grad_()
+    up = [torch.randn(n, d, device='cuda', generator=_gen(132 + k)) for k in range(2)]
+    step = lambda k: torch.autograd.grad(vocab.token_embedding(tok[k], w, 2.0), w, up[k])[0]
+    want = [step(0), step(1)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                got.append(step(k))
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    graphs, held = [], []
+    for k in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[k]):
+            held.append(step(k))
+    for _ in range(3):
+        for h in held:
+            h.zero_()
+        torch.cuda.synchronize()
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                graphs[k].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held[0], want[0]) and torch.equal(held[1], want[1])
+        assert torch.equal(step(0), want[0])
+
+
+@pytest.mark.parametrize('m', [20, 400, 6000])
 def test_captured_and_replayed(m):
     """a step captured once and replayed on new inputs gives the eager step's bits, with eager work in between"""
     cases = [_case(m, 500, 48, torch.float32, 80 + k, absent=0.2) for k in range(4)]
