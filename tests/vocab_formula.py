@@ -1,0 +1,73 @@
+"""The vocabulary cross entropy's formulas in 64 bits, with bounds on how far the kernels may be off, element by element.
+
+X_i is the largest element of a row of hidden states (or of the weight), X the largest of all of them, u(t) = finfo(t).eps / 2.
+ * Operands: two fp16 numbers for fp32, off by 2^-22 |x|; what falls below the smallest fp16 number adds min(2^-23 X_i, 2^-38 X).
+ * Products: lo * lo is left out (2^-22 |x w|), 2^-23 per term and plane for the accumulation.
+ * G = g (p - y): 2^-22 (two fp16 numbers: fp32 and fp16) or 2^-11 (bf16) of itself, and min(2^-39 max |g|, 2^-21 |g_i|) below the smallest
+   fp16 number, if it is not 0 to begin with.
+ * p: with d_iv the error of a logit and e_i = log sum exp(l + d) - log sum exp(l) what these do to the normaliser, E = d + e + (exponentials
+   and sums) stands on both sides of the quotient: p (e^E - 1).  An entry so far below the row's largest that its p is 0 whatever the error,
+   and a largest entry so far above all others that its p is 1, have no error of that kind.
+"""
+import torch
+
+
+def u(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def below(x):
+    """what the smallest fp16 number costs an element of each row"""
+    top = x.abs().max(1, keepdim=True).values
+    return torch.minimum(2.0 ** -23 * top, 2.0 ** -38 * top.max())
+
+
+def formula(x, w, b, t, grad_rows, extra=0.0):
+    """loss per row and its bound, (dx, dw, db) and their bounds; ``extra``: error of every logit beside the above"""
+    dtype = x.dtype
+    split = dtype == torch.float32
+    there = t >= 0
+    xd = torch.where(there[:, None], x.detach().double(), 0.0)
+    wd = w.detach().double()
+    (m, k), v = xd.shape, wd.shape[0]
+    l = xd @ wd.t() + (b.detach().double() if b is not None else 0.0)
+    at = t.clamp(min=0)[:, None]
+    lse = torch.logsumexp(l, 1)
+    loss = torch.where(there, lse - l.gather(1, at)[:, 0], 0.0)
+    size = torch.where(torch.isinf(l), 0.0, l.abs())
+    planes = 3 if split else 1
+    xa, wa, xb, wb = xd.abs(), wd.abs(), below(xd), below(wd)
+    delta = ((3 * 2.0 ** -22 if split else 0.0) + planes * k * 2.0 ** -23) * (xa @ wa.t()) + 6 * 2.0 ** -24 * size + extra
+    delta += xb * wa.sum(1) + xa.sum(1, keepdim=True) * wb.t()
+    delta = torch.where(torch.isinf(l), 0.0, delta)
+    e = torch.logsumexp(l + delta, 1) - lse
+    # sums: of up to 64 terms in a lane, then of tiles and workgroups; rounding of the exponentials' arguments is in delta
+    sums = 2.0 ** -22 + 4 * 2.0 ** -24 * lse.abs() + (64 + v / 16 + 32) * 2.0 ** -24
+    loss_bound = torch.where(there, delta.gather(1, at)[:, 0] + e + sums + 4 * 2.0 ** -24 * (loss.abs() + lse.abs()), 0.0) + 1e-30
+    E = delta + (e + 2 * sums)[:, None]
+    p = torch.exp(l - lse[:, None])
+    most = torch.exp((l - lse[:, None] + E).clamp(max=0.0))               # p is no larger than this
+    dp = torch.minimum(p * torch.expm1(E.clamp(max=50.0)), most)
+    first = l.argmax(1, keepdim=True)
+    rest = most.scatter(1, first, 0.0).sum(1, keepdim=True)               # 1 - p of the largest
+    dp = dp.scatter(1, first, torch.minimum(dp.gather(1, first), rest))
+    g = torch.where(there, grad_rows.double(), 0.0)[:, None]
+    G = (p * g).scatter_add(1, at, -g)
+    step = 2.0 ** -11 if dtype == torch.bfloat16 else 2.0 ** -22
+    floor = torch.minimum(2.0 ** -39 * g.abs().max(), 2.0 ** -21 * g.abs())
+    dG = dp * g.abs()
+    dG = dG + G.abs() * (step + 6 * 2.0 ** -24) + torch.minimum(floor, G.abs() + dG)
+    dG = torch.where(there[:, None], dG, 0.0)
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    runs = 3 if split else 1 if dtype == torch.bfloat16 else 2
+
+    def near(val, da, a, c, low, n):                                       # val = a c, a off by da, c by its own roundings
+        off = da @ c + a @ (c * ((3 * 2.0 ** -22 if split else 0.0) + runs * n * 2.0 ** -23) + low)
+        return off + val.abs() * (u(dtype) + 4 * 2.0 ** -24) + tiny + 1e-30
+
+    Ga = G.abs()
+    one = torch.ones(m, 1, dtype=torch.float64, device=x.device)
+    want = (G @ wd, G.t() @ xd, G.sum(0))
+    bounds = (near(want[0], dG, Ga, wa, wb, v), near(want[1], dG.t(), Ga.t(), xa, xb, m),
+              near(want[2][:, None], dG.t(), Ga.t(), one, 0.0 * one, m)[:, 0])
+    return loss, loss_bound, want, bounds

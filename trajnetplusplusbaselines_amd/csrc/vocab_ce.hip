@@ -2,14 +2,15 @@
 //     l_iv = hidden_i . weight_v + bias_v,   lse_i = log sum_v exp(l_iv),   loss_i = lse_i - l_i,target(i)
 //     G_iv = g_i (exp(l_iv - lse_i) - [v == target(i)]),   dhidden = G weight,   dweight = G^T hidden,   dbias_v = sum_i G_iv
 // The logits are never kept: the forward pass leaves per row the running maximum and sum of every vocabulary tile, the backward
-// pass forms the logits again, piece by piece of the vocabulary, as G in fp16 (twice fp16 for fp32 inputs), which both gradient
+// pass forms the logits again, piece by piece of the vocabulary, as G in fp16 (twice fp16 for fp32 and fp16 inputs), which both gradient
 // products read.  Forming them again costs 2 M D V operations; writing, reading and correcting the fp32 logits would cost 12 bytes
 // each, more than that for every D below about 2000.
 //
 // Numbers.  Inputs are packed once per call as fp16 times one power of two per tensor, so that its largest element lies in
 // [2^14, 2^15): bf16 and fp16 values are exact down to 2^-29 of the largest, fp32 values become two fp16 numbers (vocab_gemm.h) with an error
-// of 2^-23 of the value or 2^-40 of the largest.  G = 2^15 (g_i / max g) (p - y) is rounded to fp16 (11 bits, finer than bf16
-// by 8) or to two fp16 numbers.  All sums, maxima and statistics are fp32; the sum of the losses is fp64.
+// of 2^-23 of the value or 2^-40 of the largest.  G = 2^15 (g_i / max g) (p - y) is rounded to fp16 for bf16 gradients (11 bits, eight times
+// finer than what they are rounded to: their error grows by less than a hundredth) and to two fp16 numbers for fp32 and fp16 ones (one of them
+// would be as coarse as the fp16 gradient itself).  All sums, maxima and statistics are fp32; the sum of the losses is fp64.
 //
 // A negative target marks an absent row: its hidden state is not read (it may be NaN), its loss and gradients are zero.  Packing leaves
 // the absent rows out, so that everything behind it runs on the rows that are there (a fifth of a crowd's tracks are absent, more
@@ -34,6 +35,10 @@ static constexpr int CE_SCORE_GROUPS = 2, CE_SCORE_GROUPS_FROM = 20480;
 static constexpr int CE_JOIN_BLOCKS = 1 << 20;         // a grid holds fewer than 2^32 threads
 // rows up to which scoring reads the inputs in place: 64 x 65536 x 512 bf16 37 us against 62 packed, fp32 74 against 127
 static constexpr int CE_SCORE_ROWS = 64;
+
+// G as two fp16 numbers: panels of both (SPLIT operands), or one plane of panels behind the other
+template <typename T, bool SPLIT> static constexpr bool CE_TWO_PLANES = !SPLIT && std::is_same<T, half_t>::value;
+static inline int ce_g_planes(int dtype) { return dtype == TNP_BF16 ? 1 : 2; }
 
 struct CeScalars {            // head of the saved area
     int ex, ew;               // packed = value * 2^-e
@@ -235,6 +240,7 @@ struct CeLogits {
     const float2 *stat;       // [Mp] (largest logit, base 2; 1 / sum of 2^(l - largest)), padding (+inf, 0), no such target (.., NaN)
     const float *grad, *gmax; // reduction none: [M], largest |grad|
     half_t *g;                // panels of Mp rows, column 0 = vocabulary entry v0
+    int64_t g_plane;          // elements from a plane of G to the next
 };
 
 // bias in base 2; a finite one stays finite (the lowest value of fp32 as a mask: where it masks a whole row, all entries are alike)
@@ -362,11 +368,12 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) ce_logits_kernel(CeLogits a, c
                         for (int e = 0; e < 8; ++e) {
                             const float v = acc[i][j][8 * c + e];
                             hi[e] = (half_t)v;
-                            if (SPLIT) lo[e] = (half_t)(v - (float)hi[e]);
+                            if (SPLIT || CE_TWO_PLANES<T, SPLIT>) lo[e] = (half_t)(v - (float)hi[e]);
                         }
                         half_t *o = out + (SPLIT ? (i * 2 + c) * a.Mp * 32 : i * a.Mp * 32 + c * 16) + at;
                         *(half8 *)o = hi;
                         if (SPLIT) *(half8 *)(o + 16) = lo;
+                        if (CE_TWO_PLANES<T, SPLIT>) *(half8 *)(o + a.g_plane) = lo;
                     }
                 }
             }
@@ -662,7 +669,7 @@ struct CeGrads {
     const float *grad, *gmax;
     const int64_t *target;
     const int32_t *orig;      // dhidden: the caller's row of a row that is there
-    int64_t M;
+    int64_t M, g_plane;
     int reduction, D, zero_blocks;
     float *part_b;            // dbias: [w.splits][ldb] sums in G's stored column order, or NULL
     int64_t ldb;
@@ -680,7 +687,7 @@ __device__ __forceinline__ void ce_grad_tile(const CeGrads &a, const CeGrad &c, 
     if (z >= c.splits || !gemm_tile_of(bid - z * per, tiles_r, c.tiles_d, tr, td)) return;
     const int64_t r0 = (int64_t)tr * BM;
     const int d0 = td * BN;
-    const int64_t steps = WEIGHT ? ce_padded(live) / PC : c.steps;
+    const int64_t plane_steps = WEIGHT ? ce_padded(live) / PC : c.steps, steps = plane_steps * (CE_TWO_PLANES<T, SPLIT> ? 2 : 1);
     const int s0 = (int)(steps * z / c.splits), s1 = (int)(steps * (z + 1) / c.splits);
     f32x16 acc[TM][TN];
     const int gp = WEIGHT ? (int)(r0 / PC) : 0, op = d0 / PC;
@@ -693,6 +700,7 @@ __device__ __forceinline__ void ce_grad_tile(const CeGrads &a, const CeGrad &c, 
     for (int i = 0; i < TM; ++i) asum[i] = 0.0f;
     TileGemm<SPLIT, WEIGHT, true, BM, BN, WM, WN, NST> g;
     g.init(c.g, c.o, WEIGHT ? 0 : r0, gp, c.g_panels - gp, c.ok0, op, c.o_panels - op, lds);
+    if (CE_TWO_PLANES<T, SPLIT>) g.two_planes(a.g_plane, (int)plane_steps);
     g.first(s0, s1);
     g.template run<WEIGHT>(s0, s1, acc, sums, asum);
     if (sums) {
@@ -882,7 +890,7 @@ static constexpr size_t CE_PIECE_BYTES = (size_t)1 << 30;      // of 288 GB; 163
 static CeBackward ce_backward_layout(const tnp_vocab_ce *p, void *ws) {
     CeBackward b;
     const CeShape s = ce_shape(p);
-    const int planes = s.split ? 2 : 1, ks = s.split ? 16 : 32;
+    const int planes = ce_g_planes(p->dtype), ks = s.split ? 16 : 32, runs = s.split ? 1 : planes;     // runs of the products over G
     int64_t most = (int64_t)(CE_PIECE_BYTES / ((size_t)s.Mp * 2 * planes)) / 256 * 256;
     if (most < 256) most = 256;
     b.pieces = (int)((s.Vp + most - 1) / most);
@@ -892,7 +900,7 @@ static CeBackward ce_backward_layout(const tnp_vocab_ce *p, void *ws) {
     // 256 x 256 tiles (eight waves) where they are many steps' work: 16384 x 4096 x 512 bf16 backward 248 us against 285, 8192 x 16384 x
     // 128 (65536 tile steps) 229 against 218
     const int64_t td = (p->D + 127) / 128, small_x = s.Mp / 128 * td, small_w = b.piece / 128 * td;
-    const int sx = b.piece / ks, sw = (int)(s.Mp / ks);
+    const int sx = b.piece / ks * runs, sw = (int)(s.Mp / ks) * runs;
     b.tile = small_x * sx + small_w * sw >= 131072 && p->D > 128 ? 256 : 128;
     // both products share a launch: every workgroup gets about the same number of steps, at least 8
     const int64_t tx = s.Mp / b.tile * ((p->D + b.tile - 1) / b.tile), tw = b.piece / b.tile * ((p->D + b.tile - 1) / b.tile);
@@ -1051,11 +1059,12 @@ static int ce_backward(const tnp_vocab_ce *p, const CeBackward &b, const float *
         const int v0 = k * b.piece, cols = sh.Vp - v0 < b.piece ? sh.Vp - v0 : b.piece, live = sh.V - v0 < cols ? sh.V - v0 : cols;
         CeLogits a = {};
         a.w = w; a.x = x; a.sc = sv.sc; a.tc = sv.tc; a.orig = sv.orig; a.Mp = sh.Mp; a.V = sh.V; a.v0 = v0; a.steps = sh.panels;
-        a.stat = sv.stat; a.grad = p->reduction == 0 ? grad : nullptr; a.gmax = b.gmax; a.g = b.g; a.v_shares = ce_logit_shares(sh, cols);
+        a.stat = sv.stat; a.grad = p->reduction == 0 ? grad : nullptr; a.gmax = b.gmax; a.g = b.g; a.g_plane = (int64_t)b.piece * sh.Mp; a.v_shares = ce_logit_shares(sh, cols);
         if ((rc = ce_logits<T, SPLIT, true>(a, cols, ce_big(sh), (const T *)p->bias, s))) return rc;
         const bool last = k == b.pieces - 1;
         const int ks = SPLIT ? 16 : 32;
         CeGrads c = {};
+        c.g_plane = (int64_t)b.piece * sh.Mp;
         c.sc = sv.sc; c.grad = grad; c.gmax = b.gmax; c.target = p->target; c.orig = sv.orig; c.M = sh.M; c.reduction = p->reduction; c.D = sh.D;
         c.zero_blocks = dhidden && k == 0 ? (int)(sh.Mp / 64 < 512 ? sh.Mp / 64 : 512) : 0;
         c.x.g = c.w.g = GemmOperand{b.g, sh.Mp, 0};

@@ -63,8 +63,8 @@ template <bool KS, bool SPLIT, int BR, int NW> struct TileStage {
             }
         }
     }
-    __device__ __forceinline__ void load(int step, char *lds, int wave) const {
-        const half_t *b = base + step * advance;
+    __device__ __forceinline__ void load(int step, int64_t plane, char *lds, int wave) const {
+        const half_t *b = base + step * advance + plane;
 #pragma unroll
         for (int j = 0; j < INSTR; ++j)
             __builtin_amdgcn_global_load_lds((const TNP_GLB void *)(b + off[j]), (TNP_LDS void *)(lds + (wave + j * NW) * 1024), 16, 0, 0);
@@ -215,6 +215,9 @@ template <int TM> __device__ __forceinline__ void step_row_sums(const half8 (&fa
 // four waves the other workgroups on the CU fill that time.
 //
 // SUMS: with `sums` (the same for the wave), asum[] gathers the row sums of a as well (step_row_sums).
+//
+// An unsplit a may have a second plane, `plane` elements behind the first: the steps from `wrap` on run over it, with b's steps from the
+// first one again.
 template <bool SPLIT, bool A_KS, bool B_KS, int BM, int BN, int WM, int WN, int NST> struct TileGemm {
     static constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, STAGE = (BM + BN) * 64;
     static constexpr bool TURNS = NW == 8;
@@ -225,20 +228,26 @@ template <bool SPLIT, bool A_KS, bool B_KS, int BM, int BN, int WM, int WN, int 
     SA sa;
     SB sb;
     char *lds;
-    int lane, wave;
+    int lane, wave, wrap;
+    int64_t plane;
 
     __device__ __forceinline__ void init(const GemmOperand &a, const GemmOperand &b, int64_t ar, int64_t ap, int al, int64_t br, int64_t bp, int bl,
                                          char *lds_) {
         lds = lds_;
         lane = threadIdx.x & 63;
         wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        wrap = INT32_MAX;
+        plane = 0;
         sa.init(a, ar, ap, al, wave, lane);
         sb.init(b, br, bp, bl, wave, lane);
     }
     __device__ __forceinline__ void a_rows(int rows) { sa.base += (int64_t)rows * 32; }
+    __device__ __forceinline__ void two_planes(int64_t plane_, int wrap_) { plane = plane_; wrap = wrap_; }
     __device__ __forceinline__ void load(int s, int stage) {
-        sa.load(s, lds + stage * STAGE, wave);
-        sb.load(s, lds + stage * STAGE + BM * 64, wave);
+        const bool second = s >= wrap;
+        const int k = second ? s - wrap : s;
+        sa.load(k, second ? plane : 0, lds + stage * STAGE, wave);
+        sb.load(k, 0, lds + stage * STAGE + BM * 64, wave);
     }
     __device__ __forceinline__ void first(int s0, int s1) {
 #pragma unroll

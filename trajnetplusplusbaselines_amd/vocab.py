@@ -133,8 +133,8 @@ def vocab_cross_entropy(hidden, weight, target, bias=None, reduction='mean'):
 
     fp32 operands are multiplied as two fp16 numbers each, scaled by the largest finite element of their tensor: an element below
     2^-16 of that one loses relative precision (2^-40 of the largest remains), a row of valid targets that holds an infinity gives
-    NaN.  Gradients: (p - y) times the upstream gradient is rounded to fp16 (fp32 operands: two fp16 numbers) on one scale for all rows;
-    parts below 2^-29 of the largest lose relative precision."""
+    NaN.  Gradients: (p - y) times the upstream gradient is rounded to fp16 (fp32 and fp16 operands: two fp16 numbers) on one scale for
+    all rows; parts below 2^-29 of the largest lose relative precision."""
     if torch.compiler.is_compiling():
         from . import ops  # noqa: F401  (registers the operators)
         return torch.ops.trajnet.vocab_cross_entropy(hidden, weight, target, bias, reduction)[0]
