@@ -31,3 +31,79 @@ def _check(x, w, b, t, up=None, extra=0.0):
 def test_gradients_are_rounded_once(dtype, m, v, d):
     """G does not add a rounding of the gradients' own size (fp16: it is held in two numbers)"""
     _check(*_case(m, v, d, dtype, m + 3 * v + d, absent=0.2 if m > 4 else 0.0))
+
+
+# ---- one row, one entry of another magnitude ---------------------------------------------------------------------------------
+def _scaled(x, rows, factor):
+    with torch.no_grad():
+        x[rows] = (x[rows].double() * factor).to(x.dtype)
+
+
+def _score(x, w, b, t):
+    """losses of 40 rows at a time without a gradient: the inputs in place"""
+    with torch.no_grad():
+        return torch.cat([vocab.vocab_cross_entropy(x[k:k + 40], w, t[k:k + 40], bias=b, reduction='none') for k in range(0, x.shape[0], 40)])
+
+
+@pytest.mark.parametrize('dtype,factor', [(torch.float32, 2.0 ** 20), (torch.float32, 2.0 ** 40), (torch.float32, 2.0 ** 70), (torch.bfloat16, 2.0 ** 30),
+                                          (torch.bfloat16, 2.0 ** 40), (torch.bfloat16, 2.0 ** 70), (torch.float16, 2.0 ** 25)])
+@pytest.mark.parametrize('m,v,d', [(130, 90, 24), (300, 700, 65)])
+def test_a_row_of_another_magnitude_leaves_the_others_alone(dtype, factor, m, v, d):
+    x, w, b, t = _case(m, v, d, dtype, 17 * m + d, absent=0.2)
+    live = torch.nonzero(t >= 0)[:, 0]
+    if dtype == torch.float16:                          # small rows and one of ordinary size times 2^12: fp16 holds no more
+        _scaled(x, slice(None), 2.0 ** -13)
+        _scaled(w, slice(None), 2.0 ** 12)
+    _scaled(x, live[[7]], factor)
+    _check(x, w, b, t)
+    loss, bound, _, _ = formula(x, w, b, t, torch.ones(m, device='cuda'))
+    _within(_score(x, w, b, t), loss, bound)
+
+
+@pytest.mark.parametrize('dtype,factor', [(torch.float32, 2.0 ** 40), (torch.float32, 2.0 ** 70), (torch.bfloat16, 2.0 ** 40)])
+@pytest.mark.parametrize('masked', [True, False])
+@pytest.mark.parametrize('m,v,d', [(130, 90, 24), (300, 700, 65)])
+def test_an_entry_of_another_magnitude_leaves_the_others_alone(dtype, factor, masked, m, v, d):
+    """a row of the weight 2^40 times as large as the others, masked by the bias or winning wherever its logit is positive"""
+    x, w, b, t = _case(m, v, d, dtype, 19 * m + d, absent=0.2)
+    hit = v // 2
+    t[t == hit] = 0
+    _scaled(w, [hit], factor)
+    if masked:
+        with torch.no_grad():
+            b[hit] = float('-inf')
+    _check(x, w, b, t)
+    loss, bound, _, _ = formula(x, w, b, t, torch.ones(m, device='cuda'))
+    _within(_score(x, w, b, t), loss, bound)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_rows_and_entries_over_many_magnitudes(dtype):
+    """hidden states over 2^48 and weights over 2^48, their products of ordinary size: every tenth row and entry meets its like"""
+    m, v, d = 300, 500, 40
+    x, w, b, t = _case(m, v, d, dtype, 23, absent=0.1)
+    with torch.no_grad():
+        # column block k of both is the rows' magnitude class: x 2^(12 k) there, w 2^(-12 k), zero elsewhere
+        cls_x, cls_w = torch.arange(m, device='cuda') % 5, torch.arange(v, device='cuda') % 5
+        col = torch.arange(d, device='cuda') // 8
+        x.copy_(torch.where(col == cls_x[:, None], x * 2.0 ** (12 * cls_x[:, None].double()), 0.0 * x).to(dtype))
+        w.copy_(torch.where(col == cls_w[:, None], w * 2.0 ** (-12 * cls_w[:, None].double()), 0.0).to(dtype))
+        x[t < 0] = float('nan')
+    _check(x, w, b, t)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_magnitudes_at_the_ends_of_the_types(dtype):
+    """all rows near the largest and all weights near the smallest normal number: exponents whose sum alone would pass fp32's"""
+    top = 14.0 if dtype == torch.float16 else 120.0
+    x, w, b, t = _case(150, 80, 16, dtype, 29, absent=0.1)
+    _scaled(x, slice(None), 2.0 ** top)
+    _scaled(w, slice(None), 2.0 ** -top)
+    _check(x, w, b, t)
+    with torch.no_grad():
+        # logits that are exactly zero although both exponents are at their largest: no product of the scales may make NaN of them
+        x.copy_(torch.where(torch.arange(16, device='cuda') < 8, 2.0 ** top, 0.0).to(dtype).expand(150, 16))
+        w.copy_(torch.where(torch.arange(16, device='cuda') < 8, 0.0, 2.0 ** top).to(dtype).expand(80, 16))
+        loss = vocab.vocab_cross_entropy(x, w, t, bias=b, reduction='none')
+        zero, bound, _, _ = formula(torch.zeros_like(x), torch.zeros_like(w), b, t, torch.ones(150, device='cuda'))
+        _within(loss, zero, bound)

@@ -7,8 +7,10 @@
 // each, more than that for every D below about 2000.
 //
 // Numbers.  Inputs are packed once per call as fp16 times one power of two per tensor, so that its largest element lies in
-// [2^14, 2^15): bf16 and fp16 values are exact down to 2^-29 of the largest, fp32 values become two fp16 numbers (vocab_gemm.h) with an error
-// of 2^-23 of the value or 2^-40 of the largest.  G = 2^15 (g_i / max g) (p - y) is rounded to fp16 for bf16 gradients (11 bits, eight times
+// [2^14, 2^15); a row whose largest element is below 2^-16 of that gets a power of two of its own (a "far" row), so that no row's bits go by
+// another's size.  bf16 and fp16 values are exact down to 2^-12 of their row's largest, fp32 values become two fp16 numbers (vocab_gemm.h); an error of
+// 2^-23 of the value or of its row's largest, usually 2^-40 of the latter.  Logits of far rows or entries get their powers of two one by one;
+// the gradient products, where rows are summed over, take far rows in classes (vocab_gemm.h), one run each.  G = 2^15 (g_i / max g) (p - y) is rounded to fp16 for bf16 gradients (11 bits, eight times
 // finer than what they are rounded to: their error grows by less than a hundredth) and to two fp16 numbers for fp32 and fp16 ones (one of them
 // would be as coarse as the fp16 gradient itself).  All sums, maxima and statistics are fp32; the sum of the losses is fp64.
 //
@@ -44,7 +46,9 @@ struct CeScalars {            // head of the saved area
     int ex, ew;               // packed = value * 2^-e
     uint32_t ticket;          // last-workgroup counter of the loss sum
     int live;                 // rows that are there
+    uint32_t x_classes, w_classes;      // bit c: rows of class c (vocab_gemm.h) among the hidden states, the weight
 };
+static constexpr int CE_FAR = 16;      // binades below the tensor's largest element from which on a row has its own scale
 __device__ __forceinline__ int ce_padded(int live) { return (live + 255) & ~255; }
 
 struct CeShape {
@@ -107,7 +111,10 @@ __global__ void __launch_bounds__(256) ce_amax_kernel(const T *x, int64_t ldx, i
     __syncthreads();
     if (threadIdx.x == 0) {
         part[blockIdx.x] = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
-        if (blockIdx.x == 0) sc->ticket = 0;
+        if (blockIdx.x == 0) {
+            sc->ticket = 0;
+            sc->x_classes = sc->w_classes = 1;
+        }
     }
 }
 
@@ -120,16 +127,17 @@ __device__ __forceinline__ int ce_exponent(float a) {
 }
 
 // sixteen rows into panels (vocab_gemm.h): lane = (row, 16-byte chunk), so a panel is written as one contiguous kilobyte.  This lane's
-// row: src row `from` (negative: zeros) to dst row `to` (negative: nothing)
+// row: src row `from` (negative: zeros) to dst row `to` (negative: nothing), times 2^-e.  Returns the largest finite |element| that this lane has seen.
 template <typename T, int VE, bool SPLIT>
-__device__ __forceinline__ void ce_pack_rows(const T *src, int64_t ld, int64_t from_row, int64_t to, int D, int e, half_t *dst, int64_t panel_rows,
-                                             int panels, int lane) {
+__device__ __forceinline__ float ce_pack_rows_at(const T *src, int64_t ld, int64_t from_row, int64_t to, int D, int e, half_t *dst,
+                                                 int64_t panel_rows, int panels, int lane) {
     constexpr int NV = 8;                                        // values per chunk; a split chunk is the hi or the lo half of eight
     const bool live = from_row >= 0;
     const int ch = lane & 3, c0 = SPLIT ? (ch & 1) * 8 : ch * 8;
     constexpr int U = 4;                                         // panels in flight
     const T *from = src + (live ? from_row : 0) * ld;                 // rows and columns that are not there: row 0, column 0, not used
     half_t *out = dst + (to < 0 ? 0 : to) * 32 + ch * 8;
+    float top = 0.0f;
     for (int p = 0; p < panels; p += U) {
         Pack<T, VE> q[U][NV / VE];
 #pragma unroll
@@ -146,19 +154,36 @@ __device__ __forceinline__ void ce_pack_rows(const T *src, int64_t ld, int64_t f
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
                 const bool there = live && (p + u) * (SPLIT ? 16 : 32) + c0 + k < D;
-                const float v = there ? ldexpf(to_f32(q[u][k / VE].v[k % VE]), -e) : 0.0f;
+                const float x = there ? to_f32(q[u][k / VE].v[k % VE]) : 0.0f, v = ldexpf(x, -e);
                 const half_t hi = (half_t)v;
                 o[k] = SPLIT && ch >= 2 ? (fabsf(v) < 65504.0f ? (half_t)(v - (float)hi) : (half_t)0.0f) : hi;
+                top = fmaxf(top, fabsf(x) < __builtin_inff() ? fabsf(x) : 0.0f);
             }
             if (to >= 0) *(half8 *)(out + (p + u) * panel_rows * 32) = o;
         }
     }
+    return top;
+}
+
+// the same on the tensor's exponent e, and once more on their own the rows that are far below it; exps[to]: the row's exponent
+template <typename T, int VE, bool SPLIT>
+__device__ __forceinline__ void ce_pack_rows(const T *src, int64_t ld, int64_t from_row, int64_t to, int D, int e, half_t *dst, int64_t panel_rows,
+                                             int panels, int lane, int32_t *exps, uint32_t *classes) {
+    float top = ce_pack_rows_at<T, VE, SPLIT>(src, ld, from_row, to, D, e, dst, panel_rows, panels, lane);
+    top = fmaxf(top, __shfl_xor(top, 1));                        // the row's four lanes
+    top = fmaxf(top, __shfl_xor(top, 2));
+    const int own = ce_exponent(top);
+    const bool far = top > 0.0f && own < e - CE_FAR;
+    if (to >= 0 && (lane & 3) == 0) exps[to] = far ? own : e;
+    if (!__any(far)) return;
+    ce_pack_rows_at<T, VE, SPLIT>(src, ld, from_row, far ? to : -1, D, own, dst, panel_rows, panels, lane);
+    if (far && to >= 0 && (lane & 3) == 0) atomicOr(classes, 1u << row_class(own - e));
 }
 
 template <typename T, int VX, int VW, bool SPLIT>
 __global__ void __launch_bounds__(256) ce_pack_kernel(const T *x, int64_t ldx, const int64_t *target, const T *w, int64_t ldw, CeShape sh,
                                                       const float *part, const int *count, CeScalars *sc, half_t *xp, half_t *wp, int32_t *orig,
-                                                      int32_t *tc, int x_blocks) {
+                                                      int32_t *tc, int32_t *xe, int32_t *we, int x_blocks) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tid = threadIdx.x;
     const bool is_w = (int)blockIdx.x >= x_blocks;
     __shared__ float red[4];
@@ -185,7 +210,7 @@ __global__ void __launch_bounds__(256) ce_pack_kernel(const T *x, int64_t ldx, c
         if (tid == 0 && (int)blockIdx.x == x_blocks) sc->ew = e;
         const int blocks = gridDim.x - x_blocks;
         for (int64_t r = ((int)blockIdx.x - x_blocks) * 64 + wave * 16 + (lane >> 2); r < sh.Vp; r += blocks * 64)
-            ce_pack_rows<T, VW, SPLIT>(w, ldw, r < sh.V ? r : -1, r, sh.D, e, wp, sh.Vp, sh.panels, lane);
+            ce_pack_rows<T, VW, SPLIT>(w, ldw, r < sh.V ? r : -1, r, sh.D, e, wp, sh.Vp, sh.panels, lane, we, &sc->w_classes);
         return;
     }
     int base = cnt[0].x + cnt[1].x + cnt[2].x + cnt[3].x;
@@ -213,13 +238,14 @@ __global__ void __launch_bounds__(256) ce_pack_kernel(const T *x, int64_t ldx, c
         __syncthreads();
         for (int g = wave * 16; g < num; g += 64) {
             const int i = g + (lane >> 2);
-            ce_pack_rows<T, VX, SPLIT>(x, ldx, i < num ? list[i] : -1, i < num ? base + i : -1, sh.D, e, xp, sh.Mp, sh.panels, lane);
+            ce_pack_rows<T, VX, SPLIT>(x, ldx, i < num ? list[i] : -1, i < num ? base + i : -1, sh.D, e, xp, sh.Mp, sh.panels, lane, xe,
+                                        &sc->x_classes);
         }
         base += num;
     }
     // zero rows up to the next multiple of 256
     for (int64_t r = live + (int64_t)blockIdx.x * 64 + wave * 16 + (lane >> 2); r - (lane >> 2) < ce_padded(live); r += (int64_t)x_blocks * 64)
-        ce_pack_rows<T, VX, SPLIT>(x, ldx, -1, r < ce_padded(live) ? r : -1, sh.D, e, xp, sh.Mp, sh.panels, lane);
+        ce_pack_rows<T, VX, SPLIT>(x, ldx, -1, r < ce_padded(live) ? r : -1, sh.D, e, xp, sh.Mp, sh.panels, lane, xe, &sc->x_classes);
 }
 
 // ---- logits: statistics forward, G backward ---------------------------------------------------------------------------------
@@ -231,6 +257,7 @@ struct CeLogits {
     GemmOperand w, x;
     const CeScalars *sc;
     const int32_t *tc, *orig; // of the rows that are there: target (V: none such), row of the caller
+    const int32_t *xe, *we;   // exponents of hidden rows and vocabulary entries
     int64_t Mp;
     int V, v0, tiles_v, v_shares, steps;
     // forward
@@ -266,7 +293,10 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) ce_logits_kernel(CeLogits a, c
     const int tv0 = (int)((int64_t)a.tiles_v * vs / a.v_shares), tv1 = (int)((int64_t)a.tiles_v * (vs + 1) / a.v_shares);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
     const int wm = wave / WN, wn = wave % WN;
-    const float scale = ldexpf(CE_LOG2E, a.sc->ex + a.sc->ew);
+    // rows or entries on scales of their own, or scales whose product could leave fp32's range: every logit by itself
+    const int ex_all = a.sc->ex + a.sc->ew;
+    const bool each = (a.sc->x_classes | a.sc->w_classes) != 1 || ex_all > 96 || ex_all < -96;
+    const float scale = each ? 1.0f : ldexpf(CE_LOG2E, ex_all);
     // this lane's rows
     uint32_t row[TN];
     int tc[TN];
@@ -298,11 +328,31 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) ce_logits_kernel(CeLogits a, c
         if ((int)threadIdx.x < BM) tb[threadIdx.x] = b_next;     // read behind the barriers of run(); the other half is still being read
         f32x16 acc[TM][TN];
         float none[TM];
-        g.template run<false>(0, a.steps, acc, false, none);
+        g.template run<false, false>(0, a.steps, acc, false, none, RowScales{});
         if (tv + 1 < tv1) {
             b_next = next_bias(tv + 1);
             g.a_rows(BM);
             g.first(0, a.steps);
+        }
+        if (each) {
+            int ex[TN];
+#pragma unroll
+            for (int j = 0; j < TN; ++j) ex[j] = a.xe[row[j]];
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    __builtin_amdgcn_sched_barrier(0);           // four exponents at a time: all of them spill registers
+                    const int4 ew = *(const int4 *)(a.we + a.v0 + tv * BM + wm * TM * 32 + i * 32 + 8 * q + 4 * h);
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) {
+                        acc[i][j][4 * q + 0] = ldexpf(acc[i][j][4 * q + 0] * CE_LOG2E, ex[j] + ew.x);
+                        acc[i][j][4 * q + 1] = ldexpf(acc[i][j][4 * q + 1] * CE_LOG2E, ex[j] + ew.y);
+                        acc[i][j][4 * q + 2] = ldexpf(acc[i][j][4 * q + 2] * CE_LOG2E, ex[j] + ew.z);
+                        acc[i][j][4 * q + 3] = ldexpf(acc[i][j][4 * q + 3] * CE_LOG2E, ex[j] + ew.w);
+                    }
+                }
+            __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int i = 0; i < TM; ++i)
@@ -657,6 +707,7 @@ struct CeGrad {
     int64_t rows, out0;       // dweight: output rows of this call, the first one's index in the output
     int tiles_d, steps, splits, blocks;
     int64_t ok0;              // first row of the other operand
+    const int32_t *o_exps;    // exponents of its rows, from there
     int g_panels, o_panels;
     void *out;                // final output (nothing to add up), [..][D]
     float *part;              // [splits][part_rows][D] sums, or NULL
@@ -674,6 +725,15 @@ struct CeGrads {
     float *part_b;            // dbias: [w.splits][ldb] sums in G's stored column order, or NULL
     int64_t ldb;
 };
+
+template <int TM, int TN> __device__ __forceinline__ void ce_rescale(f32x16 (&acc)[TM][TN], int by) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = ldexpf(acc[i][j][e], by);
+}
 
 // WEIGHT: dweight (G read transposed, output rows = vocabulary entries in G's stored column order), else dhidden
 template <typename T, bool SPLIT, bool WEIGHT, int BM, int BN, int WM, int WN, int NST>
@@ -701,8 +761,23 @@ __device__ __forceinline__ void ce_grad_tile(const CeGrads &a, const CeGrad &c, 
     TileGemm<SPLIT, WEIGHT, true, BM, BN, WM, WN, NST> g;
     g.init(c.g, c.o, WEIGHT ? 0 : r0, gp, c.g_panels - gp, c.ok0, op, c.o_panels - op, lds);
     if (CE_TWO_PLANES<T, SPLIT>) g.two_planes(a.g_plane, (int)plane_steps);
-    g.first(s0, s1);
-    g.template run<WEIGHT>(s0, s1, acc, sums, asum);
+    const uint32_t classes = WEIGHT ? a.sc->x_classes : a.sc->w_classes;
+    if (classes == 1) {
+        g.first(s0, s1);
+        g.template run<WEIGHT, false>(s0, s1, acc, sums, asum, RowScales{});
+    } else {
+        int at = -1;                                           // the class on whose scale acc is
+        decltype(g)::clear(acc);
+        for (int k = ROW_CLASSES - 1; k >= 0; --k) {
+            if (!(classes >> k & 1)) continue;
+            if (at >= 0) ce_rescale(acc, 16 * (k - at));
+            at = k;
+            g.first(s0, s1);
+            // the row sums of G know no classes: with the first run
+            g.template run<WEIGHT, true>(s0, s1, acc, sums && k == 0, asum,
+                                         RowScales{c.o_exps, WEIGHT ? a.sc->ex : a.sc->ew, k, c.o.perm});
+        }
+    }
     if (sums) {
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
@@ -810,7 +885,7 @@ static CeShape ce_shape(const tnp_vocab_ce *p) {
     return s;
 }
 
-struct CeSaved { CeScalars *sc; float2 *stat; int32_t *tc, *orig; half_t *x, *w; size_t bytes; };
+struct CeSaved { CeScalars *sc; float2 *stat; int32_t *tc, *orig, *xe, *we; half_t *x, *w; size_t bytes; };
 static CeSaved ce_saved(const CeShape &s, void *base) {
     CeSaved v;
     char *p = (char *)base;
@@ -818,6 +893,8 @@ static CeSaved ce_saved(const CeShape &s, void *base) {
     v.stat = (float2 *)p; p += s.Mp * 8;               // Mp and Vp are multiples of 256: every part stays aligned
     v.tc = (int32_t *)p; p += s.Mp * 4;
     v.orig = (int32_t *)p; p += s.Mp * 4;
+    v.xe = (int32_t *)p; p += s.Mp * 4;
+    v.we = (int32_t *)p; p += (size_t)s.Vp * 4;
     v.x = (half_t *)p; p += (size_t)s.Mp * s.panels * 64;
     v.w = (half_t *)p; p += (size_t)s.Vp * s.panels * 64;
     v.bytes = (size_t)(p - (char *)base);
@@ -1009,7 +1086,7 @@ static int ce_pack(const tnp_vocab_ce *p, const CeShape &sh, const CeForward &f,
     const int xb = ce_x_blocks(p->M), wb = sh.Vp / 64 < 2048 ? sh.Vp / 64 : 2048;
     hipLaunchKernelGGL((ce_pack_kernel<T, VX, VW, SPLIT>), dim3(xb + wb), dim3(256), 0, s, (const T *)p->hidden, p->ld_hidden, p->target,
                        (const T *)p->weight, p->ld_weight, sh, f.amax, f.count, f.saved.sc, f.saved.x, f.saved.w,
-                       f.saved.orig, f.saved.tc, xb);
+                       f.saved.orig, f.saved.tc, f.saved.xe, f.saved.we, xb);
     TNP_HIP(hipGetLastError());
     return 0;
 }
@@ -1029,7 +1106,7 @@ static int ce_forward(const tnp_vocab_ce *p, const CeForward &f, float *loss, hi
         CeLogits a = {};
         a.w = GemmOperand{f.saved.w, sh.Vp, 0};
         a.x = GemmOperand{f.saved.x, sh.Mp, 0};
-        a.sc = f.saved.sc; a.tc = f.saved.tc; a.orig = f.saved.orig; a.Mp = sh.Mp; a.V = sh.V; a.v0 = 0; a.steps = sh.panels;
+        a.sc = f.saved.sc; a.tc = f.saved.tc; a.orig = f.saved.orig; a.xe = f.saved.xe; a.we = f.saved.we; a.Mp = sh.Mp; a.V = sh.V; a.v0 = 0; a.steps = sh.panels;
         a.part = f.part; a.tlogit = f.tlogit; a.v_shares = ce_logit_shares(sh, sh.Vp);
         if ((rc = ce_logits<T, SPLIT, false>(a, sh.Vp, ce_big(sh), (const T *)p->bias, s))) return rc;
     }
@@ -1058,7 +1135,7 @@ static int ce_backward(const tnp_vocab_ce *p, const CeBackward &b, const float *
     for (int k = 0; k < b.pieces; ++k) {
         const int v0 = k * b.piece, cols = sh.Vp - v0 < b.piece ? sh.Vp - v0 : b.piece, live = sh.V - v0 < cols ? sh.V - v0 : cols;
         CeLogits a = {};
-        a.w = w; a.x = x; a.sc = sv.sc; a.tc = sv.tc; a.orig = sv.orig; a.Mp = sh.Mp; a.V = sh.V; a.v0 = v0; a.steps = sh.panels;
+        a.w = w; a.x = x; a.sc = sv.sc; a.tc = sv.tc; a.orig = sv.orig; a.xe = sv.xe; a.we = sv.we; a.Mp = sh.Mp; a.V = sh.V; a.v0 = v0; a.steps = sh.panels;
         a.stat = sv.stat; a.grad = p->reduction == 0 ? grad : nullptr; a.gmax = b.gmax; a.g = b.g; a.g_plane = (int64_t)b.piece * sh.Mp; a.v_shares = ce_logit_shares(sh, cols);
         if ((rc = ce_logits<T, SPLIT, true>(a, cols, ce_big(sh), (const T *)p->bias, s))) return rc;
         const bool last = k == b.pieces - 1;
@@ -1069,10 +1146,10 @@ static int ce_backward(const tnp_vocab_ce *p, const CeBackward &b, const float *
         c.zero_blocks = dhidden && k == 0 ? (int)(sh.Mp / 64 < 512 ? sh.Mp / 64 : 512) : 0;
         c.x.g = c.w.g = GemmOperand{b.g, sh.Mp, 0};
         c.x.g_panels = c.w.g_panels = cols / ks; c.x.o_panels = c.w.o_panels = sh.panels;
-        c.x.o = w; c.x.o.perm = 1; c.x.ok0 = v0;
+        c.x.o = w; c.x.o.perm = 1; c.x.ok0 = v0; c.x.o_exps = sv.we + v0;
         c.x.out = dhidden; c.x.part = b.part_x; c.x.part_rows = sh.Mp; c.x.splits = b.splits_x;
         c.x.steps = cols / ks; c.x.add = k > 0;
-        c.w.o = x;
+        c.w.o = x; c.w.o_exps = sv.xe;
         c.w.rows = live; c.w.out0 = v0; c.w.out = dweight; c.w.part = b.part_w; c.w.part_rows = b.piece; c.w.splits = b.splits_w;
         c.part_b = dbias ? b.part_b : nullptr; c.ldb = b.piece;
         rc = b.tile == 256 ? ce_launch_grads<T, SPLIT, 256, 256, 2, 4, 4>(c, s) : ce_launch_grads<T, SPLIT, 128, 128, 2, 2, 4>(c, s);

@@ -29,6 +29,21 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 #define TNP_LDS __attribute__((address_space(3)))
 #define TNP_GLB __attribute__((address_space(1)))
 
+// Rows of an operand that is read as KS (its rows are the k of the product) may lie in memory on scales of their own: row r holds the
+// value times 2^-exps[r].  Rows are taken by CLASSES of sixteen binades, one run of the product each, from the smallest numbers to the
+// largest: a run multiplies the operand, in registers, by 2^(exps[r] - top + 16 class) where the row is of its class and by zero elsewhere,
+// and the accumulator is brought onto the next class's scale in between.  No row's bits are lost to another's size, and an
+// operand whose rows share one scale (class 0 alone, exps == top) needs none of it.
+static constexpr int ROW_CLASSES = 32;
+__device__ __forceinline__ int row_class(int shift) {              // shift <= 0: binades below the top
+    const int c = -shift >> 4;
+    return c < ROW_CLASSES ? c : ROW_CLASSES - 1;
+}
+struct RowScales {
+    const int32_t *exps;     // of the operand's row ok0
+    int top, cls, perm;      // perm: GemmOperand's
+};
+
 struct GemmOperand {
     const half_t *p;     // panel 0, row 0
     int64_t rows;        // rows of a panel (a multiple of 256)
@@ -204,6 +219,24 @@ template <int TM> __device__ __forceinline__ void step_row_sums(const half8 (&fa
                 asum[i] = __builtin_amdgcn_fdot2(half2v{fa[2 * i + w][2 * e], fa[2 * i + w][2 * e + 1]}, one, asum[i], false);
 }
 
+// One step's KS operand times its rows' scales; row: of the step's first k value
+template <bool SPLIT, int NB> __device__ __forceinline__ void step_scale(half8 (&f)[2 * NB], const RowScales &rs, int row, int lane) {
+#pragma unroll
+    for (int w = 0; w < (SPLIT ? 1 : 2); ++w) {
+        half8 sc;
+        const int h = lane >> 5;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int shift = rs.exps[row + 16 * w + (rs.perm ? (e & 3) + 8 * (e >> 2) + 4 * h : 8 * h + e)] - rs.top;
+            sc[e] = row_class(shift) == rs.cls ? (half_t)ldexpf(1.0f, shift + 16 * rs.cls) : (half_t)0.0f;
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int p = 0; p < (SPLIT ? 2 : 1); ++p) f[2 * b + (SPLIT ? p : w)] *= sc;
+    }
+}
+
 // One workgroup's products: init() takes the tile at (row ar, panel ap) of a and (br, bp) of b (al / bl: panels from there to the last,
 // KS), first() starts to fetch its steps [s0, s1), run() accumulates them into acc.  After run() the ring is free: first() of the next
 // tile (a_rows() moves a KC operand a on by whole rows) can be called before this one's results are used, which hides its latency.
@@ -218,6 +251,8 @@ template <int TM> __device__ __forceinline__ void step_row_sums(const half8 (&fa
 //
 // An unsplit a may have a second plane, `plane` elements behind the first: the steps from `wrap` on run over it, with b's steps from the
 // first one again.
+//
+// SCALED: b's rows on scales of their own (RowScales); acc is added to, not set.
 template <bool SPLIT, bool A_KS, bool B_KS, int BM, int BN, int WM, int WN, int NST> struct TileGemm {
     static constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, STAGE = (BM + BN) * 64;
     static constexpr bool TURNS = NW == 8;
@@ -263,14 +298,18 @@ template <bool SPLIT, bool A_KS, bool B_KS, int BM, int BN, int WM, int WN, int 
             stage_barrier<0>();
         }
     }
-    template <bool SUMS> __device__ __forceinline__ void run(int s0, int s1, f32x16 (&acc)[TM][TN], bool sums, float (&asum)[TM]) {
-        const int wm = wave / WN, wn = wave % WN;
+    static __device__ __forceinline__ void clear(f32x16 (&acc)[TM][TN]) {
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
             for (int j = 0; j < TN; ++j)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+    }
+    template <bool SUMS, bool SCALED>
+    __device__ __forceinline__ void run(int s0, int s1, f32x16 (&acc)[TM][TN], bool sums, float (&asum)[TM], const RowScales &rs) {
+        const int wm = wave / WN, wn = wave % WN;
+        if (!SCALED) clear(acc);
         if (s0 >= s1) return;
         landed(s1 - 1 - s0);
         if (TURNS && wave >= 4) stage_barrier_only();
@@ -280,6 +319,7 @@ template <bool SPLIT, bool A_KS, bool B_KS, int BM, int BN, int WM, int WN, int 
             const char *la = lds + cur * STAGE, *lb = la + BM * 64;
             step_frags<SB, B_KS, SPLIT, TN>(lb, wn * TN * 32, lane, fb);
             step_frags<SA, A_KS, SPLIT, TM>(la, wm * TM * 32, lane, fa);
+            if constexpr (SCALED) step_scale<SPLIT, TN>(fb, rs, (s < wrap ? s : s - wrap) * SB::KSTEP, lane);
             if (s + NST - 1 < s1) load(s + NST - 1, cur == 0 ? NST - 1 : cur - 1);   // the buffer that every wave left one barrier ago
             cur = cur + 1 == NST ? 0 : cur + 1;
             if (TURNS) {

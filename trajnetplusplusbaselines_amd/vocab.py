@@ -85,7 +85,7 @@ def saved_bytes(rows, entries, columns, dtype):
     """tnp_vocab_ce_saved_bytes() from the sizes alone (they may be symbolic while a graph is traced)"""
     panels = (columns + 15) // 16 if dtype == torch.float32 else (columns + 31) // 32
     up = lambda n: (n + 255) // 256 * 256
-    return 256 + 16 * up(rows) + 64 * panels * (up(rows) + up(entries))
+    return 256 + 20 * up(rows) + 4 * up(entries) + 64 * panels * (up(rows) + up(entries))
 
 
 def check_cross_entropy(hidden, weight, target, bias, reduction):
@@ -131,9 +131,10 @@ def vocab_cross_entropy(hidden, weight, target, bias=None, reduction='mean'):
     a scalar ('mean' over the rows that are there, 0 if there are none; 'sum') or target's shape ('none').  target < 0: an absent
     row -- its hidden state is not read, its loss and gradient are 0; target >= V: NaN.  Differentiable in hidden, weight and bias.
 
-    fp32 operands are multiplied as two fp16 numbers each, scaled by the largest finite element of their tensor: an element below
-    2^-16 of that one loses relative precision (2^-40 of the largest remains), a row of valid targets that holds an infinity gives
-    NaN.  Gradients: (p - y) times the upstream gradient is rounded to fp16 (fp32 and fp16 operands: two fp16 numbers) on one scale for
+    fp32 operands are multiplied as two fp16 numbers each, scaled by the largest finite element of their tensor or, where all of a row
+    (of hidden or of weight) is below 2^-16 of that one, of their row: no row's result goes by another's size.  Within a row, an element below
+    2^-16 of the row's largest may lose relative precision (2^-23 of the row's largest remains, usually 2^-40).  Rows with a valid
+    target that hold an infinity, and an fp32 weight that holds one, give NaN.  Gradients: (p - y) times the upstream gradient is rounded to fp16 (fp32 and fp16 operands: two fp16 numbers) on one scale for
     all rows; parts below 2^-29 of the largest lose relative precision."""
     if torch.compiler.is_compiling():
         from . import ops  # noqa: F401  (registers the operators)
