@@ -107,3 +107,43 @@ def test_magnitudes_at_the_ends_of_the_types(dtype):
         loss = vocab.vocab_cross_entropy(x, w, t, bias=b, reduction='none')
         zero, bound, _, _ = formula(torch.zeros_like(x), torch.zeros_like(w), b, t, torch.ones(150, device='cuda'))
         _within(loss, zero, bound)
+
+
+# ---- upstream gradients, row by row ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('bad', [float('inf'), float('-inf'), float('nan')])
+def test_an_upstream_gradient_that_is_no_number_stays_with_its_row(dtype, bad):
+    x, w, b, t = _case(200, 90, 24, dtype, 31, absent=0.2)
+    live = torch.nonzero(t >= 0)[:, 0]
+    up = torch.randn(200, device='cuda', generator=_gen(32))
+    up[live[9]] = bad
+    fine = torch.ones(200, dtype=torch.bool, device='cuda')
+    fine[live[9]] = False
+    for others in (1.0, 0.0):
+        u = torch.where(fine, up * others, up)
+        _, _, want, bounds = formula(x, w, b, t, torch.where(fine, u, 0.0))
+        out = vocab.vocab_cross_entropy(x, w, t, bias=b, reduction='none')
+        dx, dw, db = torch.autograd.grad(out, (x, w, b), u)
+        _within(dx[fine], want[0][fine], bounds[0][fine])
+        assert not bool(torch.isfinite(dx[live[9]]).any())
+        assert not bool(torch.isfinite(dw[t[live[9]]]).any()) and not bool(torch.isfinite(db[t[live[9]]]))
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('m,v,d', [(130, 90, 24), (600, 700, 65)])
+def test_upstream_gradients_over_many_magnitudes(dtype, m, v, d):
+    """rows weighted from 1 to 2^-60: each row's gradient keeps its own precision"""
+    x, w, b, t = _case(m, v, d, dtype, 37 + m, absent=0.2)
+    up = torch.randn(m, device='cuda', generator=_gen(38)) * 2.0 ** (-60.0 * torch.rand(m, device='cuda', generator=_gen(39)))
+    if dtype == torch.float16:
+        up = torch.randn(m, device='cuda', generator=_gen(38)) * 2.0 ** (14.0 - 28.0 * torch.rand(m, device='cuda', generator=_gen(39)))
+    _check(x, w, b, t, up)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_magnitudes_of_rows_and_of_upstream_gradients_together(dtype):
+    x, w, b, t = _case(400, 300, 40, dtype, 41, absent=0.1)
+    far = 2.0 ** torch.randint(-40, 1, (400, 1), device='cuda', generator=_gen(42)).double()
+    with torch.no_grad():
+        x.copy_((x.double() * far).to(dtype))
+    _check(x, w, b, t, (torch.randn(400, device='cuda', generator=_gen(43)).double() / far[:, 0] * 2.0 ** -20).float())

@@ -10,7 +10,8 @@
 // [2^14, 2^15); a row whose largest element is below 2^-16 of that gets a power of two of its own (a "far" row), so that no row's bits go by
 // another's size.  bf16 and fp16 values are exact down to 2^-12 of their row's largest, fp32 values become two fp16 numbers (vocab_gemm.h); an error of
 // 2^-23 of the value or of its row's largest, usually 2^-40 of the latter.  Logits of far rows or entries get their powers of two one by one;
-// the gradient products, where rows are summed over, take far rows in classes (vocab_gemm.h), one run each.  G = 2^15 (g_i / max g) (p - y) is rounded to fp16 for bf16 gradients (11 bits, eight times
+// the gradient products, where rows are summed over, take far rows in classes (vocab_gemm.h), one run each.  G = 2^15 (g_i / max g) (p - y),
+// with a power of two per row instead of 1 / max g where the row's upstream gradient is below 2^-18 of the largest, is rounded to fp16 for bf16 gradients (11 bits, eight times
 // finer than what they are rounded to: their error grows by less than a hundredth) and to two fp16 numbers for fp32 and fp16 ones (one of them
 // would be as coarse as the fp16 gradient itself).  All sums, maxima and statistics are fp32; the sum of the losses is fp64.
 //
@@ -49,6 +50,10 @@ struct CeScalars {            // head of the saved area
     uint32_t x_classes, w_classes;      // bit c: rows of class c (vocab_gemm.h) among the hidden states, the weight
 };
 static constexpr int CE_FAR = 16;      // binades below the tensor's largest element from which on a row has its own scale
+struct CeUpstream {           // reduction none, head of the backward pass's workspace
+    float gmax;               // largest finite |grad| of the rows that are there, 1 where that is 0
+    uint32_t classes;         // bit c: rows of class c, by their hidden state's scale and their gradient's together
+};
 __device__ __forceinline__ int ce_padded(int live) { return (live + 255) & ~255; }
 
 struct CeShape {
@@ -265,7 +270,9 @@ struct CeLogits {
     float *tlogit;            // [Mp] target's logit, base 2
     // backward
     const float2 *stat;       // [Mp] (largest logit, base 2; 1 / sum of 2^(l - largest)), padding (+inf, 0), no such target (.., NaN)
-    const float *grad, *gmax; // reduction none: [M], largest |grad|
+    const float *grad;        // reduction none: [M]
+    CeUpstream *up;           // ... what is known of it
+    int32_t *gs;              // ... binades [Mp] by which a row of G lies below the largest gradient's scale
     half_t *g;                // panels of Mp rows, column 0 = vocabulary entry v0
     int64_t g_plane;          // elements from a plane of G to the next
 };
@@ -275,6 +282,18 @@ template <typename T> __device__ __forceinline__ float ce_bias(const T *bias, in
     if (!bias) return 0.0f;
     const float b = to_f32(bias[v]), l = b * CE_LOG2E;
     return fabsf(b) < __builtin_inff() ? fminf(fmaxf(l, -3.402823466e38f), 3.402823466e38f) : l;
+}
+
+// A row's factor of G: 2^15 g / (largest finite g); from 2^-18 of that on 2^14 .. 2^16 with `below` binades to be taken off later, so that the
+// row keeps its bits.  An infinity or a NaN is the row's own.
+__device__ __forceinline__ float ce_row_factor(float g, float gmax, int &below) {
+    if (!(fabsf(g) < __builtin_inff())) return g;
+    const float r = g / gmax;
+    if (g == 0.0f || fabsf(r) >= 0x1p-18f) return 32768.0f * r;
+    int eg, em;
+    const float mg = frexpf(g, &eg), mm = frexpf(gmax, &em);      // mg / mm in (1/2, 2)
+    below = eg - em + 1;
+    return 16384.0f * (mg / mm);
 }
 
 // A workgroup keeps its BN hidden rows and walks over a share of the vocabulary's tiles, the next tile's first steps in flight while it
@@ -310,7 +329,15 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) ce_logits_kernel(CeLogits a, c
         if (BACK) {
             const float2 st = a.stat[row[j]];
             f[j] = tc[j] >= 0 ? 32768.0f : 0.0f;
-            if (a.grad && tc[j] >= 0) f[j] = *a.gmax > 0.0f ? 32768.0f * (a.grad[a.orig[row[j]]] / *a.gmax) : 0.0f;
+            if (a.grad) {
+                int below = 0;
+                if (tc[j] >= 0) f[j] = ce_row_factor(a.grad[a.orig[row[j]]], a.up->gmax, below);
+                if (vs == 0 && wm == 0 && h == 0) {
+                    a.gs[row[j]] = below;
+                    const int shift = a.xe[row[j]] - a.sc->ex + below;
+                    if (shift) atomicOr(&a.up->classes, 1u << row_class(shift));
+                }
+            }
             m[j] = st.x;
             pf[j] = st.y * f[j];                                 // f (p - y) = 2^(l - top) (f / sum) - f y
         }
@@ -672,24 +699,22 @@ template <bool PACKED> __global__ void __launch_bounds__(256) ce_rows_kernel(CeR
     }
 }
 
-// largest |grad| over the rows that are there (reduction none)
-__global__ void __launch_bounds__(1024) ce_gmax_kernel(const float *grad, const int64_t *target, int64_t M, float *gmax) {
+// largest finite |grad| over the rows that are there (reduction none); a row whose gradient is no number keeps that to itself
+__global__ void __launch_bounds__(1024) ce_gmax_kernel(const float *grad, const int64_t *target, int64_t M, CeUpstream *up) {
     __shared__ float sh[16];
     float a = 0.0f;
     for (int64_t i = threadIdx.x; i < M; i += 1024)
         if (target[i] >= 0) {
             const float g = fabsf(grad[i]);
-            a = g > a || g != g ? g : a;                     // NaN stays
+            a = g < __builtin_inff() ? fmaxf(a, g) : a;
         }
-    for (int o = 32; o; o >>= 1) {
-        const float b = __shfl_xor(a, o);
-        a = b > a || b != b ? b : a;
-    }
+    for (int o = 32; o; o >>= 1) a = fmaxf(a, __shfl_xor(a, o));
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = a;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int k = 1; k < 16; ++k) a = sh[k] > a || sh[k] != sh[k] ? sh[k] : a;
-        *gmax = a;
+        for (int k = 1; k < 16; ++k) a = fmaxf(a, sh[k]);
+        up->gmax = a > 0.0f ? a : 1.0f;
+        up->classes = 1;
     }
 }
 
@@ -697,8 +722,8 @@ __global__ void __launch_bounds__(1024) ce_gmax_kernel(const float *grad, const 
 // what takes a sum over G back to the gradient: 2^-15 times the other operand's scale, a power of two, and then max g (in one factor a
 // small max g would lose bits below the smallest normal number)
 struct CeFactor { float two, g; };
-__device__ __forceinline__ CeFactor ce_unscale(const CeScalars *sc, const float *grad, const float *gmax, int reduction, int e) {
-    const float g = reduction == 0 ? *gmax : reduction == 1 ? grad[0] / (float)(sc->live > 0 ? sc->live : 1) : grad[0];
+__device__ __forceinline__ CeFactor ce_unscale(const CeScalars *sc, const float *grad, const CeUpstream *up, int reduction, int e) {
+    const float g = reduction == 0 ? up->gmax : reduction == 1 ? grad[0] / (float)(sc->live > 0 ? sc->live : 1) : grad[0];
     return CeFactor{ldexpf(1.0f, e - 15), g};
 }
 
@@ -717,7 +742,9 @@ struct CeGrad {
 struct CeGrads {
     CeGrad x, w;              // dhidden, dweight
     const CeScalars *sc;
-    const float *grad, *gmax;
+    const float *grad;
+    const CeUpstream *up;     // reduction none, as in CeLogits; gs else NULL
+    const int32_t *gs;
     const int64_t *target;
     const int32_t *orig;      // dhidden: the caller's row of a row that is there
     int64_t M, g_plane;
@@ -725,6 +752,26 @@ struct CeGrads {
     float *part_b;            // dbias: [w.splits][ldb] sums in G's stored column order, or NULL
     int64_t ldb;
 };
+
+// dbias's sums over rows on scales of their own, from memory: asum[i] += what this lane's half of the rows of steps [s0, s1) adds to G's
+// column col + 32 i + (lane & 31)
+template <bool SPLIT, int TM>
+__device__ __forceinline__ void ce_row_sums(const CeGrads &a, const CeGrad &c, int64_t col, int s0, int s1, int plane_steps, float (&asum)[TM], int lane) {
+    constexpr int PC = SPLIT ? 16 : 32;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        const int64_t v = col + i * 32 + (lane & 31);
+        const half_t *g = c.g.p + v / PC * c.g.rows * 32 + v % PC;
+        for (int s = s0; s < s1; ++s) {
+            const bool second = s >= plane_steps;
+            const int k0 = (second ? s - plane_steps : s) * PC;
+            for (int k = k0 + (lane >> 5); k < k0 + PC; k += 2) {
+                const half_t *at = g + (second ? a.g_plane : 0) + (int64_t)k * 32;
+                asum[i] += ldexpf(SPLIT ? (float)at[0] + (float)at[16] : (float)at[0], a.gs ? a.gs[k] : 0);
+            }
+        }
+    }
+}
 
 template <int TM, int TN> __device__ __forceinline__ void ce_rescale(f32x16 (&acc)[TM][TN], int by) {
 #pragma unroll
@@ -761,11 +808,12 @@ __device__ __forceinline__ void ce_grad_tile(const CeGrads &a, const CeGrad &c, 
     TileGemm<SPLIT, WEIGHT, true, BM, BN, WM, WN, NST> g;
     g.init(c.g, c.o, WEIGHT ? 0 : r0, gp, c.g_panels - gp, c.ok0, op, c.o_panels - op, lds);
     if (CE_TWO_PLANES<T, SPLIT>) g.two_planes(a.g_plane, (int)plane_steps);
-    const uint32_t classes = WEIGHT ? a.sc->x_classes : a.sc->w_classes;
+    const uint32_t classes = !WEIGHT ? a.sc->w_classes : a.gs ? a.up->classes : a.sc->x_classes;
     if (classes == 1) {
         g.first(s0, s1);
         g.template run<WEIGHT, false>(s0, s1, acc, sums, asum, RowScales{});
     } else {
+        if (sums) ce_row_sums<SPLIT, TM>(a, c, r0 + wm * TM * 32, s0, s1, (int)plane_steps, asum, lane);
         int at = -1;                                           // the class on whose scale acc is
         decltype(g)::clear(acc);
         for (int k = ROW_CLASSES - 1; k >= 0; --k) {
@@ -773,9 +821,8 @@ __device__ __forceinline__ void ce_grad_tile(const CeGrads &a, const CeGrad &c, 
             if (at >= 0) ce_rescale(acc, 16 * (k - at));
             at = k;
             g.first(s0, s1);
-            // the row sums of G know no classes: with the first run
-            g.template run<WEIGHT, true>(s0, s1, acc, sums && k == 0, asum,
-                                         RowScales{c.o_exps, WEIGHT ? a.sc->ex : a.sc->ew, k, c.o.perm});
+            g.template run<false, true>(s0, s1, acc, false, asum,
+                                         RowScales{c.o_exps, WEIGHT ? a.gs : nullptr, WEIGHT ? a.sc->ex : a.sc->ew, k, c.o.perm});
         }
     }
     if (sums) {
@@ -786,7 +833,7 @@ __device__ __forceinline__ void ce_grad_tile(const CeGrads &a, const CeGrad &c, 
         }
     }
     if (!c.out) return;                                        // only dbias is asked for
-    const CeFactor f = ce_unscale(a.sc, a.grad, a.gmax, a.reduction, WEIGHT ? a.sc->ex : a.sc->ew);
+    const CeFactor f = ce_unscale(a.sc, a.grad, a.up, a.reduction, WEIGHT ? a.sc->ex : a.sc->ew);
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -796,6 +843,7 @@ __device__ __forceinline__ void ce_grad_tile(const CeGrads &a, const CeGrad &c, 
             const int64_t row = r0 + wm * TM * 32 + i * 32 + loc;
             if (row >= rows) continue;
             const int64_t to = WEIGHT ? c.out0 + row : c.part ? 0 : a.orig[row];
+            const int below = !WEIGHT && a.gs ? a.gs[row] : 0;
 #pragma unroll
             for (int j = 0; j < TN; ++j) {
                 const int d = d0 + wn * TN * 32 + j * 32 + (lane & 31);
@@ -805,7 +853,7 @@ __device__ __forceinline__ void ce_grad_tile(const CeGrads &a, const CeGrad &c, 
                     float *p = c.part + ((int64_t)z * c.part_rows + row) * a.D + d;
                     *p = c.add ? *p + v : v;
                 } else {
-                    ((T *)c.out)[to * a.D + d] = from_f32<T>(v * f.two * f.g);
+                    ((T *)c.out)[to * a.D + d] = from_f32<T>(ldexpf(v * f.two * f.g, below));
                 }
             }
         }
@@ -833,7 +881,7 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) ce_grads_kernel(CeGrads a) {
 template <typename T, int VE>
 __device__ __forceinline__ void ce_join(const CeGrads &a, const CeGrad &c, bool weight, int bid, int blocks) {
     const int64_t n = (weight ? c.rows : (int64_t)a.sc->live) * a.D, stride = c.part_rows * a.D;
-    const CeFactor f = ce_unscale(a.sc, a.grad, a.gmax, a.reduction, weight ? a.sc->ex : a.sc->ew);
+    const CeFactor f = ce_unscale(a.sc, a.grad, a.up, a.reduction, weight ? a.sc->ex : a.sc->ew);
     for (int64_t k = ((int64_t)bid * 256 + threadIdx.x) * VE; k < n; k += (int64_t)blocks * 256 * VE) {
         const int64_t row = k / a.D;
         float v[VE];
@@ -851,9 +899,10 @@ __device__ __forceinline__ void ce_join(const CeGrads &a, const CeGrad &c, bool 
 #pragma unroll
                     for (int e = 0; e < VE; ++e) v[e] += p[u].v[e];
         }
+        const int below = !weight && a.gs ? a.gs[row] : 0;
         T *out = (T *)c.out + (weight ? c.out0 + row : (int64_t)a.orig[row]) * a.D + (k - row * a.D);
 #pragma unroll
-        for (int e = 0; e < VE; ++e) out[e] = from_f32<T>(v[e] * f.two * f.g);
+        for (int e = 0; e < VE; ++e) out[e] = from_f32<T>(ldexpf(v[e] * f.two * f.g, below));
     }
 }
 
@@ -868,7 +917,7 @@ __global__ void __launch_bounds__(256) ce_join_kernel(CeGrads a, int bx, int bw,
     const int pos = (v & ~12) | ((v & 4) << 1) | ((v & 8) >> 1);
     float s = 0.0f;
     for (int k = 0; k < a.w.splits; ++k) s += a.part_b[k * a.ldb + pos];
-    const CeFactor f = ce_unscale(a.sc, a.grad, a.gmax, a.reduction, 0);
+    const CeFactor f = ce_unscale(a.sc, a.grad, a.up, a.reduction, 0);
     dbias[v] = from_f32<T>(s * f.two * f.g);
 }
 
@@ -959,7 +1008,9 @@ struct CeBackward {
     int64_t ldg;
     half_t *g;
     int tile, splits_x, splits_w;
-    float *gmax, *part_x, *part_w, *part_b;
+    CeUpstream *up;
+    int32_t *gs;
+    float *part_x, *part_w, *part_b;
     size_t bytes;
 };
 static constexpr size_t CE_PIECE_BYTES = (size_t)1 << 30;      // of 288 GB; 16384 x 65536 x 1024 bf16 backward 7.59 ms with 256 MB, 6.42 with 512, 6.32, 6.27 with 2 GB
@@ -987,7 +1038,9 @@ static CeBackward ce_backward_layout(const tnp_vocab_ce *p, void *ws) {
     b.splits_x = (int)(nx < 1 ? 1 : nx);
     b.splits_w = (int)(nw < 1 ? 1 : nw);
     char *w = (char *)ws;
-    b.gmax = (float *)w; w += 256;
+    b.up = (CeUpstream *)w; w += 256;
+    b.gs = p->reduction == 0 ? (int32_t *)w : nullptr;
+    if (b.gs) w += ce_up((size_t)s.Mp * 4);
     b.g = (half_t *)w; w += ce_up((size_t)s.Mp * b.ldg * 2);
     b.part_x = b.splits_x > 1 || b.pieces > 1 ? (float *)w : nullptr;
     if (b.part_x) w += ce_up((size_t)b.splits_x * s.Mp * p->D * 4);
@@ -1128,7 +1181,7 @@ static int ce_backward(const tnp_vocab_ce *p, const CeBackward &b, const float *
     const CeSaved sv = ce_saved(sh, p->saved);
     int rc;
     if (p->reduction == 0) {
-        hipLaunchKernelGGL(ce_gmax_kernel, dim3(1), dim3(1024), 0, s, grad, p->target, p->M, b.gmax);
+        hipLaunchKernelGGL(ce_gmax_kernel, dim3(1), dim3(1024), 0, s, grad, p->target, p->M, b.up);
         TNP_HIP(hipGetLastError());
     }
     const GemmOperand w{sv.w, sh.Vp, 0}, x{sv.x, sh.Mp, 0};
@@ -1136,13 +1189,13 @@ static int ce_backward(const tnp_vocab_ce *p, const CeBackward &b, const float *
         const int v0 = k * b.piece, cols = sh.Vp - v0 < b.piece ? sh.Vp - v0 : b.piece, live = sh.V - v0 < cols ? sh.V - v0 : cols;
         CeLogits a = {};
         a.w = w; a.x = x; a.sc = sv.sc; a.tc = sv.tc; a.orig = sv.orig; a.xe = sv.xe; a.we = sv.we; a.Mp = sh.Mp; a.V = sh.V; a.v0 = v0; a.steps = sh.panels;
-        a.stat = sv.stat; a.grad = p->reduction == 0 ? grad : nullptr; a.gmax = b.gmax; a.g = b.g; a.g_plane = (int64_t)b.piece * sh.Mp; a.v_shares = ce_logit_shares(sh, cols);
+        a.stat = sv.stat; a.grad = p->reduction == 0 ? grad : nullptr; a.up = b.up; a.gs = b.gs; a.g = b.g; a.g_plane = (int64_t)b.piece * sh.Mp; a.v_shares = ce_logit_shares(sh, cols);
         if ((rc = ce_logits<T, SPLIT, true>(a, cols, ce_big(sh), (const T *)p->bias, s))) return rc;
         const bool last = k == b.pieces - 1;
         const int ks = SPLIT ? 16 : 32;
         CeGrads c = {};
         c.g_plane = (int64_t)b.piece * sh.Mp;
-        c.sc = sv.sc; c.grad = grad; c.gmax = b.gmax; c.target = p->target; c.orig = sv.orig; c.M = sh.M; c.reduction = p->reduction; c.D = sh.D;
+        c.sc = sv.sc; c.grad = grad; c.up = b.up; c.gs = b.gs; c.target = p->target; c.orig = sv.orig; c.M = sh.M; c.reduction = p->reduction; c.D = sh.D;
         c.zero_blocks = dhidden && k == 0 ? (int)(sh.Mp / 64 < 512 ? sh.Mp / 64 : 512) : 0;
         c.x.g = c.w.g = GemmOperand{b.g, sh.Mp, 0};
         c.x.g_panels = c.w.g_panels = cols / ks; c.x.o_panels = c.w.o_panels = sh.panels;

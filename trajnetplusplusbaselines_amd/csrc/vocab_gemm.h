@@ -41,6 +41,7 @@ __device__ __forceinline__ int row_class(int shift) {              // shift <= 0
 }
 struct RowScales {
     const int32_t *exps;     // of the operand's row ok0
+    const int32_t *other;    // binades (<= 0) that a's columns of these rows are to be taken by as well, or NULL
     int top, cls, perm;      // perm: GemmOperand's
 };
 
@@ -223,11 +224,13 @@ template <int TM> __device__ __forceinline__ void step_row_sums(const half8 (&fa
 template <bool SPLIT, int NB> __device__ __forceinline__ void step_scale(half8 (&f)[2 * NB], const RowScales &rs, int row, int lane) {
 #pragma unroll
     for (int w = 0; w < (SPLIT ? 1 : 2); ++w) {
+        __builtin_amdgcn_sched_barrier(0);                           // eight scales at a time: more of them spill registers
         half8 sc;
         const int h = lane >> 5;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const int shift = rs.exps[row + 16 * w + (rs.perm ? (e & 3) + 8 * (e >> 2) + 4 * h : 8 * h + e)] - rs.top;
+            const int r = row + 16 * w + (rs.perm ? (e & 3) + 8 * (e >> 2) + 4 * h : 8 * h + e);
+            const int shift = rs.exps[r] - rs.top + (rs.other ? rs.other[r] : 0);
             sc[e] = row_class(shift) == rs.cls ? (half_t)ldexpf(1.0f, shift + 16 * rs.cls) : (half_t)0.0f;
         }
 #pragma unroll
