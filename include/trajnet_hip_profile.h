@@ -56,6 +56,17 @@ TNP_API int tnp_profile_end(void);
  * ----------------------------------------------------------------------------------------- */
 TNP_API int tnp_tuning_set(const char *key, long value);
 
+/* -------------------------------------------------------------------------------------------
+ * What the vocabulary cross entropy chooses for these sizes and this dtype (tests hold a case to the kernels it is meant for).
+ * TNP_VOCAB_LOGIT_TILE: rows and columns of a tile of logits, 128 or 256; 0: scored from the inputs in place (`saved` NULL and few rows).
+ * TNP_VOCAB_GRAD_TILE: of a tile of the gradient products.  TNP_VOCAB_PIECES: pieces of the vocabulary that the backward pass takes.
+ * -1: arguments that the entries refuse, or an unknown `which`.
+ * ----------------------------------------------------------------------------------------- */
+#define TNP_VOCAB_LOGIT_TILE 0
+#define TNP_VOCAB_GRAD_TILE  1
+#define TNP_VOCAB_PIECES     2
+TNP_API int tnp_vocab_ce_plan(const tnp_vocab_ce *args, int which);
+
 #ifdef __cplusplus
 }
 #endif

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from tests.test_gpu_vocab import _case, _gen, _within
-from tests.vocab_formula import formula
+from tests.vocab_formula import LARGE, formula, plan
 from trajnetplusplusbaselines_amd import vocab
 
 pytestmark = pytest.mark.gpu
@@ -147,3 +147,79 @@ def test_magnitudes_of_rows_and_of_upstream_gradients_together(dtype):
     with torch.no_grad():
         x.copy_((x.double() * far).to(dtype))
     _check(x, w, b, t, (torch.randn(400, device='cuda', generator=_gen(43)).double() / far[:, 0] * 2.0 ** -20).float())
+
+
+# ---- tiles of 256 ------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('reduction', ['mean', 'none'])
+@pytest.mark.parametrize('m,v,d,dtype,pieces', LARGE)
+def test_large_tiles_with_absent_rows(m, v, d, dtype, pieces, reduction):
+    assert plan(m, v, d, dtype) == (256, 256, pieces)
+    x, w, b, t = _case(m, v, d, dtype, 51, absent=0.2)
+    n = int((t >= 0).sum())
+    if reduction == 'none':
+        _check(x, w, b, t, torch.randn(m, device='cuda', generator=_gen(52)))
+        return
+    loss, bound, want, bounds = formula(x, w, b, t, torch.full((m,), 1.0 / n, dtype=torch.float64, device='cuda'))
+    out = vocab.vocab_cross_entropy(x, w, t, bias=b)
+    _within(out.detach(), loss.sum() / n, (bound.sum() + 2.0 ** -23 * loss.sum()) / n)
+    got = torch.autograd.grad(out, (x, w, b))
+    for a, e, lim in zip(got, want, bounds):
+        _within(a, e, lim)
+    again = torch.autograd.grad(vocab.vocab_cross_entropy(x, w, t, bias=b), (x, w, b))
+    assert all(torch.equal(p, q) for p, q in zip(got, again))
+    with torch.no_grad():
+        _within(vocab.vocab_cross_entropy(x, w, t, bias=b, reduction='none'), loss, bound)
+
+
+@pytest.mark.parametrize('m,v,d,dtype,pieces', LARGE)
+def test_large_tiles_with_rows_of_other_magnitudes(m, v, d, dtype, pieces):
+    x, w, b, t = _case(m, v, d, dtype, 53, absent=0.1)
+    live = torch.nonzero(t >= 0)[:, 0]
+    if dtype == torch.float16:
+        _scaled(x, slice(None), 2.0 ** -13)
+        _scaled(w, slice(None), 2.0 ** 12)
+        _scaled(x, live[[3, 2000]], 2.0 ** 25)
+    else:
+        _scaled(x, live[[3, 2000, 3001]], 2.0 ** 40)
+        _scaled(x, live[[4]], 2.0 ** 20)
+        _scaled(w, [v // 3, v - 1], 2.0 ** -30)
+        hit = v // 2
+        t[t == hit] = 0
+        _scaled(w, [hit], 2.0 ** 30)
+        with torch.no_grad():
+            b[hit] = float('-inf')
+    up = torch.randn(m, device='cuda', generator=_gen(54))
+    up[live[::7]] *= 2.0 ** -30
+    _check(x, w, b, t, up)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_large_tiles_captured_and_replayed(dtype):
+    """the step's bits on new inputs, with eager work between the replays; the second inputs have rows of other magnitudes"""
+    m, v, d = (6000, 12001, 264) if dtype == torch.float32 else (6000, 12001, 500)
+    cases = [_case(m, v, d, dtype, 60 + k, absent=0.2) for k in range(2)]
+    _scaled(cases[1][0], torch.nonzero(cases[1][3] >= 0)[:, 0][[5]], 2.0 ** 40)
+
+    def step(x, w, b, t):
+        loss = vocab.vocab_cross_entropy(x, w, t, bias=b)
+        return [loss] + list(torch.autograd.grad(loss, (x, w, b)))
+
+    bufs = [z.detach().clone().requires_grad_(i < 3) for i, z in enumerate(cases[0])]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*bufs)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(*bufs)
+    for k in (1, 0, 1):
+        with torch.no_grad():
+            for buf, src in zip(bufs, cases[k]):
+                buf.copy_(src)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [h.detach().clone() for h in held]
+        want = step(*[z.detach().clone().requires_grad_(i < 3) for i, z in enumerate(cases[k])])
+        assert all(torch.equal(p, q.detach()) for p, q in zip(got, want))

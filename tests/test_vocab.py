@@ -128,3 +128,15 @@ def test_fake_implementations():
         loss, saved = torch.ops.trajnet.vocab_cross_entropy(out, w, tok, None, 'mean')
         assert loss.shape == () and loss.dtype == torch.float32 and saved.dtype == torch.uint8
         assert torch.ops.trajnet.vocab_cross_entropy(out, w, tok, torch.empty(30, dtype=torch.bfloat16), 'none')[0].shape == (5, 7)
+
+
+def test_the_plans_that_the_gpu_tests_are_written_for():
+    """a threshold that moves a case to other kernels shows here"""
+    from tests.vocab_formula import LARGE, plan
+    for m, v, d, dtype, pieces in LARGE:
+        assert plan(m, v, d, dtype) == (256, 256, pieces)
+    assert plan(300, 700, 65, torch.float32) == (128, 128, 1)
+    assert plan(64, 700, 65, torch.float32, train=False)[0] == 0 and plan(65, 700, 65, torch.float32, train=False)[0] == 128
+    assert plan(4000, 8200, 72, torch.bfloat16) == (128, 128, 1)
+    assert plan(20000, 34000, 40, torch.bfloat16)[2] == 2
+    assert plan(0, 0, 0, torch.float32) == (-1, -1, -1)

@@ -9,7 +9,11 @@ X_i is the largest element of a row of hidden states (or of the weight), X the l
    and sums) stands on both sides of the quotient: p (e^E - 1).  An entry so far below the row's largest that its p is 0 whatever the error,
    and a largest entry so far above all others that its p is 1, have no error of that kind.
 """
+import ctypes
+
 import torch
+
+from trajnetplusplusbaselines_amd import _lib
 
 
 def u(dtype):
@@ -71,3 +75,22 @@ def formula(x, w, b, t, grad_rows, extra=0.0):
     bounds = (near(want[0], dG, Ga, wa, wb, v), near(want[1], dG.t(), Ga.t(), xa, xb, m),
               near(want[2][:, None], dG.t(), Ga.t(), one, 0.0 * one, m)[:, 0])
     return loss, loss_bound, want, bounds
+
+
+class VocabCe(ctypes.Structure):
+    """struct tnp_vocab_ce of include/trajnet_hip.h"""
+    _fields_ = [('dtype', ctypes.c_int32), ('reduction', ctypes.c_int32), ('M', ctypes.c_int64), ('V', ctypes.c_int32),
+                ('D', ctypes.c_int32), ('hidden', ctypes.c_void_p), ('ld_hidden', ctypes.c_int64), ('weight', ctypes.c_void_p),
+                ('ld_weight', ctypes.c_int64), ('bias', ctypes.c_void_p), ('target', ctypes.c_void_p), ('saved', ctypes.c_void_p)]
+
+
+def plan(m, v, d, dtype, train=True):
+    """(tile of the logits, tile of the gradient products, pieces of the vocabulary) that the library chooses"""
+    a = VocabCe(dtype=(torch.float32, torch.bfloat16, torch.float16).index(dtype), M=m, V=v, D=d, ld_hidden=d, ld_weight=d,
+                saved=1 << 20 if train else None)
+    return tuple(_lib.lib().tnp_vocab_ce_plan(ctypes.byref(a), which) for which in range(3))
+
+
+# cases of the 256 x 256 tiles (eight waves): rows, entries and columns that fill no tile; the last in several pieces
+LARGE = [(6000, 12001, 264, torch.float32, 1), (6000, 12001, 500, torch.bfloat16, 1), (6000, 12001, 264, torch.float16, 1),
+         (20001, 14003, 150, torch.float32, 2)]

@@ -207,6 +207,7 @@ def lib():
     L.tnp_vocab_ce_saved_bytes.argtypes = [_fp]
     L.tnp_vocab_ce_workspace_bytes.restype = ctypes.c_size_t
     L.tnp_vocab_ce_workspace_bytes.argtypes = [_fp, ctypes.c_int]
+    L.tnp_vocab_ce_plan.argtypes = [_fp, ctypes.c_int]
     L.tnp_vocab_ce_forward.argtypes = [_fp, _fp, _fp, ctypes.c_size_t, _fp]
     L.tnp_vocab_ce_backward.argtypes = [_fp, _fp, _fp, _fp, _fp, _fp, ctypes.c_size_t, _fp]
     if L.tnp_abi_version() != ABI_VERSION:

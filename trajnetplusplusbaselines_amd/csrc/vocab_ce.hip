@@ -20,6 +20,7 @@
 // where only some are predicted); their number stays on the device, launches are sized for all rows and the workgroups behind the
 // last row end at once.  A target >= V is an error that shows: NaN loss, NaN gradients.
 #include "vocab_gemm.h"
+#include "../../include/trajnet_hip_profile.h"
 
 #include <math.h>
 
@@ -1233,6 +1234,14 @@ extern "C" TNP_API size_t tnp_vocab_ce_saved_bytes(const tnp_vocab_ce *args) {
 extern "C" TNP_API size_t tnp_vocab_ce_workspace_bytes(const tnp_vocab_ce *args, int backward) {
     if (ce_check(args, "tnp_vocab_ce_workspace_bytes")) return 0;
     return backward ? ce_backward_layout(args, nullptr).bytes : ce_forward_layout(args, nullptr).bytes;
+}
+
+extern "C" TNP_API int tnp_vocab_ce_plan(const tnp_vocab_ce *args, int which) {
+    if (ce_check(args, "tnp_vocab_ce_plan")) return -1;
+    if (which == TNP_VOCAB_LOGIT_TILE) return ce_scores(args) ? 0 : ce_big(ce_shape(args)) ? 256 : 128;
+    if (which == TNP_VOCAB_GRAD_TILE) return ce_backward_layout(args, nullptr).tile;
+    if (which == TNP_VOCAB_PIECES) return ce_backward_layout(args, nullptr).pieces;
+    TNP_FAIL(-1, "tnp_vocab_ce_plan: unknown question %d", which);
 }
 
 extern "C" TNP_API int tnp_vocab_ce_forward(const tnp_vocab_ce *args, float *loss, void *workspace, size_t workspace_bytes, void *stream) {
