@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from tests.test_gpu_vocab import _case, _gen, _within
-from tests.vocab_formula import LARGE, formula, plan
+from tests.vocab_formula import LARGE, far_biases, formula, plan
 from trajnetplusplusbaselines_amd import vocab
 
 pytestmark = pytest.mark.gpu
@@ -223,3 +223,30 @@ def test_large_tiles_captured_and_replayed(dtype):
         got = [h.detach().clone() for h in held]
         want = step(*[z.detach().clone().requires_grad_(i < 3) for i, z in enumerate(cases[k])])
         assert all(torch.equal(p, q.detach()) for p, q in zip(got, want))
+
+
+# ---- the normaliser at large logits ------------------------------------------------------------------------------------------
+def offset_case(size, entries, device):
+    """logits around ``size`` that are exact in base 2 but for 2^-20 (tests/vocab_formula.py: far_biases): they are biases alone,
+    hidden states and weight meet in zeros"""
+    g = torch.Generator().manual_seed(7)
+    shift, far = far_biases(size)
+    m, v, d = 20, entries, 16
+    x, w = torch.rand(m, d, generator=g) * 2 - 1, torch.randn(v, d, generator=g)
+    x[:, :8] = 0.0
+    w[:, 8:] = 0.0
+    b = far[torch.randint(far.numel(), (v,), generator=g)]
+    t = torch.randint(v, (m,), generator=g)
+    leaf = lambda z: z.to(device).requires_grad_()
+    return leaf(x), leaf(w), leaf(b), t.to(device), shift
+
+
+@pytest.mark.parametrize('entries', [32, 36, 42, 58])
+def test_the_normaliser_keeps_its_precision_at_large_logits(entries):
+    """what one rounded log-sum-exp would lose (test_vocab.py shows that its gradients are out of these bounds) is kept"""
+    x, w, b, t, shift = offset_case(1e4, entries, 'cuda')
+    up = torch.ones(20, device='cuda')
+    _, _, want, bounds = formula(x, w, b.detach().double() - shift, t, up, extra=2.0 ** -19)
+    out = vocab.vocab_cross_entropy(x, w, t, bias=b, reduction='none')
+    for a, e, lim in zip(torch.autograd.grad(out, (x, w, b), up), want, bounds):
+        _within(a, e, lim)

@@ -140,3 +140,22 @@ def test_the_plans_that_the_gpu_tests_are_written_for():
     assert plan(4000, 8200, 72, torch.bfloat16) == (128, 128, 1)
     assert plan(20000, 34000, 40, torch.bfloat16)[2] == 2
     assert plan(0, 0, 0, torch.float32) == (-1, -1, -1)
+
+
+@pytest.mark.parametrize('entries', [32, 36, 42, 58])
+def test_one_rounded_log_sum_exp_is_out_of_the_bounds_of_large_logits(entries):
+    """the check of the normaliser's precision on the GPU tells the two forms apart: exp(l - top) / sum, formed here in fp32, is inside
+    its bounds, exp(l - lse) with lse rounded to fp32 is not"""
+    from tests.test_gpu_vocab_range import offset_case
+    from tests.vocab_formula import formula
+    x, w, b, t, shift = offset_case(1e4, entries, 'cpu')
+    _, _, want, bounds = formula(x, w, b.detach().double() - shift, t, torch.ones(20), extra=2.0 ** -19)
+    l = (b.detach() * torch.tensor(1.4426950408889634, dtype=torch.float32)).expand(20, entries)
+    top = l.max(1, keepdim=True).values
+    e = torch.exp2(l - top)
+    total = e.sum(1, keepdim=True)
+    for p, inside in ((e / total, True), (torch.exp2(l - (top + torch.log2(total))), False)):
+        G = p.double().scatter_add(1, t[:, None], torch.full((20, 1), -1.0, dtype=torch.float64))
+        got = (G @ w.detach().double(), G.t() @ x.detach().double(), G.sum(0))
+        off = [float(((a - c).abs() / lim).max()) for a, c, lim in zip(got, want, bounds)]
+        assert (max(off) < 1.0) == inside and (inside or min(off) > 1.0), off

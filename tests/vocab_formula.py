@@ -77,6 +77,18 @@ def formula(x, w, b, t, grad_rows, extra=0.0):
     return loss, loss_bound, want, bounds
 
 
+def far_biases(size):
+    """(shift, biases): fp32 numbers around ``size`` whose base-2 forms, as the kernels round them, keep the biases' differences to 2^-20:
+    a common offset of that size then costs nothing but what the normaliser loses"""
+    ulp = float(torch.finfo(torch.float32).eps) * 2.0 ** torch.floor(torch.log2(torch.tensor(size))).item()
+    b = (size + torch.arange(-4000, 4001, dtype=torch.float64) * ulp).float()
+    log2e = torch.tensor(1.4426950408889634, dtype=torch.float32)
+    off = (b * log2e).double() - b.double() * 1.4426950408889634
+    middle = off[4000]
+    keep = b[(off - middle).abs() < 2.0 ** -20]
+    return size, keep
+
+
 class VocabCe(ctypes.Structure):
     """struct tnp_vocab_ce of include/trajnet_hip.h"""
     _fields_ = [('dtype', ctypes.c_int32), ('reduction', ctypes.c_int32), ('M', ctypes.c_int64), ('V', ctypes.c_int32),
