@@ -159,3 +159,16 @@ def test_one_rounded_log_sum_exp_is_out_of_the_bounds_of_large_logits(entries):
         got = (G @ w.detach().double(), G.t() @ x.detach().double(), G.sum(0))
         off = [float(((a - c).abs() / lim).max()) for a, c, lim in zip(got, want, bounds)]
         assert (max(off) < 1.0) == inside and (inside or min(off) > 1.0), off
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+def test_what_is_held_of_the_logits_at_a_time(dtype):
+    """a piece of the vocabulary: 1 GB, or 256 entries of all rows where that is more"""
+    from tests.vocab_formula import plan
+    each = 2 if dtype == torch.bfloat16 else 4
+    for m, v in ((1, 1 << 23), (300, 70000), (16384, 65536), (100001, 50021), (1 << 20, 3000), (1 << 23, 5), (1 << 23, 1000)):
+        up = lambda n: (n + 255) // 256 * 256
+        pieces = plan(m, v, 64, dtype)[2]
+        piece = up(-(-up(v) // pieces))
+        assert up(m) * piece * each <= max(1 << 30, up(m) * 256 * each)
+        assert (pieces - 1) * piece < up(v) <= pieces * piece
