@@ -1,6 +1,8 @@
 """Build libtrajnet_hip.so (gfx950) in-tree with hipcc.  No torch dependency: the library is a plain
-C-ABI shared object (include/trajnet_hip.h); hipcc cross-compiles without a GPU.  Beside it _trajnet_torch.so, host code that
-makes autograd nodes of two of its operators."""
+C-ABI shared object (include/trajnet_hip.h); hipcc cross-compiles without a GPU.
+
+Beside it, where a torch for ROCm is installed, _trajnet_torch.so: host code that makes autograd nodes of two of the library's operators
+(vocab.py).  The library is linked first and does not depend on it."""
 import importlib.util
 import os
 import subprocess
@@ -31,18 +33,30 @@ def hipcc():
     return 'hipcc'
 
 
+def torch_folder():
+    """folder of an installed torch for ROCm, or None"""
+    spec = importlib.util.find_spec('torch')
+    folder = spec.submodule_search_locations[0] if spec and spec.submodule_search_locations else None
+    return folder if folder and os.path.exists(os.path.join(folder, 'lib', 'libc10_hip.so')) else None
+
+
 def needs_build():
-    if not (os.path.exists(OUT) and os.path.exists(TORCH_OUT)):
+    outs = [OUT] + ([TORCH_OUT] if torch_folder() else [])
+    if not all(os.path.exists(o) for o in outs):
         return True
-    t = min(os.path.getmtime(OUT), os.path.getmtime(TORCH_OUT))
+    t = min(os.path.getmtime(o) for o in outs)
     deps = [os.path.join(HERE, f) for f in SOURCES + HEADERS + [TORCH_SOURCE]] + [os.path.abspath(__file__)]
     return any(os.path.exists(d) and os.path.getmtime(d) > t for d in deps)
 
 
 def torch_command():
-    torch = importlib.util.find_spec('torch').submodule_search_locations[0]
+    """None where there is no torch for ROCm"""
+    torch = torch_folder()
+    if torch is None:
+        return None
     inc = [os.path.join(torch, 'include'), os.path.join(torch, 'include', 'torch', 'csrc', 'api', 'include'), sysconfig.get_paths()['include']]
-    return [hipcc(), '-std=c++17', '-O2', '-fPIC', '-shared', '-fvisibility=hidden', '-w'] + ['-I' + i for i in inc] + [
+    # warnings of this file, not of torch's headers
+    return [hipcc(), '-std=c++17', '-O2', '-fPIC', '-shared', '-fvisibility=hidden', '-Wall'] + [a for i in inc for a in ('-isystem', i)] + [
         os.path.join(HERE, TORCH_SOURCE), '-o', TORCH_OUT, '-L' + os.path.join(torch, 'lib'), '-ltorch_python', '-ltorch_cpu', '-lc10', '-lc10_hip']
 
 
@@ -65,17 +79,20 @@ def build(force=False, verbose=False):
             print(' '.join(cmd))
         cmds.append(cmd)
         objs.append(obj)
-    cmds.append(torch_command())
+    torch_cmd = torch_command()
     if verbose:
-        print(' '.join(cmds[-1]))
+        print(' '.join(torch_cmd) if torch_cmd else 'no torch for ROCm: %s is not built' % TORCH_OUT)
     # translation units are independent: compile them side by side
     from concurrent.futures import ThreadPoolExecutor
-    with ThreadPoolExecutor(max_workers=min(len(cmds), os.cpu_count() or 4)) as pool:
+    with ThreadPoolExecutor(max_workers=min(len(cmds) + 1, os.cpu_count() or 4)) as pool:
+        beside = pool.submit(subprocess.check_call, torch_cmd) if torch_cmd else None
         list(pool.map(subprocess.check_call, cmds))
-    cmd = [hipcc(), '--offload-arch=gfx950', '-shared', '-fPIC', '-o', OUT] + objs
-    if verbose:
-        print(' '.join(cmd))
-    subprocess.check_call(cmd)
+        cmd = [hipcc(), '--offload-arch=gfx950', '-shared', '-fPIC', '-o', OUT] + objs
+        if verbose:
+            print(' '.join(cmd))
+        subprocess.check_call(cmd)
+    if beside:
+        beside.result()                  # raises what the torch file's compiler said, the library being there
     return OUT
 
 
