@@ -109,6 +109,32 @@ def test_magnitudes_at_the_ends_of_the_types(dtype):
         _within(loss, zero, bound)
 
 
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_infinite_weights_and_hidden_states_follow_the_formula(dtype):
+    x, w, b, t = _case(150, 80, 40, dtype, 47, absent=0.1)
+    with torch.no_grad():
+        x[:, 5].abs_()                                  # nowhere zero: tanh of a normal number
+        w[11, 5] = float('-inf')                        # -inf logits everywhere: the entry is masked
+        x[t < 0] = float('nan')
+    t[t == 11] = 12
+    _check(x, w, b, t)                                  # the hidden states' gradient: NaN in that column, as 0 * inf is
+    loss, bound, _, _ = formula(x, w, b, t, torch.ones(150, device='cuda'))
+    _within(_score(x, w, b, t), loss, bound)
+    # logits of both infinities in the weight's and in the hidden states' rows: the same rows are NaN, scored and packed
+    with torch.no_grad():
+        x[::2, 5].neg_()
+        w[13, 7] = float('inf')
+        live = torch.nonzero(t >= 0)[:, 0]
+        x[live[20], 9] = float('inf')
+        want = torch.log_softmax(torch.where((t >= 0)[:, None], x.double(), 0.0) @ w.double().t() + b.double(), 1)
+        want = torch.where(t >= 0, -want.gather(1, t.clamp(min=0)[:, None])[:, 0], 0.0)
+        got = vocab.vocab_cross_entropy(x, w, t, bias=b, reduction='none')
+        assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.isnan(_score(x, w, b, t)), torch.isnan(want))
+        fine = torch.isfinite(want)
+        assert bool(fine[live].any()) and torch.equal(got == float('inf'), want == float('inf'))
+        _within(got[fine], want[fine], 1e-4 * (1 + want[fine]))
+
+
 # ---- upstream gradients, row by row ------------------------------------------------------------------------------------------
 @pytest.mark.parametrize('dtype', DTYPES)
 @pytest.mark.parametrize('bad', [float('inf'), float('-inf'), float('nan')])

@@ -22,7 +22,7 @@ def u(dtype):
 
 def below(x):
     """what the smallest fp16 number costs an element of each row"""
-    top = x.abs().max(1, keepdim=True).values
+    top = torch.where(torch.isfinite(x), x.abs(), 0.0).max(1, keepdim=True).values
     return torch.minimum(2.0 ** -23 * top, 2.0 ** -38 * top.max())
 
 
@@ -35,6 +35,7 @@ def formula(x, w, b, t, grad_rows, extra=0.0):
     wd = w.detach().double()
     (m, k), v = xd.shape, wd.shape[0]
     l = xd @ wd.t() + (b.detach().double() if b is not None else 0.0)
+    l = torch.where(there[:, None], l, 0.0)
     at = t.clamp(min=0)[:, None]
     lse = torch.logsumexp(l, 1)
     loss = torch.where(there, lse - l.gather(1, at)[:, 0], 0.0)
@@ -71,8 +72,8 @@ def formula(x, w, b, t, grad_rows, extra=0.0):
 
     Ga = G.abs()
     one = torch.ones(m, 1, dtype=torch.float64, device=x.device)
-    want = (G @ wd, G.t() @ xd, G.sum(0))
-    bounds = (near(want[0], dG, Ga, wa, wb, v), near(want[1], dG.t(), Ga.t(), xa, xb, m),
+    want = (torch.where(there[:, None], G @ wd, 0.0), G.t() @ xd, G.sum(0))    # an absent row has no gradient, whatever the weight holds
+    bounds = (torch.where(there[:, None], near(want[0], dG, Ga, wa, wb, v), tiny), near(want[1], dG.t(), Ga.t(), xa, xb, m),
               near(want[2][:, None], dG.t(), Ga.t(), one, 0.0 * one, m)[:, 0])
     return loss, loss_bound, want, bounds
 

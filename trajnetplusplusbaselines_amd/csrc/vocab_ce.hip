@@ -162,7 +162,9 @@ __device__ __forceinline__ float ce_pack_rows_at(const T *src, int64_t ld, int64
                 const bool there = live && (p + u) * (SPLIT ? 16 : 32) + c0 + k < D;
                 const float x = there ? to_f32(q[u][k / VE].v[k % VE]) : 0.0f, v = ldexpf(x, -e);
                 const half_t hi = (half_t)v;
-                o[k] = SPLIT && ch >= 2 ? (fabsf(v) < 65504.0f ? (half_t)(v - (float)hi) : (half_t)0.0f) : hi;
+                // an infinity is the lo half, beside a hi of zero: it meets the other operand's hi alone, whose sign is the value's
+                const bool inf = SPLIT && fabsf(v) == __builtin_inff();
+                o[k] = SPLIT && ch >= 2 ? (inf ? hi : (half_t)(v - (float)hi)) : inf ? (half_t)0.0f : hi;
                 top = fmaxf(top, fabsf(x) < __builtin_inff() ? fabsf(x) : 0.0f);
             }
             if (to >= 0) *(half8 *)(out + (p + u) * panel_rows * 32) = o;
@@ -423,7 +425,7 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) ce_logits_kernel(CeLogits a, c
                     if (mine) a.tlogit[row[j]] = l;
                 }
             } else {
-                const bool any = __any(mine);
+                const bool any = __any(mine), edge = (ti + 1) * BN > live;
                 // stored order inside 16 columns: 0 1 2 3 8 9 10 11 | 4 5 6 7 12 13 14 15 -- what one lane holds, 16 bytes at a time, at a
                 // wave's base and a lane's offset of 32 bits
                 half_t *out = a.g + (int64_t)(tv * BM / 32 + wm * TM) * (SPLIT ? 2 : 1) * a.Mp * 32;
@@ -434,6 +436,10 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) ce_logits_kernel(CeLogits a, c
                                                                  // 128 fp32 backward 493 us against 458)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_amdgcn_exp2f(acc[i][j][e] - m[j]) * pf[j];
+                    if (edge) {                                  // rows behind the last: 0 times an infinite weight is no number
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) acc[i][j][e] = tc[j] >= 0 ? acc[i][j][e] : 0.0f;
+                    }
                     if (any) {
 #pragma unroll
                         for (int e = 0; e < 16; ++e)

@@ -133,8 +133,8 @@ def vocab_cross_entropy(hidden, weight, target, bias=None, reduction='mean'):
 
     fp32 operands are multiplied as two fp16 numbers each, scaled by the largest finite element of their tensor or, where all of a row
     (of hidden or of weight) is below 2^-16 of that one, of their row: no row's result goes by another's size.  Within a row, an element below
-    2^-16 of the row's largest may lose relative precision (2^-23 of the row's largest remains, usually 2^-40).  Rows with a valid
-    target that hold an infinity, and an fp32 weight that holds one, give NaN.  Gradients: (p - y) times the upstream gradient is rounded to fp16 (fp32 and fp16 operands: two fp16 numbers); parts of a
+    2^-16 of the row's largest may lose relative precision (2^-23 of the row's largest remains, usually 2^-40).  Infinities are
+    multiplied as the formula says (a logit of -inf masks its entry; two infinities that meet may give NaN).  Gradients: (p - y) times the upstream gradient is rounded to fp16 (fp32 and fp16 operands: two fp16 numbers); parts of a
     row below 2^-29 of the largest lose relative precision (2^-40 of the largest upstream gradient remains, and 2^-22 of the row's own). An
     upstream gradient that is no number spoils its own row of hidden's gradient, and the sums over rows."""
     if torch.compiler.is_compiling():
