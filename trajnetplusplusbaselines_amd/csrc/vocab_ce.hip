@@ -173,16 +173,20 @@ __device__ __forceinline__ float ce_pack_rows_at(const T *src, int64_t ld, int64
     return top;
 }
 
-// the same on the tensor's exponent e, and once more on their own the rows that are far below it; exps[to]: the row's exponent
+// the same on the tensor's exponent e, and once more on their own the rows that are far below it; exps[to], scales[to]: the row's exponent
+// and its word for the gradient products
 template <typename T, int VE, bool SPLIT>
 __device__ __forceinline__ void ce_pack_rows(const T *src, int64_t ld, int64_t from_row, int64_t to, int D, int e, half_t *dst, int64_t panel_rows,
-                                             int panels, int lane, int32_t *exps, uint32_t *classes) {
+                                             int panels, int lane, int32_t *exps, int32_t *scales, uint32_t *classes) {
     float top = ce_pack_rows_at<T, VE, SPLIT>(src, ld, from_row, to, D, e, dst, panel_rows, panels, lane);
     top = fmaxf(top, __shfl_xor(top, 1));                        // the row's four lanes
     top = fmaxf(top, __shfl_xor(top, 2));
     const int own = ce_exponent(top);
     const bool far = top > 0.0f && own < e - CE_FAR;
-    if (to >= 0 && (lane & 3) == 0) exps[to] = far ? own : e;
+    if (to >= 0 && (lane & 3) == 0) {
+        exps[to] = far ? own : e;
+        scales[to] = row_scale(far ? own - e : 0);
+    }
     if (!__any(far)) return;
     ce_pack_rows_at<T, VE, SPLIT>(src, ld, from_row, far ? to : -1, D, own, dst, panel_rows, panels, lane);
     if (far && to >= 0 && (lane & 3) == 0) atomicOr(classes, 1u << row_class(own - e));
@@ -191,7 +195,7 @@ __device__ __forceinline__ void ce_pack_rows(const T *src, int64_t ld, int64_t f
 template <typename T, int VX, int VW, bool SPLIT>
 __global__ void __launch_bounds__(256) ce_pack_kernel(const T *x, int64_t ldx, const int64_t *target, const T *w, int64_t ldw, CeShape sh,
                                                       const float *part, const int *count, CeScalars *sc, half_t *xp, half_t *wp, int32_t *orig,
-                                                      int32_t *tc, int32_t *xe, int32_t *we, int x_blocks) {
+                                                      int32_t *tc, int32_t *xe, int32_t *xs, int32_t *we, int32_t *ws, int x_blocks) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tid = threadIdx.x;
     const bool is_w = (int)blockIdx.x >= x_blocks;
     __shared__ float red[4];
@@ -218,7 +222,7 @@ __global__ void __launch_bounds__(256) ce_pack_kernel(const T *x, int64_t ldx, c
         if (tid == 0 && (int)blockIdx.x == x_blocks) sc->ew = e;
         const int blocks = gridDim.x - x_blocks;
         for (int64_t r = ((int)blockIdx.x - x_blocks) * 64 + wave * 16 + (lane >> 2); r < sh.Vp; r += blocks * 64)
-            ce_pack_rows<T, VW, SPLIT>(w, ldw, r < sh.V ? r : -1, r, sh.D, e, wp, sh.Vp, sh.panels, lane, we, &sc->w_classes);
+            ce_pack_rows<T, VW, SPLIT>(w, ldw, r < sh.V ? r : -1, r, sh.D, e, wp, sh.Vp, sh.panels, lane, we, ws, &sc->w_classes);
         return;
     }
     int base = cnt[0].x + cnt[1].x + cnt[2].x + cnt[3].x;
@@ -246,14 +250,14 @@ __global__ void __launch_bounds__(256) ce_pack_kernel(const T *x, int64_t ldx, c
         __syncthreads();
         for (int g = wave * 16; g < num; g += 64) {
             const int i = g + (lane >> 2);
-            ce_pack_rows<T, VX, SPLIT>(x, ldx, i < num ? list[i] : -1, i < num ? base + i : -1, sh.D, e, xp, sh.Mp, sh.panels, lane, xe,
+            ce_pack_rows<T, VX, SPLIT>(x, ldx, i < num ? list[i] : -1, i < num ? base + i : -1, sh.D, e, xp, sh.Mp, sh.panels, lane, xe, xs,
                                         &sc->x_classes);
         }
         base += num;
     }
     // zero rows up to the next multiple of 256
     for (int64_t r = live + (int64_t)blockIdx.x * 64 + wave * 16 + (lane >> 2); r - (lane >> 2) < ce_padded(live); r += (int64_t)x_blocks * 64)
-        ce_pack_rows<T, VX, SPLIT>(x, ldx, -1, r < ce_padded(live) ? r : -1, sh.D, e, xp, sh.Mp, sh.panels, lane, xe, &sc->x_classes);
+        ce_pack_rows<T, VX, SPLIT>(x, ldx, -1, r < ce_padded(live) ? r : -1, sh.D, e, xp, sh.Mp, sh.panels, lane, xe, xs, &sc->x_classes);
 }
 
 // ---- logits: statistics forward, G backward ---------------------------------------------------------------------------------
@@ -275,7 +279,7 @@ struct CeLogits {
     const float2 *stat;       // [Mp] (largest logit, base 2; 1 / sum of 2^(l - largest)), padding (+inf, 0), no such target (.., NaN)
     const float *grad;        // reduction none: [M]
     CeUpstream *up;           // ... what is known of it
-    int32_t *gs;              // ... binades [Mp] by which a row of G lies below the largest gradient's scale
+    int32_t *gs, *xs;         // ... binades [Mp] by which a row of G lies below the largest gradient's scale, words of these and the hidden states' together
     half_t *g;                // panels of Mp rows, column 0 = vocabulary entry v0
     int64_t g_plane;          // elements from a plane of G to the next
 };
@@ -338,6 +342,7 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) ce_logits_kernel(CeLogits a, c
                 if (vs == 0 && wm == 0 && h == 0) {
                     a.gs[row[j]] = below;
                     const int shift = a.xe[row[j]] - a.sc->ex + below;
+                    a.xs[row[j]] = row_scale(shift);
                     if (shift) atomicOr(&a.up->classes, 1u << row_class(shift));
                 }
             }
@@ -739,7 +744,7 @@ struct CeGrad {
     int64_t rows, out0;       // dweight: output rows of this call, the first one's index in the output
     int tiles_d, steps, splits, blocks;
     int64_t ok0;              // first row of the other operand
-    const int32_t *o_exps;    // exponents of its rows, from there
+    const int32_t *o_scales;  // its rows' words (vocab_gemm.h), from there
     int g_panels, o_panels;
     void *out;                // final output (nothing to add up), [..][D]
     float *part;              // [splits][part_rows][D] sums, or NULL
@@ -759,26 +764,6 @@ struct CeGrads {
     float *part_b;            // dbias: [w.splits][ldb] sums in G's stored column order, or NULL
     int64_t ldb;
 };
-
-// dbias's sums over rows on scales of their own, from memory: asum[i] += what this lane's half of the rows of steps [s0, s1) adds to G's
-// column col + 32 i + (lane & 31)
-template <bool SPLIT, int TM>
-__device__ __forceinline__ void ce_row_sums(const CeGrads &a, const CeGrad &c, int64_t col, int s0, int s1, int plane_steps, float (&asum)[TM], int lane) {
-    constexpr int PC = SPLIT ? 16 : 32;
-#pragma unroll
-    for (int i = 0; i < TM; ++i) {
-        const int64_t v = col + i * 32 + (lane & 31);
-        const half_t *g = c.g.p + v / PC * c.g.rows * 32 + v % PC;
-        for (int s = s0; s < s1; ++s) {
-            const bool second = s >= plane_steps;
-            const int k0 = (second ? s - plane_steps : s) * PC;
-            for (int k = k0 + (lane >> 5); k < k0 + PC; k += 2) {
-                const half_t *at = g + (second ? a.g_plane : 0) + (int64_t)k * 32;
-                asum[i] += ldexpf(SPLIT ? (float)at[0] + (float)at[16] : (float)at[0], a.gs ? a.gs[k] : 0);
-            }
-        }
-    }
-}
 
 template <int TM, int TN> __device__ __forceinline__ void ce_rescale(f32x16 (&acc)[TM][TN], int by) {
 #pragma unroll
@@ -820,17 +805,20 @@ __device__ __forceinline__ void ce_grad_tile(const CeGrads &a, const CeGrad &c, 
         g.first(s0, s1);
         g.template run<WEIGHT, false>(s0, s1, acc, sums, asum, RowScales{});
     } else {
-        if (sums) ce_row_sums<SPLIT, TM>(a, c, r0 + wm * TM * 32, s0, s1, (int)plane_steps, asum, lane);
-        int at = -1;                                           // the class on whose scale acc is
+        int at = 0;                                            // the class on whose scale acc is
         decltype(g)::clear(acc);
         for (int k = ROW_CLASSES - 1; k >= 0; --k) {
             if (!(classes >> k & 1)) continue;
-            if (at >= 0) ce_rescale(acc, 16 * (k - at));
+            const RowScales rs{c.o_scales, WEIGHT ? a.gs : nullptr, k};
+            int c0 = s0, c1 = s1;
+            class_steps<PC>(rs, CE_TWO_PLANES<T, SPLIT> ? (int)plane_steps : INT32_MAX, c0, c1, lane);
+            if (c0 == c1) continue;
+            if (at) ce_rescale(acc, 16 * (k - at));
             at = k;
-            g.first(s0, s1);
-            g.template run<false, true>(s0, s1, acc, false, asum,
-                                         RowScales{c.o_exps, WEIGHT ? a.gs : nullptr, WEIGHT ? a.sc->ex : a.sc->ew, k, c.o.perm});
+            g.first(c0, c1);
+            g.template run<WEIGHT, true>(c0, c1, acc, sums, asum, rs);
         }
+        if (at) ce_rescale(acc, -16 * at);
     }
     if (sums) {
 #pragma unroll
@@ -941,7 +929,7 @@ static CeShape ce_shape(const tnp_vocab_ce *p) {
     return s;
 }
 
-struct CeSaved { CeScalars *sc; float2 *stat; int32_t *tc, *orig, *xe, *we; half_t *x, *w; size_t bytes; };
+struct CeSaved { CeScalars *sc; float2 *stat; int32_t *tc, *orig, *xe, *xs, *we, *ws; half_t *x, *w; size_t bytes; };
 static CeSaved ce_saved(const CeShape &s, void *base) {
     CeSaved v;
     char *p = (char *)base;
@@ -950,7 +938,9 @@ static CeSaved ce_saved(const CeShape &s, void *base) {
     v.tc = (int32_t *)p; p += s.Mp * 4;
     v.orig = (int32_t *)p; p += s.Mp * 4;
     v.xe = (int32_t *)p; p += s.Mp * 4;
+    v.xs = (int32_t *)p; p += s.Mp * 4;
     v.we = (int32_t *)p; p += (size_t)s.Vp * 4;
+    v.ws = (int32_t *)p; p += (size_t)s.Vp * 4;
     v.x = (half_t *)p; p += (size_t)s.Mp * s.panels * 64;
     v.w = (half_t *)p; p += (size_t)s.Vp * s.panels * 64;
     v.bytes = (size_t)(p - (char *)base);
@@ -1016,7 +1006,7 @@ struct CeBackward {
     half_t *g;
     int tile, splits_x, splits_w;
     CeUpstream *up;
-    int32_t *gs;
+    int32_t *gs, *xs;
     float *part_x, *part_w, *part_b;
     size_t bytes;
 };
@@ -1049,7 +1039,8 @@ static CeBackward ce_backward_layout(const tnp_vocab_ce *p, void *ws) {
     char *w = (char *)ws;
     b.up = (CeUpstream *)w; w += 256;
     b.gs = p->reduction == 0 ? (int32_t *)w : nullptr;
-    if (b.gs) w += ce_up((size_t)s.Mp * 4);
+    b.xs = b.gs ? b.gs + s.Mp : nullptr;
+    if (b.gs) w += ce_up((size_t)s.Mp * 8);
     b.g = (half_t *)w; w += ce_up((size_t)s.Mp * b.ldg * 2);
     b.part_x = b.splits_x > 1 || b.pieces > 1 ? (float *)w : nullptr;
     if (b.part_x) w += ce_up((size_t)b.splits_x * s.Mp * p->D * 4);
@@ -1148,7 +1139,7 @@ static int ce_pack(const tnp_vocab_ce *p, const CeShape &sh, const CeForward &f,
     const int xb = ce_x_blocks(p->M), wb = sh.Vp / 64 < 2048 ? sh.Vp / 64 : 2048;
     hipLaunchKernelGGL((ce_pack_kernel<T, VX, VW, SPLIT>), dim3(xb + wb), dim3(256), 0, s, (const T *)p->hidden, p->ld_hidden, p->target,
                        (const T *)p->weight, p->ld_weight, sh, f.amax, f.count, f.saved.sc, f.saved.x, f.saved.w,
-                       f.saved.orig, f.saved.tc, f.saved.xe, f.saved.we, xb);
+                       f.saved.orig, f.saved.tc, f.saved.xe, f.saved.xs, f.saved.we, f.saved.ws, xb);
     TNP_HIP(hipGetLastError());
     return 0;
 }
@@ -1198,7 +1189,7 @@ static int ce_backward(const tnp_vocab_ce *p, const CeBackward &b, const float *
         const int v0 = k * b.piece, cols = sh.Vp - v0 < b.piece ? sh.Vp - v0 : b.piece, live = sh.V - v0 < cols ? sh.V - v0 : cols;
         CeLogits a = {};
         a.w = w; a.x = x; a.sc = sv.sc; a.tc = sv.tc; a.orig = sv.orig; a.xe = sv.xe; a.we = sv.we; a.Mp = sh.Mp; a.V = sh.V; a.v0 = v0; a.steps = sh.panels;
-        a.stat = sv.stat; a.grad = p->reduction == 0 ? grad : nullptr; a.up = b.up; a.gs = b.gs; a.g = b.g; a.g_plane = (int64_t)b.piece * sh.Mp; a.v_shares = ce_logit_shares(sh, cols);
+        a.stat = sv.stat; a.grad = p->reduction == 0 ? grad : nullptr; a.up = b.up; a.gs = b.gs; a.xs = b.xs; a.g = b.g; a.g_plane = (int64_t)b.piece * sh.Mp; a.v_shares = ce_logit_shares(sh, cols);
         if ((rc = ce_logits<T, SPLIT, true>(a, cols, ce_big(sh), (const T *)p->bias, s))) return rc;
         const bool last = k == b.pieces - 1;
         const int ks = SPLIT ? 16 : 32;
@@ -1208,10 +1199,10 @@ static int ce_backward(const tnp_vocab_ce *p, const CeBackward &b, const float *
         c.zero_blocks = dhidden && k == 0 ? (int)(sh.Mp / 64 < 512 ? sh.Mp / 64 : 512) : 0;
         c.x.g = c.w.g = GemmOperand{b.g, sh.Mp, 0};
         c.x.g_panels = c.w.g_panels = cols / ks; c.x.o_panels = c.w.o_panels = sh.panels;
-        c.x.o = w; c.x.o.perm = 1; c.x.ok0 = v0; c.x.o_exps = sv.we + v0;
+        c.x.o = w; c.x.o.perm = 1; c.x.ok0 = v0; c.x.o_scales = sv.ws + v0;
         c.x.out = dhidden; c.x.part = b.part_x; c.x.part_rows = sh.Mp; c.x.splits = b.splits_x;
         c.x.steps = cols / ks; c.x.add = k > 0;
-        c.w.o = x; c.w.o_exps = sv.xe;
+        c.w.o = x; c.w.o_scales = b.xs ? b.xs : sv.xs;
         c.w.rows = live; c.w.out0 = v0; c.w.out = dweight; c.w.part = b.part_w; c.w.part_rows = b.piece; c.w.splits = b.splits_w;
         c.part_b = dbias ? b.part_b : nullptr; c.ldb = b.piece;
         rc = b.tile == 256 ? ce_launch_grads<T, SPLIT, 256, 256, 2, 4, 4>(c, s) : ce_launch_grads<T, SPLIT, 128, 128, 2, 2, 4>(c, s);

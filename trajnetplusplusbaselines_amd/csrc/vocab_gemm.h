@@ -23,27 +23,49 @@
 namespace tnp {
 
 typedef half_t half8 __attribute__((ext_vector_type(8)));
-typedef short short4v __attribute__((ext_vector_type(4)));
+typedef int int2v __attribute__((ext_vector_type(2)));
+typedef int int4v __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 #define TNP_LDS __attribute__((address_space(3)))
 #define TNP_GLB __attribute__((address_space(1)))
 
-// Rows of an operand that is read as KS (its rows are the k of the product) may lie in memory on scales of their own: row r holds the
-// value times 2^-exps[r].  Rows are taken by CLASSES of sixteen binades, one run of the product each, from the smallest numbers to the
-// largest: a run multiplies the operand, in registers, by 2^(exps[r] - top + 16 class) where the row is of its class and by zero elsewhere,
+// Rows of an operand that is read as KS (its rows are the k of the product) may lie in memory on scales of their own, row r by `shift`
+// binades (<= 0) below the top one's.  Rows are taken by CLASSES of sixteen binades, one run of the product each, from the smallest numbers to
+// the largest: a run multiplies the operand, in registers, by 2^(shift + 16 class) where the row is of its class and by zero elsewhere,
 // and the accumulator is brought onto the next class's scale in between.  No row's bits are lost to another's size, and an
-// operand whose rows share one scale (class 0 alone, exps == top) needs none of it.
+// operand whose rows share one scale (class 0 alone, no shifts) needs none of it.  A run goes from the first to the last step that has a row of
+// its class, so that a few such rows cost little.
+//
+// A row's scale is one word: class << 16 | that fp16 number.  A wave reads a step's words by scalar loads (vector loads would wait for the tiles in
+// flight), one step ahead: forward and backward of 24576 x 1024 x 128 fp32 with one row 2^40 times as large 232 us (vector loads 488), without such a
+// row 148; a run with scales takes 1.4 times one without.
 static constexpr int ROW_CLASSES = 32;
-__device__ __forceinline__ int row_class(int shift) {              // shift <= 0: binades below the top
+__device__ __forceinline__ int row_class(int shift) {
     const int c = -shift >> 4;
     return c < ROW_CLASSES ? c : ROW_CLASSES - 1;
 }
+__device__ __forceinline__ int32_t row_scale(int shift) {
+    const int c = row_class(shift);
+    return c << 16 | __builtin_bit_cast(uint16_t, (half_t)ldexpf(1.0f, shift + 16 * c));
+}
 struct RowScales {
-    const int32_t *exps;     // of the operand's row ok0
-    const int32_t *other;    // binades (<= 0) that a's columns of these rows are to be taken by as well, or NULL
-    int top, cls, perm;      // perm: GemmOperand's
+    const int32_t *scales;   // of the operand's row ok0
+    const int32_t *sums;     // binades that the row sums of a are to be taken by (not the product: it is in `scales`), or NULL
+    int cls;
+    // which of sixteen rows is lane half h's e-th value; perm: GemmOperand's
+    static __device__ __forceinline__ constexpr int at(int e, int h, int perm) { return perm ? (e & 3) + 8 * (e >> 2) + 4 * h : 8 * h + e; }
 };
+// sixteen words at a wave-uniform address, by scalar loads
+struct Row16 { int32_t v[16]; };
+__device__ __forceinline__ Row16 row16(const int32_t *p, int row) {
+    typedef const __attribute__((address_space(4))) int32_t *Constant;
+    const Constant c = (Constant)(p + __builtin_amdgcn_readfirstlane(row));
+    Row16 r;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) r.v[k] = c[k];
+    return r;
+}
 
 struct GemmOperand {
     const half_t *p;     // panel 0, row 0
@@ -105,8 +127,8 @@ template <bool KS, bool SPLIT, int BR, int NW> struct TileStage {
 // 32-column blocks of KS tiles at the LDS addresses a[], k rows 0 .. 3 and (R4 bytes on) 4 .. 7 of every half.  One asm block that ends
 // with its own wait: as builtins these reads would first wait for every global_load_lds in flight, that is for the tiles of the
 // next steps.
-typedef int int2v __attribute__((ext_vector_type(2)));
-typedef int int4v __attribute__((ext_vector_type(4)));
+
+
 template <int R4> __device__ __forceinline__ void ks_read(const uint32_t (&a)[2], half8 (&f)[2]) {
     int2v r[4];
     asm volatile(
@@ -220,24 +242,98 @@ template <int TM> __device__ __forceinline__ void step_row_sums(const half8 (&fa
                 asum[i] = __builtin_amdgcn_fdot2(half2v{fa[2 * i + w][2 * e], fa[2 * i + w][2 * e + 1]}, one, asum[i], false);
 }
 
-// One step's KS operand times its rows' scales; row: of the step's first k value
-template <bool SPLIT, int NB> __device__ __forceinline__ void step_scale(half8 (&f)[2 * NB], const RowScales &rs, int row, int lane) {
+// a step's words; row: of the step's first k value
+template <bool SPLIT, bool SUMS> struct StepWords {
+    static constexpr int N = SPLIT ? 1 : 2;
+    Row16 scales[N], sums[SUMS ? N : 1];
+    __device__ __forceinline__ void load(const RowScales &rs, int row) {
+#pragma unroll
+        for (int w = 0; w < N; ++w) scales[w] = row16(rs.scales, row + 16 * w);
+        if (SUMS && rs.sums)
+#pragma unroll
+            for (int w = 0; w < N; ++w) sums[SUMS ? w : 0] = row16(rs.sums, row + 16 * w);
+    }
+};
+
+// One step's KS operand times its rows' scales
+template <bool SPLIT, bool PERM, int NB, typename Words>
+__device__ __forceinline__ void step_scale(half8 (&f)[2 * NB], const RowScales &rs, const Words &words, int lane) {
 #pragma unroll
     for (int w = 0; w < (SPLIT ? 1 : 2); ++w) {
-        __builtin_amdgcn_sched_barrier(0);                           // eight scales at a time: more of them spill registers
-        half8 sc;
-        const int h = lane >> 5;
+        __builtin_amdgcn_sched_barrier(0);                           // sixteen rows at a time: more of them spill registers
+        const Row16 &r = words.scales[w];
+        uint32_t bits[16];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int r = row + 16 * w + (rs.perm ? (e & 3) + 8 * (e >> 2) + 4 * h : 8 * h + e);
-            const int shift = rs.exps[r] - rs.top + (rs.other ? rs.other[r] : 0);
-            sc[e] = row_class(shift) == rs.cls ? (half_t)ldexpf(1.0f, shift + 16 * rs.cls) : (half_t)0.0f;
+        for (int k = 0; k < 16; ++k) bits[k] = r.v[k] >> 16 == rs.cls ? r.v[k] & 0xffff : 0;
+        int4v sc;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            const uint32_t low = bits[RowScales::at(e, 0, PERM)] | bits[RowScales::at(e + 1, 0, PERM)] << 16,
+                           high = bits[RowScales::at(e, 1, PERM)] | bits[RowScales::at(e + 1, 1, PERM)] << 16;
+            sc[e / 2] = lane >> 5 ? high : low;
         }
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int p = 0; p < (SPLIT ? 2 : 1); ++p) f[2 * b + (SPLIT ? p : w)] *= sc;
+            for (int p = 0; p < (SPLIT ? 2 : 1); ++p) f[2 * b + (SPLIT ? p : w)] *= __builtin_bit_cast(half8, sc);
     }
+}
+
+// the sums of step_row_sums over the rows of one class, each by the binades that its sums are to be taken by
+template <bool SPLIT, int TM, typename Words>
+__device__ __forceinline__ void step_row_sums(const half8 (&fa)[2 * TM], float (&asum)[TM], const RowScales &rs, const Words &words, int lane) {
+#pragma unroll
+    for (int w = 0; w < (SPLIT ? 1 : 2); ++w) {
+        __builtin_amdgcn_sched_barrier(0);
+        const Row16 &r = words.scales[w];
+        float by[16];
+        if (rs.sums) {
+            const Row16 &n = words.sums[w];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) by[k] = r.v[k] >> 16 == rs.cls && n.v[k] > -127 ? __uint_as_float((uint32_t)(127 + n.v[k]) << 23) : 0.0f;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) by[k] = r.v[k] >> 16 == rs.cls ? 1.0f : 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float b = lane >> 5 ? by[8 + e] : by[e];
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                asum[i] = fmaf((float)fa[2 * i + w][e], b, asum[i]);
+                if (SPLIT) asum[i] = fmaf((float)fa[2 * i + 1][e], b, asum[i]);
+            }
+        }
+    }
+}
+
+// The steps of [s0, s1) from the first to the last that has a row of the class, the same for all lanes.
+template <int KSTEP> __device__ __forceinline__ void class_steps(const RowScales &rs, int wrap, int &s0, int &s1, int lane) {
+    if (rs.cls == 0 || (s0 < wrap && s1 > wrap)) return;             // most rows' class, or both planes of the other operand: all of them
+    const int back = s0 >= wrap ? wrap : 0, end = (s1 - back) * KSTEP;
+    int first = INT32_MAX, last = -1;
+    constexpr int U = 16;                                            // words in flight
+    for (int r0 = (s0 - back) * KSTEP + lane; r0 < end; r0 += 64 * U) {
+        int32_t v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = rs.scales[r0 + u * 64 < end ? r0 + u * 64 : r0];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int r = r0 + u * 64;
+            if (r >= end || v[u] >> 16 != rs.cls) continue;
+            first = first < r ? first : r;
+            last = r;
+        }
+    }
+    for (int o = 32; o; o >>= 1) {
+        const int f = __shfl_xor(first, o), l = __shfl_xor(last, o);
+        first = first < f ? first : f;
+        last = last > l ? last : l;
+    }
+    first = __builtin_amdgcn_readfirstlane(first);
+    last = __builtin_amdgcn_readfirstlane(last);
+    s1 = last < 0 ? s0 : back + last / KSTEP + 1;
+    s0 = last < 0 ? s0 : back + first / KSTEP;
 }
 
 // One workgroup's products: init() takes the tile at (row ar, panel ap) of a and (br, bp) of b (al / bl: panels from there to the last,
@@ -255,7 +351,7 @@ template <bool SPLIT, int NB> __device__ __forceinline__ void step_scale(half8 (
 // An unsplit a may have a second plane, `plane` elements behind the first: the steps from `wrap` on run over it, with b's steps from the
 // first one again.
 //
-// SCALED: b's rows on scales of their own (RowScales); acc is added to, not set.
+// SCALED: b's rows on scales of their own (RowScales), in G's stored order of them where a is read as KC; acc is added to, not set.
 template <bool SPLIT, bool A_KS, bool B_KS, int BM, int BN, int WM, int WN, int NST> struct TileGemm {
     static constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, STAGE = (BM + BN) * 64;
     static constexpr bool TURNS = NW == 8;
@@ -318,11 +414,14 @@ template <bool SPLIT, bool A_KS, bool B_KS, int BM, int BN, int WM, int WN, int 
         if (TURNS && wave >= 4) stage_barrier_only();
         int cur = 0;
         half8 fa[2 * TM], fb[2 * TN];
+        auto row = [&](int s) { return (s < wrap ? s : s - wrap) * SB::KSTEP; };
+        StepWords<SPLIT, SUMS> words;
+        if constexpr (SCALED) words.load(rs, row(s0));
         for (int s = s0; s < s1; ++s) {
             const char *la = lds + cur * STAGE, *lb = la + BM * 64;
             step_frags<SB, B_KS, SPLIT, TN>(lb, wn * TN * 32, lane, fb);
             step_frags<SA, A_KS, SPLIT, TM>(la, wm * TM * 32, lane, fa);
-            if constexpr (SCALED) step_scale<SPLIT, TN>(fb, rs, (s < wrap ? s : s - wrap) * SB::KSTEP, lane);
+            if constexpr (SCALED) step_scale<SPLIT, !A_KS, TN>(fb, rs, words, lane);
             if (s + NST - 1 < s1) load(s + NST - 1, cur == 0 ? NST - 1 : cur - 1);   // the buffer that every wave left one barrier ago
             cur = cur + 1 == NST ? 0 : cur + 1;
             if (TURNS) {
@@ -331,14 +430,22 @@ template <bool SPLIT, bool A_KS, bool B_KS, int BM, int BN, int WM, int WN, int 
                 __builtin_amdgcn_sched_barrier(0);
                 __builtin_amdgcn_s_setprio(1);
                 step_mfma<SPLIT, TM, TN>(fa, fb, acc);
-                if (SUMS && sums) step_row_sums<TM>(fa, asum);
+                if (SUMS && sums) {
+                    if constexpr (SCALED) step_row_sums<SPLIT, TM>(fa, asum, rs, words, lane);
+                    else step_row_sums<TM>(fa, asum);
+                }
+                if constexpr (SCALED) words.load(rs, row(s + 1 < s1 ? s + 1 : s));
                 __builtin_amdgcn_s_setprio(0);
                 __builtin_amdgcn_sched_barrier(0);
                 stage_barrier_only();
                 __builtin_amdgcn_sched_barrier(0);
             } else {
                 step_mfma<SPLIT, TM, TN>(fa, fb, acc);
-                if (SUMS && sums) step_row_sums<TM>(fa, asum);
+                if (SUMS && sums) {
+                    if constexpr (SCALED) step_row_sums<SPLIT, TM>(fa, asum, rs, words, lane);
+                    else step_row_sums<TM>(fa, asum);
+                }
+                if constexpr (SCALED) words.load(rs, row(s + 1 < s1 ? s + 1 : s));
                 landed(s1 - 2 - s);                                // after the last step: every wave is done with the ring
             }
         }

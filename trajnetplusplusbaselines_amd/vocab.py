@@ -85,7 +85,7 @@ def saved_bytes(rows, entries, columns, dtype):
     """tnp_vocab_ce_saved_bytes() from the sizes alone (they may be symbolic while a graph is traced)"""
     panels = (columns + 15) // 16 if dtype == torch.float32 else (columns + 31) // 32
     up = lambda n: (n + 255) // 256 * 256
-    return 256 + 20 * up(rows) + 4 * up(entries) + 64 * panels * (up(rows) + up(entries))
+    return 256 + 24 * up(rows) + 8 * up(entries) + 64 * panels * (up(rows) + up(entries))
 
 
 def check_cross_entropy(hidden, weight, target, bias, reduction):
