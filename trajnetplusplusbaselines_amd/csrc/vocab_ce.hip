@@ -173,6 +173,12 @@ __device__ __forceinline__ float ce_pack_rows_at(const T *src, int64_t ld, int64
     return top;
 }
 
+// classes |= the wave's bits: one atomic per wave, none where they are there already
+__device__ __forceinline__ void ce_add_classes(uint32_t *classes, uint32_t bits) {
+    for (int o = 32; o; o >>= 1) bits |= __shfl_xor(bits, o);
+    if ((threadIdx.x & 63) == 0 && (bits & ~__hip_atomic_load(classes, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))) atomicOr(classes, bits);
+}
+
 // the same on the tensor's exponent e, and once more on their own the rows that are far below it; exps[to], scales[to]: the row's exponent
 // and its word for the gradient products
 template <typename T, int VE, bool SPLIT>
@@ -189,7 +195,7 @@ __device__ __forceinline__ void ce_pack_rows(const T *src, int64_t ld, int64_t f
     }
     if (!__any(far)) return;
     ce_pack_rows_at<T, VE, SPLIT>(src, ld, from_row, far ? to : -1, D, own, dst, panel_rows, panels, lane);
-    if (far && to >= 0 && (lane & 3) == 0) atomicOr(classes, 1u << row_class(own - e));
+    ce_add_classes(classes, far && to >= 0 ? 1u << row_class(own - e) : 0);
 }
 
 template <typename T, int VX, int VW, bool SPLIT>
@@ -339,11 +345,11 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) ce_logits_kernel(CeLogits a, c
             if (a.grad) {
                 int below = 0;
                 if (tc[j] >= 0) f[j] = ce_row_factor(a.grad[a.orig[row[j]]], a.up->gmax, below);
-                if (vs == 0 && wm == 0 && h == 0) {
-                    a.gs[row[j]] = below;
+                if (vs == 0 && wm == 0) {
                     const int shift = a.xe[row[j]] - a.sc->ex + below;
-                    a.xs[row[j]] = row_scale(shift);
-                    if (shift) atomicOr(&a.up->classes, 1u << row_class(shift));
+                    if (h == 0) a.gs[row[j]] = below;
+                    if (h == 0) a.xs[row[j]] = row_scale(shift);
+                    if (__any(shift)) ce_add_classes(&a.up->classes, shift ? 1u << row_class(shift) : 0);
                 }
             }
             m[j] = st.x;
