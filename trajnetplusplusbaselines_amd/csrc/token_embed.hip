@@ -5,9 +5,10 @@
 // fault), nothing backward.
 //
 // Forward: one pass, bound by memory.  Backward of few tokens: every token's workgroup looks for its like (embed_small_kernel).  Of more:
-// the tokens are sorted (a stable radix sort of (token, i) pairs, digits of up to
-// 10 bits), so that all rows of one token are neighbours; chunks of 8, 16 or 32 sorted positions are summed by one group of lanes each,
-// whatever the distribution of the tokens -- a table row that owns half of the batch is split over many chunks and joined.
+// the tokens are sorted (a stable radix sort of (token, i) pairs, digits of up to 10 bits), so that all rows of one token are
+// neighbours; chunks of 8, 16 or 32 sorted positions are summed by one group of lanes each, whatever the distribution of the tokens.  What
+// goes by it is the join of a run over many chunks, one workgroup per run and block of columns: 262144 x 256 bf16 takes 78 us with the tokens
+// spread over 65536 rows, 89 with ~ u^6 (the longest run has 41000 rows), 151 with all of them alike.
 // Every gradient row is read once and every table row written once; table rows without a token are zeroed by their own workgroups,
 // which find them by binary search in the sorted tokens.
 #include "vocab_types.h"

@@ -66,7 +66,7 @@ struct CeShape {
 
 // ---- scales and packing -----------------------------------------------------------------------------------------------------
 // largest finite |element| of rows [r0, r1): the rows' accesses one after the other, four in flight per lane.  16384 + 65536 rows of 1024 bf16:
-// 38 us, 4.4 TB/s; packing them reads from the caches behind it: 59 us for 168 MB in and as much out
+// 38 us, 4.4 TB/s; packing them reads from the caches behind it: 57 us for 168 MB in and as much out
 template <typename T, int VE>
 __device__ __forceinline__ float ce_rows_amax(const T *x, int64_t ld, int64_t r0, int64_t r1, const int64_t *target, int D) {
     const uint32_t per = (uint32_t)D / VE, n = (uint32_t)(r1 - r0) * per;
@@ -269,8 +269,9 @@ __global__ void __launch_bounds__(256) ce_pack_kernel(const T *x, int64_t ldx, c
 // ---- logits: statistics forward, G backward ---------------------------------------------------------------------------------
 // The vocabulary runs over the rows of the matrix instruction, so a lane holds 16 logits of ONE hidden row per 32 x 32 block and
 // maxima, sums and exponentials stay inside the lane; the two halves of a wave meet once per share of the vocabulary.  16384 x 65536 x 1024
-// bf16: 2.16 ms of statistics (1.02 PFLOP/s), 2.26 with G written (2 GB); 4096 x 16384 x 512 fp32: 182 and 212 us (377 and 324 TFLOP/s; a
-// library product in fp32: 138).  Bound by the matrix cores' rate under load, the exponentials of a tile come on top.
+// bf16: 2.05 ms of statistics (1.07 PFLOP/s), 2.18 with G written (2 GB); 4096 x 16384 x 512 fp32: 179 and 209 us (384 and 329 TFLOP/s; a
+// library product in fp32: 138).  The matrix pipe is busy for 53 to 64 % of the cycles, at 1.9 GHz; the exponentials of a tile, three
+// vector instructions per matrix instruction, and its barriers take the rest.
 struct CeLogits {
     GemmOperand w, x;
     const CeScalars *sc;
@@ -861,9 +862,9 @@ __device__ __forceinline__ void ce_grad_tile(const CeGrads &a, const CeGrad &c, 
 }
 
 // Both gradient products in one launch: they read the same G, and the workgroups of one fill what the other's leave idle.  The last
-// workgroups zero dhidden of the absent rows.  16384 x 65536 x 1024 bf16 2 x 1.98 ms: 1.11 PFLOP/s (library products of these sizes 1.14 and
-// 1.51); 4096 x 16384 x 512 fp32 360 us: 382 TFLOP/s; 19700 x 1024 x 128 fp32 51 us: 203.  This loop with the operands left in place
-// reaches 1.3 PFLOP/s, which is the matrix cores' power.
+// workgroups zero dhidden of the absent rows.  16384 x 65536 x 1024 bf16 2 x 2.02 ms: 1.09 PFLOP/s (library products of these sizes 1.14 and
+// 1.51); 4096 x 16384 x 512 fp32 355 us: 387 TFLOP/s; 19700 x 1024 x 128 fp32 51 us: 203; 1237 x 5003 x 201 fp16, two planes of G, 48 us (one: 23).
+// The matrix pipe is busy for 58 % (bf16) and 67 % (fp32) of the cycles, at 1.9 GHz, 34 % in the third case, whose tiles have few steps.
 template <typename T, bool SPLIT, int BM, int BN, int WM, int WN, int NST>
 __global__ void __launch_bounds__(WM *WN * 64, 2) ce_grads_kernel(CeGrads a) {
     extern __shared__ __attribute__((aligned(1024))) char lds[];

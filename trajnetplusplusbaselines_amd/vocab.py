@@ -129,7 +129,8 @@ def vocab_cross_entropy(hidden, weight, target, bias=None, reduction='mean'):
 
     hidden [..., D], weight [V, D], bias [V] (may hold -inf: masked entries) of one dtype, target [...] int64 / int32.  Returns fp32:
     a scalar ('mean' over the rows that are there, 0 if there are none; 'sum') or target's shape ('none').  target < 0: an absent
-    row -- its hidden state is not read, its loss and gradient are 0; target >= V: NaN.  Differentiable in hidden, weight and bias.
+    row -- its hidden state is not read, its loss and gradient are 0; target >= V: NaN.  Differentiable in hidden, weight and bias; until its
+    backward pass a call keeps packed copies of hidden and of weight, so that one call on stacked rows keeps less than several.
 
     fp32 operands are multiplied as two fp16 numbers each, scaled by the largest finite element of their tensor or, where all of a row
     (of hidden or of weight) is below 2^-16 of that one, of their row: no row's result goes by another's size.  Within a row, an element below
