@@ -11,9 +11,9 @@
 // another's size.  bf16 and fp16 values are exact down to 2^-12 of their row's largest, fp32 values become two fp16 numbers (vocab_gemm.h); an error of
 // 2^-23 of the value or of its row's largest, usually 2^-40 of the latter.  Logits of far rows or entries get their powers of two one by one;
 // the gradient products, where rows are summed over, take far rows in classes (vocab_gemm.h), one run each.  G = 2^15 (g_i / max g) (p - y),
-// with a power of two per row instead of 1 / max g where the row's upstream gradient is below 2^-18 of the largest, is rounded to fp16 for bf16 gradients (11 bits, eight times
-// finer than what they are rounded to: their error grows by less than a hundredth) and to two fp16 numbers for fp32 and fp16 ones (one of them
-// would be as coarse as the fp16 gradient itself).  All sums, maxima and statistics are fp32; the sum of the losses is fp64.
+// with a power of two per row instead of 1 / max g where the row's upstream gradient is below 2^-18 of the largest, is rounded to fp16 for
+// bf16 gradients (11 bits, eight times finer than what they are rounded to: their error grows by less than a hundredth) and to two fp16
+// numbers for fp32 and fp16 ones (one of them would be as coarse as the fp16 gradient itself).  All sums, maxima and statistics are fp32; the sum of the losses is fp64.
 //
 // A negative target marks an absent row: its hidden state is not read (it may be NaN), its loss and gradients are zero.  Packing leaves
 // the absent rows out, so that everything behind it runs on the rows that are there (a fifth of a crowd's tracks are absent, more
@@ -298,8 +298,8 @@ template <typename T> __device__ __forceinline__ float ce_bias(const T *bias, in
     return fabsf(b) < __builtin_inff() ? fminf(fmaxf(l, -3.402823466e38f), 3.402823466e38f) : l;
 }
 
-// A row's factor of G: 2^15 g / (largest finite g); from 2^-18 of that on 2^14 .. 2^16 with `below` binades to be taken off later, so that the
-// row keeps its bits.  An infinity or a NaN is the row's own.
+// A row's factor of G: 2^15 g / (largest finite g); below 2^-18 of that one it is 2^13 .. 2^15 in magnitude, with `below` binades (negative) to be
+// applied later, so that the row keeps its bits.  An infinity or a NaN is the row's own.
 __device__ __forceinline__ float ce_row_factor(float g, float gmax, int &below) {
     if (!(fabsf(g) < __builtin_inff())) return g;
     const float r = g / gmax;
